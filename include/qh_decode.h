@@ -213,6 +213,64 @@ int qh_mlp_layer_w8a8(float* out, const float* x, const qh_tensor* gate_w, const
                       const qh_tensor* down_w, void* stream);
 
 /* ======================================================================
+ * Packed sequences: the int8 projection, the delta rule and the attention of
+ * the ops above for many tokens, of one sequence or of several.  No counterpart
+ * in the reference, whose ops take one token.
+ *
+ * Operands are [rows][heads][dim] in place, element (r, h, d) at
+ * p + r * ld + h * hs + d (strides in elements, so that slices of a fused
+ * projection and head-major tensors need no copy).  Pointers and strides are
+ * multiples of 16 bytes where not said otherwise; the stride of a dimension with
+ * one entry does not count.  Inputs may repeat rows (a stride of 0), outputs may
+ * not; an output that shares memory with an input is QH_EINVAL.
+ *
+ * Sequences stand one after another: sequence i has the rows cu[i] .. cu[i + 1]
+ * (cu [n_seq + 1] int32, on the device).  Empty sequences are allowed; rows
+ * outside every sequence are left as they were; a sequence whose bounds are out
+ * of order or outside the array is taken as empty.  max_len, max_q and max_k
+ * are the caller's bounds on the lengths: they choose the form of the kernels
+ * and the size of the workspace, longer sequences are computed all the same.
+ *
+ * Nothing is allocated; scratch is the caller's workspace (256-byte aligned, at
+ * least the bytes its query names, NULL allowed for 0; nothing in it lasts from
+ * one call to the next).  Calls that can run at the same time, captured graphs
+ * among them, need a workspace each.
+ * ==================================================================== */
+#define QH_F32 0
+#define QH_BF16 1
+#define QH_GEMM_MAX_IN 131056        /* int32 sums of int8 products cannot overflow */
+#define QH_GEMM_MAX_TOKENS (1 << 20)
+#define QH_GEMM_MAX_OUT (1 << 24)
+
+/* y[t][o] = float(sum_i xq[t][i] * w[o][i]) * sx[t] * scale[o] for all tokens t: qh_gemv_i8_w8a8 of every row of
+ * xq (int8, ldx a multiple of 16), the fp32 y bit for bit; QH_BF16 rounds it once more.  qh_quant_rows quantises
+ * the activations (a row a token).  in: a multiple of 16, up to QH_GEMM_MAX_IN.  y: any alignment and row stride. */
+int qh_gemm_i8_w8a8(void* y, int64_t ldy, int type, const int8_t* w, const float* scale, const int8_t* xq, int64_t ldx,
+                    const float* sx, int tokens, int out, int in, void* stream);
+
+/* The gated delta rule (qh_delta_rule_layer) along each sequence: q, k [tokens][k_heads][128], v, out
+ * [tokens][heads][128] of `type`, g (the log of the decay, at most 0) and beta [tokens][heads] fp32 with rows ldg and
+ * ldb apart (any alignment), state [n_seq][heads][128][128] fp32 read and updated in place.  Value head h takes key
+ * head h / (heads / k_heads).  q and k as the caller normalised them.  An empty sequence keeps its state. */
+size_t qh_delta_rule_seq_workspace(int tokens, int n_seq, int heads, int max_len);
+int qh_delta_rule_seq(void* out, int64_t ldo, int64_t hso, const void* q, int64_t ldq, int64_t hsq, const void* k, int64_t ldk,
+                      int64_t hsk, const void* v, int64_t ldv, int64_t hsv, int type, const float* g, int64_t ldg,
+                      const float* beta, int64_t ldb, float* state, const int32_t* cu, int n_seq, int tokens, int max_len,
+                      int k_heads, int heads, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Causal attention: q, out [q_rows][heads][head_dim], k, v [k_rows][kv_heads][head_dim], head_dim 128 or 256.
+ * Sequence i's keys are the rows k_start[i] .. + k_len[i] of k and v (device arrays: packed keys, or a slot of a
+ * cache of several), the new tokens' own among them: row r of q_len sees the first r + 1 + k_len - q_len.
+ * out = softmax(scale q k^T) v over those; 0 for a row that sees none; NaN for the rows of a sequence whose keys
+ * do not lie inside the array.  Keys a row does not see have no influence on it, whatever they hold.
+ * Query head h takes kv head h / (heads / kv_heads). */
+size_t qh_attention_seq_workspace(int q_rows, int n_seq, int max_q, int max_k, int heads, int kv_heads, int head_dim);
+int qh_attention_seq(void* out, int64_t ldo, int64_t hso, const void* q, int64_t ldq, int64_t hsq, const void* k, int64_t ldk,
+                     int64_t hsk, const void* v, int64_t ldv, int64_t hsv, int type, const int32_t* cu_q,
+                     const int64_t* k_start, const int32_t* k_len, int n_seq, int q_rows, int64_t k_rows, int max_q, int max_k,
+                     int heads, int kv_heads, int head_dim, float scale, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ======================================================================
  * Weight blob layout (scripts/pack_weights.py:25-101, emit_weight_index.py:13-22)
  * ==================================================================== */
 

@@ -114,6 +114,7 @@ def _lib() -> ctypes.CDLL:
         lib.qh_engine_device_ptr.argtypes = [ctypes.c_void_p, ctypes.c_int]
         if torch is not None:   # (not at the package's import, which host-only users of the layout and packer share)
             _Short.f32, _Short.i8, _Short.i32 = torch.float32, torch.int8, torch.int32
+            _Short.i64, _Short.bf16 = torch.int64, torch.bfloat16
             _Short.device = getattr(torch._C, "_cuda_getDevice", None)
             _Short.stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
             _Short.tensor = torch.Tensor
@@ -214,7 +215,7 @@ def _call(name: str, *args) -> None:
 # types, so ctypes converts each argument once; the current stream's handle is read without building
 # a Stream object.  (A projection call took 10.7 us where this takes 5.4.)
 
-_V, _I, _FL = ctypes.c_void_p, ctypes.c_int, ctypes.c_float
+_V, _I, _FL, _L = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_int64
 _OPS = {
     "qh_gemv_i8": [_V] * 4 + [_I] * 2 + [_V],
     "qh_gemv_f32": [_V] * 3 + [_I] * 2 + [_V],
@@ -238,6 +239,9 @@ _OPS = {
     "qh_quant_rows_bf16": [_V] * 3 + [_I] * 2 + [_V],
     "qh_gemv_i8_w8a8": [_V] * 6 + [_I] * 2 + [_V],
     "qh_matvec_i8": [_V] * 5 + [_I] * 4 + [_V],
+    "qh_gemm_i8_w8a8": [_V, _L, _I] + [_V] * 3 + [_L, _V] + [_I] * 3 + [_V],
+    "qh_delta_rule_seq": [_V, _L, _L] * 4 + [_I, _V, _L, _V, _L, _V, _V] + [_I] * 5 + [_V, ctypes.c_size_t, _V],
+    "qh_attention_seq": [_V, _L, _L] * 4 + [_I, _V, _V, _V, _I, _I, _L] + [_I] * 5 + [_FL, _V, ctypes.c_size_t, _V],
 }
 for _n in ("deltanet", "attention", "mlp"):
     _OPS[f"qh_{_n}_layer_w8a8"] = _OPS[f"qh_{_n}_layer"]
@@ -256,7 +260,7 @@ def _op(name: str):
 
 class _Short:
     """torch's tensor class, dtypes and raw stream query, looked up once by _lib (torch may be absent)."""
-    tensor = f32 = i8 = i32 = device = stream = None
+    tensor = f32 = i8 = i32 = i64 = bf16 = device = stream = None
 
 
 def _slow(t, kind: str, n: int, what: str) -> Optional[int]:
@@ -488,6 +492,159 @@ def quant_rows(q, scale, w, rows: int, cols: int, stream=None):
                    _st(stream))
     if st:
         _check(st, name)
+
+
+# ---------------------------------------------------------------- packed sequences
+# Tensors carry their own sizes and strides here: operands are [rows, heads, dim] with a unit last stride,
+# the other two as the caller has them.  Every tensor has to be on the current device, whose stream the call
+# takes.
+
+F32, BF16 = 0, 1
+
+
+def _on(t, what: str):
+    """A tensor on the current device."""
+    if getattr(t, "is_cuda", False) is not True:
+        raise TypeError(f"{what}: expected a torch CUDA tensor, got {getattr(t, 'device', type(t).__name__)}")
+    if _Short.device is not None and t.get_device() != _Short.device():
+        raise ValueError(f"{what}: tensor is on {t.device}, the current device is {_Short.device()}")
+    return t
+
+
+def _type(t, what: str) -> int:
+    if t.dtype is _Short.f32:
+        return F32
+    if t.dtype is _Short.bf16:
+        return BF16
+    raise TypeError(f"{what}: dtype {t.dtype}, expected float32 or bfloat16")
+
+
+def _r3(t, dt, shape, what: str):
+    """(address, row stride, head stride) of an operand [rows, heads, dim] of the given dtype and shape."""
+    _on(t, what)
+    if t.dtype is not dt:
+        raise TypeError(f"{what}: dtype {t.dtype}, expected {dt}")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{what}: shape {tuple(t.shape)}, expected {shape}")
+    ld, hs, one = t.stride()
+    if one != 1 and shape[2] > 1:
+        raise ValueError(f"{what}: the last dimension has stride {one}, expected 1")
+    return t.data_ptr(), ld, hs
+
+
+def _r2(t, dt, shape, what: str):
+    """(address, row stride) of an operand [rows, dim]."""
+    _on(t, what)
+    if t.dtype is not dt:
+        raise TypeError(f"{what}: dtype {t.dtype}, expected {dt}")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{what}: shape {tuple(t.shape)}, expected {shape}")
+    ld, one = t.stride()
+    if one != 1 and shape[1] > 1:
+        raise ValueError(f"{what}: the last dimension has stride {one}, expected 1")
+    return t.data_ptr(), ld
+
+
+def _c(t, dt, shape, what: str) -> int:
+    """Address of a contiguous tensor of the given dtype and shape."""
+    _on(t, what)
+    if t.dtype is not dt:
+        raise TypeError(f"{what}: dtype {t.dtype}, expected {dt}")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{what}: shape {tuple(t.shape)}, expected {shape}")
+    if not t.is_contiguous():
+        raise ValueError(f"{what}: tensor is not contiguous")
+    return t.data_ptr()
+
+
+def _ws(t):
+    """(address, bytes) of a workspace; None where the call needs none."""
+    if t is None:
+        return None, 0
+    _on(t, "workspace")
+    if not t.is_contiguous():
+        raise ValueError("workspace: tensor is not contiguous")
+    return t.data_ptr() or None, t.numel() * t.element_size()
+
+
+def _dims(t, n: int, what: str):
+    if getattr(t, "ndim", None) != n:
+        raise ValueError(f"{what}: expected a tensor with {n} dimensions")
+    return t.shape
+
+
+def gemm_i8_w8a8(y, w, scale, xq, sx, stream=None):
+    """gemv_i8_w8a8 for many tokens: y[t, o] = (sum_i xq[t, i] w[o, i]) * sx[t] * scale[o].
+
+    xq int8 [tokens, in] (quant_rows makes it and sx, a row a token), w int8 [out, in], y [tokens, out]
+    float32 (gemv_i8_w8a8's bits) or bfloat16; xq and y may be slices of wider rows."""
+    lib = _op("qh_gemm_i8_w8a8")
+    tokens, out = _dims(y, 2, "y")
+    in_ = _dims(w, 2, "w")[1]
+    yp, ldy = _r2(y, y.dtype, (tokens, out), "y")
+    xp, ldx = _r2(xq, _Short.i8, (tokens, in_), "xq")
+    st = lib(yp, ldy, _type(y, "y"), _c(w, _Short.i8, (out, in_), "w"), _c(scale, _Short.f32, (out,), "scale"), xp, ldx,
+             _c(sx, _Short.f32, (tokens,), "sx"), tokens, out, in_, _st(stream))
+    if st:
+        _check(st, "qh_gemm_i8_w8a8")
+
+
+def delta_rule_seq_workspace(tokens: int, n_seq: int, heads: int, max_len: int) -> int:
+    """Bytes of device scratch delta_rule_seq takes from its caller."""
+    f = _lib().qh_delta_rule_seq_workspace
+    f.restype = ctypes.c_size_t
+    return int(f(int(tokens), int(n_seq), int(heads), int(max_len)))
+
+
+def delta_rule_seq(out, q, k, v, g, beta, S, cu, workspace, max_len: int, stream=None):
+    """The gated delta rule (delta_rule_layer) along each of several packed sequences.
+
+    q, k [tokens, k_heads, 128], v, out [tokens, heads, 128] (float32 or bfloat16, any row and head
+    strides), g, beta float32 [tokens, heads], S float32 [n_seq, heads, 128, 128] (updated in place), cu
+    int32 [n_seq + 1] on the device: sequence i has the rows cu[i] .. cu[i + 1].  max_len bounds the
+    sequences' lengths (it chooses the kernels' form); workspace: delta_rule_seq_workspace(...) bytes."""
+    lib = _op("qh_delta_rule_seq")
+    tokens, heads, _ = _dims(v, 3, "v")
+    kh = _dims(k, 3, "k")[1]
+    n = _dims(S, 4, "S")[0]
+    dt, ty = v.dtype, _type(v, "v")
+    gp, ldg = _r2(g, _Short.f32, (tokens, heads), "g")
+    bp, ldb = _r2(beta, _Short.f32, (tokens, heads), "beta")
+    st = lib(*_r3(out, dt, (tokens, heads, LV), "out"), *_r3(q, dt, (tokens, kh, LK), "q"), *_r3(k, dt, (tokens, kh, LK), "k"),
+             *_r3(v, dt, (tokens, heads, LV), "v"), ty, gp, ldg, bp, ldb, _c(S, _Short.f32, (n, heads, LK, LV), "S"),
+             _c(cu, _Short.i32, (n + 1,), "cu"), n, tokens, int(max_len), kh, heads, *_ws(workspace), _st(stream))
+    if st:
+        _check(st, "qh_delta_rule_seq")
+
+
+def attention_seq_workspace(q_rows: int, n_seq: int, max_q: int, max_k: int, heads: int, kv_heads: int, head_dim: int) -> int:
+    """Bytes of device scratch attention_seq takes from its caller."""
+    f = _lib().qh_attention_seq_workspace
+    f.restype = ctypes.c_size_t
+    return int(f(int(q_rows), int(n_seq), int(max_q), int(max_k), int(heads), int(kv_heads), int(head_dim)))
+
+
+def attention_seq(out, q, k, v, cu_q, k_start, k_len, workspace, max_q: int, max_k: int, scale: Optional[float] = None,
+                  stream=None):
+    """Causal attention of packed queries, each sequence over its own rows of a K/V array.
+
+    q, out [q_rows, heads, dim], k, v [k_rows, kv_heads, dim] (float32 or bfloat16, dim 128 or 256, any row
+    and head strides); cu_q int32 [n_seq + 1], k_start int64 [n_seq] and k_len int32 [n_seq] on the device:
+    sequence i's keys are the rows k_start[i] .. + k_len[i], the new tokens' own among them, and row r of
+    q_len sees the first r + 1 + k_len - q_len (0 comes out where it sees none).  scale: 1 / sqrt(dim) if
+    None.  max_q and max_k bound the sequences' rows and keys (they choose the kernels' form); workspace:
+    attention_seq_workspace(...) bytes."""
+    lib = _op("qh_attention_seq")
+    rows, heads, d = _dims(q, 3, "q")
+    krows, kvh, _ = _dims(k, 3, "k")
+    n = _dims(k_len, 1, "k_len")[0]
+    dt, ty = q.dtype, _type(q, "q")
+    st = lib(*_r3(out, dt, (rows, heads, d), "out"), *_r3(q, dt, (rows, heads, d), "q"), *_r3(k, dt, (krows, kvh, d), "k"),
+             *_r3(v, dt, (krows, kvh, d), "v"), ty, _c(cu_q, _Short.i32, (n + 1,), "cu_q"), _c(k_start, _Short.i64, (n,), "k_start"),
+             _c(k_len, _Short.i32, (n,), "k_len"), n, rows, krows, int(max_q), int(max_k), heads, kvh, d,
+             float(d ** -0.5 if scale is None else scale), *_ws(workspace), _st(stream))
+    if st:
+        _check(st, "qh_attention_seq")
 
 
 # ---------------------------------------------------------------- layout / synthetic weights

@@ -1,0 +1,112 @@
+// Operators over packed sequences (qh_seq_ops.hip and the kernels beside it): an int8 matrix product for
+// the activations of many tokens, the gated delta rule and causal attention.  Sequences stand one after
+// another in the rows of an array; cu[i] .. cu[i + 1] are sequence i's rows.  cu, and the key ranges of
+// attention, are device data that the host does not see, so the kernels bound every index themselves:
+// the rules are the functions here, which the CPU tests compile too.
+#pragma once
+#include <stddef.h>
+#include <stdint.h>
+
+#if defined(__HIPCC__)
+#include <hip/hip_runtime.h>
+#define QH_SEQ_FN __host__ __device__ __forceinline__
+#else
+#define QH_SEQ_FN inline
+#endif
+
+namespace qh {
+
+// Rows of one sequence.
+struct SeqSpan {
+  int start, len;
+};
+// Sequence i's rows from its two bounds; bounds out of order or outside [0, rows] leave it without rows.
+QH_SEQ_FN SeqSpan seq_span(int a, int b, int rows) {
+  if (a < 0 || b < a || b > rows) return {0, 0};
+  return {a, b - a};
+}
+// Keys of one sequence: the row its keys start at in an array of k_rows, and their number; a range that
+// does not lie inside the array, or is longer than kMaxKeys, gives -1 (the sequence's outputs are then NaN).
+constexpr int kMaxKeys = 1 << 30;
+QH_SEQ_FN int key_len(int64_t start, int len, int64_t k_rows) {
+  if (len < 0 || len > kMaxKeys || start < 0 || start > k_rows || (int64_t)len > k_rows - start) return -1;
+  return len;
+}
+// Row tiles of a sequence of len rows.
+QH_SEQ_FN int seq_tiles(int len, int tile) { return len / tile + (len % tile != 0); }
+// The most tiles that n sequences of `rows` rows in all can have.
+QH_SEQ_FN int64_t seq_tiles_max(int64_t rows, int n, int tile) {
+  const int64_t t = rows / tile + n;
+  return t < rows ? t : rows;   // (each tile holds a row)
+}
+// Keys that row `row` of q_len sees of k_len: the last rows stand at the last keys.  Not below 0.
+QH_SEQ_FN int keys_seen(int row, int q_len, int k_len) {
+  const int64_t n = (int64_t)row + 1 + k_len - q_len;
+  return n < 0 ? 0 : (int)n;
+}
+
+}  // namespace qh
+
+#if defined(__HIPCC__)
+namespace qh {
+
+// One operand [rows][heads][dim] in place: element (r, h, d) at p + r * ld + h * hs + d.
+struct SeqIn {
+  const void* p = nullptr;
+  int64_t ld = 0, hs = 0;
+};
+struct SeqOut {
+  void* p = nullptr;
+  int64_t ld = 0, hs = 0;
+};
+
+struct GemmSeq {
+  SeqOut y;                       // [tokens][out], fp32 or bf16
+  const int8_t* w = nullptr;      // [out][in]
+  const float* scale = nullptr;   // [out]
+  SeqIn x;                        // [tokens][in] int8
+  const float* sx = nullptr;      // [tokens]
+  int tokens = 0, out = 0, in = 0;
+  int bf16 = 0;                   // type of y
+};
+
+struct DeltaSeq {
+  SeqOut out;                     // [tokens][heads][128]
+  SeqIn q, k, v;                  // [tokens][k_heads][128], [tokens][heads][128]; the type of out
+  const float* g = nullptr;       // [tokens][heads], rows ldg apart
+  const float* beta = nullptr;
+  int64_t ldg = 0, ldb = 0;
+  float* S = nullptr;             // [n_seq][heads][128][128]
+  const int32_t* cu = nullptr;
+  int n_seq = 0, tokens = 0, k_heads = 0, heads = 0;
+  int bf16 = 0;
+};
+
+struct AttnSeq {
+  SeqOut out;                     // [q_rows][heads][dim]
+  SeqIn q, k, v;                  // [q_rows][heads][dim], [k_rows][kv_heads][dim]; the type of out
+  const int32_t* cu_q = nullptr;  // [n_seq + 1]
+  const int64_t* k_start = nullptr;
+  const int32_t* k_len = nullptr;
+  int n_seq = 0, q_rows = 0;
+  int64_t k_rows = 0;
+  int heads = 0, kv_heads = 0, dim = 0;
+  float scale = 0.0f;
+  int bf16 = 0;
+  float* part = nullptr;          // split partials (see attn_split)
+  int chunk = 0, nsplit = 1;      // keys of a split; splits a sequence of max_k keys has
+};
+
+hipError_t launch_gemm_seq(const GemmSeq& a, hipStream_t s);
+hipError_t launch_delta_seq(const DeltaSeq& a, hipStream_t s);
+hipError_t launch_attn_seq(const AttnSeq& a, hipStream_t s);
+
+// The split of the keys for few query rows (qh_attn_seq.hip), and the bytes its partials take.
+struct AttnSplit {
+  int chunk, nsplit;
+  size_t bytes;
+};
+AttnSplit attn_seq_split(int64_t q_rows, int n_seq, int max_k, int heads, int kv_heads, int dim);
+
+}  // namespace qh
+#endif
