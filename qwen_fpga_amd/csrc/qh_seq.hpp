@@ -68,6 +68,7 @@ struct GemmSeq {
   const float* sx = nullptr;      // [tokens]
   int tokens = 0, out = 0, in = 0;
   int bf16 = 0;                   // type of y
+  int wide = 0;                   // y takes four outputs in one store (set by the launch)
 };
 
 struct DeltaSeq {
