@@ -1,7 +1,6 @@
 // Causal attention with grouped heads over packed sequences.  Row r of a sequence with q_len rows and k_len
 // keys sees the first r + 1 + k_len - q_len keys:  out = softmax(scale q K^T) V  over those; 0 without any.
-#include "qh_device.hpp"
-#include "qh_seq.hpp"
+#include "qh_seq_device.hpp"
 
 namespace qh {
 
@@ -13,38 +12,6 @@ namespace {
 
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kNegInf = -__builtin_inff();
-
-// The sequence and the tile in it of row tile b (tiles of `tile` rows; a token is `mult` rows).
-struct TileAt {
-  int seq, tile;
-  SeqSpan sp;
-};
-__device__ __forceinline__ bool find_tile(const int32_t* cu, int n_seq, int rows, int mult, int tile, int b, TileAt& o) {
-  const int lane = threadIdx.x & 63;
-  int base = 0;
-  for (int s0 = 0; s0 < n_seq; s0 += 64) {
-    const int i = s0 + lane;
-    SeqSpan sp = {0, 0};
-    if (i < n_seq) sp = seq_span(as_global(cu)[i], as_global(cu)[i + 1], rows);
-    const int n = seq_tiles(sp.len * mult, tile);
-    int inc = n;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const int t = __shfl_up(inc, d);
-      if (lane >= d) inc += t;
-    }
-    const uint64_t past = __ballot(base + inc > b);
-    if (past != 0) {
-      const int l = __builtin_ctzll(past);
-      o.seq = s0 + l;
-      o.tile = b - base - (__builtin_amdgcn_readlane(inc, l) - __builtin_amdgcn_readlane(n, l));
-      o.sp = {__builtin_amdgcn_readlane(sp.start, l), __builtin_amdgcn_readlane(sp.len, l)};
-      return true;
-    }
-    base += __builtin_amdgcn_readlane(inc, 63);
-  }
-  return false;
-}
 
 __device__ __forceinline__ bool non_finite(float v) { return (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u; }
 

@@ -81,6 +81,7 @@ struct DeltaSeq {
   const int32_t* cu = nullptr;
   int n_seq = 0, tokens = 0, k_heads = 0, heads = 0;
   int bf16 = 0;
+  float* ws = nullptr;            // delta_seq_workspace bytes: in chunks; null: token by token
 };
 
 struct AttnSeq {
@@ -101,6 +102,10 @@ struct AttnSeq {
 hipError_t launch_gemm_seq(const GemmSeq& a, hipStream_t s);
 hipError_t launch_delta_seq(const DeltaSeq& a, hipStream_t s);
 hipError_t launch_attn_seq(const AttnSeq& a, hipStream_t s);
+
+// Sequences of up to this many tokens run token by token.
+constexpr int kDeltaStepLen = 12;
+size_t delta_seq_workspace(int tokens, int n_seq, int heads, int max_len);
 
 // The split of the keys for few query rows (qh_attn_seq.hip), and the bytes its partials take.
 struct AttnSplit {

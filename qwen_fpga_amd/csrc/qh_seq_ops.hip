@@ -13,6 +13,7 @@ hipStream_t S(void* s) { return reinterpret_cast<hipStream_t>(s); }
 
 constexpr int64_t kMaxStride = (int64_t)1 << 40;   // elements; keeps every offset inside 64 bits
 constexpr int64_t kMaxUnits = 0x7fffffff;          // workgroups, and rows times heads
+constexpr int kMaxGridY = 65535;
 
 // An operand [rows][heads][dim] with its element size, to check it and to compare it with another.
 struct View {
@@ -86,8 +87,9 @@ int qh_gemm_i8_w8a8(void* y, int64_t ldy, int type, const int8_t* w, const float
 }
 
 size_t qh_delta_rule_seq_workspace(int tokens, int n_seq, int heads, int max_len) {
-  (void)tokens, (void)n_seq, (void)heads, (void)max_len;
-  return 0;
+  if (tokens <= 0 || n_seq <= 0 || heads <= 0 || (int64_t)n_seq * heads * 8 > kMaxUnits || (int64_t)tokens * heads > kMaxUnits)
+    return 0;
+  return delta_seq_workspace(tokens, n_seq, heads, max_len);
 }
 
 int qh_delta_rule_seq(void* out, int64_t ldo, int64_t hso, const void* q, int64_t ldq, int64_t hsq, const void* k, int64_t ldk,
@@ -97,7 +99,7 @@ int qh_delta_rule_seq(void* out, int64_t ldo, int64_t hso, const void* q, int64_
   if (!type_ok(type) || n_seq < 0 || tokens < 0 || max_len < 0 || k_heads <= 0 || heads <= 0 || heads % k_heads != 0)
     return QH_EINVAL;
   if (tokens == 0 || n_seq == 0) return QH_OK;
-  if ((int64_t)n_seq * heads * 8 > kMaxUnits || (int64_t)tokens * heads > kMaxUnits) return QH_ERANGE;
+  if ((int64_t)n_seq * heads * 8 > kMaxUnits || (int64_t)tokens * heads > kMaxUnits || heads > kMaxGridY) return QH_ERANGE;
   const int eb = type == QH_BF16 ? 2 : 4;
   const View vo{out, tokens, heads, QH_LV, ldo, hso, eb}, vq{q, tokens, k_heads, QH_LK, ldq, hsq, eb},
       vk{k, tokens, k_heads, QH_LK, ldk, hsk, eb}, vv{v, tokens, heads, QH_LV, ldv, hsv, eb};
@@ -129,6 +131,7 @@ int qh_delta_rule_seq(void* out, int64_t ldo, int64_t hso, const void* q, int64_
   a.k_heads = k_heads;
   a.heads = heads;
   a.bf16 = type == QH_BF16;
+  a.ws = need > 0 ? static_cast<float*>(workspace) : nullptr;
   return hip_status(launch_delta_seq(a, S(stream)));
 }
 

@@ -193,6 +193,41 @@ def test_delta_full_resets(q, torch_cuda):
     delta_check(torch, out, S, delta_oracle(torch, *host, lens), lens, False)
 
 
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+@pytest.mark.parametrize("which", ["q", "k", "v", "g", "beta", "S"])
+@pytest.mark.parametrize("bad", [math.nan, math.inf], ids=str)
+def test_delta_non_finite_inputs(q, torch_cuda, bf16, which, bad):
+    """A token that is not finite has no influence on those before it, on other heads or on other sequences,
+    and a query's none on the state; what comes after it shows it."""
+    torch = torch_cuda
+    lens, at = [100, 80], 75                      # in the second chunk of the first sequence
+    host, _ = delta_inputs(torch, 14, lens, 2, 2, bf16, decay=0.05)
+    run = lambda h: (lambda S: (delta_run(q, torch, [x.cuda() for x in h[:5]], S, lens).cpu(), S.cpu()))(h[5].cuda())
+    clean, S0 = run(host)
+    i = ["q", "k", "v", "g", "beta", "S"].index(which)
+    if which == "S":
+        host[5][0, 0, :, 9] = bad                 # one column of one head
+    elif which in ("g", "beta"):
+        host[i][at, 0] = bad
+    else:
+        host[i][at, 0, 5] = bad
+    out, S = run(host)
+    first = 0 if which == "S" else at
+    ok = lambda x, y: (x.double() - y.double()).abs().max().item() <= 1e-3 * y.double().abs().max().item() + (BF if bf16 else 0)
+    assert torch.isfinite(out[:first]).all() and (first == 0 or ok(out[:first], clean[:first]))
+    assert torch.equal(out[100:], clean[100:]) and torch.equal(S[1], S0[1])
+    assert ok(out[:100, 1], clean[:100, 1]) and ok(S[0, 1], S0[0, 1])       # the other head
+    if which == "q":
+        assert not torch.isfinite(out[at, 0]).any() and ok(S[0, 0], S0[0, 0])
+        assert torch.isfinite(out[at + 1:100, 0]).all()
+    elif which == "S":
+        assert not torch.isfinite(S[0, 0, :, 9]).any()
+        keep = [c for c in range(128) if c != 9]
+        assert ok(out[:100, 0][:, keep], clean[:100, 0][:, keep]) and ok(S[0, 0][:, keep], S0[0, 0][:, keep])
+    else:
+        assert not torch.isfinite(out[at:100, 0]).all() and not torch.isfinite(S[0, 0]).all()
+
+
 def test_delta_prompt_then_tokens(q, torch_cuda):
     """A prompt in one call, in two, and token by token through the one-token op: the same within tolerance."""
     torch = torch_cuda
