@@ -13,6 +13,77 @@ namespace {
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kNegInf = -__builtin_inff();
 
+// The work of the split form.  A unit is 16 rows of a sequence (tokens x query heads of one kv head) and one chunk
+// of its keys; chunks hold the same number of keys in every sequence, chosen from all sequences' keys (which only
+// the device knows) so that the units come to about kFill, two workgroups for each CU: 16 sequences of 15 to 8191
+// keys took 55 us with chunks cut from the longest one's length and XX with this.
+struct Unit {
+  SeqSpan sp;
+  int64_t ks;   // the sequence's keys: first row, number (key_len)
+  int kl;
+  int tile, split, nsplit, chunk;
+  int first;    // unit (before kv heads) of the tile's first split
+};
+constexpr int kFill = 512, kMinChunk = 128;
+// Unit b of the split kernel, or (JOIN) the units of row tile b.
+template <bool JOIN>
+__device__ __forceinline__ bool find_unit(const AttnSeq& a, int b, Unit& o) {
+  const int lane = threadIdx.x & 63, G = a.heads / a.kv_heads;
+  SeqSpan sp;   // of sequence s0 + lane, as of its keys and tiles
+  int64_t ks;
+  int kl, tiles, chunk = kMaxKeys;
+  auto load = [&](int s0) {
+    const int i = min(s0 + lane, a.n_seq - 1);
+    ks = as_global(a.k_start)[i];
+    const int n = as_global(a.k_len)[i];
+    sp = seq_span(as_global(a.cu_q)[i], as_global(a.cu_q)[i + 1], a.q_rows);
+    kl = key_len(ks, n, a.k_rows);
+    tiles = s0 + lane < a.n_seq ? seq_tiles(sp.len * G, 16) : 0;
+  };
+  load(0);
+  if (!a.whole) {
+    int64_t work = (int64_t)tiles * max(kl, 0);   // keys of all row tiles
+    for (int s0 = 64; s0 < a.n_seq; s0 += 64) {
+      load(s0);
+      work += (int64_t)tiles * max(kl, 0);
+    }
+    if (a.n_seq > 64) load(0);
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) work += __shfl_xor(work, d);
+    const int64_t c = (work * a.kv_heads + kFill - 1) / kFill;
+    chunk = (int)min(max((c + 63) / 64 * 64, (int64_t)kMinChunk), (int64_t)kMaxKeys);
+  }
+  int base = 0, first = 0;   // of the next 64 sequences: tiles (JOIN) or units, units
+  for (int s0 = 0; s0 < a.n_seq; s0 += 64) {
+    if (s0 > 0) load(s0);
+    const int ns = max(seq_tiles(max(kl, 0), chunk), 1);
+    int iu = tiles * ns, it = tiles;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const int tu = __shfl_up(iu, d), tt = __shfl_up(it, d);
+      if (lane >= d) iu += tu, it += tt;
+    }
+    const uint64_t past = __ballot(base + (JOIN ? it : iu) > b);
+    if (past != 0) {
+      const int l = __builtin_ctzll(past);
+      auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
+      o.sp = {of(sp.start), of(sp.len)};
+      o.ks = (int64_t)((uint64_t)(uint32_t)of((int)(ks >> 32)) << 32 | (uint32_t)of((int)ks));
+      o.kl = of(kl);
+      o.nsplit = of(ns);
+      o.chunk = chunk;
+      const int in = b - base - (of(JOIN ? it : iu) - of(JOIN ? tiles : tiles * ns));
+      o.tile = JOIN ? in : in / o.nsplit;
+      o.split = JOIN ? 0 : in - o.tile * o.nsplit;
+      o.first = first + of(iu) - of(tiles * ns) + o.tile * o.nsplit;
+      return o.tile >= 0 && o.tile < of(tiles);   // (bounds that overlap can make more tiles than an int counts)
+    }
+    base += __builtin_amdgcn_readlane(JOIN ? it : iu, 63);
+    first += __builtin_amdgcn_readlane(iu, 63);
+  }
+  return false;
+}
+
 __device__ __forceinline__ bool non_finite(float v) { return (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u; }
 
 // Sets the non-finite elements of 16 bytes to zero; true if there was one.
@@ -43,45 +114,41 @@ __device__ __forceinline__ float elem(const u32x4& v, int e) {
     return __uint_as_float(v[e]);
 }
 
-// Splits' partials: for each (row tile, kv head, split) 16 rows of D sums, 16 maxima, 16 sums of exponentials.
-__device__ __forceinline__ size_t part_at(size_t unit, int split, int nsplit, int D) {
-  return (unit * nsplit + split) * (size_t)(16 * D + 32);
-}
+// Partials of a unit and kv head: 16 rows of D sums, their maxima, their sums of exponentials.
+constexpr size_t part_floats(int D) { return 16 * D + 32; }
 
 // Few query rows: a workgroup takes 16 rows (tokens x query heads of one kv head) and one chunk of the keys,
 // its four waves every fourth step of KT keys.  Per step a wave forms S^T = K Q^T, so that a lane holds the
 // scores of one row, and O^T = V^T P^T, whose operand P^T those registers are (the keys of a step stand in the
 // order in which the lanes hold them).
 template <bool BF16, int D>
-__global__ __launch_bounds__(256) void attn_split_kernel(const AttnSeq a) {
+__global__ __launch_bounds__(256, 2) void attn_split_kernel(const AttnSeq a) {
   constexpr int EV = BF16 ? 8 : 4;        // elements of 16 bytes
   constexpr int KT = BF16 ? 32 : 16;      // keys of a step
   constexpr int NQ = D / (4 * EV);        // 16-byte pieces of a row in a lane
   constexpr int NG = D / (16 * EV);
   constexpr int NK = BF16 ? 8 : 4;        // V rows of a lane in a step
   constexpr int NT = D / 16;
+  constexpr bool kQLds = D == 256;   // the query rows in LDS where two waves a SIMD would not hold them
   __shared__ __attribute__((aligned(16))) float lacc[2][64][NT * 4 + 4];
+  __shared__ u32x4 lq[kQLds ? NQ : 1][64];
   __shared__ float lm[2][16], ll[2][16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, j = lane & 15;
   const int G = a.heads / a.kv_heads;
-  const int unit = blockIdx.x, kvh = unit % a.kv_heads, split = blockIdx.y;
-  TileAt at;
-  if (!find_tile(a.cu_q, a.n_seq, a.q_rows, G, 16, unit / a.kv_heads, at)) return;
-  const int64_t ks = as_global(a.k_start)[at.seq];
-  const int kl = key_len(ks, as_global(a.k_len)[at.seq], a.k_rows);
+  const int kvh = (int)blockIdx.x % a.kv_heads;
+  Unit at;
+  if (!find_unit<false>(a, (int)blockIdx.x / a.kv_heads, at)) return;
+  const int64_t ks = at.ks;
+  const int kl = at.kl;
   const int rows = at.sp.len * G, r0 = 16 * at.tile;
   const int row = min(r0 + j, rows - 1), tok = row / G, hq = kvh * G + row % G;
   const int seen = keys_seen(tok, at.sp.len, kl);                                    // this lane's row
   const int end = keys_seen(min(r0 + 15, rows - 1) / G, at.sp.len, kl);              // the tile's last row
   const int all = keys_seen(r0 / G, at.sp.len, kl);                                  // its first
-  const int k0 = split * a.chunk, k1 = min(end, a.nsplit == split + 1 ? end : k0 + a.chunk);
-  if (split > 0 && k0 >= end) return;
+  const int k0 = at.split * at.chunk, k1 = min(end, at.split + 1 == at.nsplit ? end : k0 + at.chunk);
+  if (at.split > 0 && k0 >= end) return;   // (no row of the tile sees it)
 
-  u32x4 qv[NQ];
-  const char* qp = static_cast<const char*>(a.q.p) + ((at.sp.start + tok) * a.q.ld + hq * a.q.hs) * (BF16 ? 2 : 4) + 16 * g;
-#pragma unroll
-  for (int s = 0; s < NQ; ++s) qv[s] = *as_global(reinterpret_cast<const u32x4*>(qp + 64 * s));
   f32x4 acc[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -90,36 +157,56 @@ __global__ __launch_bounds__(256) void attn_split_kernel(const AttnSeq a) {
   const int64_t kld = a.k.ld * (BF16 ? 2 : 4), vld = a.v.ld * (BF16 ? 2 : 4);
   const char* kp = static_cast<const char*>(a.k.p) + (ks * a.k.ld + kvh * a.k.hs) * (BF16 ? 2 : 4) + 16 * g;
   const char* vp = static_cast<const char*>(a.v.p) + (ks * a.v.ld + kvh * a.v.hs) * (BF16 ? 2 : 4) + 16 * j;
-  for (int kb = k0 + KT * wave; kb < k1; kb += 4 * KT) {
-    u32x4 kv[KT / 16][NQ], vv[NK][NG];
+  u32x4 kv[KT / 16][NQ], vv[NK][NG];   // a step's rows; the next step's are loaded as soon as these are used
+  auto load_k = [&](int kb) {
 #pragma unroll
     for (int t = 0; t < KT / 16; ++t) {
       const char* p = kp + min(kb + 16 * t + j, k1 - 1) * kld;
 #pragma unroll
       for (int s = 0; s < NQ; ++s) kv[t][s] = *as_global(reinterpret_cast<const u32x4*>(p + 64 * s));
     }
+  };
+  auto load_v = [&](int kb) {
 #pragma unroll
     for (int i = 0; i < NK; ++i) {
       const char* p = vp + min(kb + 16 * (i >> 2) + 4 * g + (i & 3), k1 - 1) * vld;
 #pragma unroll
       for (int s = 0; s < NG; ++s) vv[i][s] = *as_global(reinterpret_cast<const u32x4*>(p + 256 * s));
     }
+  };
+  int kb = k0 + KT * wave;
+  if (kb < k1) load_k(kb), load_v(kb);
+  u32x4 qv[kQLds ? 1 : NQ];
+  const char* qp = static_cast<const char*>(a.q.p) + ((at.sp.start + tok) * a.q.ld + hq * a.q.hs) * (BF16 ? 2 : 4) + 16 * g;
+  if constexpr (kQLds) {
+#pragma unroll
+    for (int s = 0; s < NQ / 4; ++s)
+      lq[4 * s + wave][lane] = *as_global(reinterpret_cast<const u32x4*>(qp + 64 * (4 * s + wave)));
+    __syncthreads();
+  } else {
+#pragma unroll
+    for (int s = 0; s < NQ; ++s) qv[s] = *as_global(reinterpret_cast<const u32x4*>(qp + 64 * s));
+  }
+  for (; kb < k1; kb += 4 * KT) {
     f32x4 st[KT / 16];
 #pragma unroll
-    for (int t = 0; t < KT / 16; ++t) {
-      st[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int t = 0; t < KT / 16; ++t) st[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int s = 0; s < NQ; ++s) {
+    for (int s = 0; s < NQ; ++s) {
+      const u32x4 qs = kQLds ? lq[kQLds ? s : 0][lane] : qv[kQLds ? 0 : s];
+#pragma unroll
+      for (int t = 0; t < KT / 16; ++t) {
         if constexpr (BF16) {
-          st[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kv[t][s]), __builtin_bit_cast(bf16x8, qv[s]),
+          st[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kv[t][s]), __builtin_bit_cast(bf16x8, qs),
                                                           st[t], 0, 0, 0);
         } else {
 #pragma unroll
           for (int c = 0; c < 4; ++c)
-            st[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kv[t][s][c]), __uint_as_float(qv[s][c]), st[t], 0, 0, 0);
+            st[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kv[t][s][c]), __uint_as_float(qs[c]), st[t], 0, 0, 0);
         }
       }
     }
+    load_k(min(kb + 4 * KT, k1 - 1));
     float p[NK], mx = kNegInf;
 #pragma unroll
     for (int i = 0; i < NK; ++i) {
@@ -175,6 +262,7 @@ __global__ __launch_bounds__(256) void attn_split_kernel(const AttnSeq a) {
           for (int i = 0; i < 4; ++i)
             acc[4 * s + c] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vv[i][s][c]), p[i], acc[4 * s + c], 0, 0, 0);
     }
+    load_v(min(kb + 4 * KT, k1 - 1));
     if (__ballot(bad) != 0) {
       for (int key = kb; key < min(kb + KT, k1); ++key) {
         const char* q = static_cast<const char*>(a.v.p) + ((ks + key) * a.v.ld + kvh * a.v.hs) * (BF16 ? 2 : 4);
@@ -218,7 +306,7 @@ __global__ __launch_bounds__(256) void attn_split_kernel(const AttnSeq a) {
     }
   }
   if (wave != 0 || r0 + j >= rows) return;
-  if (a.nsplit == 1) {
+  if (at.nsplit == 1) {
     const float inv = kl < 0 ? __builtin_nanf("") : seen == 0 ? 0.0f : 1.0f / l;
     char* op = static_cast<char*>(a.out.p) + ((at.sp.start + tok) * a.out.ld + hq * a.out.hs) * (BF16 ? 2 : 4);
 #pragma unroll
@@ -239,7 +327,7 @@ __global__ __launch_bounds__(256) void attn_split_kernel(const AttnSeq a) {
         *as_global_w(reinterpret_cast<u32x4*>(op + 256 * s + 16 * (4 * g + r))) = o;
       }
   } else {
-    float* pp = a.part + part_at(unit, split, a.nsplit, D);
+    float* pp = a.part + (size_t)blockIdx.x * part_floats(D);   // (unit first + split, kv head)
 #pragma unroll
     for (int s = 0; s < NG; ++s)
 #pragma unroll
@@ -252,69 +340,97 @@ __global__ __launch_bounds__(256) void attn_split_kernel(const AttnSeq a) {
   }
 }
 
-// Joins the splits of one row: four waves take every fourth split.
+// Joins the splits of a tile's rows, every fourth row in a workgroup: sixteen waves take every sixteenth split, four
+// in flight, each with a running maximum of its own.
 template <bool BF16, int D>
-__global__ __launch_bounds__(256) void attn_join_kernel(const AttnSeq a) {
-  constexpr int W = D / 64;   // elements of a lane
-  __shared__ float lo[4][D], lsum[4];
+__global__ __launch_bounds__(1024) void attn_join_kernel(const AttnSeq a) {
+  constexpr int W = D / 64, NW = 16, U = 4;   // elements of a lane; waves; splits in flight
+  typedef float vec __attribute__((ext_vector_type(W)));
+  __shared__ vec lo[NW][64];
+  __shared__ float lsum[NW], lmax[NW];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int G = a.heads / a.kv_heads;
-  const int unit = blockIdx.x, kvh = unit % a.kv_heads, j = blockIdx.y;
-  TileAt at;
-  if (!find_tile(a.cu_q, a.n_seq, a.q_rows, G, 16, unit / a.kv_heads, at)) return;
-  const int kl = key_len(as_global(a.k_start)[at.seq], as_global(a.k_len)[at.seq], a.k_rows);
-  const int rows = at.sp.len * G, row = 16 * at.tile + j;
-  if (row >= rows) return;
-  const int tok = row / G, hq = kvh * G + row % G;
-  const int seen = keys_seen(tok, at.sp.len, kl);
-  const int ns = min(seq_tiles(seen, a.chunk), a.nsplit);   // splits that this row sees (the rest hold no key of it)
-  const float* pp = a.part + part_at(unit, 0, a.nsplit, D);
-  constexpr size_t kStep = 16 * D + 32;
-  float m = kNegInf;
-  for (int s = lane; s < ns; s += 64) m = fmaxf(m, as_global(pp)[s * kStep + 16 * D + j]);
-  m = xor_max<64>(m);
-  const float mu = m == kNegInf ? 0.0f : m;
-  float acc[W] = {}, l = 0.0f;
-  for (int s = wave; s < ns; s += 4) {
-    const float e = __builtin_amdgcn_exp2f(as_global(pp)[s * kStep + 16 * D + j] - mu);
-    l += e * as_global(pp)[s * kStep + 16 * D + 16 + j];
+  const int kvh = (int)blockIdx.x % a.kv_heads;
+  Unit at;
+  if (!find_unit<true>(a, (int)blockIdx.x / a.kv_heads, at)) return;
+  if (at.nsplit == 1) return;   // written by the split kernel
+  if (at.first < 0 || (int64_t)(at.first + at.nsplit) * a.kv_heads > (int64_t)gridDim.x + kFill) return;   // past its grid
+  const int rows = at.sp.len * G;
+  const size_t step = part_floats(D) * a.kv_heads;
+  const float* pp = a.part + ((size_t)at.first * a.kv_heads + kvh) * part_floats(D);
+  for (int j = blockIdx.y; j < 16 && 16 * at.tile + j < rows; j += 4) {
+    const int row = 16 * at.tile + j, tok = row / G, hq = kvh * G + row % G;
+    const int seen = keys_seen(tok, at.sp.len, at.kl);
+    const int ns = min(seq_tiles(seen, at.chunk), at.nsplit);   // splits that this row sees (the rest hold no key of it)
+    float m = kNegInf, l = 0.0f;
+    vec acc = {};
+    for (int s0 = wave; s0 < ns; s0 += NW * U) {
+      float mv[U], lv[U], mn = m;
+      vec av[U];
 #pragma unroll
-    for (int w = 0; w < W; ++w) acc[w] += e * as_global(pp)[s * kStep + j * D + 64 * w + lane];
+      for (int u = 0; u < U; ++u) {
+        const float* p = pp + min(s0 + NW * u, ns - 1) * step;
+        mv[u] = s0 + NW * u < ns ? as_global(p)[16 * D + j] : kNegInf;
+        lv[u] = as_global(p)[16 * D + 16 + j];
+        av[u] = *as_global(reinterpret_cast<const vec*>(p + j * D) + lane);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) mn = fmaxf(mn, mv[u]);
+      const float mu = mn == kNegInf ? 0.0f : mn, al = __builtin_amdgcn_exp2f(m - mu);
+      m = mn;
+      l *= al;
+      acc *= al;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float e = __builtin_amdgcn_exp2f(mv[u] - mu);
+        if (s0 + NW * u < ns) l += e * lv[u], acc += e * av[u];
+      }
+    }
+    __syncthreads();   // the row before has been read
+    lo[wave][lane] = acc;
+    if (lane == 0) lsum[wave] = l, lmax[wave] = m;
+    __syncthreads();
+    if (wave != 0) continue;
+    m = kNegInf;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) m = fmaxf(m, lmax[w]);
+    const float mu = m == kNegInf ? 0.0f : m;
+    acc = vec{};
+    l = 0.0f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float e = __builtin_amdgcn_exp2f(lmax[w] - mu);
+      acc += e * lo[w][lane];
+      l += e * lsum[w];
+    }
+    acc *= seen == 0 ? 0.0f : 1.0f / l;
+    const int64_t to = (at.sp.start + tok) * a.out.ld + hq * a.out.hs + W * lane;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      if constexpr (BF16)
+        as_global_w(static_cast<__bf16*>(a.out.p))[to + w] = (__bf16)acc[w];
+      else
+        as_global_w(static_cast<float*>(a.out.p))[to + w] = acc[w];
+    }
   }
-#pragma unroll
-  for (int w = 0; w < W; ++w) lo[wave][64 * w + lane] = acc[w];
-  if (lane == 0) lsum[wave] = l;
-  __syncthreads();
-  if ((int)threadIdx.x >= D) return;
-  l = (lsum[0] + lsum[1]) + (lsum[2] + lsum[3]);
-  const float inv = kl < 0 ? __builtin_nanf("") : seen == 0 ? 0.0f : 1.0f / l;
-  const int d = threadIdx.x;
-  const float v = ((lo[0][d] + lo[1][d]) + (lo[2][d] + lo[3][d])) * inv;
-  const int64_t o = (at.sp.start + tok) * a.out.ld + hq * a.out.hs + d;
-  if constexpr (BF16)
-    as_global_w(static_cast<__bf16*>(a.out.p))[o] = (__bf16)v;
-  else
-    as_global_w(static_cast<float*>(a.out.p))[o] = v;
 }
 
 template <bool BF16, int D>
 hipError_t launch(const AttnSeq& a, hipStream_t s) {
-  const unsigned units = (unsigned)(seq_tiles_max((int64_t)a.q_rows * (a.heads / a.kv_heads), a.n_seq, 16) * a.kv_heads);
-  attn_split_kernel<BF16, D><<<dim3(units, a.nsplit), 256, 0, s>>>(a);
-  if (a.nsplit > 1) attn_join_kernel<BF16, D><<<dim3(units, 16), 256, 0, s>>>(a);
+  const unsigned tiles = (unsigned)(seq_tiles_max((int64_t)a.q_rows * (a.heads / a.kv_heads), a.n_seq, 16) * a.kv_heads);
+  attn_split_kernel<BF16, D><<<a.whole ? tiles : tiles + kFill, 256, 0, s>>>(a);
+  if (!a.whole) attn_join_kernel<BF16, D><<<dim3(tiles, 4), 1024, 0, s>>>(a);
   return hipGetLastError();
 }
 
 }  // namespace
 
-AttnSplit attn_seq_split(int64_t q_rows, int n_seq, int max_k, int heads, int kv_heads, int dim) {
-  const int64_t units = seq_tiles_max(q_rows * (heads / kv_heads), n_seq, 16) * kv_heads;
-  const int64_t want = units >= 1024 ? 1 : 2048 / (units > 0 ? units : 1);   // splits that fill the chip
-  int64_t chunk = (max_k + want - 1) / want;
-  chunk = (chunk + 127) / 128 * 128;
-  if (chunk < 128) chunk = 128;
-  const int64_t n = max_k > chunk ? (max_k + chunk - 1) / chunk : 1;
-  return {(int)chunk, (int)n, n > 1 ? (size_t)(units * n) * (16 * dim + 32) * sizeof(float) : 0};
+bool attn_seq_whole(int max_k) { return max_k <= kMinChunk; }
+
+size_t attn_seq_workspace(int64_t q_rows, int n_seq, int max_k, int heads, int kv_heads, int dim) {
+  if (attn_seq_whole(max_k)) return 0;
+  const int64_t tiles = seq_tiles_max(q_rows * (heads / kv_heads), n_seq, 16) * kv_heads;
+  return (size_t)(tiles + kFill) * part_floats(dim) * sizeof(float);
 }
 
 hipError_t launch_attn_seq(const AttnSeq& a, hipStream_t s) {

@@ -95,8 +95,8 @@ struct AttnSeq {
   int heads = 0, kv_heads = 0, dim = 0;
   float scale = 0.0f;
   int bf16 = 0;
-  float* part = nullptr;          // split partials (see attn_split)
-  int chunk = 0, nsplit = 1;      // keys of a split; splits a sequence of max_k keys has
+  float* part = nullptr;          // partials of the split form
+  int whole = 0;                  // the split form with one chunk of all keys (nothing to join)
 };
 
 hipError_t launch_gemm_seq(const GemmSeq& a, hipStream_t s);
@@ -107,12 +107,9 @@ hipError_t launch_attn_seq(const AttnSeq& a, hipStream_t s);
 constexpr int kDeltaStepLen = 12;
 size_t delta_seq_workspace(int tokens, int n_seq, int heads, int max_len);
 
-// The split of the keys for few query rows (qh_attn_seq.hip), and the bytes its partials take.
-struct AttnSplit {
-  int chunk, nsplit;
-  size_t bytes;
-};
-AttnSplit attn_seq_split(int64_t q_rows, int n_seq, int max_k, int heads, int kv_heads, int dim);
+// Whether max_k keys are too few to split, and the bytes of workspace of a call.
+bool attn_seq_whole(int max_k);
+size_t attn_seq_workspace(int64_t q_rows, int n_seq, int max_k, int heads, int kv_heads, int dim);
 
 }  // namespace qh
 #endif

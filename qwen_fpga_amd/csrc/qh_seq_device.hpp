@@ -30,7 +30,7 @@ __device__ __forceinline__ bool find_tile(const int32_t* cu, int n_seq, int rows
       o.seq = s0 + l;
       o.tile = b - base - (__builtin_amdgcn_readlane(inc, l) - __builtin_amdgcn_readlane(n, l));
       o.sp = {__builtin_amdgcn_readlane(sp.start, l), __builtin_amdgcn_readlane(sp.len, l)};
-      return true;
+      return o.tile >= 0 && o.tile < __builtin_amdgcn_readlane(n, l);   // (overlapping bounds can overflow the count)
     }
     base += __builtin_amdgcn_readlane(inc, 63);
   }

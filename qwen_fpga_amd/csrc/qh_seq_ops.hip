@@ -139,7 +139,7 @@ size_t qh_attention_seq_workspace(int q_rows, int n_seq, int max_q, int max_k, i
   if (q_rows <= 0 || n_seq <= 0 || max_q < 0 || max_k < 0 || max_k > kMaxKeys || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 ||
       (head_dim != 128 && head_dim != 256) || (int64_t)q_rows * heads > kMaxUnits)
     return 0;
-  return attn_seq_split(q_rows, n_seq, max_k, heads, kv_heads, head_dim).bytes;
+  return attn_seq_workspace(q_rows, n_seq, max_k, heads, kv_heads, head_dim);
 }
 
 int qh_attention_seq(void* out, int64_t ldo, int64_t hso, const void* q, int64_t ldq, int64_t hsq, const void* k, int64_t ldk,
@@ -161,10 +161,10 @@ int qh_attention_seq(void* out, int64_t ldo, int64_t hso, const void* q, int64_t
   if (!cu_q || !k_start || !k_len) return QH_EINVAL;
   const View vc = flat(cu_q, n_seq + 1, 4), vt = flat(k_start, n_seq, 8), vl = flat(k_len, n_seq, 4);
   if (overlap_any(vo, vq, vc, vt, vl) || (k_rows > 0 && overlap_any(vo, vk, vv))) return QH_EINVAL;
-  const AttnSplit sp = attn_seq_split(q_rows, n_seq, max_k, heads, kv_heads, head_dim);
-  if (sp.bytes > 0) {
-    if (!workspace || workspace_bytes < sp.bytes || (reinterpret_cast<uintptr_t>(workspace) & 255)) return QH_EINVAL;
-    const View vw = flat(workspace, sp.bytes, 1);
+  const size_t need = attn_seq_workspace(q_rows, n_seq, max_k, heads, kv_heads, head_dim);
+  if (need > 0) {
+    if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255)) return QH_EINVAL;
+    const View vw = flat(workspace, need, 1);
     if (overlap_any(vw, vo, vq, vc, vt, vl) || (k_rows > 0 && overlap_any(vw, vk, vv))) return QH_EINVAL;
   }
   AttnSeq a;
@@ -184,8 +184,7 @@ int qh_attention_seq(void* out, int64_t ldo, int64_t hso, const void* q, int64_t
   a.scale = scale;
   a.bf16 = type == QH_BF16;
   a.part = static_cast<float*>(workspace);
-  a.chunk = sp.chunk;
-  a.nsplit = sp.nsplit;
+  a.whole = need == 0;
   return hip_status(launch_attn_seq(a, S(stream)));
 }
 
