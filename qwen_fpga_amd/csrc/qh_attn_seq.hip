@@ -1,17 +1,33 @@
 // Causal attention with grouped heads over packed sequences.  Row r of a sequence with q_len rows and k_len
 // keys sees the first r + 1 + k_len - q_len keys:  out = softmax(scale q K^T) V  over those; 0 without any.
+#include <type_traits>
+
 #include "qh_seq_device.hpp"
 
 namespace qh {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 namespace {
 
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kNegInf = -__builtin_inff();
+
+// find_tile, and the sequence's keys.
+struct KeyTileAt : TileAt {
+  int64_t ks;
+  int kl;
+};
+__device__ __forceinline__ bool find_key_tile(const AttnSeq& a, int mult, int tile, int b, KeyTileAt& o) {
+  if (!find_tile(a.cu_q, a.n_seq, a.q_rows, mult, tile, b, o)) return false;
+  o.ks = as_global(a.k_start)[o.seq];
+  o.kl = key_len(o.ks, as_global(a.k_len)[o.seq], a.k_rows);
+  return true;
+}
 
 // The work of the split form.  A unit is 16 rows of a sequence (tokens x query heads of one kv head) and one chunk
 // of its keys; chunks hold the same number of keys in every sequence, chosen from all sequences' keys (which only
@@ -415,8 +431,264 @@ __global__ __launch_bounds__(1024) void attn_join_kernel(const AttnSeq a) {
   }
 }
 
+// Prompts, bfloat16: a workgroup takes 256 rows (tokens x query heads of one kv head) over all the keys they see.
+// As in the split form the products are S^T = K Q^T and O^T = V^T P^T, and P never leaves the registers.  K and V
+// come 32 keys at a time through a ring of LDS stages that global -> LDS loads fill three ahead.  16-byte chunk c of
+// key r stands at chunk c ^ (r % 16) of K's rows (32 keys of one chunk lie in all banks) and c ^ 4 (r % 4) of V's
+// (four keys of 32 elements do, as the transposing read takes them).  The running maximum moves only when a score
+// passes it by more than 8 (a factor of 256, exact in the sums), so that the sums are rarely rescaled.
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+
+template <int D>
+__global__ __launch_bounds__(2 * D, 2) void attn_tile_kernel(const AttnSeq a) {
+  constexpr int NW = D / 32, RB = 256 / D;  // waves; blocks of 32 rows of a wave
+  constexpr int kKeys = 32, kRing = 4, CH = D / 8, kHalf = kKeys * D * 2, kStage = 2 * kHalf;
+  constexpr int NI = kHalf / (1024 * NW);   // loads of a wave for K's part of a stage (and for V's)
+  constexpr int NS = D / 16, NT = D / 32;
+  __shared__ __attribute__((aligned(256))) char lds[kRing * kStage];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int h = lane >> 5, j = lane & 31;
+  const int G = a.heads / a.kv_heads;
+  const int kvh = (int)blockIdx.x % a.kv_heads;
+  KeyTileAt at;   // the last tiles, which see the most keys, first
+  if (!find_key_tile(a, G, 256, ((int)gridDim.x - 1 - (int)blockIdx.x) / a.kv_heads, at)) return;
+  const int rows = at.sp.len * G, r0 = 256 * at.tile, w0 = r0 + 32 * RB * wave;
+  auto sees = [&](int row) { return keys_seen(min(row, rows - 1) / G, at.sp.len, at.kl); };
+  const int end = sees(r0 + 255), wend = w0 < rows ? sees(w0 + 32 * RB - 1) : 0;
+  int seen[RB];
+  u32x4 qf[RB][NS];
+  const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;   // (-q) k |scale|: a maximum stays one
+  const float sc = fabsf(a.scale) * kLog2e;
+#pragma unroll
+  for (int b = 0; b < RB; ++b) {
+    const int row = min(w0 + 32 * b + j, rows - 1), tok = row / G, hq = kvh * G + row % G;
+    seen[b] = keys_seen(tok, at.sp.len, at.kl);
+    const char* qp = static_cast<const char*>(a.q.p) + ((at.sp.start + tok) * a.q.ld + hq * a.q.hs) * 2 + 16 * h;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      qf[b][s] = *as_global(reinterpret_cast<const u32x4*>(qp + 32 * s));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) qf[b][s][e] ^= flip;
+    }
+  }
+  // a wave's loads: LDS places 64 (NI wave + i) + lane of a stage's K (V) rows
+  const char* kp = static_cast<const char*>(a.k.p) + (at.ks * a.k.ld + kvh * a.k.hs) * 2;
+  const char* vp = static_cast<const char*>(a.v.p) + (at.ks * a.v.ld + kvh * a.v.hs) * 2;
+  const uint32_t kld = (uint32_t)a.k.ld * 2, vld = (uint32_t)a.v.ld * 2;   // (below 2^25: the launch's rule)
+  auto k_off = [&](int i, int last) {   // last: the last row of the stage that is there
+    const int place = 64 * (NI * wave + i) + lane, r = place / CH;
+    return min(r, last) * kld + 16 * ((place % CH) ^ (r & 15));
+  };
+  auto v_off = [&](int i, int last) {
+    const int place = 64 * (NI * wave + i) + lane, r = place / CH;
+    return min(r, last) * vld + 16 * ((place % CH) ^ ((r & 3) << 2));
+  };
+  uint32_t ko[NI], vo[NI];
+#pragma unroll
+  for (int i = 0; i < NI; ++i) ko[i] = k_off(i, kKeys), vo[i] = v_off(i, kKeys);
+  const uint32_t lds0 = lds_address(lds);
+  auto put = [&](int it, int i, uint32_t k, uint32_t v) {
+    const uint32_t base = lds0 + (it & (kRing - 1)) * kStage + (NI * wave + i) * 1024;
+    load_to_lds(kp + (size_t)it * kKeys * kld, k, base);
+    load_to_lds(vp + (size_t)it * kKeys * vld, v, base + kHalf);
+  };
+  auto stage = [&](int it) {
+    const int last = end - 1 - kKeys * it;
+    if (last >= kKeys - 1) {
+#pragma unroll
+      for (int i = 0; i < NI; ++i) put(it, i, ko[i], vo[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NI; ++i) put(it, i, k_off(i, last), v_off(i, last));
+    }
+  };
+  f32x16 acc[RB][NT];
+#pragma unroll
+  for (int b = 0; b < RB; ++b)
+#pragma unroll
+    for (int t = 0; t < NT; ++t) acc[b][t] = f32x16{};
+  float m[RB], l[RB];
+#pragma unroll
+  for (int b = 0; b < RB; ++b) m[b] = kNegInf, l[b] = 0.0f;
+  const int n = seq_tiles(end, kKeys);
+#pragma unroll
+  for (int i = 0; i < kRing - 1; ++i)
+    if (i < n) stage(i);
+  // places of a lane's first fragments; those of the others are these, xor-ed by the chunk and moved by whole 256 bytes
+  const int vx = (lane & 15) >> 2;   // the key of four that this lane's transposing read brings
+  uint32_t kl0 = lds0 + j * D * 2 + 16 * (h ^ (j & 15));
+  uint32_t vl0 = lds0 + kHalf + (4 * h + vx) * D * 2 + 32 * ((lane >> 4) & 1) + 16 * ((lane & 3) >> 1) + 8 * (lane & 1) + 64 * vx;
+  auto wait = [&](int it) {
+    // this wave's loads of the stage have landed (those of the next two stay in flight) and its reads of the stage
+    // before are done; after the barrier every wave's
+    if (it + 2 < n)
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(4 * NI) : "memory");
+    else if (it + 1 < n)
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * NI) : "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (it + kRing - 1 < n) stage(it + kRing - 1);
+  };
+  // 32 keys.  PART: some row may see them only in part.
+  auto step = [&](int it, auto PART) {
+    constexpr bool part = decltype(PART)::value;
+    const int kb = kKeys * it;
+    // (opaque, so that the places are formed where they are used: held over the loop they would not fit the registers)
+    uint32_t kl = kl0 + (it & (kRing - 1)) * kStage, vl = vl0 + (it & (kRing - 1)) * kStage;
+    asm volatile("" : "+v"(kl), "+v"(vl));
+    f32x16 st[RB];
+#pragma unroll
+    for (int b = 0; b < RB; ++b) st[b] = f32x16{};
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      const u32x4 kf = *lds_at<u32x4>((kl ^ (32 * (s & 7))) + 256 * (s >> 3));
+#pragma unroll
+      for (int b = 0; b < RB; ++b)
+        st[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, kf), __builtin_bit_cast(bf16x8, qf[b][s]), st[b], 0, 0, 0);
+    }
+    if constexpr (!part) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
+#pragma unroll
+      for (int i = 0; i < NS - 3; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x8, RB, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x8, 3 * RB, 0);
+    }
+    if constexpr (part) {
+#pragma unroll
+      for (int b = 0; b < RB; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (kb + 8 * (r >> 2) + 4 * h + (r & 3) >= seen[b]) st[b][r] = kNegInf;
+    }
+    float mt[RB];
+    bool up[RB], any = false;
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+      float x = st[b][0];
+#pragma unroll
+      for (int r = 1; r < 16; ++r) x = fmaxf(x, st[b][r]);
+      x = fmaxf(x, xor_perm<32>(x));
+      mt[b] = x == kNegInf ? kNegInf : x * sc;   // (0 times it is not it)
+      up[b] = mt[b] > m[b] + 8.0f;
+      any |= up[b];
+    }
+    if (__ballot(any) != 0) {
+#pragma unroll
+      for (int b = 0; b < RB; ++b) {   // (a row's own scores decide, so that other rows have no influence on it)
+        const float mn = up[b] ? mt[b] : m[b], al = __builtin_amdgcn_exp2f(m[b] - (mn == kNegInf ? 0.0f : mn));
+        m[b] = mn;
+        l[b] *= al;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[b][t][r] *= al;
+      }
+    }
+    u32x4 pf[RB][2];
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+      const float mu = m[b] == kNegInf ? 0.0f : m[b];
+      float ps = 0.0f;
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) {
+        float p[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[b][r + e], sc, -mu));
+          if constexpr (part) p[e] = st[b][r + e] == kNegInf ? 0.0f : p[e];   // (a scale of 0)
+          ps += p[e];
+        }
+        const bf16x2 pk = {(__bf16)p[0], (__bf16)p[1]};
+        pf[b][r >> 3][(r >> 1) & 3] = __builtin_bit_cast(uint32_t, pk);
+      }
+      l[b] += ps;
+    }
+    bool bad = false;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) {   // keys 16 kk + 4 h .., + 8 of d = 32 t + lane % 32
+        const uint32_t p = (vl ^ (64 * (t & 3))) + 256 * (t >> 2) + 16 * kk * D * 2;
+        union {
+          i16x4 h[2];
+          u32x4 v;
+        } u;
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+          u.h[q] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_at<i16x4>(p + 8 * q * D * 2));
+        // (see attn_split_kernel: what is not finite in V goes only to the rows that see it)
+        if constexpr (part) bad |= zero_non_finite<true>(u.v);
+#pragma unroll
+        for (int b = 0; b < RB; ++b)
+          acc[b][t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, u.v), __builtin_bit_cast(bf16x8, pf[b][kk]),
+                                                              acc[b][t], 0, 0, 0);
+      }
+    if constexpr (!part) {   // fragments on their way ahead of the product they are for
+      __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+      for (int i = 0; i < 2 * NT - 2; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x8, RB, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x8, 2 * RB, 0);
+    }
+    if constexpr (part) {
+      if (__ballot(bad) != 0) {
+        for (int key = kb; key < min(kb + kKeys, end); ++key) {
+          const __bf16* q = static_cast<const __bf16*>(a.v.p) + (at.ks + key) * a.v.ld + kvh * a.v.hs + 4 * h;
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const float e = (float)as_global(q)[32 * t + 8 * (r >> 2) + (r & 3)];
+              if (non_finite(e))
+#pragma unroll
+                for (int b = 0; b < RB; ++b)
+                  if (key < seen[b]) acc[b][t][r] += e;
+            }
+        }
+      }
+    }
+  };
+  const int full = sees(r0) / kKeys;   // steps that every row sees whole
+  int it = 0;
+  for (; it < full; ++it) {
+    wait(it);
+    step(it, std::false_type{});
+  }
+  for (; it < n; ++it) {
+    wait(it);
+    if (kKeys * it < wend) step(it, std::true_type{});
+  }
+#pragma unroll
+  for (int b = 0; b < RB; ++b) {
+    l[b] = l[b] + xor_perm<32>(l[b]);
+    const int row = w0 + 32 * b + j, tok = row / G, hq = kvh * G + row % G;
+    if (row >= rows) continue;
+    const float inv = at.kl < 0 ? __builtin_nanf("") : seen[b] == 0 ? 0.0f : 1.0f / l[b];
+    char* op = static_cast<char*>(a.out.p) + ((at.sp.start + tok) * a.out.ld + hq * a.out.hs) * 2;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const bf16x4 o = {(__bf16)(acc[b][t][r] * inv), (__bf16)(acc[b][t][r + 1] * inv), (__bf16)(acc[b][t][r + 2] * inv),
+                          (__bf16)(acc[b][t][r + 3] * inv)};
+        *as_global_w(reinterpret_cast<bf16x4*>(op + (32 * t + 2 * r + 4 * h) * 2)) = o;
+      }
+  }
+}
+
 template <bool BF16, int D>
 hipError_t launch(const AttnSeq& a, hipStream_t s) {
+  if constexpr (BF16)
+    if (a.tile) {
+      const int64_t t = seq_tiles_max((int64_t)a.q_rows * (a.heads / a.kv_heads), a.n_seq, 256) * a.kv_heads;
+      attn_tile_kernel<D><<<(unsigned)t, 2 * D, 0, s>>>(a);
+      return hipGetLastError();
+    }
   const unsigned tiles = (unsigned)(seq_tiles_max((int64_t)a.q_rows * (a.heads / a.kv_heads), a.n_seq, 16) * a.kv_heads);
   attn_split_kernel<BF16, D><<<a.whole ? tiles : tiles + kFill, 256, 0, s>>>(a);
   if (!a.whole) attn_join_kernel<BF16, D><<<dim3(tiles, 4), 1024, 0, s>>>(a);

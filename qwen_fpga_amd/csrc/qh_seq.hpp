@@ -96,6 +96,7 @@ struct AttnSeq {
   float scale = 0.0f;
   int bf16 = 0;
   float* part = nullptr;          // partials of the split form
+  int tile = 0;                   // the form for prompts
   int whole = 0;                  // the split form with one chunk of all keys (nothing to join)
 };
 

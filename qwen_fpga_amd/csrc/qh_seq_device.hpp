@@ -37,4 +37,23 @@ __device__ __forceinline__ bool find_tile(const int32_t* cu, int n_seq, int rows
   return false;
 }
 
+// LDS by its 32-bit address.
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+  return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)p;
+}
+template <typename T>
+__device__ __forceinline__ __attribute__((address_space(3))) T* lds_at(uint32_t p) {
+  return (__attribute__((address_space(3))) T*)(uintptr_t)p;
+}
+
+// 16 bytes per lane from base + off (base the same for the wave) to LDS at `to` + 16 lane (`to` the same for the
+// wave).  In assembly, so that the caller counts the loads in flight itself (s_waitcnt vmcnt before the barrier that
+// hands a stage over): the compiler waits for every such load before any transposing LDS read.  Nothing is
+// returned to a register.
+__device__ __forceinline__ void load_to_lds(const char* base, uint32_t off, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+               :: "s"(__builtin_amdgcn_readfirstlane(to)), "v"(off), "s"(base)
+               : "memory", "m0");
+}
+
 }  // namespace qh

@@ -185,6 +185,7 @@ int qh_attention_seq(void* out, int64_t ldo, int64_t hso, const void* q, int64_t
   a.bf16 = type == QH_BF16;
   a.part = static_cast<float*>(workspace);
   a.whole = need == 0;
+  a.tile = (int64_t)max_q * (heads / kv_heads) >= 128 && ldk < (1 << 24) && ldv < (1 << 24);
   return hip_status(launch_attn_seq(a, S(stream)));
 }
 
