@@ -8,18 +8,24 @@
 // so with T = (I + A)^-1 a chunk is five matrix products.  T and P do not depend on the state: one launch forms
 // them for all chunks at once (delta_chunk_kernel), a second follows the state through them (delta_scan_kernel).
 // c is summed and subtracted in 64 bits: a factor e^{c_t - c_j} near 1 may stand between sums in the thousands.
-// All products are fp32 (v_mfma_f32_16x16x4_f32: row l % 16 and column l % 16 of lane l, depth l / 16; a lane ends
-// with rows 4 (l / 16) .. + 3 of column l % 16).  What a lane holds of a result is what it has to bring as the
-// next product's right operand, four depths in four instructions, so results chain without a shuffle.
+//
+// The products run on the matrix cores at fp32 precision.  A float is the sum of three bfloat16 exactly (its 24 bits
+// cut into three eights, by masking), so an fp32 product is the six largest of the nine partial products (what is
+// left out is below 2^-22 of the largest), and one with a bfloat16 operand is three: 6 and 3 MFMAs of 16 cycles do
+// what takes eight of 32 in v_mfma_f32_16x16x4_f32.  That one stays for the small triangular products with T and P.
+// In all of them lane l has row l % 16 of the left and column l % 16 of the right operand, at the depths of lane group
+// l / 16, and ends with rows 4 (l / 16) .. + 3 of column l % 16: what a lane holds of a result is what it has to
+// bring as the next product's right operand, so results chain without a shuffle.
 #include "qh_seq_device.hpp"
 
 namespace qh {
 
-typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
 
 namespace {
 
@@ -72,15 +78,6 @@ __device__ __forceinline__ f32x4 load4(const void* p, int64_t at) {
     return f32x4{(float)t[0], (float)t[1], (float)t[2], (float)t[3]};
   } else {
     return *as_global(reinterpret_cast<const f32x4*>(static_cast<const float*>(p) + at));
-  }
-}
-template <bool BF16>
-__device__ __forceinline__ f32x2 load2(const void* p, int64_t at) {
-  if constexpr (BF16) {
-    const bf16x2 t = *as_global(reinterpret_cast<const bf16x2*>(static_cast<const __bf16*>(p) + at));
-    return f32x2{(float)t[0], (float)t[1]};
-  } else {
-    return *as_global(reinterpret_cast<const f32x2*>(static_cast<const float*>(p) + at));
   }
 }
 __device__ __forceinline__ bool finite(float v) { return (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u; }
@@ -157,139 +154,233 @@ __global__ __launch_bounds__(256) void delta_step_kernel(const DeltaSeq a) {
   for (int e = 0; e < 8; ++e) *as_global_w(Sp + e * (kD / 4)) = s[e];
 }
 
-// T, P and the row factors of one chunk and head.
+// Two floats as pairs of bfloat16: the top eight bits of each, the next eight, the last eight.
+__device__ __forceinline__ void cut2(float x, float y, uint32_t& hi, uint32_t& mid, uint32_t& lo) {
+  const uint32_t xu = __float_as_uint(x), yu = __float_as_uint(y);
+  hi = __builtin_amdgcn_perm(yu, xu, 0x07060302u);
+  const float x1 = x - __uint_as_float(xu & 0xffff0000u), y1 = y - __uint_as_float(yu & 0xffff0000u);
+  const uint32_t x1u = __float_as_uint(x1), y1u = __float_as_uint(y1);
+  mid = __builtin_amdgcn_perm(y1u, x1u, 0x07060302u);
+  const float x2 = x1 - __uint_as_float(x1u & 0xffff0000u), y2 = y1 - __uint_as_float(y1u & 0xffff0000u);
+  lo = __builtin_amdgcn_perm(__float_as_uint(y2), __float_as_uint(x2), 0x07060302u);
+}
+// Eight elements as NP parts: a bfloat16 input as it is, fp32 in three.
+template <bool BF16>
+struct Parts {
+  static constexpr int NP = BF16 ? 1 : 3;
+  u32x4 p[NP];
+};
+template <bool BF16>
+struct Raw8 {   // eight elements as they lie in memory
+  u32x4 v[BF16 ? 1 : 2];
+};
+template <bool BF16>
+__device__ __forceinline__ Raw8<BF16> raw8(const void* p, int64_t at) {
+  Raw8<BF16> o;
+  const u32x4* q = reinterpret_cast<const u32x4*>(static_cast<const char*>(p) + at * (BF16 ? 2 : 4));
+  o.v[0] = *as_global(q);
+  if constexpr (!BF16) o.v[1] = *as_global(q + 1);
+  return o;
+}
+template <bool BF16>
+__device__ __forceinline__ Parts<BF16> parts(const Raw8<BF16>& r) {
+  Parts<BF16> o;
+  if constexpr (BF16) {
+    o.p[0] = r.v[0];
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      uint32_t hi, mid, lo;
+      cut2(__uint_as_float(r.v[e >> 1][2 * (e & 1)]), __uint_as_float(r.v[e >> 1][2 * (e & 1) + 1]), hi, mid, lo);
+      o.p[0][e] = hi, o.p[1][e] = mid, o.p[2][e] = lo;
+    }
+  }
+  return o;
+}
+template <bool BF16>
+__device__ __forceinline__ bool any_non_finite(const Raw8<BF16>& r) {
+  bool bad = false;
+#pragma unroll
+  for (int q = 0; q < (BF16 ? 1 : 2); ++q)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      bad |= (r.v[q][e] & 0x7f800000u) == 0x7f800000u;
+      if constexpr (BF16) bad |= (r.v[q][e] & 0x7f80u) == 0x7f80u;
+    }
+  return bad;
+}
+__device__ __forceinline__ f32x4 mfma32(const u32x4& x, const u32x4& y, const f32x4& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y), c, 0, 0, 0);
+}
+// Depth 32 of a product: x in NX parts, y in NY, the smallest partial products first.
+template <int NX, int NY>
+__device__ __forceinline__ f32x4 mul(const u32x4 (&x)[NX], const u32x4 (&y)[NY], f32x4 c) {
+#pragma unroll
+  for (int o = NX + NY - 2 < 2 ? NX + NY - 2 : 2; o >= 0; --o)
+#pragma unroll
+    for (int i = o < NX ? o : NX - 1; i >= 0; --i)
+      if (o - i < NY) c = mfma32(x[i], y[o - i], c);
+  return c;
+}
+// A chunk's keys in LDS, a part [64][128] bfloat16 after another: 16-byte piece c of token t at piece c ^ (t % 16),
+// so that 16 tokens' pieces of one place lie in all banks.
+constexpr int kPart = kC * kD * 2;
+__device__ __forceinline__ int key_at(int t, int c) { return t * (kD * 2) + 16 * (c ^ (t & 15)); }
+
+// T, P and the row factors of one chunk, for the value heads of one key head.  Wave i forms the tiles (i, j <= i) of
+// K K^T and Q K^T once; every head scales them.
 template <bool BF16>
 __global__ __launch_bounds__(256) void delta_chunk_kernel(const DeltaSeq a) {
-  constexpr int LD = kC + 4;
-  __shared__ __attribute__((aligned(16))) float al[kC * LD], tl[kC * LD];   // A; T
+  constexpr int LD = kC + 4, NP = Parts<BF16>::NP;
+  __shared__ __attribute__((aligned(256))) char kl[NP * kPart < kC * LD * 4 ? kC * LD * 4 : NP * kPart];
+  __shared__ __attribute__((aligned(16))) float al[kC * LD];   // A
+  float* tl = reinterpret_cast<float*>(kl);                    // T, over the keys
   __shared__ double cs[kC];
   __shared__ float bt[kC];
   __shared__ int bad_in[4];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int g4 = 4 * (lane >> 4), j = lane & 15;
+  const int g = lane >> 4, g4 = 4 * g, j = lane & 15;
   TileAt at;
   if (!find_tile(a.cu, a.n_seq, a.tokens, 1, kC, blockIdx.x, at)) return;
-  const int h = blockIdx.y, hk = h / (a.heads / a.k_heads);
+  const int hk = blockIdx.y, rep = a.heads / a.k_heads;
   const int t0 = at.sp.start + kC * at.tile, n = min(kC, at.sp.start + at.sp.len - t0);   // n >= 1 tokens
-  float* ws = a.ws + chunk_at(a, at.seq, at.sp.start, at.tile, h);
   bool bad = false;
-  if (wave == 0) {
-    // a log decay below -1e5 is 0 as a factor like any below -104, and finite in the sums
-    float gv = 0.0f, be = 0.0f;
-    if (lane < n) {
-      gv = as_global(a.g)[(t0 + lane) * a.ldg + h];
-      be = as_global(a.beta)[(t0 + lane) * a.ldb + h];
-      if (gv < -1e5f) gv = -1e5f;
-      bad = !finite(gv) || !finite(be);
-    }
-    double c = gv;
-#pragma unroll
-    for (int d = 1; d < kC; d *= 2) {
-      const double t = __shfl_up(c, d);
-      if (lane >= d) c += t;
-    }
-    const double last = __shfl(c, kC - 1);
-    cs[lane] = c;
-    bt[lane] = be;
-    const float ec = dev_expf((float)c);
-    *as_global_w(reinterpret_cast<f32x4*>(ws + kOffRow) + lane) = f32x4{be, be * ec, ec, dev_expf((float)(last - c))};
-  }
-  // wave's share of the rows: all of q, k (the tiles below) and v are looked at for values that are not finite
-  for (int u = threadIdx.x; u < kC * kD / 4; u += 256) {
-    const int64_t r = t0 + min(u >> 5, n - 1);
-    const f32x4 x = load4<BF16>(a.v.p, r * a.v.ld + h * a.v.hs + 4 * (u & 31));
-    bad |= !finite(x[0]) || !finite(x[1]) || !finite(x[2]) || !finite(x[3]);
-  }
-  __syncthreads();
-  // the ten tiles (i, jj), dealt to the waves
-  constexpr int kDeal[4][3] = {{tri(3, 0), tri(3, 1), tri(3, 2)}, {tri(2, 0), tri(2, 1), tri(2, 2)}, {tri(3, 3), tri(1, 0), -1}, {tri(1, 1), tri(0, 0), -1}};
-#pragma unroll
-  for (int u = 0; u < 3; ++u) {
-    int tile = -1;
-#pragma unroll
-    for (int w = 0; w < 4; ++w)
-      if (wave == w) tile = kDeal[w][u];
-    if (tile < 0) break;
-    const int i = tile < 1 ? 0 : tile < 3 ? 1 : tile < 6 ? 2 : 3, jj = tile - tri(i, 0);
-    const int64_t rt = t0 + min(16 * i + j, n - 1), rj = t0 + min(16 * jj + j, n - 1);
-    f32x4 G = {0.0f, 0.0f, 0.0f, 0.0f}, P = G;   // row (depth of the later products): j; column: t
-#pragma unroll
-    for (int s = 0; s < kD / 16; ++s) {
-      const f32x4 kj = load4<BF16>(a.k.p, rj * a.k.ld + hk * a.k.hs + 16 * s + g4), kt = load4<BF16>(a.k.p, rt * a.k.ld + hk * a.k.hs + 16 * s + g4),
-                  qt = load4<BF16>(a.q.p, rt * a.q.ld + hk * a.q.hs + 16 * s + g4);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) bad |= !finite(kj[e]) || !finite(kt[e]) || !finite(qt[e]);
-      G = mfma4(kj, kt, G);
-      P = mfma4(kj, qt, P);
-    }
-    const int t = 16 * i + j;
-    const double ct = cs[t];
-    const float be = bt[t];
-    f32x4 av;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int jr = 16 * jj + g4 + r;
-      const float e = jr <= t ? dev_expf((float)(ct - cs[jr])) : 0.0f;
-      av[r] = jr < t ? be * e * G[r] : 0.0f;
-      P[r] = jr <= t ? e * P[r] : 0.0f;
-    }
-    *as_lds_w(reinterpret_cast<f32x4*>(al + t * LD + 16 * jj + g4)) = av;
-    *as_global_w(reinterpret_cast<f32x4*>(ws + kOffP + tile * 256) + lane) = P;
-  }
-  const uint64_t any = __ballot(bad);
-  if (lane == 0) bad_in[wave] = any != 0;
-  __syncthreads();
-  if (threadIdx.x == 0) ws[kOffFlag] = (bad_in[0] | bad_in[1] | bad_in[2] | bad_in[3]) ? 1.0f : 0.0f;
-  // the diagonal tiles' inverses: lane's column j of T_ii, row after row
+  f32x4 G[4], P[4];   // tile (wave, jj): lane's token t = 16 wave + l % 16, tokens j = 16 jj + 4 (l / 16) ..
   {
-    const float* ad = al + 16 * wave * LD + 16 * wave;
-    float x[16];
+    const int64_t r = t0 + min(16 * wave + j, n - 1);
+    Parts<BF16> kp[4], qp[4];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      float s = r == j ? 1.0f : 0.0f;
+    for (int s = 0; s < 4; ++s) {
+      const Raw8<BF16> kr = raw8<BF16>(a.k.p, r * a.k.ld + hk * a.k.hs + 32 * s + 8 * g), qr = raw8<BF16>(a.q.p, r * a.q.ld + hk * a.q.hs + 32 * s + 8 * g);
+      bad |= any_non_finite<BF16>(kr) || any_non_finite<BF16>(qr);
+      kp[s] = parts<BF16>(kr);
+      qp[s] = parts<BF16>(qr);
 #pragma unroll
-      for (int k = 0; k < r; ++k) s = __builtin_fmaf(-as_lds(ad)[r * LD + k], x[k], s);
-      x[r] = s;
+      for (int p = 0; p < NP; ++p) *as_lds_w(reinterpret_cast<u32x4*>(kl + p * kPart + key_at(16 * wave + j, 4 * s + g))) = kp[s].p[p];
     }
-    if (lane < 16)
+    __syncthreads();
 #pragma unroll
-      for (int r = 0; r < 16; ++r) tl[(16 * wave + r) * LD + 16 * wave + j] = x[r];
-  }
-  __syncthreads();
-  // the tiles below them, a column of tiles per wave: T_ij = -T_ii sum_{k=j}^{i-1} A_ik T_kj
-  f32x4 tc[4];   // T_kj, rows g4 .. of column j
+    for (int jj = 0; jj < 4; ++jj) {
+      G[jj] = P[jj] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      if (jj > wave) continue;
 #pragma unroll
-  for (int c = 0; c < 3; ++c) {
-    if (wave != c) continue;
+      for (int s = 0; s < 4; ++s) {
+        u32x4 x[NP];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) tc[c][r] = as_lds(tl)[(16 * c + g4 + r) * LD + 16 * c + j];
-#pragma unroll
-    for (int i = c + 1; i < 4; ++i) {
-      f32x4 z = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int k = c; k < i; ++k) z = mfma4(*as_lds(reinterpret_cast<const f32x4*>(al + (16 * i + j) * LD + 16 * k + g4)), tc[k], z);
-      f32x4 m = mfma4(*as_lds(reinterpret_cast<const f32x4*>(tl + (16 * i + j) * LD + 16 * i + g4)), z, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        tc[i][r] = -m[r];
-        tl[(16 * i + g4 + r) * LD + 16 * c + j] = -m[r];
+        for (int p = 0; p < NP; ++p) x[p] = *as_lds(reinterpret_cast<const u32x4*>(kl + p * kPart + key_at(16 * jj + j, 4 * s + g)));
+        G[jj] = mul(x, kp[s].p, G[jj]);
+        P[jj] = mul(x, qp[s].p, P[jj]);
       }
     }
   }
-  __syncthreads();
-  for (int u = wave; u < kTiles; u += 4) {
-    const int i = u < 1 ? 0 : u < 3 ? 1 : u < 6 ? 2 : 3, c = u - tri(i, 0);
-    *as_global_w(reinterpret_cast<f32x4*>(ws + u * 256) + lane) =
-        *as_lds(reinterpret_cast<const f32x4*>(tl + (16 * i + j) * LD + 16 * c + g4));
+  const bool bad_qk = bad;
+  for (int h = hk * rep; h < (hk + 1) * rep; ++h) {
+    float* ws = a.ws + chunk_at(a, at.seq, at.sp.start, at.tile, h);
+    bad = bad_qk;
+    if (wave == 0) {
+      // a log decay below -1e5 is 0 as a factor like any below -104, and finite in the sums
+      float gv = 0.0f, be = 0.0f;
+      if (lane < n) {
+        gv = as_global(a.g)[(t0 + lane) * a.ldg + h];
+        be = as_global(a.beta)[(t0 + lane) * a.ldb + h];
+        if (gv < -1e5f) gv = -1e5f;
+        bad |= !finite(gv) || !finite(be);
+      }
+      double c = gv;
+#pragma unroll
+      for (int d = 1; d < kC; d *= 2) {
+        const double t = __shfl_up(c, d);
+        if (lane >= d) c += t;
+      }
+      const double last = __shfl(c, kC - 1);
+      cs[lane] = c;
+      bt[lane] = be;
+      const float ec = dev_expf((float)c);
+      *as_global_w(reinterpret_cast<f32x4*>(ws + kOffRow) + lane) = f32x4{be, be * ec, ec, dev_expf((float)(last - c))};
+    }
+#pragma unroll
+    for (int u = 0; u < kC * kD / 8 / 256; ++u) {
+      const int e = 256 * u + threadIdx.x;
+      bad |= any_non_finite<BF16>(raw8<BF16>(a.v.p, (int64_t)(t0 + min(e >> 4, n - 1)) * a.v.ld + h * a.v.hs + 8 * (e & 15)));
+    }
+    const uint64_t any = __ballot(bad);
+    if (lane == 0) bad_in[wave] = any != 0;
+    __syncthreads();
+    const int t = 16 * wave + j;
+    const double ct = cs[t];
+    const float be = bt[t];
+#pragma unroll
+    for (int jj = 0; jj < 4; ++jj) {
+      if (jj > wave) continue;
+      f32x4 av, pv;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int jr = 16 * jj + g4 + r;
+        const float e = jr <= t ? dev_expf((float)(ct - cs[jr])) : 0.0f;
+        av[r] = jr < t ? be * e * G[jj][r] : 0.0f;
+        pv[r] = jr <= t ? e * P[jj][r] : 0.0f;
+      }
+      *as_lds_w(reinterpret_cast<f32x4*>(al + t * LD + 16 * jj + g4)) = av;
+      *as_global_w(reinterpret_cast<f32x4*>(ws + kOffP + tri(wave, jj) * 256) + lane) = pv;
+    }
+    if (threadIdx.x == 0) ws[kOffFlag] = (bad_in[0] | bad_in[1] | bad_in[2] | bad_in[3]) ? 1.0f : 0.0f;
+    __syncthreads();
+    // the diagonal tiles' inverses: lane's column j of T_ii, row after row
+    {
+      const float* ad = al + 16 * wave * LD + 16 * wave;
+      float x[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        float s = r == j ? 1.0f : 0.0f;
+#pragma unroll
+        for (int k = 0; k < r; ++k) s = __builtin_fmaf(-as_lds(ad)[r * LD + k], x[k], s);
+        x[r] = s;
+      }
+      if (lane < 16)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) tl[(16 * wave + r) * LD + 16 * wave + j] = x[r];
+    }
+    __syncthreads();
+    // the tiles below them, a column of tiles per wave: T_ij = -T_ii sum_{k=j}^{i-1} A_ik T_kj
+    f32x4 tc[4];   // T_kj, rows g4 .. of column j
+#pragma unroll
+    for (int c = 0; c < 3; ++c) {
+      if (wave != c) continue;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) tc[c][r] = as_lds(tl)[(16 * c + g4 + r) * LD + 16 * c + j];
+#pragma unroll
+      for (int i = c + 1; i < 4; ++i) {
+        f32x4 z = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int k = c; k < i; ++k) z = mfma4(*as_lds(reinterpret_cast<const f32x4*>(al + (16 * i + j) * LD + 16 * k + g4)), tc[k], z);
+        const f32x4 m = mfma4(*as_lds(reinterpret_cast<const f32x4*>(tl + (16 * i + j) * LD + 16 * i + g4)), z, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          tc[i][r] = -m[r];
+          tl[(16 * i + g4 + r) * LD + 16 * c + j] = -m[r];
+        }
+      }
+    }
+    __syncthreads();
+    for (int u = wave; u < kTiles; u += 4) {
+      const int i = u < 1 ? 0 : u < 3 ? 1 : u < 6 ? 2 : 3, c = u - tri(i, 0);
+      *as_global_w(reinterpret_cast<f32x4*>(ws + u * 256) + lane) =
+          *as_lds(reinterpret_cast<const f32x4*>(tl + (16 * i + j) * LD + 16 * c + g4));
+    }
+    __syncthreads();   // T and the sums have been read
   }
 }
 
-// The state's way through the chunks: a workgroup takes one sequence, one head and 16 of its columns.  Every wave
-// holds the whole 128 x 16 slice (s[w][c], lane l: rows 32 w + 8 (l / 16) + 2 r + c of column l % 16), wave w
-// works on the chunk's tokens 16 w .. + 15 and updates the rows 32 w .. + 31.
+// The state's way through the chunks: a workgroup takes one sequence, one head and 16 of its columns.  Wave w owns the
+// state's rows 32 w .. + 31 (lane: 32 w + 8 (l / 16) .. + 7 of column l % 16) and the chunk's tokens 16 w .. + 15.  The
+// waves exchange through LDS the state's parts, the tokens' right sides R and their d.
 template <bool BF16>
 __global__ __launch_bounds__(256) void delta_scan_kernel(const DeltaSeq a) {
-  __shared__ f32x4 rl[4][64], dl[4][64], el[4][64], sl[4][2][64];
+  constexpr int NP = Parts<BF16>::NP;
+  __shared__ __attribute__((aligned(256))) char kl[2][NP * kPart];   // keys of this chunk and the next
+  __shared__ f32x4 rl[4][64], dl[4][64];                             // R, d
+  __shared__ u32x2 el[4][3][64];                                     // parts of e^{c_63 - c_t} d_t
+  __shared__ u32x4 sl[4][3][64];                                     // parts of the state
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, j = lane & 15;
   // the eight slices of a head on one of the eight XCDs, whose L2 then holds the head's q, k, T and P
@@ -300,35 +391,29 @@ __global__ __launch_bounds__(256) void delta_scan_kernel(const DeltaSeq a) {
   if (sp.len == 0) return;
   const int col = 16 * slice + j;
   float* Sp = a.S + ((size_t)seq * a.heads + h) * kD * kD + col;
-  f32x4 s[4][2];
-#pragma unroll
-  for (int w = 0; w < 4; ++w)
-#pragma unroll
-    for (int c = 0; c < 2; ++c)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) s[w][c][r] = as_global(Sp)[(32 * w + 8 * g + 2 * r + c) * kD];
-
-  f32x4 kf[4][2], qf[4][2], tf[4], pf[4], row[4];   // operands of one chunk, each reloaded as soon as it is used
-  f32x2 kt[4][4];
-  float vv[4];
   const int nc = seq_tiles(sp.len, kC);
   auto token = [&](int c, int t) -> int64_t { return min(sp.start + kC * c + t, sp.start + sp.len - 1); };
   auto ws = [&](int c) { return a.ws + chunk_at(a, seq, sp.start, c, h); };
-  auto load_kv = [&](int c) {
+
+  float s[8];            // this wave's rows of the state
+  u32x4 sp4[4][3];       // all rows' parts: depths 32 w + 8 (l / 16) ..
+  Raw8<BF16> kr[4], qr[4];   // a chunk's operands on their way
+  Parts<BF16> kp[4];
+  f32x4 tf[4], pf[4], row[4];
+  float vv[4];
+  auto load_k = [&](int c) {
     const int64_t at = token(c, 16 * wave + j) * a.k.ld + hk * a.k.hs + 8 * g;
 #pragma unroll
-    for (int w = 0; w < 4; ++w)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) kf[w][e] = load4<BF16>(a.k.p, at + 32 * w + 4 * e);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) vv[r] = load1<BF16>(a.v.p, token(c, 16 * wave + 4 * g + r) * a.v.ld + h * a.v.hs + col);
+    for (int w = 0; w < 4; ++w) kr[w] = raw8<BF16>(a.k.p, at + 32 * w);
   };
   auto load_q = [&](int c) {
     const int64_t at = token(c, 16 * wave + j) * a.q.ld + hk * a.q.hs + 8 * g;
 #pragma unroll
-    for (int w = 0; w < 4; ++w)
+    for (int w = 0; w < 4; ++w) qr[w] = raw8<BF16>(a.q.p, at + 32 * w);
+  };
+  auto load_v = [&](int c) {
 #pragma unroll
-      for (int e = 0; e < 2; ++e) qf[w][e] = load4<BF16>(a.q.p, at + 32 * w + 4 * e);
+    for (int r = 0; r < 4; ++r) vv[r] = load1<BF16>(a.v.p, token(c, 16 * wave + 4 * g + r) * a.v.ld + h * a.v.hs + col);
   };
   auto load_tile = [&](int c, int off, f32x4 (&f)[4]) {
     const f32x4* p = reinterpret_cast<const f32x4*>(ws(c) + off) + lane;
@@ -336,26 +421,62 @@ __global__ __launch_bounds__(256) void delta_scan_kernel(const DeltaSeq a) {
     for (int t = 0; t < 4; ++t)
       if (t <= wave) f[t] = *as_global(p + tri(wave, t) * 64);
   };
-  auto load_kt = [&](int c) {
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        kt[t][r] = load2<BF16>(a.k.p, token(c, 16 * t + 4 * g + r) * a.k.ld + hk * a.k.hs + 32 * wave + 2 * j);
-  };
   auto load_row = [&](int c) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) row[r] = *as_global(reinterpret_cast<const f32x4*>(ws(c) + kOffRow) + 16 * wave + 4 * g + r);
   };
-  load_kv(0), load_row(0), load_q(0), load_tile(0, 0, tf), load_kt(0), load_tile(0, kOffP, pf);
+  // the keys that arrived, as this wave's left operand and to LDS for the state's update
+  auto put_k = [&](int c) {
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      kp[w] = parts<BF16>(kr[w]);
+#pragma unroll
+      for (int p = 0; p < NP; ++p) *as_lds_w(reinterpret_cast<u32x4*>(kl[c & 1] + p * kPart + key_at(16 * wave + j, 4 * w + g))) = kp[w].p[p];
+    }
+  };
+  auto put_s = [&]() {
+    u32x4 p[3];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      uint32_t hi, mid, lo;
+      cut2(s[2 * e], s[2 * e + 1], hi, mid, lo);
+      p[0][e] = hi, p[1][e] = mid, p[2][e] = lo;
+    }
+#pragma unroll
+    for (int q = 0; q < 3; ++q) sl[wave][q][lane] = p[q];
+  };
+  auto get_s = [&]() {
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+#pragma unroll
+      for (int q = 0; q < 3; ++q) sp4[w][q] = sl[w][q][lane];
+  };
+  load_k(0), load_v(0), load_row(0), load_q(0), load_tile(0, 0, tf), load_tile(0, kOffP, pf);
   float flag = as_global(ws(0))[kOffFlag], decay = as_global(ws(0))[kOffRow + 4 * (kC - 1) + 2];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) s[e] = as_global(Sp)[(32 * wave + 8 * g + e) * kD];
+  put_s();
+  put_k(0);
+  lds_barrier();
+  get_s();
   const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+  // this lane's place in the transposing reads of the keys: token 4 (l / 16) + l % 16 / 4 (+ 16 tile), rows
+  // 32 wave + 8 (l % 4) + 4 c .. + 3
+  const int kt0 = 4 * g + (j >> 2), kc0 = 4 * wave + (j & 3);
   for (int c = 0; c < nc; ++c) {
     const int nx = min(c + 1, nc - 1);
     const float dec = decay;
+    load_k(nx);
     if (flag != 0.0f) {
       // an input that is not finite: the products below would carry it to tokens before it (0 times it is not
-      // 0), so the chunk runs token by token, in every wave alike
+      // 0), so the chunk runs token by token, in every wave alike (lane: rows 32 w + 8 (l / 16) .. + 7 of all w)
+      float st[32];
+      lds_barrier();   // the state's parts have been read
+#pragma unroll
+      for (int e = 0; e < 8; ++e) *reinterpret_cast<float*>(reinterpret_cast<char*>(&sl[wave][e >> 2][lane]) + 4 * (e & 3)) = s[e];
+      lds_barrier();
+#pragma unroll
+      for (int e = 0; e < 32; ++e) st[e] = *reinterpret_cast<const float*>(reinterpret_cast<const char*>(&sl[e >> 3][(e >> 2) & 1][lane]) + 4 * (e & 3));
       const int t1 = min(kC, sp.len - kC * c);
       for (int t = 0; t < t1; ++t) {
         const int64_t tk = sp.start + kC * c + t;
@@ -363,45 +484,47 @@ __global__ __launch_bounds__(256) void delta_scan_kernel(const DeltaSeq a) {
         const float v1 = load1<BF16>(a.v.p, tk * a.v.ld + h * a.v.hs + col);
         float x = 0.0f, y = 0.0f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float sv = s[w][e & 1][e >> 1] * de;
-            s[w][e & 1][e >> 1] = sv;
-            x = __builtin_fmaf(sv, load1<BF16>(a.k.p, tk * a.k.ld + hk * a.k.hs + 32 * w + 8 * g + e), x);
-          }
+        for (int e = 0; e < 32; ++e) {
+          st[e] *= de;
+          x = __builtin_fmaf(st[e], load1<BF16>(a.k.p, tk * a.k.ld + hk * a.k.hs + 32 * (e >> 3) + 8 * g + (e & 7)), x);
+        }
         x = x + xor_perm<16>(x);
         x = x + xor_perm<32>(x);
         const float d = (v1 - x) * be;
 #pragma unroll
-        for (int w = 0; w < 4; ++w)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float sv = __builtin_fmaf(load1<BF16>(a.k.p, tk * a.k.ld + hk * a.k.hs + 32 * w + 8 * g + e), d, s[w][e & 1][e >> 1]);
-            s[w][e & 1][e >> 1] = sv;
-            y = __builtin_fmaf(sv, load1<BF16>(a.q.p, tk * a.q.ld + hk * a.q.hs + 32 * w + 8 * g + e), y);
-          }
+        for (int e = 0; e < 32; ++e) {
+          st[e] = __builtin_fmaf(load1<BF16>(a.k.p, tk * a.k.ld + hk * a.k.hs + 32 * (e >> 3) + 8 * g + (e & 7)), d, st[e]);
+          y = __builtin_fmaf(st[e], load1<BF16>(a.q.p, tk * a.q.ld + hk * a.q.hs + 32 * (e >> 3) + 8 * g + (e & 7)), y);
+        }
         y = y + xor_perm<16>(y);
         y = y + xor_perm<32>(y);
         if (wave == 0 && g == 0) store1<BF16>(a.out.p, tk * a.out.ld + h * a.out.hs + col, y);
       }
-      load_kv(nx), load_row(nx), load_q(nx), load_tile(nx, 0, tf), load_kt(nx), load_tile(nx, kOffP, pf);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        s[e] = st[e];
+#pragma unroll
+        for (int w = 1; w < 4; ++w)
+          if (wave == w) s[e] = st[8 * w + e];
+      }
+      lds_barrier();
+      put_s();
+      if (c + 1 < nc) put_k(nx);
+      load_v(nx), load_row(nx), load_q(nx), load_tile(nx, 0, tf), load_tile(nx, kOffP, pf);
       flag = as_global(ws(nx))[kOffFlag], decay = as_global(ws(nx))[kOffRow + 4 * (kC - 1) + 2];
+      lds_barrier();
+      get_s();
       continue;
     }
-    f32x4 x = zero, y = zero, d = zero, R, ec;
+    f32x4 x[2] = {zero, zero}, y[2] = {zero, zero}, d = zero, R;
 #pragma unroll
-    for (int w = 0; w < 4; ++w)
+    for (int w = 0; w < 4; ++w) x[w & 1] = mul(kp[w].p, sp4[w], x[w & 1]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[w][e >> 2][e & 3], s[w][e & 1][e >> 1], x, 0, 0, 0);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) R[r] = row[r][0] * vv[r] - row[r][1] * x[r];
+    for (int r = 0; r < 4; ++r) R[r] = row[r][0] * vv[r] - row[r][1] * (x[0][r] + x[1][r]);
     rl[wave][lane] = R;
-    load_kv(nx);
+    load_v(nx);
 #pragma unroll
-    for (int w = 0; w < 4; ++w)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) y = __builtin_amdgcn_mfma_f32_16x16x4f32(qf[w][e >> 2][e & 3], s[w][e & 1][e >> 1], y, 0, 0, 0);
+    for (int w = 0; w < 4; ++w) y[w & 1] = mul(parts<BF16>(qr[w]).p, sp4[w], y[w & 1]);
     load_q(nx);
     lds_barrier();
 #pragma unroll
@@ -409,58 +532,70 @@ __global__ __launch_bounds__(256) void delta_scan_kernel(const DeltaSeq a) {
       if (t <= wave) d = mfma4(tf[t], rl[t][lane], d);
     load_tile(nx, 0, tf);
     dl[wave][lane] = d;
+    {
+      u32x2 p[3];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) ec[r] = d[r] * row[r][3];
-    el[wave][lane] = ec;
+      for (int e = 0; e < 2; ++e) {
+        uint32_t hi, mid, lo;
+        cut2(d[2 * e] * row[2 * e][3], d[2 * e + 1] * row[2 * e + 1][3], hi, mid, lo);
+        p[0][e] = hi, p[1][e] = mid, p[2][e] = lo;
+      }
 #pragma unroll
-    for (int r = 0; r < 4; ++r) y[r] *= row[r][2];
+      for (int q = 0; q < 3; ++q) el[wave][q][lane] = p[q];
+    }
+    f32x4 o;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) o[r] = (y[0][r] + y[1][r]) * row[r][2];
     load_row(nx);
     lds_barrier();
-    f32x4 n0, n1;
+    f32x4 sn[2];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      f32x4 o0 = s[0][0], o1 = s[0][1];
+    for (int e = 0; e < 8; ++e) sn[e >> 2][e & 3] = s[e] * dec;
 #pragma unroll
-      for (int w = 1; w < 4; ++w)
-        if (wave == w) o0 = s[w][0], o1 = s[w][1];
-      n0[r] = o0[r] * dec;
-      n1[r] = o1[r] * dec;
-    }
+    for (int kk = 0; kk < 2; ++kk) {   // depth: tokens 32 kk + 4 (l / 16) .., + 16
+      u32x4 ep[3];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const f32x4 e = el[t][lane];
+      for (int q = 0; q < 3; ++q) {
+        const u32x2 e0 = el[2 * kk][q][lane], e1 = el[2 * kk + 1][q][lane];
+        ep[q] = u32x4{e0[0], e0[1], e1[0], e1[1]};
+      }
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        n0 = __builtin_amdgcn_mfma_f32_16x16x4f32(kt[t][r][0], e[r], n0, 0, 0, 0);
-        n1 = __builtin_amdgcn_mfma_f32_16x16x4f32(kt[t][r][1], e[r], n1, 0, 0, 0);
+      for (int cc = 0; cc < 2; ++cc) {
+        u32x4 kt[NP];
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+          union {
+            i16x4 h[2];
+            u32x4 v;
+          } un;
+#pragma unroll
+          for (int q = 0; q < 2; ++q)
+            un.h[q] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)as_lds_w(
+                kl[c & 1] + p * kPart + key_at(32 * kk + 16 * q + kt0, kc0) + 8 * cc));
+          kt[p] = un.v;
+        }
+        sn[cc] = mul(kt, ep, sn[cc]);
       }
     }
-    sl[wave][0][lane] = n0;
-    sl[wave][1][lane] = n1;
-    load_kt(nx);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s[e] = sn[e >> 2][e & 3];
+    put_s();
+    if (c + 1 < nc) put_k(nx);
 #pragma unroll
     for (int t = 0; t < 4; ++t)
-      if (t <= wave) y = mfma4(pf[t], dl[t][lane], y);
+      if (t <= wave) o = mfma4(pf[t], dl[t][lane], o);
     load_tile(nx, kOffP, pf);
     flag = as_global(ws(nx))[kOffFlag], decay = as_global(ws(nx))[kOffRow + 4 * (kC - 1) + 2];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int t = kC * c + 16 * wave + 4 * g + r;
-      if (t < sp.len) store1<BF16>(a.out.p, (int64_t)(sp.start + t) * a.out.ld + h * a.out.hs + col, y[r]);
+      if (t < sp.len) store1<BF16>(a.out.p, (int64_t)(sp.start + t) * a.out.ld + h * a.out.hs + col, o[r]);
     }
     lds_barrier();
-#pragma unroll
-    for (int w = 0; w < 4; ++w)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) s[w][e] = sl[w][e][lane];
+    get_s();
   }
-  if (wave == 0)
 #pragma unroll
-    for (int w = 0; w < 4; ++w)
-#pragma unroll
-      for (int c = 0; c < 2; ++c)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) as_global_w(Sp)[(32 * w + 8 * g + 2 * r + c) * kD] = s[w][c][r];
+  for (int e = 0; e < 8; ++e) as_global_w(Sp)[(32 * wave + 8 * g + e) * kD] = s[e];
 }
 
 template <bool BF16>
@@ -468,7 +603,7 @@ hipError_t launch(const DeltaSeq& a, hipStream_t s) {
   if (a.ws == nullptr) {
     delta_step_kernel<BF16><<<(unsigned)(((int64_t)a.n_seq * a.heads * 8 + 3) / 4), 256, 0, s>>>(a);
   } else {
-    delta_chunk_kernel<BF16><<<dim3((unsigned)seq_tiles_max(a.tokens, a.n_seq, kC), a.heads), 256, 0, s>>>(a);
+    delta_chunk_kernel<BF16><<<dim3((unsigned)seq_tiles_max(a.tokens, a.n_seq, kC), a.k_heads), 256, 0, s>>>(a);
     delta_scan_kernel<BF16><<<(unsigned)(((int64_t)a.n_seq * a.heads + 7) / 8 * 64), 256, 0, s>>>(a);
   }
   return hipGetLastError();
