@@ -20,6 +20,7 @@
 
 namespace qh {
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -33,7 +34,7 @@ constexpr int kD = 128;
 constexpr int kC = 64;                       // tokens of a chunk
 // A chunk's and head's part of the workspace, in floats: T and P as ten 16 x 16 tiles each (lower triangle,
 // tile (i, j) at i (i + 1) / 2 + j; lane l's four values: row l % 16, columns 4 (l / 16) ..), the row factors
-// {beta, beta e^c, e^c, e^{c_63 - c}}, and whether an input is not finite.
+// {beta, beta e^c, e^c, e^{c_63 - c}}, whether an input is not finite, e^{c_63}.
 constexpr int kTiles = 10, kOffP = kTiles * 256, kOffRow = 2 * kTiles * 256, kOffFlag = kOffRow + 4 * kC,
               kChunkFloats = kOffFlag + 64;
 __device__ __forceinline__ constexpr int tri(int i, int j) { return i * (i + 1) / 2 + j; }
@@ -297,6 +298,7 @@ __global__ __launch_bounds__(256) void delta_chunk_kernel(const DeltaSeq a) {
       bt[lane] = be;
       const float ec = dev_expf((float)c);
       *as_global_w(reinterpret_cast<f32x4*>(ws + kOffRow) + lane) = f32x4{be, be * ec, ec, dev_expf((float)(last - c))};
+      if (lane == kC - 1) ws[kOffFlag + 1] = ec;
     }
 #pragma unroll
     for (int u = 0; u < kC * kD / 8 / 256; ++u) {
@@ -371,17 +373,22 @@ __global__ __launch_bounds__(256) void delta_chunk_kernel(const DeltaSeq a) {
   }
 }
 
-// The state's way through the chunks: a workgroup takes one sequence, one head and 16 of its columns.  Wave w owns the
-// state's rows 32 w .. + 31 (lane: 32 w + 8 (l / 16) .. + 7 of column l % 16) and the chunk's tokens 16 w .. + 15.  The
-// waves exchange through LDS the state's parts, the tokens' right sides R and their d.
+// The state's way through the chunks: a workgroup takes one sequence, one head and 16 of its columns.  What bounds it
+// is the chain from one chunk's state to the next, so four waves do that alone: R = beta v - beta e^c K S, d = T R,
+// S' = e^{c_63} S + K^T (e^{c_63 - c} d); wave w owns the state's rows 32 w .. + 31 (lane: 32 w + 8 (l / 16) .. + 7 of
+// column l % 16) and the chunk's tokens 16 w .. + 15.  The other four, one beside each on its SIMD, do what the chain
+// does not wait for: the next chunk's keys and T brought to LDS in parts, Q S and P d, the outputs.  With one set of
+// four waves doing everything in turn a chunk took 8.7 thousand cycles (fp32) and 6.0 (bfloat16).
 template <bool BF16>
-__global__ __launch_bounds__(256) void delta_scan_kernel(const DeltaSeq a) {
+__global__ __launch_bounds__(512, BF16 ? 4 : 2) void delta_scan_kernel(const DeltaSeq a) {
   constexpr int NP = Parts<BF16>::NP;
-  __shared__ __attribute__((aligned(256))) char kl[2][NP * kPart];   // keys of this chunk and the next
-  __shared__ f32x4 rl[4][64], dl[4][64];                             // R, d
-  __shared__ u32x2 el[4][3][64];                                     // parts of e^{c_63 - c_t} d_t
-  __shared__ u32x4 sl[4][3][64];                                     // parts of the state
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  __shared__ __attribute__((aligned(256))) char kl[2][NP * kPart];   // parts of the keys, this chunk's and the next one's
+  __shared__ u32x4 tl[6][3][64];          // parts of T: rows 16 w, depth 32 kk at w + (w == 3) + kk, kk <= w / 2
+  __shared__ u32x4 sl[4][3][64];          // parts of the state
+  __shared__ f32x4 sf[BF16 ? 1 : 4][2][64];   // the state itself (fp32: for Q S)
+  __shared__ u32x2 rl[4][3][64], el[4][3][64];   // parts of R and of e^{c_63 - c_t} d_t
+  __shared__ f32x4 dl[4][64];             // d
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & 3;
   const int g = lane >> 4, j = lane & 15;
   // the eight slices of a head on one of the eight XCDs, whose L2 then holds the head's q, k, T and P
   const int b = blockIdx.x, u = (b & 7) + 8 * (b >> 6), slice = (b >> 3) & 7;
@@ -394,208 +401,281 @@ __global__ __launch_bounds__(256) void delta_scan_kernel(const DeltaSeq a) {
   const int nc = seq_tiles(sp.len, kC);
   auto token = [&](int c, int t) -> int64_t { return min(sp.start + kC * c + t, sp.start + sp.len - 1); };
   auto ws = [&](int c) { return a.ws + chunk_at(a, seq, sp.start, c, h); };
-
-  float s[8];            // this wave's rows of the state
-  u32x4 sp4[4][3];       // all rows' parts: depths 32 w + 8 (l / 16) ..
-  Raw8<BF16> kr[4], qr[4];   // a chunk's operands on their way
-  Parts<BF16> kp[4];
-  f32x4 tf[4], pf[4], row[4];
-  float vv[4];
-  auto load_k = [&](int c) {
-    const int64_t at = token(c, 16 * wave + j) * a.k.ld + hk * a.k.hs + 8 * g;
+  auto load_flag = [&](int c) { return *as_global(reinterpret_cast<const f32x2*>(ws(c) + kOffFlag)); };
+  auto load_row = [&](int c, f32x4 (&row)[4]) {
 #pragma unroll
-    for (int w = 0; w < 4; ++w) kr[w] = raw8<BF16>(a.k.p, at + 32 * w);
+    for (int r = 0; r < 4; ++r) row[r] = *as_global(reinterpret_cast<const f32x4*>(ws(c) + kOffRow) + 16 * w + 4 * g + r);
   };
-  auto load_q = [&](int c) {
-    const int64_t at = token(c, 16 * wave + j) * a.q.ld + hk * a.q.hs + 8 * g;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) qr[w] = raw8<BF16>(a.q.p, at + 32 * w);
-  };
-  auto load_v = [&](int c) {
-#pragma unroll
-    for (int r = 0; r < 4; ++r) vv[r] = load1<BF16>(a.v.p, token(c, 16 * wave + 4 * g + r) * a.v.ld + h * a.v.hs + col);
-  };
-  auto load_tile = [&](int c, int off, f32x4 (&f)[4]) {
+  auto load_tile = [&](int c, int off, f32x4 (&f)[4]) {   // tiles past the diagonal: one that is there, not used
     const f32x4* p = reinterpret_cast<const f32x4*>(ws(c) + off) + lane;
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
-      if (t <= wave) f[t] = *as_global(p + tri(wave, t) * 64);
+    for (int t = 0; t < 4; ++t) f[t] = *as_global(p + tri(w, min(t, w)) * 64);
   };
-  auto load_row = [&](int c) {
-#pragma unroll
-    for (int r = 0; r < 4; ++r) row[r] = *as_global(reinterpret_cast<const f32x4*>(ws(c) + kOffRow) + 16 * wave + 4 * g + r);
-  };
-  // the keys that arrived, as this wave's left operand and to LDS for the state's update
-  auto put_k = [&](int c) {
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      kp[w] = parts<BF16>(kr[w]);
-#pragma unroll
-      for (int p = 0; p < NP; ++p) *as_lds_w(reinterpret_cast<u32x4*>(kl[c & 1] + p * kPart + key_at(16 * wave + j, 4 * w + g))) = kp[w].p[p];
-    }
-  };
-  auto put_s = [&]() {
-    u32x4 p[3];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      uint32_t hi, mid, lo;
-      cut2(s[2 * e], s[2 * e + 1], hi, mid, lo);
-      p[0][e] = hi, p[1][e] = mid, p[2][e] = lo;
-    }
-#pragma unroll
-    for (int q = 0; q < 3; ++q) sl[wave][q][lane] = p[q];
-  };
-  auto get_s = [&]() {
-#pragma unroll
-    for (int w = 0; w < 4; ++w)
-#pragma unroll
-      for (int q = 0; q < 3; ++q) sp4[w][q] = sl[w][q][lane];
-  };
-  load_k(0), load_v(0), load_row(0), load_q(0), load_tile(0, 0, tf), load_tile(0, kOffP, pf);
-  float flag = as_global(ws(0))[kOffFlag], decay = as_global(ws(0))[kOffRow + 4 * (kC - 1) + 2];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) s[e] = as_global(Sp)[(32 * wave + 8 * g + e) * kD];
-  put_s();
-  put_k(0);
-  lds_barrier();
-  get_s();
   const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
-  // this lane's place in the transposing reads of the keys: token 4 (l / 16) + l % 16 / 4 (+ 16 tile), rows
-  // 32 wave + 8 (l % 4) + 4 c .. + 3
-  const int kt0 = 4 * g + (j >> 2), kc0 = 4 * wave + (j & 3);
-  for (int c = 0; c < nc; ++c) {
-    const int nx = min(c + 1, nc - 1);
-    const float dec = decay;
-    load_k(nx);
-    if (flag != 0.0f) {
-      // an input that is not finite: the products below would carry it to tokens before it (0 times it is not
-      // 0), so the chunk runs token by token, in every wave alike (lane: rows 32 w + 8 (l / 16) .. + 7 of all w)
-      float st[32];
-      lds_barrier();   // the state's parts have been read
+  int c = 0;
+  if (wave < 4) {
+    float s[8];
+    auto put_s = [&]() {
+      u32x4 p[3];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) *reinterpret_cast<float*>(reinterpret_cast<char*>(&sl[wave][e >> 2][lane]) + 4 * (e & 3)) = s[e];
-      lds_barrier();
-#pragma unroll
-      for (int e = 0; e < 32; ++e) st[e] = *reinterpret_cast<const float*>(reinterpret_cast<const char*>(&sl[e >> 3][(e >> 2) & 1][lane]) + 4 * (e & 3));
-      const int t1 = min(kC, sp.len - kC * c);
-      for (int t = 0; t < t1; ++t) {
-        const int64_t tk = sp.start + kC * c + t;
-        const float de = dev_expf(as_global(a.g)[tk * a.ldg + h]), be = as_global(a.beta)[tk * a.ldb + h];
-        const float v1 = load1<BF16>(a.v.p, tk * a.v.ld + h * a.v.hs + col);
-        float x = 0.0f, y = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          st[e] *= de;
-          x = __builtin_fmaf(st[e], load1<BF16>(a.k.p, tk * a.k.ld + hk * a.k.hs + 32 * (e >> 3) + 8 * g + (e & 7)), x);
-        }
-        x = x + xor_perm<16>(x);
-        x = x + xor_perm<32>(x);
-        const float d = (v1 - x) * be;
-#pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          st[e] = __builtin_fmaf(load1<BF16>(a.k.p, tk * a.k.ld + hk * a.k.hs + 32 * (e >> 3) + 8 * g + (e & 7)), d, st[e]);
-          y = __builtin_fmaf(st[e], load1<BF16>(a.q.p, tk * a.q.ld + hk * a.q.hs + 32 * (e >> 3) + 8 * g + (e & 7)), y);
-        }
-        y = y + xor_perm<16>(y);
-        y = y + xor_perm<32>(y);
-        if (wave == 0 && g == 0) store1<BF16>(a.out.p, tk * a.out.ld + h * a.out.hs + col, y);
+      for (int e = 0; e < 4; ++e) {
+        uint32_t hi, mid, lo;
+        cut2(s[2 * e], s[2 * e + 1], hi, mid, lo);
+        p[0][e] = hi, p[1][e] = mid, p[2][e] = lo;
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        s[e] = st[e];
+      for (int q = 0; q < 3; ++q) sl[w][q][lane] = p[q];
+      if constexpr (!BF16)
 #pragma unroll
-        for (int w = 1; w < 4; ++w)
-          if (wave == w) s[e] = st[8 * w + e];
-      }
-      lds_barrier();
-      put_s();
-      if (c + 1 < nc) put_k(nx);
-      load_v(nx), load_row(nx), load_q(nx), load_tile(nx, 0, tf), load_tile(nx, kOffP, pf);
-      flag = as_global(ws(nx))[kOffFlag], decay = as_global(ws(nx))[kOffRow + 4 * (kC - 1) + 2];
-      lds_barrier();
-      get_s();
-      continue;
-    }
-    f32x4 x[2] = {zero, zero}, y[2] = {zero, zero}, d = zero, R;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) x[w & 1] = mul(kp[w].p, sp4[w], x[w & 1]);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) R[r] = row[r][0] * vv[r] - row[r][1] * (x[0][r] + x[1][r]);
-    rl[wave][lane] = R;
-    load_v(nx);
-#pragma unroll
-    for (int w = 0; w < 4; ++w) y[w & 1] = mul(parts<BF16>(qr[w]).p, sp4[w], y[w & 1]);
-    load_q(nx);
-    lds_barrier();
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-      if (t <= wave) d = mfma4(tf[t], rl[t][lane], d);
-    load_tile(nx, 0, tf);
-    dl[wave][lane] = d;
-    {
+        for (int q = 0; q < 2; ++q) sf[w][q][lane] = f32x4{s[4 * q], s[4 * q + 1], s[4 * q + 2], s[4 * q + 3]};
+    };
+    auto put_parts = [&](u32x2 (&to)[4][3][64], const f32x4& v) {
       u32x2 p[3];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         uint32_t hi, mid, lo;
-        cut2(d[2 * e] * row[2 * e][3], d[2 * e + 1] * row[2 * e + 1][3], hi, mid, lo);
+        cut2(v[2 * e], v[2 * e + 1], hi, mid, lo);
         p[0][e] = hi, p[1][e] = mid, p[2][e] = lo;
       }
 #pragma unroll
-      for (int q = 0; q < 3; ++q) el[wave][q][lane] = p[q];
-    }
-    f32x4 o;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) o[r] = (y[0][r] + y[1][r]) * row[r][2];
-    load_row(nx);
-    lds_barrier();
-    f32x4 sn[2];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) sn[e >> 2][e & 3] = s[e] * dec;
-#pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {   // depth: tokens 32 kk + 4 (l / 16) .., + 16
-      u32x4 ep[3];
+      for (int q = 0; q < 3; ++q) to[w][q][lane] = p[q];
+    };
+    auto get_parts = [&](const u32x2 (&from)[4][3][64], int kk, u32x4 (&p)[3]) {   // depths: rows 4 (l / 16) .. of two tiles
 #pragma unroll
       for (int q = 0; q < 3; ++q) {
-        const u32x2 e0 = el[2 * kk][q][lane], e1 = el[2 * kk + 1][q][lane];
-        ep[q] = u32x4{e0[0], e0[1], e1[0], e1[1]};
+        const u32x2 x = from[2 * kk][q][lane], y = from[2 * kk + 1][q][lane];
+        p[q] = u32x4{x[0], x[1], y[0], y[1]};
       }
+    };
+    // this lane's place in the transposing reads of the keys: token 4 (l / 16) + l % 16 / 4 (+ 16 tile), rows
+    // 32 w + 8 (l % 4) + 4 cc .. + 3
+    const int kt0 = 4 * g + (j >> 2), kc0 = 4 * w + (j & 3);
 #pragma unroll
-      for (int cc = 0; cc < 2; ++cc) {
-        u32x4 kt[NP];
+    for (int e = 0; e < 8; ++e) s[e] = as_global(Sp)[(32 * w + 8 * g + e) * kD];
+    while (c < nc) {
+      if (as_global(ws(c))[kOffFlag] != 0.0f) {
+        // an input that is not finite: the products below would carry it to tokens before it (0 times it is not
+        // 0), so the chunk runs token by token, in all four waves alike (lane: rows 32 w + 8 (l / 16) .. + 7 of all w)
+        float st[32];
+        float* x0 = reinterpret_cast<float*>(sl);
 #pragma unroll
-        for (int p = 0; p < NP; ++p) {
-          union {
-            i16x4 h[2];
-            u32x4 v;
-          } un;
+        for (int e = 0; e < 8; ++e) x0[(w * 8 + e) * 64 + lane] = s[e];
+        lds_barrier();
 #pragma unroll
-          for (int q = 0; q < 2; ++q)
-            un.h[q] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)as_lds_w(
-                kl[c & 1] + p * kPart + key_at(32 * kk + 16 * q + kt0, kc0) + 8 * cc));
-          kt[p] = un.v;
+        for (int e = 0; e < 32; ++e) st[e] = x0[e * 64 + lane];
+        const int t1 = min(kC, sp.len - kC * c);
+        for (int t = 0; t < t1; ++t) {
+          const int64_t tk = sp.start + kC * c + t;
+          const float de = dev_expf(as_global(a.g)[tk * a.ldg + h]), be = as_global(a.beta)[tk * a.ldb + h];
+          const float v1 = load1<BF16>(a.v.p, tk * a.v.ld + h * a.v.hs + col);
+          float x = 0.0f, y = 0.0f;
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            st[e] *= de;
+            x = __builtin_fmaf(st[e], load1<BF16>(a.k.p, tk * a.k.ld + hk * a.k.hs + 32 * (e >> 3) + 8 * g + (e & 7)), x);
+          }
+          x = x + xor_perm<16>(x);
+          x = x + xor_perm<32>(x);
+          const float d = (v1 - x) * be;
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            st[e] = __builtin_fmaf(load1<BF16>(a.k.p, tk * a.k.ld + hk * a.k.hs + 32 * (e >> 3) + 8 * g + (e & 7)), d, st[e]);
+            y = __builtin_fmaf(st[e], load1<BF16>(a.q.p, tk * a.q.ld + hk * a.q.hs + 32 * (e >> 3) + 8 * g + (e & 7)), y);
+          }
+          y = y + xor_perm<16>(y);
+          y = y + xor_perm<32>(y);
+          if (wave == 0 && g == 0) store1<BF16>(a.out.p, tk * a.out.ld + h * a.out.hs + col, y);
         }
-        sn[cc] = mul(kt, ep, sn[cc]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          s[e] = st[e];
+#pragma unroll
+          for (int q = 1; q < 4; ++q)
+            if (w == q) s[e] = st[8 * q + e];
+        }
+        lds_barrier();   // every wave has read the state
+        ++c;
+        continue;
       }
+      f32x4 row[4];
+      float vv[4];
+      auto load_v = [&](int c) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) vv[r] = load1<BF16>(a.v.p, token(c, 16 * w + 4 * g + r) * a.v.ld + h * a.v.hs + col);
+      };
+      load_v(c);
+      load_row(c, row);
+      f32x2 fd = load_flag(c);
+      put_s();
+      for (;;) {
+        lds_barrier();   // C: the state, the keys and T are there
+        const int nx = min(c + 1, nc - 1);
+        const float dec = fd[1];
+        fd = load_flag(nx);
+        f32x4 x[2] = {zero, zero}, R;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          u32x4 kp[NP], s3[3];
+#pragma unroll
+          for (int p = 0; p < NP; ++p) kp[p] = *as_lds(reinterpret_cast<const u32x4*>(kl[c & 1] + p * kPart + key_at(16 * w + j, 4 * q + g)));
+#pragma unroll
+          for (int p = 0; p < 3; ++p) s3[p] = sl[q][p][lane];
+          x[q & 1] = mul(kp, s3, x[q & 1]);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) R[r] = row[r][0] * vv[r] - row[r][1] * (x[0][r] + x[1][r]);
+        put_parts(rl, R);
+        load_v(nx);
+        u32x4 tp[2][3];
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk)
+          if (kk <= w >> 1)
+#pragma unroll
+            for (int p = 0; p < 3; ++p) tp[kk][p] = tl[w + (w == 3) + kk][p][lane];
+        lds_barrier();   // A: R is there
+        f32x4 d[2] = {zero, zero};
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk)
+          if (kk <= w >> 1) {
+            u32x4 rp[3];
+            get_parts(rl, kk, rp);
+            d[kk] = mul(tp[kk], rp, d[kk]);
+          }
+        d[0] += d[1];
+        dl[w][lane] = d[0];
+        f32x4 e;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) e[r] = d[0][r] * row[r][3];
+        put_parts(el, e);
+        load_row(nx, row);
+        u32x4 kt[2][2][NP];   // K^T: this wave's rows (two tiles), depth tokens 32 kk + 4 (l / 16) .., + 16
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+          for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+            for (int p = 0; p < NP; ++p) {
+              union {
+                i16x4 h[2];
+                u32x4 v;
+              } un;
+#pragma unroll
+              for (int q = 0; q < 2; ++q)
+                un.h[q] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)as_lds_w(
+                    kl[c & 1] + p * kPart + key_at(32 * kk + 16 * q + kt0, kc0) + 8 * cc));
+              kt[kk][cc][p] = un.v;
+            }
+        lds_barrier();   // B: d is there
+        f32x4 sn[2];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) sn[q >> 2][q & 3] = s[q] * dec;
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+          u32x4 ep[3];
+          get_parts(el, kk, ep);
+#pragma unroll
+          for (int cc = 0; cc < 2; ++cc) sn[cc] = mul(kt[kk][cc], ep, sn[cc]);
+        }
+#pragma unroll
+        for (int q = 0; q < 8; ++q) s[q] = sn[q >> 2][q & 3];
+        if (++c >= nc || fd[0] != 0.0f) break;
+        put_s();
+      }
+      lds_barrier();   // every wave has read what it needs of the chunk
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) s[e] = sn[e >> 2][e & 3];
-    put_s();
-    if (c + 1 < nc) put_k(nx);
+    for (int e = 0; e < 8; ++e) as_global_w(Sp)[(32 * w + 8 * g + e) * kD] = s[e];
+  } else {
+    while (c < nc) {
+      if (as_global(ws(c))[kOffFlag] != 0.0f) {
+        lds_barrier();
+        lds_barrier();
+        ++c;
+        continue;
+      }
+      Raw8<BF16> kr[4], qr[4];
+      f32x4 tf[4], pf[4], row[4];
+      auto load_k = [&](int c) {
+        const int64_t at = token(c, 16 * w + j) * a.k.ld + hk * a.k.hs + 8 * g;
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
-      if (t <= wave) o = mfma4(pf[t], dl[t][lane], o);
-    load_tile(nx, kOffP, pf);
-    flag = as_global(ws(nx))[kOffFlag], decay = as_global(ws(nx))[kOffRow + 4 * (kC - 1) + 2];
+        for (int q = 0; q < 4; ++q) kr[q] = raw8<BF16>(a.k.p, at + 32 * q);
+      };
+      auto load_q = [&](int c) {
+        const int64_t at = token(c, 16 * w + j) * a.q.ld + hk * a.q.hs + 8 * g;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int t = kC * c + 16 * wave + 4 * g + r;
-      if (t < sp.len) store1<BF16>(a.out.p, (int64_t)(sp.start + t) * a.out.ld + h * a.out.hs + col, o[r]);
+        for (int q = 0; q < 4; ++q) qr[q] = raw8<BF16>(a.q.p, at + 32 * q);
+      };
+      auto put_k = [&](int c) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const Parts<BF16> kp = parts<BF16>(kr[q]);
+#pragma unroll
+          for (int p = 0; p < NP; ++p) *as_lds_w(reinterpret_cast<u32x4*>(kl[c & 1] + p * kPart + key_at(16 * w + j, 4 * q + g))) = kp.p[p];
+        }
+      };
+      auto put_t = [&]() {
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk)
+          if (kk <= w >> 1) {
+            u32x4 p[3];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int t = 2 * kk + (e >> 1);
+              const float x = t <= w ? tf[t][2 * (e & 1)] : 0.0f, y = t <= w ? tf[t][2 * (e & 1) + 1] : 0.0f;
+              uint32_t hi, mid, lo;
+              cut2(x, y, hi, mid, lo);
+              p[0][e] = hi, p[1][e] = mid, p[2][e] = lo;
+            }
+#pragma unroll
+            for (int q = 0; q < 3; ++q) tl[w + (w == 3) + kk][q][lane] = p[q];
+          }
+      };
+      load_k(c), load_tile(c, 0, tf);
+      load_q(c), load_tile(c, kOffP, pf), load_row(c, row);
+      f32x2 fd = load_flag(c);
+      put_k(c);
+      put_t();
+      load_k(min(c + 1, nc - 1)), load_tile(min(c + 1, nc - 1), 0, tf);
+      for (;;) {
+        lds_barrier();   // C
+        const int nx = min(c + 1, nc - 1), n2 = min(c + 2, nc - 1);
+        fd = load_flag(nx);
+        f32x4 y[2] = {zero, zero}, o[2] = {zero, zero};
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          if constexpr (BF16) {
+            u32x4 s3[3];
+#pragma unroll
+            for (int p = 0; p < 3; ++p) s3[p] = sl[q][p][lane];
+            y[q & 1] = mul(qr[q].v, s3, y[q & 1]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) y[e] = mfma4(__builtin_bit_cast(f32x4, qr[q].v[e]), sf[q][e][lane], y[e]);
+          }
+        }
+        load_q(nx);
+        lds_barrier();   // A
+        put_k(c + 1);
+        load_k(n2);
+        lds_barrier();   // B: T has been read, d is there
+        put_t();
+        load_tile(n2, 0, tf);
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+          if (t <= w) o[t & 1] = mfma4(pf[t], dl[t][lane], o[t & 1]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int t = kC * c + 16 * w + 4 * g + r;
+          const float v = (y[0][r] + y[1][r]) * row[r][2] + (o[0][r] + o[1][r]);
+          if (t < sp.len) store1<BF16>(a.out.p, (int64_t)(sp.start + t) * a.out.ld + h * a.out.hs + col, v);
+        }
+        load_tile(nx, kOffP, pf);
+        load_row(nx, row);
+        if (++c >= nc || fd[0] != 0.0f) break;
+      }
+      lds_barrier();
     }
-    lds_barrier();
-    get_s();
   }
-#pragma unroll
-  for (int e = 0; e < 8; ++e) as_global_w(Sp)[(32 * wave + 8 * g + e) * kD] = s[e];
 }
 
 template <bool BF16>
@@ -604,7 +684,7 @@ hipError_t launch(const DeltaSeq& a, hipStream_t s) {
     delta_step_kernel<BF16><<<(unsigned)(((int64_t)a.n_seq * a.heads * 8 + 3) / 4), 256, 0, s>>>(a);
   } else {
     delta_chunk_kernel<BF16><<<dim3((unsigned)seq_tiles_max(a.tokens, a.n_seq, kC), a.k_heads), 256, 0, s>>>(a);
-    delta_scan_kernel<BF16><<<(unsigned)(((int64_t)a.n_seq * a.heads + 7) / 8 * 64), 256, 0, s>>>(a);
+    delta_scan_kernel<BF16><<<(unsigned)(((int64_t)a.n_seq * a.heads + 7) / 8 * 64), 512, 0, s>>>(a);
   }
   return hipGetLastError();
 }
