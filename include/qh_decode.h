@@ -252,7 +252,7 @@ int qh_gemm_i8_w8a8(void* y, int64_t ldy, int type, const int8_t* w, const float
  * [tokens][heads][128] of `type`, g (the log of the decay, at most 0) and beta [tokens][heads] fp32 with rows ldg and
  * ldb apart (any alignment), state [n_seq][heads][128][128] fp32 read and updated in place.  Value head h takes key
  * head h / (heads / k_heads).  q and k as the caller normalised them.  An empty sequence keeps its state. */
-size_t qh_delta_rule_seq_workspace(int tokens, int n_seq, int heads, int max_len);
+size_t qh_delta_rule_seq_workspace(int tokens, int n_seq, int heads, int k_heads, int type, int max_len);
 int qh_delta_rule_seq(void* out, int64_t ldo, int64_t hso, const void* q, int64_t ldq, int64_t hsq, const void* k, int64_t ldk,
                       int64_t hsk, const void* v, int64_t ldv, int64_t hsv, int type, const float* g, int64_t ldg,
                       const float* beta, int64_t ldb, float* state, const int32_t* cu, int n_seq, int tokens, int max_len,

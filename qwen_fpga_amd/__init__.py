@@ -589,11 +589,13 @@ def gemm_i8_w8a8(y, w, scale, xq, sx, stream=None):
         _check(st, "qh_gemm_i8_w8a8")
 
 
-def delta_rule_seq_workspace(tokens: int, n_seq: int, heads: int, max_len: int) -> int:
-    """Bytes of device scratch delta_rule_seq takes from its caller."""
+def delta_rule_seq_workspace(tokens: int, n_seq: int, heads: int, max_len: int, k_heads: Optional[int] = None,
+                             dtype: int = F32) -> int:
+    """Bytes of device scratch delta_rule_seq takes from its caller.  With fewer key heads than heads, or
+    dtype BF16, less is enough: pass them, or take what serves both types and any k_heads."""
     f = _lib().qh_delta_rule_seq_workspace
     f.restype = ctypes.c_size_t
-    return int(f(int(tokens), int(n_seq), int(heads), int(max_len)))
+    return int(f(int(tokens), int(n_seq), int(heads), int(heads if k_heads is None else k_heads), int(dtype), int(max_len)))
 
 
 def delta_rule_seq(out, q, k, v, g, beta, S, cu, workspace, max_len: int, stream=None):

@@ -32,16 +32,27 @@ namespace {
 
 constexpr int kD = 128;
 constexpr int kC = 64;                       // tokens of a chunk
-// A chunk's and head's part of the workspace, in floats: T and P as ten 16 x 16 tiles each (lower triangle,
-// tile (i, j) at i (i + 1) / 2 + j; lane l's four values: row l % 16, columns 4 (l / 16) ..), the row factors
-// {beta, beta e^c, e^c, e^{c_63 - c}}, whether an input is not finite, e^{c_63}.
-constexpr int kTiles = 10, kOffP = kTiles * 256, kOffRow = 2 * kTiles * 256, kOffFlag = kOffRow + 4 * kC,
-              kChunkFloats = kOffFlag + 64;
-__device__ __forceinline__ constexpr int tri(int i, int j) { return i * (i + 1) / 2 + j; }
+// A chunk's and head's part of the workspace, in floats: T and P in parts of bfloat16, as the operands that the wave of
+// the tokens 16 w .. + 15 takes (depth 32 kk: kk = 0, and 1 for the waves 2 and 3; part by part, 16 bytes a lane: row
+// l % 16, columns 32 kk + 4 (l / 16) .. and + 16); the tokens' factors beta, beta e^c, e^{c_63 - c} and e^c; whether an
+// input is not finite, e^{c_63}.  (The factors in arrays of their own: a lane that loads what it does not use reuses
+// those registers at once, and waits for the load before it.)
+constexpr int kOperand = 3 * 256, kOffP = 6 * kOperand, kOffRow = 2 * kOffP, kOffFlag = kOffRow + 4 * kC, kChunkFloats = kOffFlag + 64;
+__device__ __forceinline__ constexpr int operand(int w, int kk) { return w + (w == 3) + kk; }
 // A chunk's slot: one per started 64 rows and sequence, so sequences need no count of those before them.
 // (floor(x) + floor(y) <= floor(x + y), so a sequence's last slot lies below the next one's first.)
 __device__ __forceinline__ size_t chunk_at(const DeltaSeq& a, int seq, int start, int c, int h) {
   return ((size_t)(start / kC + seq + c) * a.heads + h) * kChunkFloats;
+}
+// Behind those, each chunk's and key head's k and q in parts: k as it stands in LDS (key_at), q as the operands
+// [tokens 16 w][depth 32 s][part][lane].  (Copies of a bfloat16 input too: its rows, a fused projection's, are powers of
+// two apart, and a head's then lie in one of an L2's sixteen channels, from which eight workgroups would read them.)
+constexpr int kPart = kC * kD * 2;
+__host__ __device__ __forceinline__ constexpr size_t chunk_slots(int tokens, int n_seq) { return (size_t)(tokens / kC) + n_seq; }
+template <int NP>
+__device__ __forceinline__ char* keys_at(const DeltaSeq& a, int seq, int start, int c, int hk) {
+  return reinterpret_cast<char*>(a.ws + chunk_slots(a.tokens, a.n_seq) * a.heads * kChunkFloats) +
+         ((size_t)(start / kC + seq + c) * a.k_heads + hk) * (2 * NP * kPart);
 }
 
 template <bool BF16>
@@ -155,6 +166,8 @@ __global__ __launch_bounds__(256) void delta_step_kernel(const DeltaSeq a) {
   for (int e = 0; e < 8; ++e) *as_global_w(Sp + e * (kD / 4)) = s[e];
 }
 
+// e^x for a difference of sums (its power of two rounded once to fp32: an error of |x| 2^-24 of what is e^x small).
+__device__ __forceinline__ float exp_of(double x) { return __builtin_amdgcn_exp2f((float)(x * 1.4426950408889634)); }
 // Two floats as pairs of bfloat16: the top eight bits of each, the next eight, the last eight.
 __device__ __forceinline__ void cut2(float x, float y, uint32_t& hi, uint32_t& mid, uint32_t& lo) {
   const uint32_t xu = __float_as_uint(x), yu = __float_as_uint(y);
@@ -225,8 +238,21 @@ __device__ __forceinline__ f32x4 mul(const u32x4 (&x)[NX], const u32x4 (&y)[NY],
 }
 // A chunk's keys in LDS, a part [64][128] bfloat16 after another: 16-byte piece c of token t at piece c ^ (t % 16),
 // so that 16 tokens' pieces of one place lie in all banks.
-constexpr int kPart = kC * kD * 2;
 __device__ __forceinline__ int key_at(int t, int c) { return t * (kD * 2) + 16 * (c ^ (t & 15)); }
+
+// Eight values of a lane to the workspace in parts.
+__device__ __forceinline__ void put_operand(float* to, int lane, const f32x4& x, const f32x4& y) {
+  u32x4 p[3];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const f32x4& v = e < 2 ? x : y;
+    uint32_t hi, mid, lo;
+    cut2(v[2 * (e & 1)], v[2 * (e & 1) + 1], hi, mid, lo);
+    p[0][e] = hi, p[1][e] = mid, p[2][e] = lo;
+  }
+#pragma unroll
+  for (int q = 0; q < 3; ++q) *as_global_w(reinterpret_cast<u32x4*>(to + 256 * q) + lane) = p[q];
+}
 
 // T, P and the row factors of one chunk, for the value heads of one key head.  Wave i forms the tiles (i, j <= i) of
 // K K^T and Q K^T once; every head scales them.
@@ -257,7 +283,13 @@ __global__ __launch_bounds__(256) void delta_chunk_kernel(const DeltaSeq a) {
       kp[s] = parts<BF16>(kr);
       qp[s] = parts<BF16>(qr);
 #pragma unroll
-      for (int p = 0; p < NP; ++p) *as_lds_w(reinterpret_cast<u32x4*>(kl + p * kPart + key_at(16 * wave + j, 4 * s + g))) = kp[s].p[p];
+      for (int p = 0; p < NP; ++p) {
+        const int at_k = p * kPart + key_at(16 * wave + j, 4 * s + g);
+        *as_lds_w(reinterpret_cast<u32x4*>(kl + at_k)) = kp[s].p[p];
+        char* to = keys_at<NP>(a, at.seq, at.sp.start, at.tile, hk);
+        *as_global_w(reinterpret_cast<u32x4*>(to + at_k)) = kp[s].p[p];
+        *as_global_w(reinterpret_cast<u32x4*>(to + NP * kPart + ((4 * wave + s) * NP + p) * 1024) + lane) = qp[s].p[p];
+      }
     }
     __syncthreads();
 #pragma unroll
@@ -296,8 +328,11 @@ __global__ __launch_bounds__(256) void delta_chunk_kernel(const DeltaSeq a) {
       const double last = __shfl(c, kC - 1);
       cs[lane] = c;
       bt[lane] = be;
-      const float ec = dev_expf((float)c);
-      *as_global_w(reinterpret_cast<f32x4*>(ws + kOffRow) + lane) = f32x4{be, be * ec, ec, dev_expf((float)(last - c))};
+      const float ec = exp_of(c);
+      ws[kOffRow + lane] = be;
+      ws[kOffRow + kC + lane] = be * ec;
+      ws[kOffRow + 2 * kC + lane] = exp_of(last - c);
+      ws[kOffRow + 3 * kC + lane] = ec;
       if (lane == kC - 1) ws[kOffFlag + 1] = ec;
     }
 #pragma unroll
@@ -311,20 +346,24 @@ __global__ __launch_bounds__(256) void delta_chunk_kernel(const DeltaSeq a) {
     const int t = 16 * wave + j;
     const double ct = cs[t];
     const float be = bt[t];
+    f32x4 pv[4];
 #pragma unroll
     for (int jj = 0; jj < 4; ++jj) {
+      pv[jj] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
       if (jj > wave) continue;
-      f32x4 av, pv;
+      f32x4 av;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int jr = 16 * jj + g4 + r;
-        const float e = jr <= t ? dev_expf((float)(ct - cs[jr])) : 0.0f;
+        const float e = jr <= t ? exp_of(ct - cs[jr]) : 0.0f;
         av[r] = jr < t ? be * e * G[jj][r] : 0.0f;
-        pv[r] = jr <= t ? e * P[jj][r] : 0.0f;
+        pv[jj][r] = jr <= t ? e * P[jj][r] : 0.0f;
       }
       *as_lds_w(reinterpret_cast<f32x4*>(al + t * LD + 16 * jj + g4)) = av;
-      *as_global_w(reinterpret_cast<f32x4*>(ws + kOffP + tri(wave, jj) * 256) + lane) = pv;
     }
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk)
+      if (kk <= wave >> 1) put_operand(ws + kOffP + operand(wave, kk) * kOperand, lane, pv[2 * kk], pv[2 * kk + 1]);
     if (threadIdx.x == 0) ws[kOffFlag] = (bad_in[0] | bad_in[1] | bad_in[2] | bad_in[3]) ? 1.0f : 0.0f;
     __syncthreads();
     // the diagonal tiles' inverses: lane's column j of T_ii, row after row
@@ -364,70 +403,89 @@ __global__ __launch_bounds__(256) void delta_chunk_kernel(const DeltaSeq a) {
       }
     }
     __syncthreads();
-    for (int u = wave; u < kTiles; u += 4) {
-      const int i = u < 1 ? 0 : u < 3 ? 1 : u < 6 ? 2 : 3, c = u - tri(i, 0);
-      *as_global_w(reinterpret_cast<f32x4*>(ws + u * 256) + lane) =
-          *as_lds(reinterpret_cast<const f32x4*>(tl + (16 * i + j) * LD + 16 * c + g4));
-    }
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk)
+      if (kk <= wave >> 1) {
+        f32x4 x[2];
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          x[q] = *as_lds(reinterpret_cast<const f32x4*>(tl + (16 * wave + j) * LD + 32 * kk + 16 * q + g4));
+          if (2 * kk + q > wave) x[q] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        put_operand(ws + operand(wave, kk) * kOperand, lane, x[0], x[1]);
+      }
     __syncthreads();   // T and the sums have been read
   }
 }
 
-// The state's way through the chunks: a workgroup takes one sequence, one head and 16 of its columns.  What bounds it
-// is the chain from one chunk's state to the next, so four waves do that alone: R = beta v - beta e^c K S, d = T R,
-// S' = e^{c_63} S + K^T (e^{c_63 - c} d); wave w owns the state's rows 32 w .. + 31 (lane: 32 w + 8 (l / 16) .. + 7 of
-// column l % 16) and the chunk's tokens 16 w .. + 15.  The other four, one beside each on its SIMD, do what the chain
-// does not wait for: the next chunk's keys and T brought to LDS in parts, Q S and P d, the outputs.  With one set of
-// four waves doing everything in turn a chunk took 8.7 thousand cycles (fp32) and 6.0 (bfloat16).
-template <bool BF16>
-__global__ __launch_bounds__(512, BF16 ? 4 : 2) void delta_scan_kernel(const DeltaSeq a) {
-  constexpr int NP = Parts<BF16>::NP;
+// The state's way through the chunks: a workgroup takes one sequence, one head and 16 NB of its columns.  What bounds it
+// is the chain from one chunk's state to the next, so four waves do that alone, one on each SIMD.  Wave w keeps the
+// state's rows 32 w .. + 31 in registers (lane: 32 w + 8 (l / 16) .. + 7 of column l % 16), which are at once its right
+// operand; per chunk it
+//   forms its rows' part of K S for all 64 tokens                                  | barrier 1
+//   adds the four parts for the tokens 16 w .. + 15: R = beta v - beta e^c K S      | barrier 2
+//   forms those tokens' d = T R                                                     | barrier 3
+//   updates its rows: e^{c_63} S + K^T (e^{c_63 - c} d).
+// Four waves beside them form the outputs e^c Q S + P d, and one brings the next chunk's keys to LDS.  All operands
+// come in parts, cut once for a head's workgroups: the fp32 MFMAs run on the vector units, and cutting there, in each
+// workgroup, held the chain up as much.  NB = 2 halves what a head's workgroups read from L2 (72 KB a chunk each in
+// bfloat16), NB = 1 makes twice as many of them.
+template <bool BF16, int NB>
+__global__ __launch_bounds__(576, 2) void delta_scan_kernel(const DeltaSeq a) {
+  constexpr int NP = Parts<BF16>::NP, NSL = 8 / NB;
   __shared__ __attribute__((aligned(256))) char kl[2][NP * kPart];   // parts of the keys, this chunk's and the next one's
-  __shared__ u32x4 tl[6][3][64];          // parts of T: rows 16 w, depth 32 kk at w + (w == 3) + kk, kk <= w / 2
-  __shared__ u32x4 sl[4][3][64];          // parts of the state
-  __shared__ f32x4 sf[BF16 ? 1 : 4][2][64];   // the state itself (fp32: for Q S)
-  __shared__ u32x2 rl[4][3][64], el[4][3][64];   // parts of R and of e^{c_63 - c_t} d_t
-  __shared__ f32x4 dl[4][64];             // d
+  __shared__ f32x4 xl[NB][4][4][64];             // [columns][token tile][wave]: the waves' parts of K S
+  __shared__ u32x4 sl[NB][4][3][64];             // parts of the state
+  __shared__ u32x2 rl[NB][4][3][64], el[NB][4][3][64], dl[NB][4][3][64];   // parts of R, of e^{c_63 - c_t} d_t, of d
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & 3;
   const int g = lane >> 4, j = lane & 15;
-  // the eight slices of a head on one of the eight XCDs, whose L2 then holds the head's q, k, T and P
-  const int b = blockIdx.x, u = (b & 7) + 8 * (b >> 6), slice = (b >> 3) & 7;
+  // the slices of a head on one of the eight XCDs, whose L2 then holds the head's operands
+  const int b = blockIdx.x, u = (b & 7) + 8 * (b / (8 * NSL)), slice = (b >> 3) % NSL;
   if (u >= a.n_seq * a.heads) return;
-  const int h = u % a.heads, seq = u / a.heads, hk = h / (a.heads / a.k_heads);
+  const int h = u % a.heads, seq = longest_first(a.cu, a.n_seq, a.tokens, u / a.heads), hk = h / (a.heads / a.k_heads);
   const SeqSpan sp = seq_span(as_global(a.cu)[seq], as_global(a.cu)[seq + 1], a.tokens);
   if (sp.len == 0) return;
-  const int col = 16 * slice + j;
+  const int col = 16 * NB * slice + j;   // (+ 16 for the second)
   float* Sp = a.S + ((size_t)seq * a.heads + h) * kD * kD + col;
   const int nc = seq_tiles(sp.len, kC);
   auto token = [&](int c, int t) -> int64_t { return min(sp.start + kC * c + t, sp.start + sp.len - 1); };
   auto ws = [&](int c) { return a.ws + chunk_at(a, seq, sp.start, c, h); };
-  auto load_flag = [&](int c) { return *as_global(reinterpret_cast<const f32x2*>(ws(c) + kOffFlag)); };
-  auto load_row = [&](int c, f32x4 (&row)[4]) {
-#pragma unroll
-    for (int r = 0; r < 4; ++r) row[r] = *as_global(reinterpret_cast<const f32x4*>(ws(c) + kOffRow) + 16 * w + 4 * g + r);
+  auto flagged = [&](int c) { return as_global(ws(c))[kOffFlag]; };
+  auto load_row = [&](int c, int which) {   // of this lane's four tokens
+    return *as_global(reinterpret_cast<const f32x4*>(ws(c) + kOffRow + kC * which) + 4 * w + g);
   };
-  auto load_tile = [&](int c, int off, f32x4 (&f)[4]) {   // tiles past the diagonal: one that is there, not used
-    const f32x4* p = reinterpret_cast<const f32x4*>(ws(c) + off) + lane;
+  auto load_operand = [&](int c, int off, u32x4 (&f)[2][3]) {   // (waves 0 and 1 have one: twice, so that the loads count alike)
 #pragma unroll
-    for (int t = 0; t < 4; ++t) f[t] = *as_global(p + tri(w, min(t, w)) * 64);
+    for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+      for (int p = 0; p < 3; ++p)
+        f[kk][p] = *as_global(reinterpret_cast<const u32x4*>(ws(c) + off + operand(w, min(kk, w >> 1)) * kOperand + 256 * p) + lane);
+  };
+  auto get_parts = [&](const u32x2 (&from)[4][3][64], int kk, u32x4 (&p)[3]) {   // depths: rows 4 (l / 16) .. of two tiles
+#pragma unroll
+    for (int q = 0; q < 3; ++q) {
+      const u32x2 x = from[2 * kk][q][lane], y = from[2 * kk + 1][q][lane];
+      p[q] = u32x4{x[0], x[1], y[0], y[1]};
+    }
   };
   const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
   int c = 0;
   if (wave < 4) {
-    float s[8];
-    auto put_s = [&]() {
-      u32x4 p[3];
+    __builtin_amdgcn_s_setprio(3);
+    float s[NB][8];
+    u32x4 s3[NB][3];   // its parts
+    auto cut_s = [&]() {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        uint32_t hi, mid, lo;
-        cut2(s[2 * e], s[2 * e + 1], hi, mid, lo);
-        p[0][e] = hi, p[1][e] = mid, p[2][e] = lo;
+      for (int n = 0; n < NB; ++n) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          uint32_t hi, mid, lo;
+          cut2(s[n][2 * e], s[n][2 * e + 1], hi, mid, lo);
+          s3[n][0][e] = hi, s3[n][1][e] = mid, s3[n][2][e] = lo;
+        }
+#pragma unroll
+        for (int q = 0; q < 3; ++q) sl[n][w][q][lane] = s3[n][q];
       }
-#pragma unroll
-      for (int q = 0; q < 3; ++q) sl[w][q][lane] = p[q];
-      if constexpr (!BF16)
-#pragma unroll
-        for (int q = 0; q < 2; ++q) sf[w][q][lane] = f32x4{s[4 * q], s[4 * q + 1], s[4 * q + 2], s[4 * q + 3]};
     };
     auto put_parts = [&](u32x2 (&to)[4][3][64], const f32x4& v) {
       u32x2 p[3];
@@ -440,114 +498,124 @@ __global__ __launch_bounds__(512, BF16 ? 4 : 2) void delta_scan_kernel(const Del
 #pragma unroll
       for (int q = 0; q < 3; ++q) to[w][q][lane] = p[q];
     };
-    auto get_parts = [&](const u32x2 (&from)[4][3][64], int kk, u32x4 (&p)[3]) {   // depths: rows 4 (l / 16) .. of two tiles
-#pragma unroll
-      for (int q = 0; q < 3; ++q) {
-        const u32x2 x = from[2 * kk][q][lane], y = from[2 * kk + 1][q][lane];
-        p[q] = u32x4{x[0], x[1], y[0], y[1]};
-      }
-    };
     // this lane's place in the transposing reads of the keys: token 4 (l / 16) + l % 16 / 4 (+ 16 tile), rows
     // 32 w + 8 (l % 4) + 4 cc .. + 3
     const int kt0 = 4 * g + (j >> 2), kc0 = 4 * w + (j & 3);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) s[e] = as_global(Sp)[(32 * w + 8 * g + e) * kD];
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[n][e] = as_global(Sp)[(32 * w + 8 * g + e) * kD + 16 * n];
     while (c < nc) {
-      if (as_global(ws(c))[kOffFlag] != 0.0f) {
+      if (flagged(c) != 0.0f) {
         // an input that is not finite: the products below would carry it to tokens before it (0 times it is not
         // 0), so the chunk runs token by token, in all four waves alike (lane: rows 32 w + 8 (l / 16) .. + 7 of all w)
-        float st[32];
-        float* x0 = reinterpret_cast<float*>(sl);
+        float* x0 = reinterpret_cast<float*>(xl);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x0[(w * 8 + e) * 64 + lane] = s[e];
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x0[(32 * n + w * 8 + e) * 64 + lane] = s[n][e];
         lds_barrier();
 #pragma unroll
-        for (int e = 0; e < 32; ++e) st[e] = x0[e * 64 + lane];
-        const int t1 = min(kC, sp.len - kC * c);
-        for (int t = 0; t < t1; ++t) {
-          const int64_t tk = sp.start + kC * c + t;
-          const float de = dev_expf(as_global(a.g)[tk * a.ldg + h]), be = as_global(a.beta)[tk * a.ldb + h];
-          const float v1 = load1<BF16>(a.v.p, tk * a.v.ld + h * a.v.hs + col);
-          float x = 0.0f, y = 0.0f;
+        for (int n = 0; n < NB; ++n) {
+          float st[32];
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            st[e] *= de;
-            x = __builtin_fmaf(st[e], load1<BF16>(a.k.p, tk * a.k.ld + hk * a.k.hs + 32 * (e >> 3) + 8 * g + (e & 7)), x);
+          for (int e = 0; e < 32; ++e) st[e] = x0[(32 * n + e) * 64 + lane];
+          const int t1 = min(kC, sp.len - kC * c);
+          for (int t = 0; t < t1; ++t) {
+            const int64_t tk = sp.start + kC * c + t;
+            const float de = dev_expf(as_global(a.g)[tk * a.ldg + h]), be = as_global(a.beta)[tk * a.ldb + h];
+            const float v1 = load1<BF16>(a.v.p, tk * a.v.ld + h * a.v.hs + col + 16 * n);
+            float x = 0.0f, y = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              st[e] *= de;
+              x = __builtin_fmaf(st[e], load1<BF16>(a.k.p, tk * a.k.ld + hk * a.k.hs + 32 * (e >> 3) + 8 * g + (e & 7)), x);
+            }
+            x = x + xor_perm<16>(x);
+            x = x + xor_perm<32>(x);
+            const float d = (v1 - x) * be;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              st[e] = __builtin_fmaf(load1<BF16>(a.k.p, tk * a.k.ld + hk * a.k.hs + 32 * (e >> 3) + 8 * g + (e & 7)), d, st[e]);
+              y = __builtin_fmaf(st[e], load1<BF16>(a.q.p, tk * a.q.ld + hk * a.q.hs + 32 * (e >> 3) + 8 * g + (e & 7)), y);
+            }
+            y = y + xor_perm<16>(y);
+            y = y + xor_perm<32>(y);
+            if (wave == 0 && g == 0) store1<BF16>(a.out.p, tk * a.out.ld + h * a.out.hs + col + 16 * n, y);
           }
-          x = x + xor_perm<16>(x);
-          x = x + xor_perm<32>(x);
-          const float d = (v1 - x) * be;
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            st[e] = __builtin_fmaf(load1<BF16>(a.k.p, tk * a.k.ld + hk * a.k.hs + 32 * (e >> 3) + 8 * g + (e & 7)), d, st[e]);
-            y = __builtin_fmaf(st[e], load1<BF16>(a.q.p, tk * a.q.ld + hk * a.q.hs + 32 * (e >> 3) + 8 * g + (e & 7)), y);
+          for (int e = 0; e < 8; ++e) {
+            s[n][e] = st[e];
+#pragma unroll
+            for (int q = 1; q < 4; ++q)
+              if (w == q) s[n][e] = st[8 * q + e];
           }
-          y = y + xor_perm<16>(y);
-          y = y + xor_perm<32>(y);
-          if (wave == 0 && g == 0) store1<BF16>(a.out.p, tk * a.out.ld + h * a.out.hs + col, y);
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          s[e] = st[e];
-#pragma unroll
-          for (int q = 1; q < 4; ++q)
-            if (w == q) s[e] = st[8 * q + e];
         }
         lds_barrier();   // every wave has read the state
         ++c;
         continue;
       }
-      f32x4 row[4];
-      float vv[4];
+      f32x4 row[3];
+      float vv[NB][4];
+      u32x4 tp[2][3];
       auto load_v = [&](int c) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) vv[r] = load1<BF16>(a.v.p, token(c, 16 * w + 4 * g + r) * a.v.ld + h * a.v.hs + col);
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int n = 0; n < NB; ++n)
+            vv[n][r] = load1<BF16>(a.v.p, token(c, 16 * w + 4 * g + r) * a.v.ld + h * a.v.hs + col + 16 * n);
       };
+      // (in the loop's order: the waits there count what is in flight on either way in)
+      f32x2 fd = *as_global(reinterpret_cast<const f32x2*>(ws(c) + kOffFlag));
       load_v(c);
-      load_row(c, row);
-      f32x2 fd = load_flag(c);
-      put_s();
+      row[0] = load_row(c, 0);
+      row[1] = load_row(c, 1);
+      load_operand(c, 0, tp);
+      row[2] = load_row(c, 2);
+      cut_s();
+      lds_barrier();   // 0: the keys are there
       for (;;) {
-        lds_barrier();   // C: the state, the keys and T are there
         const int nx = min(c + 1, nc - 1);
         const float dec = fd[1];
-        fd = load_flag(nx);
-        f32x4 x[2] = {zero, zero}, R;
+        fd = *as_global(reinterpret_cast<const f32x2*>(ws(nx) + kOffFlag));
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          u32x4 kp[NP], s3[3];
+        for (int t = 0; t < 4; ++t) {
+          u32x4 kp[NP];
 #pragma unroll
-          for (int p = 0; p < NP; ++p) kp[p] = *as_lds(reinterpret_cast<const u32x4*>(kl[c & 1] + p * kPart + key_at(16 * w + j, 4 * q + g)));
+          for (int p = 0; p < NP; ++p) kp[p] = *as_lds(reinterpret_cast<const u32x4*>(kl[c & 1] + p * kPart + key_at(16 * t + j, 4 * w + g)));
 #pragma unroll
-          for (int p = 0; p < 3; ++p) s3[p] = sl[q][p][lane];
-          x[q & 1] = mul(kp, s3, x[q & 1]);
+          for (int n = 0; n < NB; ++n) xl[n][t][w][lane] = mul(kp, s3[n], zero);
         }
+        lds_barrier();   // 1
 #pragma unroll
-        for (int r = 0; r < 4; ++r) R[r] = row[r][0] * vv[r] - row[r][1] * (x[0][r] + x[1][r]);
-        put_parts(rl, R);
+        for (int n = 0; n < NB; ++n) {
+          f32x4 x = xl[n][w][0][lane], R;
+#pragma unroll
+          for (int q = 1; q < 4; ++q) x += xl[n][w][q][lane];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) R[r] = row[0][r] * vv[n][r] - row[1][r] * x[r];
+          put_parts(rl[n], R);
+        }
         load_v(nx);
-        u32x4 tp[2][3];
+        row[0] = load_row(nx, 0);
+        row[1] = load_row(nx, 1);
+        lds_barrier();   // 2
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk)
-          if (kk <= w >> 1)
+        for (int n = 0; n < NB; ++n) {
+          f32x4 d[2] = {zero, zero};
 #pragma unroll
-            for (int p = 0; p < 3; ++p) tp[kk][p] = tl[w + (w == 3) + kk][p][lane];
-        lds_barrier();   // A: R is there
-        f32x4 d[2] = {zero, zero};
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk)
-          if (kk <= w >> 1) {
-            u32x4 rp[3];
-            get_parts(rl, kk, rp);
-            d[kk] = mul(tp[kk], rp, d[kk]);
-          }
-        d[0] += d[1];
-        dl[w][lane] = d[0];
-        f32x4 e;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) e[r] = d[0][r] * row[r][3];
-        put_parts(el, e);
-        load_row(nx, row);
+          for (int kk = 0; kk < 2; ++kk)
+            if (kk <= w >> 1) {
+              u32x4 rp[3];
+              get_parts(rl[n], kk, rp);
+              d[kk] = mul(tp[kk], rp, d[kk]);
+            }
+          d[0] += d[1];
+          put_parts(el[n], d[0] * row[2]);
+          put_parts(dl[n], d[0]);
+        }
+        load_operand(nx, 0, tp);
+        row[2] = load_row(nx, 2);
         u32x4 kt[2][2][NP];   // K^T: this wave's rows (two tiles), depth tokens 32 kk + 4 (l / 16) .., + 16
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk)
@@ -565,113 +633,123 @@ __global__ __launch_bounds__(512, BF16 ? 4 : 2) void delta_scan_kernel(const Del
                     kl[c & 1] + p * kPart + key_at(32 * kk + 16 * q + kt0, kc0) + 8 * cc));
               kt[kk][cc][p] = un.v;
             }
-        lds_barrier();   // B: d is there
-        f32x4 sn[2];
+        lds_barrier();   // 3: d and the next keys are there, this chunk's have been read
 #pragma unroll
-        for (int q = 0; q < 8; ++q) sn[q >> 2][q & 3] = s[q] * dec;
+        for (int n = 0; n < NB; ++n) {
+          f32x4 sn[2];
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-          u32x4 ep[3];
-          get_parts(el, kk, ep);
+          for (int q = 0; q < 8; ++q) sn[q >> 2][q & 3] = s[n][q] * dec;
 #pragma unroll
-          for (int cc = 0; cc < 2; ++cc) sn[cc] = mul(kt[kk][cc], ep, sn[cc]);
+          for (int kk = 0; kk < 2; ++kk) {
+            u32x4 ep[3];
+            get_parts(el[n], kk, ep);
+#pragma unroll
+            for (int cc = 0; cc < 2; ++cc) sn[cc] = mul(kt[kk][cc], ep, sn[cc]);
+          }
+#pragma unroll
+          for (int q = 0; q < 8; ++q) s[n][q] = sn[q >> 2][q & 3];
         }
-#pragma unroll
-        for (int q = 0; q < 8; ++q) s[q] = sn[q >> 2][q & 3];
         if (++c >= nc || fd[0] != 0.0f) break;
-        put_s();
+        cut_s();
       }
       lds_barrier();   // every wave has read what it needs of the chunk
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) as_global_w(Sp)[(32 * w + 8 * g + e) * kD] = s[e];
-  } else {
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) as_global_w(Sp)[(32 * w + 8 * g + e) * kD + 16 * n] = s[n][e];
+  } else if (wave < 8) {   // outputs
     while (c < nc) {
-      if (as_global(ws(c))[kOffFlag] != 0.0f) {
+      if (flagged(c) != 0.0f) {
         lds_barrier();
         lds_barrier();
         ++c;
         continue;
       }
-      Raw8<BF16> kr[4], qr[4];
-      f32x4 tf[4], pf[4], row[4];
-      auto load_k = [&](int c) {
-        const int64_t at = token(c, 16 * w + j) * a.k.ld + hk * a.k.hs + 8 * g;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) kr[q] = raw8<BF16>(a.k.p, at + 32 * q);
-      };
+      u32x4 qp[4][NP], pp[2][3];
+      f32x4 row;
       auto load_q = [&](int c) {
-        const int64_t at = token(c, 16 * w + j) * a.q.ld + hk * a.q.hs + 8 * g;
+        const char* from = keys_at<NP>(a, seq, sp.start, c, hk) + NP * kPart + 4 * NP * 1024 * w;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) qr[q] = raw8<BF16>(a.q.p, at + 32 * q);
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+          for (int p = 0; p < NP; ++p) qp[q][p] = *as_global(reinterpret_cast<const u32x4*>(from + (q * NP + p) * 1024) + lane);
       };
-      auto put_k = [&](int c) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const Parts<BF16> kp = parts<BF16>(kr[q]);
-#pragma unroll
-          for (int p = 0; p < NP; ++p) *as_lds_w(reinterpret_cast<u32x4*>(kl[c & 1] + p * kPart + key_at(16 * w + j, 4 * q + g))) = kp.p[p];
-        }
-      };
-      auto put_t = [&]() {
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk)
-          if (kk <= w >> 1) {
-            u32x4 p[3];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int t = 2 * kk + (e >> 1);
-              const float x = t <= w ? tf[t][2 * (e & 1)] : 0.0f, y = t <= w ? tf[t][2 * (e & 1) + 1] : 0.0f;
-              uint32_t hi, mid, lo;
-              cut2(x, y, hi, mid, lo);
-              p[0][e] = hi, p[1][e] = mid, p[2][e] = lo;
-            }
-#pragma unroll
-            for (int q = 0; q < 3; ++q) tl[w + (w == 3) + kk][q][lane] = p[q];
-          }
-      };
-      load_k(c), load_tile(c, 0, tf);
-      load_q(c), load_tile(c, kOffP, pf), load_row(c, row);
-      f32x2 fd = load_flag(c);
-      put_k(c);
-      put_t();
-      load_k(min(c + 1, nc - 1)), load_tile(min(c + 1, nc - 1), 0, tf);
+      load_q(c);   // (in the loop's order)
+      row = load_row(c, 3);
+      load_operand(c, kOffP, pp);
+      float flag = flagged(c);
+      lds_barrier();   // 0
       for (;;) {
-        lds_barrier();   // C
-        const int nx = min(c + 1, nc - 1), n2 = min(c + 2, nc - 1);
-        fd = load_flag(nx);
-        f32x4 y[2] = {zero, zero}, o[2] = {zero, zero};
+        const int nx = min(c + 1, nc - 1);
+        flag = flagged(nx);
+        lds_barrier();   // 1: the state is there
+        f32x4 o[NB];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          if constexpr (BF16) {
-            u32x4 s3[3];
+        for (int n = 0; n < NB; ++n) {
+          f32x4 y[2] = {zero, zero};
 #pragma unroll
-            for (int p = 0; p < 3; ++p) s3[p] = sl[q][p][lane];
-            y[q & 1] = mul(qr[q].v, s3, y[q & 1]);
-          } else {
+          for (int q = 0; q < 4; ++q) {
+            u32x4 sp3[3];
 #pragma unroll
-            for (int e = 0; e < 2; ++e) y[e] = mfma4(__builtin_bit_cast(f32x4, qr[q].v[e]), sf[q][e][lane], y[e]);
+            for (int p = 0; p < 3; ++p) sp3[p] = sl[n][q][p][lane];
+            y[q & 1] = mul(qp[q], sp3, y[q & 1]);
           }
+          o[n] = (y[0] + y[1]) * row;
         }
         load_q(nx);
-        lds_barrier();   // A
-        put_k(c + 1);
-        load_k(n2);
-        lds_barrier();   // B: T has been read, d is there
-        put_t();
-        load_tile(n2, 0, tf);
+        row = load_row(nx, 3);
+        lds_barrier();   // 2
+        lds_barrier();   // 3: d is there, the state has been read
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
-          if (t <= w) o[t & 1] = mfma4(pf[t], dl[t][lane], o[t & 1]);
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+          for (int kk = 0; kk < 2; ++kk)
+            if (kk <= w >> 1) {
+              u32x4 dp[3];
+              get_parts(dl[n], kk, dp);
+              o[n] = mul(pp[kk], dp, o[n]);
+            }
+        load_operand(nx, kOffP, pp);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int t = kC * c + 16 * w + 4 * g + r;
-          const float v = (y[0][r] + y[1][r]) * row[r][2] + (o[0][r] + o[1][r]);
-          if (t < sp.len) store1<BF16>(a.out.p, (int64_t)(sp.start + t) * a.out.ld + h * a.out.hs + col, v);
+          if (t < sp.len)
+#pragma unroll
+            for (int n = 0; n < NB; ++n) store1<BF16>(a.out.p, (int64_t)(sp.start + t) * a.out.ld + h * a.out.hs + col + 16 * n, o[n][r]);
         }
-        load_tile(nx, kOffP, pf);
-        load_row(nx, row);
-        if (++c >= nc || fd[0] != 0.0f) break;
+        if (++c >= nc || flag != 0.0f) break;
+      }
+      lds_barrier();
+    }
+  } else {   // keys to LDS
+    const uint32_t k0 = lds_address(kl);
+    auto bring = [&](int c, int half) {
+      const char* from = keys_at<NP>(a, seq, sp.start, min(c, nc - 1), hk) + half * (NP * kPart / 2);
+      const uint32_t to = k0 + (c & 1) * (NP * kPart) + half * (NP * kPart / 2);
+#pragma unroll 4
+      for (int i = 0; i < 8 * NP; ++i) load_to_lds(from + 1024 * i, 16 * lane, to + 1024 * i);
+    };
+    while (c < nc) {
+      if (flagged(c) != 0.0f) {
+        lds_barrier();
+        lds_barrier();
+        ++c;
+        continue;
+      }
+      bring(c, 0);
+      bring(c, 1);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      lds_barrier();   // 0
+      for (;;) {
+        const float flag = flagged(min(c + 1, nc - 1));
+        bring(c + 1, 0);   // (where the chunk before this one stood: read before barrier 3)
+        lds_barrier();   // 1
+        bring(c + 1, 1);
+        lds_barrier();   // 2
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        lds_barrier();   // 3
+        if (++c >= nc || flag != 0.0f) break;
       }
       lds_barrier();
     }
@@ -684,16 +762,20 @@ hipError_t launch(const DeltaSeq& a, hipStream_t s) {
     delta_step_kernel<BF16><<<(unsigned)(((int64_t)a.n_seq * a.heads * 8 + 3) / 4), 256, 0, s>>>(a);
   } else {
     delta_chunk_kernel<BF16><<<dim3((unsigned)seq_tiles_max(a.tokens, a.n_seq, kC), a.k_heads), 256, 0, s>>>(a);
-    delta_scan_kernel<BF16><<<(unsigned)(((int64_t)a.n_seq * a.heads + 7) / 8 * 64), 512, 0, s>>>(a);
+    const int64_t heads8 = ((int64_t)a.n_seq * a.heads + 7) / 8 * 8;
+    if (BF16 && heads8 * 4 >= 512)
+      delta_scan_kernel<BF16, BF16 ? 2 : 1><<<(unsigned)(heads8 * 4), 576, 0, s>>>(a);
+    else
+      delta_scan_kernel<BF16, 1><<<(unsigned)(heads8 * 8), 576, 0, s>>>(a);
   }
   return hipGetLastError();
 }
 
 }  // namespace
 
-size_t delta_seq_workspace(int tokens, int n_seq, int heads, int max_len) {
+size_t delta_seq_workspace(int tokens, int n_seq, int heads, int k_heads, bool bf16, int max_len) {
   if (max_len <= kDeltaStepLen) return 0;
-  return ((size_t)tokens / kC + n_seq) * heads * kChunkFloats * sizeof(float);
+  return chunk_slots(tokens, n_seq) * ((size_t)heads * kChunkFloats * sizeof(float) + (size_t)k_heads * (bf16 ? 2 : 6) * kPart);
 }
 
 hipError_t launch_delta_seq(const DeltaSeq& a, hipStream_t s) { return a.bf16 ? launch<true>(a, s) : launch<false>(a, s); }

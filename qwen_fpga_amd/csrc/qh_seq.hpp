@@ -106,7 +106,7 @@ hipError_t launch_attn_seq(const AttnSeq& a, hipStream_t s);
 
 // Sequences of up to this many tokens run token by token.
 constexpr int kDeltaStepLen = 12;
-size_t delta_seq_workspace(int tokens, int n_seq, int heads, int max_len);
+size_t delta_seq_workspace(int tokens, int n_seq, int heads, int k_heads, bool bf16, int max_len);
 
 // Whether max_k keys are too few to split, and the bytes of workspace of a call.
 bool attn_seq_whole(int max_k);

@@ -37,6 +37,21 @@ __device__ __forceinline__ bool find_tile(const int32_t* cu, int n_seq, int rows
   return false;
 }
 
+// The sequence in place i when each 64 sequences stand with the longest first (the earlier of equal ones): the
+// workgroups that have most to do are then not the last to start.
+__device__ __forceinline__ int longest_first(const int32_t* cu, int n_seq, int rows, int i) {
+  const int lane = threadIdx.x & 63, s0 = i & ~63, n = min(n_seq - s0, 64);
+  int len = -1;
+  if (lane < n) len = seq_span(as_global(cu)[s0 + lane], as_global(cu)[s0 + lane + 1], rows).len;
+  int rank = 0;
+  for (int l = 0; l < n; ++l) {
+    const int o = __builtin_amdgcn_readlane(len, l);
+    rank += o > len || (o == len && l < lane);
+  }
+  const uint64_t at = __ballot(lane < n && rank == (i & 63));
+  return s0 + __builtin_ctzll(at);
+}
+
 // LDS by its 32-bit address.
 __device__ __forceinline__ uint32_t lds_address(const void* p) {
   return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)p;

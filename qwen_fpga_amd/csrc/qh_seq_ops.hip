@@ -86,10 +86,11 @@ int qh_gemm_i8_w8a8(void* y, int64_t ldy, int type, const int8_t* w, const float
   return hip_status(launch_gemm_seq(a, S(stream)));
 }
 
-size_t qh_delta_rule_seq_workspace(int tokens, int n_seq, int heads, int max_len) {
-  if (tokens <= 0 || n_seq <= 0 || heads <= 0 || (int64_t)n_seq * heads * 8 > kMaxUnits || (int64_t)tokens * heads > kMaxUnits)
+size_t qh_delta_rule_seq_workspace(int tokens, int n_seq, int heads, int k_heads, int type, int max_len) {
+  if (tokens <= 0 || n_seq <= 0 || heads <= 0 || k_heads <= 0 || !type_ok(type) || (int64_t)n_seq * heads * 8 > kMaxUnits ||
+      (int64_t)tokens * heads > kMaxUnits)
     return 0;
-  return delta_seq_workspace(tokens, n_seq, heads, max_len);
+  return delta_seq_workspace(tokens, n_seq, heads, k_heads, type == QH_BF16, max_len);
 }
 
 int qh_delta_rule_seq(void* out, int64_t ldo, int64_t hso, const void* q, int64_t ldq, int64_t hsq, const void* k, int64_t ldk,
@@ -109,7 +110,7 @@ int qh_delta_rule_seq(void* out, int64_t ldo, int64_t hso, const void* q, int64_
   const View vg{g, tokens, 1, heads, ldg, 0, 4}, vb{beta, tokens, 1, heads, ldb, 0, 4},
       vs = flat(state, (int64_t)n_seq * heads * QH_LK * QH_LV, 4), vc = flat(cu, n_seq + 1, 4);
   if (overlap_any(vo, vq, vk, vv, vg, vb, vs, vc) || overlap_any(vs, vq, vk, vv, vg, vb, vc)) return QH_EINVAL;
-  const size_t need = qh_delta_rule_seq_workspace(tokens, n_seq, heads, max_len);
+  const size_t need = qh_delta_rule_seq_workspace(tokens, n_seq, heads, k_heads, type, max_len);
   if (need > 0) {
     if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255)) return QH_EINVAL;
     const View vw = flat(workspace, need, 1);
