@@ -774,7 +774,7 @@ hipError_t launch(const DeltaSeq& a, hipStream_t s) {
 }  // namespace
 
 size_t delta_seq_workspace(int tokens, int n_seq, int heads, int k_heads, bool bf16, int max_len) {
-  if (max_len <= kDeltaStepLen) return 0;
+  if (max_len <= delta_step_len((int64_t)n_seq * heads)) return 0;
   return chunk_slots(tokens, n_seq) * ((size_t)heads * kChunkFloats * sizeof(float) + (size_t)k_heads * (bf16 ? 2 : 6) * kPart);
 }
 

@@ -104,8 +104,11 @@ hipError_t launch_gemm_seq(const GemmSeq& a, hipStream_t s);
 hipError_t launch_delta_seq(const DeltaSeq& a, hipStream_t s);
 hipError_t launch_attn_seq(const AttnSeq& a, hipStream_t s);
 
-// Sequences of up to this many tokens run token by token.
-constexpr int kDeltaStepLen = 12;
+// Sequences of up to this many tokens run token by token, which costs about 0.65 us a token for few heads (sequences
+// times heads) and less for many, where chunks cost a launch more and a whole workgroup's start a sequence.  us for
+// 24 / 48 tokens: 16 heads fp32 18.2 / 33.3 token by token, 19.3 / 20.2 in chunks, bfloat16 18.6 / 33.9 and 15.6 / 15.9;
+// 512 heads fp32 41 / 72 and 135 / 139, bfloat16 42 / 75 and 74 / 77.
+inline int delta_step_len(int64_t heads) { return heads < 256 ? 24 : 48; }
 size_t delta_seq_workspace(int tokens, int n_seq, int heads, int k_heads, bool bf16, int max_len);
 
 // Whether max_k keys are too few to split, and the bytes of workspace of a call.

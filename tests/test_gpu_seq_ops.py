@@ -151,6 +151,8 @@ def delta_check(torch, out, S, want, lens, bf16):
 
 DELTA = [  # lens, key heads, heads
     ([1], 16, 16), ([1, 1, 1], 2, 2), ([1, 0, 2, 1, 4], 2, 4), ([0, 5], 1, 1), ([15, 16, 17], 1, 2), ([31, 33, 32], 2, 2),
+    ([70, 1, 0, 130, 64, 5, 66, 20], 8, 16),            # enough heads for two column tiles a workgroup
+    ([3, 60, 0] * 22 + [1, 65, 2, 129], 1, 2),          # more sequences than a wave has lanes
     ([63], 1, 1), ([64], 1, 3), ([65], 1, 1), ([127, 128, 129], 1, 1), ([200, 1, 0, 70], 1, 2), ([333], 2, 2), ([700], 1, 1),
 ]
 
