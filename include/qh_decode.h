@@ -264,7 +264,8 @@ int qh_delta_rule_seq(void* out, int64_t ldo, int64_t hso, const void* q, int64_
  * out = softmax(scale q k^T) v over those; 0 for a row that sees none; NaN for the rows of a sequence whose keys
  * do not lie inside the array.  Keys a row does not see have no influence on it, whatever they hold.
  * Query head h takes kv head h / (heads / kv_heads). */
-size_t qh_attention_seq_workspace(int q_rows, int n_seq, int max_q, int max_k, int heads, int kv_heads, int head_dim);
+size_t qh_attention_seq_workspace(int q_rows, int n_seq, int max_q, int max_k, int heads, int kv_heads, int head_dim,
+                                  int type);
 int qh_attention_seq(void* out, int64_t ldo, int64_t hso, const void* q, int64_t ldq, int64_t hsq, const void* k, int64_t ldk,
                      int64_t hsk, const void* v, int64_t ldv, int64_t hsv, int type, const int32_t* cu_q,
                      const int64_t* k_start, const int32_t* k_len, int n_seq, int q_rows, int64_t k_rows, int max_q, int max_k,

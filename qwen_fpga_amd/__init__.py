@@ -619,11 +619,13 @@ def delta_rule_seq(out, q, k, v, g, beta, S, cu, workspace, max_len: int, stream
         _check(st, "qh_delta_rule_seq")
 
 
-def attention_seq_workspace(q_rows: int, n_seq: int, max_q: int, max_k: int, heads: int, kv_heads: int, head_dim: int) -> int:
-    """Bytes of device scratch attention_seq takes from its caller."""
+def attention_seq_workspace(q_rows: int, n_seq: int, max_q: int, max_k: int, heads: int, kv_heads: int, head_dim: int,
+                            dtype: Optional[int] = None) -> int:
+    """Bytes of device scratch attention_seq takes from its caller (dtype F32 or BF16; None: enough for both)."""
     f = _lib().qh_attention_seq_workspace
     f.restype = ctypes.c_size_t
-    return int(f(int(q_rows), int(n_seq), int(max_q), int(max_k), int(heads), int(kv_heads), int(head_dim)))
+    n = (int(q_rows), int(n_seq), int(max_q), int(max_k), int(heads), int(kv_heads), int(head_dim))
+    return max(int(f(*n, t)) for t in ((F32, BF16) if dtype is None else (int(dtype),)))
 
 
 def attention_seq(out, q, k, v, cu_q, k_start, k_len, workspace, max_q: int, max_k: int, scale: Optional[float] = None,

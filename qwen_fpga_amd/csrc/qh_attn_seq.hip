@@ -1,5 +1,6 @@
 // Causal attention with grouped heads over packed sequences.  Row r of a sequence with q_len rows and k_len
 // keys sees the first r + 1 + k_len - q_len keys:  out = softmax(scale q K^T) V  over those; 0 without any.
+#include <algorithm>
 #include <type_traits>
 
 #include "qh_seq_device.hpp"
@@ -16,18 +17,6 @@ namespace {
 
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kNegInf = -__builtin_inff();
-
-// find_tile, and the sequence's keys.
-struct KeyTileAt : TileAt {
-  int64_t ks;
-  int kl;
-};
-__device__ __forceinline__ bool find_key_tile(const AttnSeq& a, int mult, int tile, int b, KeyTileAt& o) {
-  if (!find_tile(a.cu_q, a.n_seq, a.q_rows, mult, tile, b, o)) return false;
-  o.ks = as_global(a.k_start)[o.seq];
-  o.kl = key_len(o.ks, as_global(a.k_len)[o.seq], a.k_rows);
-  return true;
-}
 
 // The work of the split form.  A unit is 16 rows of a sequence (tokens x query heads of one kv head) and one chunk
 // of its keys; chunks hold the same number of keys in every sequence, chosen from all sequences' keys (which only
@@ -57,7 +46,7 @@ __device__ __forceinline__ bool find_unit(const AttnSeq& a, int b, Unit& o) {
     tiles = s0 + lane < a.n_seq ? seq_tiles(sp.len * G, 16) : 0;
   };
   load(0);
-  if (!a.whole) {
+  if (a.limit > 0) {
     int64_t work = (int64_t)tiles * max(kl, 0);   // keys of all row tiles
     for (int s0 = 64; s0 < a.n_seq; s0 += 64) {
       load(s0);
@@ -431,18 +420,117 @@ __global__ __launch_bounds__(1024) void attn_join_kernel(const AttnSeq a) {
   }
 }
 
+// The work of the form for prompts.  A tile is `tile` rows of a sequence (tokens x query heads of one kv head) over all
+// the keys they see.  Tiles that see more than `chunk` keys are big: their keys are split into units of a chunk, whose
+// sums meet in the workspace; the others are a unit each.  The chunk is about the keys of all tiles over the CUs (but
+// at least kMinTileChunk, and a 64th of the sequence), so that no unit is much longer than a CU's share.  Units start in
+// order, unit b on XCD b % 8: so the longest come first, and neighbours are about equally long.  The workgroups of an
+// XCD then walk the keys of one head side by side and find them in its L2: shares cut to the same length anywhere in
+// the tiles missed it for 38% of the reads and took 450 us, not 390, for 16k packed tokens (8 / 2 heads of 256).
+// Split and whole: one sequence of 8000 tokens 280 and 360 us, 4096 122 and 170, 1024 43 and 56, 512 36 and 36; two of
+// 8000 500 and 515; a mix of lengths that fills the chip by itself 390 and 380.
+constexpr int kTileFill = 224, kMinTileChunk = 256, kMaxTileSplits = 64;
+struct TileUnit {
+  SeqSpan sp;
+  int64_t ks;
+  int kl, tile, split, nsplit, chunk;
+  int slot;   // of the unit (JOIN: of the tile's first) among the big tiles' units
+};
+// Unit b, or (JOIN) big tile b.
+template <bool JOIN>
+__device__ __forceinline__ bool find_tile_unit(const AttnSeq& a, int tile, int b, TileUnit& o) {
+  const int lane = threadIdx.x & 63, G = a.heads / a.kv_heads;
+  SeqSpan sp;   // of sequence s0 + lane, as of its keys and tiles
+  int64_t ks;
+  int kl, nt;
+  auto load = [&](int s0) {
+    const int i = min(s0 + lane, a.n_seq - 1);
+    ks = as_global(a.k_start)[i];
+    const int n = as_global(a.k_len)[i];
+    sp = seq_span(as_global(a.cu_q)[i], as_global(a.cu_q)[i + 1], a.q_rows);
+    kl = key_len(ks, n, a.k_rows);
+    nt = s0 + lane < a.n_seq ? seq_tiles(sp.len * G, tile) : 0;
+  };
+  auto work = [&]() -> int64_t {   // keys that the sequence's tiles see, about
+    const int64_t k = max(kl, 0), past = max(k - sp.len, (int64_t)0);
+    return nt * past + (nt + 1) * min(k, (int64_t)sp.len) / 2;
+  };
+  load(0);
+  int64_t all = nt > 0 ? work() : 0;
+  for (int s0 = 64; s0 < a.n_seq; s0 += 64) {
+    load(s0);
+    all += nt > 0 ? work() : 0;
+  }
+  if (a.n_seq > 64) load(0);
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) all += __shfl_xor(all, d);
+  const int64_t share = max((all * a.kv_heads + kTileFill - 1) / kTileFill, (int64_t)kMinTileChunk);
+  int base = 0, slots = 0;   // of the next 64 sequences: units (JOIN: big tiles), the big tiles' units
+  for (int s0 = 0; s0 < a.n_seq; s0 += 64) {
+    if (s0 > 0) load(s0);
+    // the longest first: place `rank` is this lane's sequence's
+    const int n = min(a.n_seq - s0, 64), len = nt > 0 ? max(kl, 0) : -1;
+    int rank = 0;
+    for (int l = 0; l < n; ++l) {
+      const int other = __builtin_amdgcn_readlane(len, l);
+      rank += other > len || (other == len && l < lane);
+    }
+    const int64_t c64 = (max(share, (int64_t)(max(kl, 0) / kMaxTileSplits + 1)) + 31) / 32 * 32;
+    const int chunk = a.limit > 0 ? (int)min(c64, (int64_t)kMaxKeys) : kMaxKeys;
+    // the first big tile: the first whose last row sees more than a chunk
+    const int64_t tok = (int64_t)chunk - kl + sp.len;   // (the first such row's token)
+    int big = 0;
+    if (nt > 0 && kl > 0 && sp.len - 1 >= tok) big = nt - (int)min(max((tok * G + tile) / tile - 1, (int64_t)0), (int64_t)nt - 1);
+    const int ns = big > 0 ? seq_tiles(kl, chunk) : 1;
+    for (int r = 0; r < n; ++r) {
+      const int l = __builtin_ctzll(__ballot(rank == r && lane < n));
+      auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
+      int nb = of(big), nsp = of(ns);
+      if ((slots + (int64_t)nb * nsp) * a.kv_heads > a.limit) nb = 0, nsp = 1;   // no place in the workspace: not split
+      const int t = of(nt), m = JOIN ? nb : nb * nsp + t - nb;
+      if (b < base + m) {
+        int in = b - base;
+        o.sp = {of(sp.start), of(sp.len)};
+        o.ks = (int64_t)((uint64_t)(uint32_t)of((int)(ks >> 32)) << 32 | (uint32_t)of((int)ks));
+        o.kl = of(kl);
+        o.chunk = of(chunk);
+        const int rest = t - nb, first = JOIN ? nb : nb * (nsp - 1);   // units ahead of the tiles that are not split
+        o.split = o.nsplit = 1;
+        if (in >= first && in < first + rest && !JOIN) {
+          o.tile = rest - 1 - (in - first);
+          o.split = 0;
+          o.chunk = kMaxKeys;
+        } else {
+          if (in >= first) in -= rest;
+          o.tile = t - 1 - in % nb;
+          o.split = in / nb;
+          o.nsplit = nsp;
+          o.slot = slots + in % nb * nsp + o.split;
+        }
+        return o.tile >= 0 && o.tile < t;
+      }
+      base += m;
+      slots += nb * nsp;
+    }
+  }
+  return false;
+}
+constexpr size_t tile_part_floats(int tile, int D) { return (size_t)tile * (D + 2); }
+
 // Prompts, bfloat16: a workgroup takes 256 rows (tokens x query heads of one kv head) over all the keys they see.
 // As in the split form the products are S^T = K Q^T and O^T = V^T P^T, and P never leaves the registers.  K and V
 // come 32 keys at a time through a ring of LDS stages that global -> LDS loads fill three ahead.  16-byte chunk c of
 // key r stands at chunk c ^ (r % 16) of K's rows (32 keys of one chunk lie in all banks) and c ^ 4 (r % 4) of V's
 // (four keys of 32 elements do, as the transposing read takes them).  The running maximum moves only when a score
-// passes it by more than 8 (a factor of 256, exact in the sums), so that the sums are rarely rescaled.
+// passes it by more than 8 (a factor of 256, exact in the sums), so that the sums are rarely rescaled.  At full load the
+// card's power bounds it (1.85 GHz): 930 to 1050 TFLOP/s at 256 elements and long prompts, 840 at 128.  A wave holds 32
+// rows: with 64, 128 elements took 302 us for 8000 tokens of 8 heads, and 32 rows take 189.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 
 template <int D>
-__global__ __launch_bounds__(2 * D, 2) void attn_tile_kernel(const AttnSeq a) {
-  constexpr int NW = D / 32, RB = 256 / D;  // waves; blocks of 32 rows of a wave
+__global__ __launch_bounds__(512, 2) void attn_tile_kernel(const AttnSeq a) {
+  constexpr int NW = 8;                     // waves, of 32 rows each
   constexpr int kKeys = 32, kRing = 4, CH = D / 8, kHalf = kKeys * D * 2, kStage = 2 * kHalf;
   constexpr int NI = kHalf / (1024 * NW);   // loads of a wave for K's part of a stage (and for V's)
   constexpr int NS = D / 16, NT = D / 32;
@@ -451,30 +539,28 @@ __global__ __launch_bounds__(2 * D, 2) void attn_tile_kernel(const AttnSeq a) {
   const int h = lane >> 5, j = lane & 31;
   const int G = a.heads / a.kv_heads;
   const int kvh = (int)blockIdx.x % a.kv_heads;
-  KeyTileAt at;   // the last tiles, which see the most keys, first
-  if (!find_key_tile(a, G, 256, ((int)gridDim.x - 1 - (int)blockIdx.x) / a.kv_heads, at)) return;
-  const int rows = at.sp.len * G, r0 = 256 * at.tile, w0 = r0 + 32 * RB * wave;
-  auto sees = [&](int row) { return keys_seen(min(row, rows - 1) / G, at.sp.len, at.kl); };
-  const int end = sees(r0 + 255), wend = w0 < rows ? sees(w0 + 32 * RB - 1) : 0;
-  int seen[RB];
-  u32x4 qf[RB][NS];
+  TileUnit at;
+  if (!find_tile_unit<false>(a, 256, (int)blockIdx.x / a.kv_heads, at)) return;
+  const int rows = at.sp.len * G, r0 = 256 * at.tile, w0 = r0 + 32 * wave;
+  const int k0 = at.nsplit > 1 ? at.split * at.chunk : 0;   // keys are counted from here
+  auto sees = [&](int row) { return keys_seen(min(row, rows - 1) / G, at.sp.len, at.kl) - k0; };
+  const int end = min(sees(r0 + 255), at.chunk), wend = w0 < rows ? min(sees(w0 + 31), end) : 0;
+  if (at.split > 0 && end <= 0) return;   // (a unit of no key that the tile sees)
+  u32x4 qf[NS];
   const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;   // (-q) k |scale|: a maximum stays one
   const float sc = fabsf(a.scale) * kLog2e;
+  const int row = min(w0 + j, rows - 1), tok = row / G, hq = kvh * G + row % G;
+  const int seen = sees(row);
+  const char* qp = static_cast<const char*>(a.q.p) + ((at.sp.start + tok) * a.q.ld + hq * a.q.hs) * 2 + 16 * h;
 #pragma unroll
-  for (int b = 0; b < RB; ++b) {
-    const int row = min(w0 + 32 * b + j, rows - 1), tok = row / G, hq = kvh * G + row % G;
-    seen[b] = keys_seen(tok, at.sp.len, at.kl);
-    const char* qp = static_cast<const char*>(a.q.p) + ((at.sp.start + tok) * a.q.ld + hq * a.q.hs) * 2 + 16 * h;
+  for (int s = 0; s < NS; ++s) {
+    qf[s] = *as_global(reinterpret_cast<const u32x4*>(qp + 32 * s));
 #pragma unroll
-    for (int s = 0; s < NS; ++s) {
-      qf[b][s] = *as_global(reinterpret_cast<const u32x4*>(qp + 32 * s));
-#pragma unroll
-      for (int e = 0; e < 4; ++e) qf[b][s][e] ^= flip;
-    }
+    for (int e = 0; e < 4; ++e) qf[s][e] ^= flip;
   }
   // a wave's loads: LDS places 64 (NI wave + i) + lane of a stage's K (V) rows
-  const char* kp = static_cast<const char*>(a.k.p) + (at.ks * a.k.ld + kvh * a.k.hs) * 2;
-  const char* vp = static_cast<const char*>(a.v.p) + (at.ks * a.v.ld + kvh * a.v.hs) * 2;
+  const char* kp = static_cast<const char*>(a.k.p) + ((at.ks + k0) * a.k.ld + kvh * a.k.hs) * 2;
+  const char* vp = static_cast<const char*>(a.v.p) + ((at.ks + k0) * a.v.ld + kvh * a.v.hs) * 2;
   const uint32_t kld = (uint32_t)a.k.ld * 2, vld = (uint32_t)a.v.ld * 2;   // (below 2^25: the launch's rule)
   auto k_off = [&](int i, int last) {   // last: the last row of the stage that is there
     const int place = 64 * (NI * wave + i) + lane, r = place / CH;
@@ -503,14 +589,10 @@ __global__ __launch_bounds__(2 * D, 2) void attn_tile_kernel(const AttnSeq a) {
       for (int i = 0; i < NI; ++i) put(it, i, k_off(i, last), v_off(i, last));
     }
   };
-  f32x16 acc[RB][NT];
+  f32x16 acc[NT];
 #pragma unroll
-  for (int b = 0; b < RB; ++b)
-#pragma unroll
-    for (int t = 0; t < NT; ++t) acc[b][t] = f32x16{};
-  float m[RB], l[RB];
-#pragma unroll
-  for (int b = 0; b < RB; ++b) m[b] = kNegInf, l[b] = 0.0f;
+  for (int t = 0; t < NT; ++t) acc[t] = f32x16{};
+  float m = kNegInf, l = 0.0f;
   const int n = seq_tiles(end, kKeys);
 #pragma unroll
   for (int i = 0; i < kRing - 1; ++i)
@@ -537,75 +619,58 @@ __global__ __launch_bounds__(2 * D, 2) void attn_tile_kernel(const AttnSeq a) {
     // (opaque, so that the places are formed where they are used: held over the loop they would not fit the registers)
     uint32_t kl = kl0 + (it & (kRing - 1)) * kStage, vl = vl0 + (it & (kRing - 1)) * kStage;
     asm volatile("" : "+v"(kl), "+v"(vl));
-    f32x16 st[RB];
-#pragma unroll
-    for (int b = 0; b < RB; ++b) st[b] = f32x16{};
+    f32x16 st = {};
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
       const u32x4 kf = *lds_at<u32x4>((kl ^ (32 * (s & 7))) + 256 * (s >> 3));
-#pragma unroll
-      for (int b = 0; b < RB; ++b)
-        st[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, kf), __builtin_bit_cast(bf16x8, qf[b][s]), st[b], 0, 0, 0);
+      st = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, kf), __builtin_bit_cast(bf16x8, qf[s]), st, 0, 0, 0);
     }
     if constexpr (!part) {
       __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
 #pragma unroll
       for (int i = 0; i < NS - 3; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x8, RB, 0);
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
         __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
       }
-      __builtin_amdgcn_sched_group_barrier(0x8, 3 * RB, 0);
+      __builtin_amdgcn_sched_group_barrier(0x8, 3, 0);
     }
     if constexpr (part) {
 #pragma unroll
-      for (int b = 0; b < RB; ++b)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (kb + 8 * (r >> 2) + 4 * h + (r & 3) >= seen[b]) st[b][r] = kNegInf;
+      for (int r = 0; r < 16; ++r)
+        if (kb + 8 * (r >> 2) + 4 * h + (r & 3) >= seen) st[r] = kNegInf;
     }
-    float mt[RB];
-    bool up[RB], any = false;
+    float x = st[0];
 #pragma unroll
-    for (int b = 0; b < RB; ++b) {
-      float x = st[b][0];
+    for (int r = 1; r < 16; ++r) x = fmaxf(x, st[r]);
+    x = fmaxf(x, xor_perm<32>(x));
+    const float mt = x == kNegInf ? kNegInf : x * sc;   // (0 times it is not it)
+    const bool up = mt > m + 8.0f;
+    if (__ballot(up) != 0) {
+      // (a row's own scores decide, so that other rows have no influence on it)
+      const float mn = up ? mt : m, al = __builtin_amdgcn_exp2f(m - (mn == kNegInf ? 0.0f : mn));
+      m = mn;
+      l *= al;
 #pragma unroll
-      for (int r = 1; r < 16; ++r) x = fmaxf(x, st[b][r]);
-      x = fmaxf(x, xor_perm<32>(x));
-      mt[b] = x == kNegInf ? kNegInf : x * sc;   // (0 times it is not it)
-      up[b] = mt[b] > m[b] + 8.0f;
-      any |= up[b];
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[t][r] *= al;
     }
-    if (__ballot(any) != 0) {
+    u32x4 pf[2];
+    const float mu = m == kNegInf ? 0.0f : m;
+    float ps = 0.0f;
 #pragma unroll
-      for (int b = 0; b < RB; ++b) {   // (a row's own scores decide, so that other rows have no influence on it)
-        const float mn = up[b] ? mt[b] : m[b], al = __builtin_amdgcn_exp2f(m[b] - (mn == kNegInf ? 0.0f : mn));
-        m[b] = mn;
-        l[b] *= al;
+    for (int r = 0; r < 16; r += 2) {
+      float p[2];
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) acc[b][t][r] *= al;
+      for (int e = 0; e < 2; ++e) {
+        p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[r + e], sc, -mu));
+        if constexpr (part) p[e] = st[r + e] == kNegInf ? 0.0f : p[e];   // (a scale of 0)
+        ps += p[e];
       }
+      const bf16x2 pk = {(__bf16)p[0], (__bf16)p[1]};
+      pf[r >> 3][(r >> 1) & 3] = __builtin_bit_cast(uint32_t, pk);
     }
-    u32x4 pf[RB][2];
-#pragma unroll
-    for (int b = 0; b < RB; ++b) {
-      const float mu = m[b] == kNegInf ? 0.0f : m[b];
-      float ps = 0.0f;
-#pragma unroll
-      for (int r = 0; r < 16; r += 2) {
-        float p[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[b][r + e], sc, -mu));
-          if constexpr (part) p[e] = st[b][r + e] == kNegInf ? 0.0f : p[e];   // (a scale of 0)
-          ps += p[e];
-        }
-        const bf16x2 pk = {(__bf16)p[0], (__bf16)p[1]};
-        pf[b][r >> 3][(r >> 1) & 3] = __builtin_bit_cast(uint32_t, pk);
-      }
-      l[b] += ps;
-    }
+    l += ps;
     bool bad = false;
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -621,39 +686,34 @@ __global__ __launch_bounds__(2 * D, 2) void attn_tile_kernel(const AttnSeq a) {
           u.h[q] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_at<i16x4>(p + 8 * q * D * 2));
         // (see attn_split_kernel: what is not finite in V goes only to the rows that see it)
         if constexpr (part) bad |= zero_non_finite<true>(u.v);
-#pragma unroll
-        for (int b = 0; b < RB; ++b)
-          acc[b][t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, u.v), __builtin_bit_cast(bf16x8, pf[b][kk]),
-                                                              acc[b][t], 0, 0, 0);
+        acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, u.v), __builtin_bit_cast(bf16x8, pf[kk]),
+                                                         acc[t], 0, 0, 0);
       }
     if constexpr (!part) {   // fragments on their way ahead of the product they are for
       __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
 #pragma unroll
       for (int i = 0; i < 2 * NT - 2; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x8, RB, 0);
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
         __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
       }
-      __builtin_amdgcn_sched_group_barrier(0x8, 2 * RB, 0);
+      __builtin_amdgcn_sched_group_barrier(0x8, 2, 0);
     }
     if constexpr (part) {
       if (__ballot(bad) != 0) {
         for (int key = kb; key < min(kb + kKeys, end); ++key) {
-          const __bf16* q = static_cast<const __bf16*>(a.v.p) + (at.ks + key) * a.v.ld + kvh * a.v.hs + 4 * h;
+          const __bf16* q = static_cast<const __bf16*>(a.v.p) + (at.ks + k0 + key) * a.v.ld + kvh * a.v.hs + 4 * h;
 #pragma unroll
           for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
               const float e = (float)as_global(q)[32 * t + 8 * (r >> 2) + (r & 3)];
-              if (non_finite(e))
-#pragma unroll
-                for (int b = 0; b < RB; ++b)
-                  if (key < seen[b]) acc[b][t][r] += e;
+              if (non_finite(e) && key < seen) acc[t][r] += e;
             }
         }
       }
     }
   };
-  const int full = sees(r0) / kKeys;   // steps that every row sees whole
+  const int full = max(min(sees(r0), end), 0) / kKeys;   // steps that every row sees whole
   int it = 0;
   for (; it < full; ++it) {
     wait(it);
@@ -663,46 +723,117 @@ __global__ __launch_bounds__(2 * D, 2) void attn_tile_kernel(const AttnSeq a) {
     wait(it);
     if (kKeys * it < wend) step(it, std::true_type{});
   }
-#pragma unroll
-  for (int b = 0; b < RB; ++b) {
-    l[b] = l[b] + xor_perm<32>(l[b]);
-    const int row = w0 + 32 * b + j, tok = row / G, hq = kvh * G + row % G;
-    if (row >= rows) continue;
-    const float inv = at.kl < 0 ? __builtin_nanf("") : seen[b] == 0 ? 0.0f : 1.0f / l[b];
-    char* op = static_cast<char*>(a.out.p) + ((at.sp.start + tok) * a.out.ld + hq * a.out.hs) * 2;
+  l = l + xor_perm<32>(l);
+  if (w0 + j >= rows) return;
+  if (at.nsplit > 1) {
+    float* pp = a.part + ((size_t)at.slot * a.kv_heads + kvh) * tile_part_floats(256, D);
+    const int rr = row - r0;
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int r = 0; r < 16; r += 4) {
-        const bf16x4 o = {(__bf16)(acc[b][t][r] * inv), (__bf16)(acc[b][t][r + 1] * inv), (__bf16)(acc[b][t][r + 2] * inv),
-                          (__bf16)(acc[b][t][r + 3] * inv)};
-        *as_global_w(reinterpret_cast<bf16x4*>(op + (32 * t + 2 * r + 4 * h) * 2)) = o;
+      for (int r = 0; r < 16; r += 4)
+        *as_global_w(reinterpret_cast<f32x4*>(pp + rr * D + 32 * t + 2 * r + 4 * h)) =
+            f32x4{acc[t][r], acc[t][r + 1], acc[t][r + 2], acc[t][r + 3]};
+    if (h == 0) pp[256 * D + rr] = m, pp[256 * D + 256 + rr] = l;
+    return;
+  }
+  const float inv = at.kl < 0 ? __builtin_nanf("") : seen <= 0 ? 0.0f : 1.0f / l;
+  char* op = static_cast<char*>(a.out.p) + ((at.sp.start + tok) * a.out.ld + hq * a.out.hs) * 2;
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const bf16x4 o = {(__bf16)(acc[t][r] * inv), (__bf16)(acc[t][r + 1] * inv), (__bf16)(acc[t][r + 2] * inv),
+                        (__bf16)(acc[t][r + 3] * inv)};
+      *as_global_w(reinterpret_cast<bf16x4*>(op + (32 * t + 2 * r + 4 * h) * 2)) = o;
+    }
+}
+
+// Joins the units of a big tile: a wave takes a row, four units in flight.
+template <bool BF16, int D>
+__global__ __launch_bounds__(256) void attn_tile_join_kernel(const AttnSeq a, int tile) {
+  constexpr int W = D / 64, U = 4;   // elements of a lane; units in flight
+  typedef float vec __attribute__((ext_vector_type(W)));
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int G = a.heads / a.kv_heads;
+  const int kvh = (int)blockIdx.x % a.kv_heads;
+  TileUnit at;
+  if (!find_tile_unit<true>(a, tile, (int)blockIdx.x / a.kv_heads, at)) return;
+  const int rows = min(at.sp.len * G - tile * at.tile, tile);
+  const size_t step = tile_part_floats(tile, D) * a.kv_heads;
+  const float* pp = a.part + ((size_t)at.slot * a.kv_heads + kvh) * tile_part_floats(tile, D);
+  for (int j = 4 * blockIdx.y + wave; j < rows; j += 4 * gridDim.y) {
+    const int row = tile * at.tile + j, tok = row / G, hq = kvh * G + row % G;
+    const int ns = min(seq_tiles(keys_seen(tok, at.sp.len, at.kl), at.chunk), at.nsplit);   // units that this row sees
+    float m = kNegInf, l = 0.0f;
+    vec acc = {};
+    for (int s0 = 0; s0 < ns; s0 += U) {
+      float mv[U], lv[U], mn = m;
+      vec av[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float* p = pp + min(s0 + u, ns - 1) * step;
+        mv[u] = s0 + u < ns ? as_global(p)[tile * D + j] : kNegInf;
+        lv[u] = as_global(p)[tile * D + tile + j];
+        av[u] = *as_global(reinterpret_cast<const vec*>(p + j * D) + lane);
       }
+#pragma unroll
+      for (int u = 0; u < U; ++u) mn = fmaxf(mn, mv[u]);
+      const float mu = mn == kNegInf ? 0.0f : mn, al = __builtin_amdgcn_exp2f(m - mu);
+      m = mn;
+      l *= al;
+      acc *= al;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float e = __builtin_amdgcn_exp2f(mv[u] - mu);
+        if (s0 + u < ns) l += e * lv[u], acc += e * av[u];
+      }
+    }
+    acc *= ns == 0 ? 0.0f : 1.0f / l;
+    const int64_t to = (at.sp.start + tok) * a.out.ld + hq * a.out.hs + W * lane;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      if constexpr (BF16)
+        as_global_w(static_cast<__bf16*>(a.out.p))[to + w] = (__bf16)acc[w];
+      else
+        as_global_w(static_cast<float*>(a.out.p))[to + w] = acc[w];
+    }
   }
 }
 
 template <bool BF16, int D>
 hipError_t launch(const AttnSeq& a, hipStream_t s) {
-  if constexpr (BF16)
-    if (a.tile) {
-      const int64_t t = seq_tiles_max((int64_t)a.q_rows * (a.heads / a.kv_heads), a.n_seq, 256) * a.kv_heads;
-      attn_tile_kernel<D><<<(unsigned)t, 2 * D, 0, s>>>(a);
-      return hipGetLastError();
-    }
+  if (a.tile > 0) {
+    const int64_t t = seq_tiles_max((int64_t)a.q_rows * (a.heads / a.kv_heads), a.n_seq, a.tile) * a.kv_heads;
+    attn_tile_kernel<D><<<(unsigned)(t + a.limit), 512, 0, s>>>(a);
+    if (a.limit > 0) attn_tile_join_kernel<BF16, D><<<dim3((unsigned)min(t, (int64_t)a.limit / 2), 16), 256, 0, s>>>(a, a.tile);
+    return hipGetLastError();
+  }
   const unsigned tiles = (unsigned)(seq_tiles_max((int64_t)a.q_rows * (a.heads / a.kv_heads), a.n_seq, 16) * a.kv_heads);
-  attn_split_kernel<BF16, D><<<a.whole ? tiles : tiles + kFill, 256, 0, s>>>(a);
-  if (!a.whole) attn_join_kernel<BF16, D><<<dim3(tiles, 4), 1024, 0, s>>>(a);
+  attn_split_kernel<BF16, D><<<a.limit > 0 ? tiles + kFill : tiles, 256, 0, s>>>(a);
+  if (a.limit > 0) attn_join_kernel<BF16, D><<<dim3(tiles, 4), 1024, 0, s>>>(a);
   return hipGetLastError();
 }
 
 }  // namespace
 
-bool attn_seq_whole(int max_k) { return max_k <= kMinChunk; }
-
-size_t attn_seq_workspace(int64_t q_rows, int n_seq, int max_k, int heads, int kv_heads, int dim) {
-  if (attn_seq_whole(max_k)) return 0;
-  const int64_t tiles = seq_tiles_max(q_rows * (heads / kv_heads), n_seq, 16) * kv_heads;
-  return (size_t)(tiles + kFill) * part_floats(dim) * sizeof(float);
+AttnForm attn_seq_form(int64_t q_rows, int n_seq, int max_q, int max_k, int heads, int kv_heads, int dim, bool bf16) {
+  const int G = heads / kv_heads;
+  AttnForm f = {0, 0, 0};
+  if ((int64_t)max_q * G >= 128 && bf16) {
+    f.tile = 256;
+    const int64_t tiles = seq_tiles_max(q_rows * G, n_seq, f.tile) * kv_heads;
+    // two workspace places a CU: the chunks are such that more are hardly ever taken
+    if (max_k > kMinTileChunk) {
+      const int64_t splits = max_k / kMinTileChunk + 1;
+      f.limit = (int)std::min<int64_t>(2 * kTileFill, tiles * std::min<int64_t>(splits, kMaxTileSplits));
+    }
+    f.bytes = (size_t)f.limit * tile_part_floats(f.tile, dim) * sizeof(float);
+  } else if (max_k > kMinChunk) {
+    f.limit = 1;
+    f.bytes = (size_t)(seq_tiles_max(q_rows * G, n_seq, 16) * kv_heads + kFill) * part_floats(dim) * sizeof(float);
+  }
+  return f;
 }
 
 hipError_t launch_attn_seq(const AttnSeq& a, hipStream_t s) {

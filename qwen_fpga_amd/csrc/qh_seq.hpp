@@ -95,9 +95,9 @@ struct AttnSeq {
   int heads = 0, kv_heads = 0, dim = 0;
   float scale = 0.0f;
   int bf16 = 0;
-  float* part = nullptr;          // partials of the split form
-  int tile = 0;                   // the form for prompts
-  int whole = 0;                  // the split form with one chunk of all keys (nothing to join)
+  float* part = nullptr;          // partials of units whose keys are split
+  int tile = 0;                   // rows of a tile of the form for prompts; 0: the form for few rows
+  int limit = 0;                  // places in the workspace (few rows: 1: the keys may be split)
 };
 
 hipError_t launch_gemm_seq(const GemmSeq& a, hipStream_t s);
@@ -111,9 +111,12 @@ hipError_t launch_attn_seq(const AttnSeq& a, hipStream_t s);
 inline int delta_step_len(int64_t heads) { return heads < 256 ? 24 : 48; }
 size_t delta_seq_workspace(int tokens, int n_seq, int heads, int k_heads, bool bf16, int max_len);
 
-// Whether max_k keys are too few to split, and the bytes of workspace of a call.
-bool attn_seq_whole(int max_k);
-size_t attn_seq_workspace(int64_t q_rows, int n_seq, int max_k, int heads, int kv_heads, int dim);
+// The form of a call (AttnSeq's tile and limit) and the bytes of workspace it takes.
+struct AttnForm {
+  int tile, limit;
+  size_t bytes;
+};
+AttnForm attn_seq_form(int64_t q_rows, int n_seq, int max_q, int max_k, int heads, int kv_heads, int dim, bool bf16);
 
 }  // namespace qh
 #endif

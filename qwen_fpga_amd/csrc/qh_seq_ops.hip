@@ -136,11 +136,11 @@ int qh_delta_rule_seq(void* out, int64_t ldo, int64_t hso, const void* q, int64_
   return hip_status(launch_delta_seq(a, S(stream)));
 }
 
-size_t qh_attention_seq_workspace(int q_rows, int n_seq, int max_q, int max_k, int heads, int kv_heads, int head_dim) {
-  if (q_rows <= 0 || n_seq <= 0 || max_q < 0 || max_k < 0 || max_k > kMaxKeys || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 ||
+size_t qh_attention_seq_workspace(int q_rows, int n_seq, int max_q, int max_k, int heads, int kv_heads, int head_dim, int type) {
+  if (!type_ok(type) || q_rows <= 0 || n_seq <= 0 || max_q < 0 || max_k < 0 || max_k > kMaxKeys || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 ||
       (head_dim != 128 && head_dim != 256) || (int64_t)q_rows * heads > kMaxUnits)
     return 0;
-  return attn_seq_workspace(q_rows, n_seq, max_k, heads, kv_heads, head_dim);
+  return attn_seq_form(q_rows, n_seq, max_q, max_k, heads, kv_heads, head_dim, type == QH_BF16).bytes;
 }
 
 int qh_attention_seq(void* out, int64_t ldo, int64_t hso, const void* q, int64_t ldq, int64_t hsq, const void* k, int64_t ldk,
@@ -162,7 +162,8 @@ int qh_attention_seq(void* out, int64_t ldo, int64_t hso, const void* q, int64_t
   if (!cu_q || !k_start || !k_len) return QH_EINVAL;
   const View vc = flat(cu_q, n_seq + 1, 4), vt = flat(k_start, n_seq, 8), vl = flat(k_len, n_seq, 4);
   if (overlap_any(vo, vq, vc, vt, vl) || (k_rows > 0 && overlap_any(vo, vk, vv))) return QH_EINVAL;
-  const size_t need = attn_seq_workspace(q_rows, n_seq, max_k, heads, kv_heads, head_dim);
+  const AttnForm form = attn_seq_form(q_rows, n_seq, max_q, max_k, heads, kv_heads, head_dim, type == QH_BF16);
+  const size_t need = form.bytes;
   if (need > 0) {
     if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255)) return QH_EINVAL;
     const View vw = flat(workspace, need, 1);
@@ -185,8 +186,9 @@ int qh_attention_seq(void* out, int64_t ldo, int64_t hso, const void* q, int64_t
   a.scale = scale;
   a.bf16 = type == QH_BF16;
   a.part = static_cast<float*>(workspace);
-  a.whole = need == 0;
-  a.tile = (int64_t)max_q * (heads / kv_heads) >= 128 && ldk < (1 << 24) && ldv < (1 << 24);
+  a.tile = form.tile;
+  a.limit = form.limit;
+  if (a.tile > 0 && (ldk >= (1 << 24) || ldv >= (1 << 24))) a.tile = a.limit = 0;   // (that form's 32-bit offsets)
   return hip_status(launch_attn_seq(a, S(stream)));
 }
 
