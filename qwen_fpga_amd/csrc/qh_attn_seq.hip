@@ -21,7 +21,7 @@ constexpr float kNegInf = -__builtin_inff();
 // The work of the split form.  A unit is 16 rows of a sequence (tokens x query heads of one kv head) and one chunk
 // of its keys; chunks hold the same number of keys in every sequence, chosen from all sequences' keys (which only
 // the device knows) so that the units come to about kFill, two workgroups for each CU: 16 sequences of 15 to 8191
-// keys took 55 us with chunks cut from the longest one's length and XX with this.
+// keys took 55 us with chunks cut from the longest one's length and 43 with this.
 struct Unit {
   SeqSpan sp;
   int64_t ks;   // the sequence's keys: first row, number (key_len)
@@ -420,25 +420,28 @@ __global__ __launch_bounds__(1024) void attn_join_kernel(const AttnSeq a) {
   }
 }
 
-// The work of the form for prompts.  A tile is `tile` rows of a sequence (tokens x query heads of one kv head) over all
-// the keys they see.  Tiles that see more than `chunk` keys are big: their keys are split into units of a chunk, whose
-// sums meet in the workspace; the others are a unit each.  The chunk is about the keys of all tiles over the CUs (but
-// at least kMinTileChunk, and a 64th of the sequence), so that no unit is much longer than a CU's share.  Units start in
-// order, unit b on XCD b % 8: so the longest come first, and neighbours are about equally long.  The workgroups of an
-// XCD then walk the keys of one head side by side and find them in its L2: shares cut to the same length anywhere in
-// the tiles missed it for 38% of the reads and took 450 us, not 390, for 16k packed tokens (8 / 2 heads of 256).
-// Split and whole: one sequence of 8000 tokens 280 and 360 us, 4096 122 and 170, 1024 43 and 56, 512 36 and 36; two of
-// 8000 500 and 515; a mix of lengths that fills the chip by itself 390 and 380.
-constexpr int kTileFill = 224, kMinTileChunk = 256, kMaxTileSplits = 64;
+// The work of the form for prompts.  A tile is TILE rows of a sequence (tokens x query heads of one kv head) over all
+// the keys they see.  The keys of a tile that sees more than `chunk` of them are split into equal units of at most a
+// chunk, whose sums meet in the workspace; the other tiles are a unit each.  The chunk is about the keys of all tiles
+// over the CUs (but at least min_tile_chunk, and a 64th of the sequence), so that no unit is much longer than a CU's
+// share.  Units start in order, unit b on XCD b % 8: so the longest come first, and neighbours are about equally long.
+// The workgroups of an XCD then walk the keys of one head side by side and find them in its L2: shares cut to the same
+// length anywhere in the tiles missed it for 38% of the reads and took 450 us, not 390, for 16k packed tokens (8 / 2
+// heads of 256).
+// Split and whole, bfloat16: one sequence of 8000 tokens 307 and 350 us, 4096 106 and 165, 1024 44 and 55, 512 36 and
+// 36; two of 8000 478 and 498; those 16k tokens 383 and 390.  Chunks of a 256th instead of a 192nd of the work: 410 us
+// for the 16k, 165 instead of 127 for 1500 tokens of fp32 (units beyond the CUs start when the first ones end).
+constexpr int kTileFill = 192, kMaxTileSplits = 64;
+constexpr int min_tile_chunk(bool bf16) { return bf16 ? 256 : 128; }
 struct TileUnit {
   SeqSpan sp;
   int64_t ks;
-  int kl, tile, split, nsplit, chunk;
-  int slot;   // of the unit (JOIN: of the tile's first) among the big tiles' units
+  int kl, tile, split, nsplit;
+  int slot;   // of the unit (JOIN: of the tile's first) among the split tiles' units
 };
-// Unit b, or (JOIN) big tile b.
-template <bool JOIN>
-__device__ __forceinline__ bool find_tile_unit(const AttnSeq& a, int tile, int b, TileUnit& o) {
+// Unit b, or (JOIN) split tile b.
+template <bool JOIN, int TILE>
+__device__ __forceinline__ bool find_tile_unit(const AttnSeq& a, int b, TileUnit& o) {
   const int lane = threadIdx.x & 63, G = a.heads / a.kv_heads;
   SeqSpan sp;   // of sequence s0 + lane, as of its keys and tiles
   int64_t ks;
@@ -449,7 +452,7 @@ __device__ __forceinline__ bool find_tile_unit(const AttnSeq& a, int tile, int b
     const int n = as_global(a.k_len)[i];
     sp = seq_span(as_global(a.cu_q)[i], as_global(a.cu_q)[i + 1], a.q_rows);
     kl = key_len(ks, n, a.k_rows);
-    nt = s0 + lane < a.n_seq ? seq_tiles(sp.len * G, tile) : 0;
+    nt = s0 + lane < a.n_seq ? seq_tiles(sp.len * G, TILE) : 0;
   };
   auto work = [&]() -> int64_t {   // keys that the sequence's tiles see, about
     const int64_t k = max(kl, 0), past = max(k - sp.len, (int64_t)0);
@@ -464,8 +467,8 @@ __device__ __forceinline__ bool find_tile_unit(const AttnSeq& a, int tile, int b
   if (a.n_seq > 64) load(0);
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) all += __shfl_xor(all, d);
-  const int64_t share = max((all * a.kv_heads + kTileFill - 1) / kTileFill, (int64_t)kMinTileChunk);
-  int base = 0, slots = 0;   // of the next 64 sequences: units (JOIN: big tiles), the big tiles' units
+  const int64_t share = max((all * a.kv_heads + kTileFill - 1) / kTileFill, (int64_t)min_tile_chunk(a.bf16));
+  int base = 0, slots = 0;   // of the next sequence: units (JOIN: split tiles), the split tiles' units
   for (int s0 = 0; s0 < a.n_seq; s0 += 64) {
     if (s0 > 0) load(s0);
     // the longest first: place `rank` is this lane's sequence's
@@ -477,98 +480,104 @@ __device__ __forceinline__ bool find_tile_unit(const AttnSeq& a, int tile, int b
     }
     const int64_t c64 = (max(share, (int64_t)(max(kl, 0) / kMaxTileSplits + 1)) + 31) / 32 * 32;
     const int chunk = a.limit > 0 ? (int)min(c64, (int64_t)kMaxKeys) : kMaxKeys;
-    // the first big tile: the first whose last row sees more than a chunk
-    const int64_t tok = (int64_t)chunk - kl + sp.len;   // (the first such row's token)
-    int big = 0;
-    if (nt > 0 && kl > 0 && sp.len - 1 >= tok) big = nt - (int)min(max((tok * G + tile) / tile - 1, (int64_t)0), (int64_t)nt - 1);
-    const int ns = big > 0 ? seq_tiles(kl, chunk) : 1;
+    int splits = 0;   // units of the split tiles
+    for (int k = 1, c; __ballot((c = tiles_past(sp.len, kl, G, TILE, nt, (int64_t)k * chunk)) > 0) != 0; ++k) splits += k == 1 ? 2 * c : c;
     for (int r = 0; r < n; ++r) {
       const int l = __builtin_ctzll(__ballot(rank == r && lane < n));
       auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
-      int nb = of(big), nsp = of(ns);
-      if ((slots + (int64_t)nb * nsp) * a.kv_heads > a.limit) nb = 0, nsp = 1;   // no place in the workspace: not split
-      const int t = of(nt), m = JOIN ? nb : nb * nsp + t - nb;
+      const int t = of(nt), kn = of(kl), step = of(chunk), su = of(splits);
+      o.sp = {of(sp.start), of(sp.len)};
+      const bool split = su > 0 && (slots + (int64_t)su) * a.kv_heads <= a.limit;   // (there is place for it)
+      const int big = split ? tiles_past(o.sp.len, kn, G, TILE, t, step) : 0, m = JOIN ? big : t - big + (split ? su : 0);
       if (b < base + m) {
-        int in = b - base;
-        o.sp = {of(sp.start), of(sp.len)};
         o.ks = (int64_t)((uint64_t)(uint32_t)of((int)(ks >> 32)) << 32 | (uint32_t)of((int)ks));
-        o.kl = of(kl);
-        o.chunk = of(chunk);
-        const int rest = t - nb, first = JOIN ? nb : nb * (nsp - 1);   // units ahead of the tiles that are not split
-        o.split = o.nsplit = 1;
-        if (in >= first && in < first + rest && !JOIN) {
-          o.tile = rest - 1 - (in - first);
-          o.split = 0;
-          o.chunk = kMaxKeys;
-        } else {
-          if (in >= first) in -= rest;
-          o.tile = t - 1 - in % nb;
-          o.split = in / nb;
-          o.nsplit = nsp;
-          o.slot = slots + in % nb * nsp + o.split;
+        o.kl = kn;
+        int in = b - base, past = 0, k = split ? seq_tiles(kn, step) : 1;   // tiles of more than k splits
+        for (;; --k) {
+          const int c = k > 1 ? tiles_past(o.sp.len, kn, G, TILE, t, (int64_t)(k - 1) * step) - past : t - past;   // of k
+          const int u = JOIN ? c : c * k;
+          if (in < u || k == 1) {
+            o.nsplit = k;
+            o.split = k > 1 && !JOIN ? in / c : 0;
+            in -= o.split * c;
+            o.tile = t - 1 - past - in;
+            o.slot = slots + in * k + o.split;
+            return o.tile >= 0 && o.tile < t;
+          }
+          in -= u;
+          past += c;
+          slots += c * k;
         }
-        return o.tile >= 0 && o.tile < t;
       }
       base += m;
-      slots += nb * nsp;
+      slots += split ? su : 0;
     }
   }
   return false;
 }
+// Keys of each of a tile's `nsplit` units when its last row sees `end`.
+__device__ __forceinline__ int unit_keys(int end, int nsplit) { return nsplit == 1 ? kMaxKeys : (seq_tiles(end, nsplit) + 31) / 32 * 32; }
+constexpr int tile_rows(bool bf16) { return bf16 ? 256 : 128; }
 constexpr size_t tile_part_floats(int tile, int D) { return (size_t)tile * (D + 2); }
 
-// Prompts, bfloat16: a workgroup takes 256 rows (tokens x query heads of one kv head) over all the keys they see.
-// As in the split form the products are S^T = K Q^T and O^T = V^T P^T, and P never leaves the registers.  K and V
-// come 32 keys at a time through a ring of LDS stages that global -> LDS loads fill three ahead.  16-byte chunk c of
-// key r stands at chunk c ^ (r % 16) of K's rows (32 keys of one chunk lie in all banks) and c ^ 4 (r % 4) of V's
-// (four keys of 32 elements do, as the transposing read takes them).  The running maximum moves only when a score
-// passes it by more than 8 (a factor of 256, exact in the sums), so that the sums are rarely rescaled.  At full load the
-// card's power bounds it (1.85 GHz): 930 to 1050 TFLOP/s at 256 elements and long prompts, 840 at 128.  A wave holds 32
-// rows: with 64, 128 elements took 302 us for 8000 tokens of 8 heads, and 32 rows take 189.
+// Prompts: a workgroup takes 256 rows (fp32: 128; tokens x query heads of one kv head) over all the keys they see, 32
+// (16) rows a wave.  As in the split form the products are S^T = K Q^T and O^T = V^T P^T, and P never leaves the
+// registers.  K and V come 32 (16) keys at a time through a ring of LDS stages that global -> LDS loads fill three
+// ahead.  16-byte chunk c of key r stands at chunk c ^ (r % 16) of K's rows (the keys of one chunk lie in all banks)
+// and c ^ 4 (r % 4) of V's in bfloat16 (four keys of 32 elements do, as the transposing read takes them).  The running
+// maximum moves only when a score passes it by more than 8 (a factor of 256, exact in the sums), so that the sums are
+// rarely rescaled.
+// bfloat16: at full load the card's power bounds it (1.85 GHz): 930 to 1100 TFLOP/s at 256 elements and long prompts,
+// 830 at 128.  With 64 rows a wave, 128 elements took 301 us for 8000 tokens of 8 heads, and 32 rows take 190.
+// fp32: the fp32 MFMAs bound it, 89% of their cycles at 2.15 GHz; 1500 tokens 206 us in the form for few rows, 127 in
+// this, of which the join takes 10 and a CU has work for 84; 4096 tokens 98 TFLOP/s.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 
-template <int D>
+template <bool BF16, int D>
 __global__ __launch_bounds__(512, 2) void attn_tile_kernel(const AttnSeq a) {
-  constexpr int NW = 8;                     // waves, of 32 rows each
-  constexpr int kKeys = 32, kRing = 4, CH = D / 8, kHalf = kKeys * D * 2, kStage = 2 * kHalf;
-  constexpr int NI = kHalf / (1024 * NW);   // loads of a wave for K's part of a stage (and for V's)
-  constexpr int NS = D / 16, NT = D / 32;
+  constexpr int E = BF16 ? 2 : 4, kTile = tile_rows(BF16), NR = kTile / 8;   // bytes of an element; a wave's rows
+  constexpr int kKeys = BF16 ? 32 : 16, kRing = 4, CH = D * E / 16, kHalf = kKeys * D * E, kStage = 2 * kHalf;
+  constexpr int NI = kHalf / 8192;               // loads of a wave for K's part of a stage (and for V's)
+  constexpr int NS = D / 16, NT = D / NR;        // K fragments; accumulators, of VW elements of a lane
+  constexpr int VW = BF16 ? 16 : 4, NQ = NT * VW / 4;
+  typedef std::conditional_t<BF16, f32x16, f32x4> fvec;
   __shared__ __attribute__((aligned(256))) char lds[kRing * kStage];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int h = lane >> 5, j = lane & 31;
+  const int h = lane / NR, j = lane % NR;
   const int G = a.heads / a.kv_heads;
   const int kvh = (int)blockIdx.x % a.kv_heads;
   TileUnit at;
-  if (!find_tile_unit<false>(a, 256, (int)blockIdx.x / a.kv_heads, at)) return;
-  const int rows = at.sp.len * G, r0 = 256 * at.tile, w0 = r0 + 32 * wave;
-  const int k0 = at.nsplit > 1 ? at.split * at.chunk : 0;   // keys are counted from here
-  auto sees = [&](int row) { return keys_seen(min(row, rows - 1) / G, at.sp.len, at.kl) - k0; };
-  const int end = min(sees(r0 + 255), at.chunk), wend = w0 < rows ? min(sees(w0 + 31), end) : 0;
+  if (!find_tile_unit<false, kTile>(a, (int)blockIdx.x / a.kv_heads, at)) return;
+  const int rows = at.sp.len * G, r0 = kTile * at.tile, w0 = r0 + NR * wave;
+  auto all = [&](int row) { return keys_seen(min(row, rows - 1) / G, at.sp.len, at.kl); };
+  const int piece = unit_keys(all(r0 + kTile - 1), at.nsplit), k0 = at.split * piece;   // keys are counted from here
+  auto sees = [&](int row) { return all(row) - k0; };
+  const int end = min(sees(r0 + kTile - 1), piece), wend = w0 < rows ? min(sees(w0 + NR - 1), end) : 0;
   if (at.split > 0 && end <= 0) return;   // (a unit of no key that the tile sees)
   u32x4 qf[NS];
-  const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;   // (-q) k |scale|: a maximum stays one
+  const uint32_t flip = a.scale < 0.0f ? (BF16 ? 0x80008000u : 0x80000000u) : 0u;   // (-q) k |scale|: a maximum stays one
   const float sc = fabsf(a.scale) * kLog2e;
   const int row = min(w0 + j, rows - 1), tok = row / G, hq = kvh * G + row % G;
   const int seen = sees(row);
-  const char* qp = static_cast<const char*>(a.q.p) + ((at.sp.start + tok) * a.q.ld + hq * a.q.hs) * 2 + 16 * h;
+  const char* qp = static_cast<const char*>(a.q.p) + ((at.sp.start + tok) * a.q.ld + hq * a.q.hs) * E + 16 * h;
 #pragma unroll
   for (int s = 0; s < NS; ++s) {
-    qf[s] = *as_global(reinterpret_cast<const u32x4*>(qp + 32 * s));
+    qf[s] = *as_global(reinterpret_cast<const u32x4*>(qp + 16 * (64 / NR) * s));
 #pragma unroll
     for (int e = 0; e < 4; ++e) qf[s][e] ^= flip;
   }
   // a wave's loads: LDS places 64 (NI wave + i) + lane of a stage's K (V) rows
-  const char* kp = static_cast<const char*>(a.k.p) + ((at.ks + k0) * a.k.ld + kvh * a.k.hs) * 2;
-  const char* vp = static_cast<const char*>(a.v.p) + ((at.ks + k0) * a.v.ld + kvh * a.v.hs) * 2;
-  const uint32_t kld = (uint32_t)a.k.ld * 2, vld = (uint32_t)a.v.ld * 2;   // (below 2^25: the launch's rule)
+  const char* kp = static_cast<const char*>(a.k.p) + ((at.ks + k0) * a.k.ld + kvh * a.k.hs) * E;
+  const char* vp = static_cast<const char*>(a.v.p) + ((at.ks + k0) * a.v.ld + kvh * a.v.hs) * E;
+  const uint32_t kld = (uint32_t)a.k.ld * E, vld = (uint32_t)a.v.ld * E;   // (below 2^26: the launch's rule)
   auto k_off = [&](int i, int last) {   // last: the last row of the stage that is there
     const int place = 64 * (NI * wave + i) + lane, r = place / CH;
     return min(r, last) * kld + 16 * ((place % CH) ^ (r & 15));
   };
   auto v_off = [&](int i, int last) {
     const int place = 64 * (NI * wave + i) + lane, r = place / CH;
-    return min(r, last) * vld + 16 * ((place % CH) ^ ((r & 3) << 2));
+    return min(r, last) * vld + 16 * ((place % CH) ^ (BF16 ? (r & 3) << 2 : 0));
   };
   uint32_t ko[NI], vo[NI];
 #pragma unroll
@@ -589,9 +598,9 @@ __global__ __launch_bounds__(512, 2) void attn_tile_kernel(const AttnSeq a) {
       for (int i = 0; i < NI; ++i) put(it, i, k_off(i, last), v_off(i, last));
     }
   };
-  f32x16 acc[NT];
+  fvec acc[NT];
 #pragma unroll
-  for (int t = 0; t < NT; ++t) acc[t] = f32x16{};
+  for (int t = 0; t < NT; ++t) acc[t] = fvec{};
   float m = kNegInf, l = 0.0f;
   const int n = seq_tiles(end, kKeys);
 #pragma unroll
@@ -599,8 +608,11 @@ __global__ __launch_bounds__(512, 2) void attn_tile_kernel(const AttnSeq a) {
     if (i < n) stage(i);
   // places of a lane's first fragments; those of the others are these, xor-ed by the chunk and moved by whole 256 bytes
   const int vx = (lane & 15) >> 2;   // the key of four that this lane's transposing read brings
-  uint32_t kl0 = lds0 + j * D * 2 + 16 * (h ^ (j & 15));
-  uint32_t vl0 = lds0 + kHalf + (4 * h + vx) * D * 2 + 32 * ((lane >> 4) & 1) + 16 * ((lane & 3) >> 1) + 8 * (lane & 1) + 64 * vx;
+  const uint32_t kl0 = lds0 + j * D * E + 16 * (h ^ (j & 15));
+  const uint32_t vl0 = lds0 + kHalf + (BF16 ? (4 * h + vx) * D * 2 + 32 * ((lane >> 4) & 1) + 16 * ((lane & 3) >> 1) + 8 * (lane & 1) + 64 * vx
+                                            : 4 * h * D * 4 + 16 * j);
+  // a lane holds four neighbours of its row from place(i) on, i below NQ
+  auto place = [&](int i) { return BF16 ? 32 * (i >> 2) + 8 * (i & 3) + 4 * h : 64 * (i >> 2) + 16 * h + 4 * (i & 3); };
   auto wait = [&](int it) {
     // this wave's loads of the stage have landed (those of the next two stay in flight) and its reads of the stage
     // before are done; after the barrier every wave's
@@ -612,36 +624,50 @@ __global__ __launch_bounds__(512, 2) void attn_tile_kernel(const AttnSeq a) {
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     if (it + kRing - 1 < n) stage(it + kRing - 1);
   };
-  // 32 keys.  PART: some row may see them only in part.
+  // kKeys keys.  PART: some row may see them only in part.
   auto step = [&](int it, auto PART) {
     constexpr bool part = decltype(PART)::value;
     const int kb = kKeys * it;
     // (opaque, so that the places are formed where they are used: held over the loop they would not fit the registers)
     uint32_t kl = kl0 + (it & (kRing - 1)) * kStage, vl = vl0 + (it & (kRing - 1)) * kStage;
     asm volatile("" : "+v"(kl), "+v"(vl));
-    f32x16 st = {};
+    fvec st = {};
+    if constexpr (BF16) {
 #pragma unroll
-    for (int s = 0; s < NS; ++s) {
-      const u32x4 kf = *lds_at<u32x4>((kl ^ (32 * (s & 7))) + 256 * (s >> 3));
-      st = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, kf), __builtin_bit_cast(bf16x8, qf[s]), st, 0, 0, 0);
+      for (int s = 0; s < NS; ++s) {
+        const u32x4 kf = *lds_at<u32x4>((kl ^ (32 * (s & 7))) + 256 * (s >> 3));
+        st = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, kf), __builtin_bit_cast(bf16x8, qf[s]), st, 0, 0, 0);
+      }
+    } else {
+      fvec s2[2] = {};
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        const f32x4 kf = *lds_at<f32x4>((kl ^ (64 * (s & 3))) + 256 * (s >> 2));
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          s2[c & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[c], __uint_as_float(qf[s][c]), s2[c & 1], 0, 0, 0);
+      }
+      st = s2[0] + s2[1];
     }
     if constexpr (!part) {
       __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
 #pragma unroll
       for (int i = 0; i < NS - 3; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x8, BF16 ? 1 : 4, 0);
         __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
       }
-      __builtin_amdgcn_sched_group_barrier(0x8, 3, 0);
+      __builtin_amdgcn_sched_group_barrier(0x8, BF16 ? 3 : 12, 0);
     }
+    auto key_of = [&](int r) { return kb + 8 * (r >> 2) + 4 * h + (r & 3); };   // (fp32: four in all)
     if constexpr (part) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
-        if (kb + 8 * (r >> 2) + 4 * h + (r & 3) >= seen) st[r] = kNegInf;
+      for (int r = 0; r < VW; ++r)
+        if (key_of(r) >= seen) st[r] = kNegInf;
     }
     float x = st[0];
 #pragma unroll
-    for (int r = 1; r < 16; ++r) x = fmaxf(x, st[r]);
+    for (int r = 1; r < VW; ++r) x = fmaxf(x, st[r]);
+    if constexpr (!BF16) x = fmaxf(x, xor_perm<16>(x));
     x = fmaxf(x, xor_perm<32>(x));
     const float mt = x == kNegInf ? kNegInf : x * sc;   // (0 times it is not it)
     const bool up = mt > m + 8.0f;
@@ -653,61 +679,82 @@ __global__ __launch_bounds__(512, 2) void attn_tile_kernel(const AttnSeq a) {
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) acc[t][r] *= al;
+        for (int r = 0; r < VW; ++r) acc[t][r] *= al;
     }
-    u32x4 pf[2];
     const float mu = m == kNegInf ? 0.0f : m;
     float ps = 0.0f;
 #pragma unroll
-    for (int r = 0; r < 16; r += 2) {
-      float p[2];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[r + e], sc, -mu));
-        if constexpr (part) p[e] = st[r + e] == kNegInf ? 0.0f : p[e];   // (a scale of 0)
-        ps += p[e];
-      }
-      const bf16x2 pk = {(__bf16)p[0], (__bf16)p[1]};
-      pf[r >> 3][(r >> 1) & 3] = __builtin_bit_cast(uint32_t, pk);
+    for (int r = 0; r < VW; ++r) {
+      const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(st[r], sc, -mu));
+      st[r] = part && st[r] == kNegInf ? 0.0f : p;   // (a scale of 0)
+      ps += st[r];
     }
     l += ps;
-    bool bad = false;
+    bool bad = false;   // (see attn_split_kernel: what is not finite in V goes only to the rows that see it)
+    if constexpr (BF16) {
+      u32x4 pf[2];
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int kk = 0; kk < 2; ++kk) {   // keys 16 kk + 4 h .., + 8 of d = 32 t + lane % 32
-        const uint32_t p = (vl ^ (64 * (t & 3))) + 256 * (t >> 2) + 16 * kk * D * 2;
-        union {
-          i16x4 h[2];
-          u32x4 v;
-        } u;
-#pragma unroll
-        for (int q = 0; q < 2; ++q)
-          u.h[q] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_at<i16x4>(p + 8 * q * D * 2));
-        // (see attn_split_kernel: what is not finite in V goes only to the rows that see it)
-        if constexpr (part) bad |= zero_non_finite<true>(u.v);
-        acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, u.v), __builtin_bit_cast(bf16x8, pf[kk]),
-                                                         acc[t], 0, 0, 0);
+      for (int r = 0; r < 16; r += 2) {
+        const bf16x2 pk = {(__bf16)st[r], (__bf16)st[r + 1]};
+        pf[r >> 3][(r >> 1) & 3] = __builtin_bit_cast(uint32_t, pk);
       }
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {   // keys 16 kk + 4 h .., + 8 of d = 32 t + lane % 32
+          const uint32_t p = (vl ^ (64 * (t & 3))) + 256 * (t >> 2) + 16 * kk * D * 2;
+          union {
+            i16x4 h[2];
+            u32x4 v;
+          } u;
+#pragma unroll
+          for (int q = 0; q < 2; ++q)
+            u.h[q] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_at<i16x4>(p + 8 * q * D * 2));
+          if constexpr (part) bad |= zero_non_finite<true>(u.v);
+          acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, u.v), __builtin_bit_cast(bf16x8, pf[kk]),
+                                                           acc[t], 0, 0, 0);
+        }
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)   // key 4 h + r
+#pragma unroll
+        for (int t = 0; t < NT / 4; ++t) {   // d = 64 t + 4 (lane % 16) + c
+          u32x4 v = *lds_at<u32x4>(vl + r * D * 4 + 256 * t);
+          if constexpr (part) bad |= zero_non_finite<false>(v);
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            acc[4 * t + c] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[c]), st[r], acc[4 * t + c], 0, 0, 0);
+        }
+    }
     if constexpr (!part) {   // fragments on their way ahead of the product they are for
-      __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+      constexpr int kReads = BF16 ? 2 : 1, kProducts = BF16 ? 1 : 4, kSteps = BF16 ? 2 * NT : NT;
+      __builtin_amdgcn_sched_group_barrier(0x100, 2 * kReads, 0);
 #pragma unroll
-      for (int i = 0; i < 2 * NT - 2; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      for (int i = 0; i < kSteps - 2; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x8, kProducts, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, kReads, 0);
       }
-      __builtin_amdgcn_sched_group_barrier(0x8, 2, 0);
+      __builtin_amdgcn_sched_group_barrier(0x8, 2 * kProducts, 0);
     }
     if constexpr (part) {
       if (__ballot(bad) != 0) {
         for (int key = kb; key < min(kb + kKeys, end); ++key) {
-          const __bf16* q = static_cast<const __bf16*>(a.v.p) + (at.ks + k0 + key) * a.v.ld + kvh * a.v.hs + 4 * h;
+          const char* q = vp + (int64_t)key * a.v.ld * E;
 #pragma unroll
-          for (int t = 0; t < NT; ++t)
+          for (int i = 0; i < NQ; ++i)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const float e = (float)as_global(q)[32 * t + 8 * (r >> 2) + (r & 3)];
-              if (non_finite(e) && key < seen) acc[t][r] += e;
+            for (int c = 0; c < 4; ++c) {
+              float e;
+              if constexpr (BF16)
+                e = (float)as_global(reinterpret_cast<const __bf16*>(q))[place(i) + c];
+              else
+                e = as_global(reinterpret_cast<const float*>(q))[place(i) + c];
+              if (non_finite(e) && key < seen) {
+                if constexpr (BF16)
+                  acc[i >> 2][4 * (i & 3) + c] += e;
+                else
+                  acc[4 * (i >> 2) + c][i & 3] += e;
+              }
             }
         }
       }
@@ -723,48 +770,52 @@ __global__ __launch_bounds__(512, 2) void attn_tile_kernel(const AttnSeq a) {
     wait(it);
     if (kKeys * it < wend) step(it, std::true_type{});
   }
+  if constexpr (!BF16) l = l + xor_perm<16>(l);
   l = l + xor_perm<32>(l);
   if (w0 + j >= rows) return;
+  auto quad = [&](int i) {
+    if constexpr (BF16)
+      return f32x4{acc[i >> 2][4 * (i & 3)], acc[i >> 2][4 * (i & 3) + 1], acc[i >> 2][4 * (i & 3) + 2], acc[i >> 2][4 * (i & 3) + 3]};
+    else
+      return f32x4{acc[4 * (i >> 2)][i & 3], acc[4 * (i >> 2) + 1][i & 3], acc[4 * (i >> 2) + 2][i & 3], acc[4 * (i >> 2) + 3][i & 3]};
+  };
   if (at.nsplit > 1) {
-    float* pp = a.part + ((size_t)at.slot * a.kv_heads + kvh) * tile_part_floats(256, D);
+    float* pp = a.part + ((size_t)at.slot * a.kv_heads + kvh) * tile_part_floats(kTile, D);
     const int rr = row - r0;
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int r = 0; r < 16; r += 4)
-        *as_global_w(reinterpret_cast<f32x4*>(pp + rr * D + 32 * t + 2 * r + 4 * h)) =
-            f32x4{acc[t][r], acc[t][r + 1], acc[t][r + 2], acc[t][r + 3]};
-    if (h == 0) pp[256 * D + rr] = m, pp[256 * D + 256 + rr] = l;
+    for (int i = 0; i < NQ; ++i) *as_global_w(reinterpret_cast<f32x4*>(pp + rr * D + place(i))) = quad(i);
+    if (h == 0) pp[kTile * D + rr] = m, pp[kTile * D + kTile + rr] = l;
     return;
   }
   const float inv = at.kl < 0 ? __builtin_nanf("") : seen <= 0 ? 0.0f : 1.0f / l;
-  char* op = static_cast<char*>(a.out.p) + ((at.sp.start + tok) * a.out.ld + hq * a.out.hs) * 2;
+  char* op = static_cast<char*>(a.out.p) + ((at.sp.start + tok) * a.out.ld + hq * a.out.hs) * E;
 #pragma unroll
-  for (int t = 0; t < NT; ++t)
-#pragma unroll
-    for (int r = 0; r < 16; r += 4) {
-      const bf16x4 o = {(__bf16)(acc[t][r] * inv), (__bf16)(acc[t][r + 1] * inv), (__bf16)(acc[t][r + 2] * inv),
-                        (__bf16)(acc[t][r + 3] * inv)};
-      *as_global_w(reinterpret_cast<bf16x4*>(op + (32 * t + 2 * r + 4 * h) * 2)) = o;
-    }
+  for (int i = 0; i < NQ; ++i) {
+    const f32x4 o = quad(i) * inv;
+    if constexpr (BF16)
+      *as_global_w(reinterpret_cast<bf16x4*>(op + place(i) * 2)) = bf16x4{(__bf16)o[0], (__bf16)o[1], (__bf16)o[2], (__bf16)o[3]};
+    else
+      *as_global_w(reinterpret_cast<f32x4*>(op + place(i) * 4)) = o;
+  }
 }
 
-// Joins the units of a big tile: a wave takes a row, four units in flight.
+// Joins the units of a big tile: a wave takes a row at a time, eight units in flight.
 template <bool BF16, int D>
-__global__ __launch_bounds__(256) void attn_tile_join_kernel(const AttnSeq a, int tile) {
-  constexpr int W = D / 64, U = 4;   // elements of a lane; units in flight
+__global__ __launch_bounds__(256) void attn_tile_join_kernel(const AttnSeq a) {
+  constexpr int tile = tile_rows(BF16), W = D / 64, U = 8;   // elements of a lane; units in flight
   typedef float vec __attribute__((ext_vector_type(W)));
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int G = a.heads / a.kv_heads;
   const int kvh = (int)blockIdx.x % a.kv_heads;
   TileUnit at;
-  if (!find_tile_unit<true>(a, tile, (int)blockIdx.x / a.kv_heads, at)) return;
+  if (!find_tile_unit<true, tile>(a, (int)blockIdx.x / a.kv_heads, at)) return;
   const int rows = min(at.sp.len * G - tile * at.tile, tile);
+  const int piece = unit_keys(keys_seen((tile * at.tile + rows - 1) / G, at.sp.len, at.kl), at.nsplit);
   const size_t step = tile_part_floats(tile, D) * a.kv_heads;
   const float* pp = a.part + ((size_t)at.slot * a.kv_heads + kvh) * tile_part_floats(tile, D);
   for (int j = 4 * blockIdx.y + wave; j < rows; j += 4 * gridDim.y) {
     const int row = tile * at.tile + j, tok = row / G, hq = kvh * G + row % G;
-    const int ns = min(seq_tiles(keys_seen(tok, at.sp.len, at.kl), at.chunk), at.nsplit);   // units that this row sees
+    const int ns = seq_tiles(keys_seen(tok, at.sp.len, at.kl), piece);   // units that this row sees
     float m = kNegInf, l = 0.0f;
     vec acc = {};
     for (int s0 = 0; s0 < ns; s0 += U) {
@@ -805,8 +856,11 @@ template <bool BF16, int D>
 hipError_t launch(const AttnSeq& a, hipStream_t s) {
   if (a.tile > 0) {
     const int64_t t = seq_tiles_max((int64_t)a.q_rows * (a.heads / a.kv_heads), a.n_seq, a.tile) * a.kv_heads;
-    attn_tile_kernel<D><<<(unsigned)(t + a.limit), 512, 0, s>>>(a);
-    if (a.limit > 0) attn_tile_join_kernel<BF16, D><<<dim3((unsigned)min(t, (int64_t)a.limit / 2), 16), 256, 0, s>>>(a, a.tile);
+    attn_tile_kernel<BF16, D><<<(unsigned)(t + a.limit), 512, 0, s>>>(a);
+    if (a.limit > 0) {
+      const int64_t split = std::min<int64_t>(t, a.limit / 2);
+      attn_tile_join_kernel<BF16, D><<<dim3((unsigned)split, (unsigned)std::clamp<int64_t>(1024 / split, 8, a.tile / 4)), 256, 0, s>>>(a);
+    }
     return hipGetLastError();
   }
   const unsigned tiles = (unsigned)(seq_tiles_max((int64_t)a.q_rows * (a.heads / a.kv_heads), a.n_seq, 16) * a.kv_heads);
@@ -820,12 +874,18 @@ hipError_t launch(const AttnSeq& a, hipStream_t s) {
 AttnForm attn_seq_form(int64_t q_rows, int n_seq, int max_q, int max_k, int heads, int kv_heads, int dim, bool bf16) {
   const int G = heads / kv_heads;
   AttnForm f = {0, 0, 0};
-  if ((int64_t)max_q * G >= 128 && bf16) {
-    f.tile = 256;
+  // Prompts, or many short ones that see many keys.  8 / 2 heads of 256, us in this form and in the one for few rows:
+  // fp32   one of 256 tokens 49 and 31, of 512 55 and 60, of 1500 123 and 162, of 4096 700 and 820; 128 tokens behind
+  //        1500 keys 57 and 44, behind 8000 121 and 117; 16 of 128 tokens 49 and 41, behind 8000 keys 1021 and 1367
+  // bf16   one of 128 tokens 23 and 15, of 256 27 and 27, of 512 34 and 46, of 4096 112 and 378; 128 tokens behind
+  //        1500 keys 36 and 33, behind 8000 50 and 61; 16 of 128 tokens 27 and 26, behind 8000 keys 169 and 599
+  const int64_t seen = q_rows * heads * std::max(max_k, 1);
+  if ((int64_t)max_q * G >= (bf16 ? 1024 : 2048) || ((int64_t)max_q * G >= 128 && seen >= 5000000)) {
+    f.tile = tile_rows(bf16);
     const int64_t tiles = seq_tiles_max(q_rows * G, n_seq, f.tile) * kv_heads;
     // two workspace places a CU: the chunks are such that more are hardly ever taken
-    if (max_k > kMinTileChunk) {
-      const int64_t splits = max_k / kMinTileChunk + 1;
+    if (max_k > min_tile_chunk(bf16)) {
+      const int64_t splits = max_k / min_tile_chunk(bf16) + 1;
       f.limit = (int)std::min<int64_t>(2 * kTileFill, tiles * std::min<int64_t>(splits, kMaxTileSplits));
     }
     f.bytes = (size_t)f.limit * tile_part_floats(f.tile, dim) * sizeof(float);

@@ -44,6 +44,12 @@ QH_SEQ_FN int keys_seen(int row, int q_len, int k_len) {
   const int64_t n = (int64_t)row + 1 + k_len - q_len;
   return n < 0 ? 0 : (int)n;
 }
+// Of a sequence's nt tiles (`tile` rows each, G rows a token) those whose last row sees more than `keys` keys: the last.
+QH_SEQ_FN int tiles_past(int q_len, int k_len, int G, int tile, int nt, int64_t keys) {
+  const int64_t tok = keys - k_len + q_len;   // the first token that does
+  if (nt <= 0 || tok >= q_len) return 0;
+  return tok <= 0 ? nt : nt - (int)(tok * G / tile);
+}
 
 }  // namespace qh
 

@@ -14,7 +14,9 @@ Tolerances.  u = 2^-24 is half a step of fp32, 2^-8 of bfloat16 (finfo.eps / 2).
                   (n + 1) (6 sqrt(128) + 8) u times the largest state (or v) norm of a column.  bfloat16: the
                   output rounded once more.
 """
+import functools
 import math
+import sys
 
 import numpy as np
 import pytest
@@ -490,6 +492,82 @@ def test_attention_prompt_then_tokens(q, torch_cuda):
     attn_check(torch, attn_run(q, torch, *dev, [n], [n], at_k), want, False)
     one = torch.cat([attn_run(q, torch, dev[0][t:t + 1], dev[1], dev[2], [1], [t + 1], [0]) for t in range(n)])
     attn_check(torch, one, want, False)
+
+
+# The form for prompts, whatever the lengths: max_q is a bound, and a large one asks for it.
+
+@pytest.fixture
+def prompts(monkeypatch):
+    monkeypatch.setattr(sys.modules[__name__], "attn_run", functools.partial(attn_run, max_q=4096))
+
+
+@pytest.mark.parametrize("lens,ctx,h,kvh,d", ATTN + [
+    ([700], [3000], 8, 2, 256), ([130, 1], [4100, 2000], 2, 2, 128), ([40], [9000], 4, 4, 128), ([1023, 0, 513], [1023, 4, 800], 4, 1, 256),
+    ([257], [700], 12, 4, 256)], ids=str)
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+def test_prompt_form(prompts, q, torch_cuda, lens, ctx, h, kvh, d, bf16):
+    test_attention(q, torch_cuda, lens, ctx, h, kvh, d, bf16)
+
+
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+@pytest.mark.parametrize("d", [128, 256])
+def test_prompt_form_rows_without_keys(prompts, q, torch_cuda, bf16, d):
+    test_attention_rows_without_keys(q, torch_cuda, bf16, d)
+
+
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+@pytest.mark.parametrize("n,m", [(1, 200), (5, 300), (100, 100), (150, 260), (90, 1200)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf], ids=str)
+def test_prompt_form_hidden_keys_have_no_influence(prompts, q, torch_cuda, bf16, n, m, bad):
+    test_attention_hidden_keys_have_no_influence(q, torch_cuda, bf16, n, m, bad)
+
+
+def test_prompt_form_infinite_value(prompts, q, torch_cuda):
+    test_attention_infinite_value_reaches_its_element_only(q, torch_cuda)
+
+
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+def test_prompt_form_strides(prompts, q, torch_cuda, bf16):
+    test_attention_strides(q, torch_cuda, bf16)
+
+
+def test_prompt_form_large_scores(prompts, q, torch_cuda):
+    test_attention_large_scores(q, torch_cuda)
+
+
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+def test_prompt_form_bad_ranges(prompts, q, torch_cuda, bf16):
+    """As test_attention_bad_ranges, with sequences whose keys are split beside those that have none."""
+    torch = torch_cuda
+    lens, ctx = [30, 150, 7], [600, 700, 40]
+    qq, kk, vv, at_k = attn_inputs(torch, 8, lens, ctx, 2, 1, 128, bf16)
+    dev = [x.cuda() for x in (qq, kk, vv)]
+    want, tol = attn_oracle(torch, qq, kk, vv, lens, ctx, at_k, 1 / math.sqrt(128))
+    for start, length in ((-1, 700), (641, 700), (600, -1), (1 << 40, 700), (0, 1341)):
+        got = attn_run(q, torch, *dev, lens, [600, length, 40], [at_k[0], start, at_k[2]], max_k=700)
+        assert torch.isnan(got[30:180]).all()
+        for a, b in ((0, 30), (180, 187)):
+            attn_check(torch, got[a:b], (want[a:b], tol[a:b]), bf16)
+    out = torch.full(qq.shape, 7.0, dtype=qq.dtype, device="cuda")
+    ws = torch.empty(q.attention_seq_workspace(187, 3, 4096, 700, 2, 1, 128), dtype=torch.uint8, device="cuda")
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    q.attention_seq(out, *dev, i32([0, 30, 188, 187]), torch.tensor(at_k, dtype=torch.int64, device="cuda"), i32(ctx), ws, 4096, 700)
+    attn_check(torch, out[:30], (want[:30], tol[:30]), bf16)
+    assert (out[30:] == 7).all()
+
+
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+@pytest.mark.parametrize("max_q", [1, 4096])
+def test_attention_of_many_sequences(q, torch_cuda, bf16, max_q):
+    """More than the 64 sequences that a wave looks at together; long ones among empty and short ones."""
+    torch = torch_cuda
+    lens = [(5 * i) % 9 for i in range(150)]
+    ctx = [n + (7 * i) % 40 for i, n in enumerate(lens)]
+    for i, n, m in ((3, 140, 900), (64, 1, 1500), (149, 70, 70)):
+        lens[i], ctx[i] = n, m
+    qq, kk, vv, at_k = attn_inputs(torch, 10, lens, ctx, 4, 2, 128, bf16)
+    got = attn_run(q, torch, qq.cuda(), kk.cuda(), vv.cuda(), lens, ctx, at_k, max_q=max_q)
+    attn_check(torch, got, attn_oracle(torch, qq, kk, vv, lens, ctx, at_k, 1 / math.sqrt(128)), bf16)
 
 
 # ------------------------------------------------------------------ calls that cannot be answered
