@@ -4,8 +4,7 @@
 //
 // In both kernels an MFMA's A operand (rows of the result) is 16 weight rows and its B operand 16 tokens,
 // so that a lane ends with four consecutive outputs of one token.
-#include "qh_device.hpp"
-#include "qh_seq.hpp"
+#include "qh_seq_device.hpp"
 
 namespace qh {
 
@@ -53,34 +52,27 @@ __device__ __forceinline__ void put4(const GemmSeq& a, int m, int n, const i32x4
   }
 }
 
-// Few tokens, or few outputs: a wave takes 16 RT rows and 16 TT tokens, operands straight from memory into the
-// MFMAs' registers, PF steps of 64 in flight.  KS waves share the rows and every KS-th pair of steps (a 128-byte
-// line of each row) is a wave's own; their sums meet in LDS.
-template <bool BF16, int RT, int TT, int KS>
+// Few tokens, or few outputs: a workgroup takes 16 rows and 16 TT tokens, operands straight from memory into the MFMAs'
+// registers, PF steps of 64 in flight.  Every fourth pair of steps (a 128-byte line of each row) is one wave's; the four
+// waves' sums meet in LDS.  Bound by the rows' way from memory: 151936 x 1024 weights and 4 tokens 27 us, 5.7 TB/s.
+template <bool BF16, int TT>
 __global__ __launch_bounds__(256) void gemm_rows_kernel(const GemmSeq a) {
-  constexpr int PF = 4;
-  __shared__ i32x4 red[KS > 1 ? KS : 1][KS > 1 ? RT * TT : 1][64];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  constexpr int PF = 4, KS = 4;
+  __shared__ i32x4 red[KS][TT][64];
+  const int lane = threadIdx.x & 63, ks = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, j = lane & 15;
-  const int ks = KS > 1 ? wave : 0;
-  const int n0 = (KS > 1 ? (int)blockIdx.x : (int)blockIdx.x * 4 + wave) * 16 * RT, m0 = (int)blockIdx.y * 16 * TT;
-  if (n0 >= a.out) return;   // (KS == 1: a whole wave; KS > 1: never)
+  const int n0 = (int)blockIdx.x * 16, m0 = (int)blockIdx.y * 16 * TT;
   const int NC = a.in >> 4;
-  const int8_t *wp[RT], *xp[TT];
-#pragma unroll
-  for (int r = 0; r < RT; ++r) wp[r] = a.w + (size_t)min(n0 + 16 * r + j, a.out - 1) * a.in;
+  const int8_t *wp = a.w + (size_t)min(n0 + j, a.out - 1) * a.in, *xp[TT];
 #pragma unroll
   for (int t = 0; t < TT; ++t) xp[t] = static_cast<const int8_t*>(a.x.p) + (int64_t)min(m0 + 16 * t + j, a.tokens - 1) * a.x.ld;
-  i32x4 acc[RT][TT], wb[PF][RT], xb[PF][TT];
+  i32x4 acc[TT], wb[PF], xb[PF][TT];
 #pragma unroll
-  for (int r = 0; r < RT; ++r)
-#pragma unroll
-    for (int t = 0; t < TT; ++t) acc[r][t] = i32x4{0, 0, 0, 0};
+  for (int t = 0; t < TT; ++t) acc[t] = i32x4{0, 0, 0, 0};
   auto chunk = [&](int i) { return 4 * ((i >> 1) * 2 * KS + 2 * ks + (i & 1)) + g; };   // of this wave's step i
-  auto load = [&](int i, i32x4 (&w)[RT], i32x4 (&x)[TT]) {
+  auto load = [&](int i, i32x4& w, i32x4 (&x)[TT]) {
     const int c = 16 * min(chunk(i), NC - 1);
-#pragma unroll
-    for (int r = 0; r < RT; ++r) w[r] = *as_global(reinterpret_cast<const i32x4*>(wp[r] + c));
+    w = *as_global(reinterpret_cast<const i32x4*>(wp + c));
 #pragma unroll
     for (int t = 0; t < TT; ++t) x[t] = *as_global(reinterpret_cast<const i32x4*>(xp[t] + c));
   };
@@ -93,53 +85,30 @@ __global__ __launch_bounds__(256) void gemm_rows_kernel(const GemmSeq a) {
     for (int p = 0; p < PF; ++p) {
       const int i = i0 + p;
       if (i < n) {
-        const bool in = chunk(i) < NC;   // past the end of the row: nothing
+        const i32x4 wv = chunk(i) < NC ? wb[p] : i32x4{0, 0, 0, 0};   // past the end of the row: nothing
 #pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          const i32x4 wv = in ? wb[p][r] : i32x4{0, 0, 0, 0};
-#pragma unroll
-          for (int t = 0; t < TT; ++t) acc[r][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv, xb[p][t], acc[r][t], 0, 0, 0);
-        }
+        for (int t = 0; t < TT; ++t) acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv, xb[p][t], acc[t], 0, 0, 0);
         if (i + PF < n) load(i + PF, wb[p], xb[p]);
       }
     }
   }
-  if constexpr (KS > 1) {
 #pragma unroll
-    for (int r = 0; r < RT; ++r)
+  for (int t = 0; t < TT; ++t) red[ks][t][lane] = acc[t];
+  __syncthreads();
+  if (ks >= TT) return;
+  i32x4 s = red[0][ks][lane];
 #pragma unroll
-      for (int t = 0; t < TT; ++t) red[ks][r * TT + t][lane] = acc[r][t];
-    __syncthreads();
-#pragma unroll
-    for (int u = 0; u < (RT * TT + KS - 1) / KS; ++u) {
-      const int q = u * KS + ks;
-      if (q >= RT * TT) break;
-      i32x4 s = red[0][q][lane];
-#pragma unroll
-      for (int w = 1; w < KS; ++w) s += red[w][q][lane];
-      const int m = m0 + 16 * (q % TT) + j;
-      const int n = n0 + 16 * (q / TT) + 4 * g;
-      if (m < a.tokens) put4<BF16>(a, m, n, s, as_global(a.sx)[m], scale4(a, n), a.wide && n + 4 <= a.out);
-    }
-  } else {
-    f32x4 sc[RT];
-    float xs[TT];
-#pragma unroll
-    for (int r = 0; r < RT; ++r) sc[r] = scale4(a, n0 + 16 * r + 4 * g);
-#pragma unroll
-    for (int t = 0; t < TT; ++t) xs[t] = as_global(a.sx)[min(m0 + 16 * t + j, a.tokens - 1)];
-    const bool wide = a.wide && n0 + 16 * RT <= a.out;
-#pragma unroll
-    for (int t = 0; t < TT; ++t)
-      if (m0 + 16 * t + j < a.tokens)
-#pragma unroll
-        for (int r = 0; r < RT; ++r) put4<BF16>(a, m0 + 16 * t + j, n0 + 16 * r + 4 * g, acc[r][t], xs[t], sc[r], wide);
-  }
+  for (int w = 1; w < KS; ++w) s += red[w][ks][lane];
+  const int m = m0 + 16 * ks + j, o = n0 + 4 * g;
+  if (m < a.tokens) put4<BF16>(a, m, o, s, as_global(a.sx)[m], scale4(a, o), a.wide && o + 4 <= a.out);
 }
 
 // Many tokens: a workgroup takes 128 rows and 128 tokens, in steps of 64 through a ring of four LDS stages that
-// global -> LDS loads fill three steps ahead; a wave multiplies 64 x 64.  A row's 16-byte chunk c stands at chunk
-// c ^ (row / 4 % 4) of its 64 bytes, so that the 16 rows that a fragment reads lie in 16 different bank groups.
+// global -> LDS loads fill three steps ahead; a wave multiplies 64 x 64, and reads the fragments of a step beside the
+// products of the one before.  A row's 16-byte chunk c stands at chunk c ^ (row / 2 % 4) of its 64 bytes, so that eight
+// rows of a fragment, which are read at once, lie in all banks.  4096 tokens of 3584 -> 1024: 23.4 us, the loop 16.8 of
+// them (1.8 POP/s at 1.95 GHz; LDS and MFMA pipes are busy for 65 and 45% of it); 1500 tokens of 1024 -> 7168: 26.5 us,
+// two rounds of workgroups, each 8 us of loop and 5 of start and of writing 43 MB of fp32 outputs.
 constexpr int kBT = 128, kStages = 4, kStageBytes = 2 * kBT * 64;
 
 template <bool BF16>
@@ -151,21 +120,21 @@ __global__ __launch_bounds__(256, 2) void gemm_tile_kernel(const GemmSeq a, int 
   const int n0 = (b / mt) * kBT, m0 = (b % mt) * kBT;
   const int wr = 64 * (wave & 1), wt = 64 * (wave >> 1);
   const int NC = a.in >> 4, NS = (NC + 3) >> 2;
-  // a wave's loads of a step: 2 x 16 rows of w, 2 x 16 of x; lane l brings chunk (l % 4) ^ (row / 4 % 4) of row l / 4
-  const int lr = lane >> 2, lc = (lane & 3) ^ ((lr >> 2) & 3);
-  const int8_t* src[4];
+  // a wave's loads of a step: 2 x 16 rows of w, 2 x 16 of x; lane l brings chunk (l % 4) ^ (row / 2 % 4) of row l / 4
+  const int lr = lane >> 2, lc = (lane & 3) ^ ((lr >> 1) & 3);
+  const char* src[2] = {reinterpret_cast<const char*>(a.w) + (size_t)n0 * a.in, static_cast<const char*>(a.x.p) + (int64_t)m0 * a.x.ld};
+  uint32_t off[4];   // (below 128 rows of less than 2^24 bytes: the launch's rule)
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int r = 32 * wave + 16 * i + lr;
-    src[i] = a.w + (size_t)min(n0 + r, a.out - 1) * a.in;
-    src[2 + i] = static_cast<const int8_t*>(a.x.p) + (int64_t)min(m0 + r, a.tokens - 1) * a.x.ld;
+    off[i] = (uint32_t)min(r, a.out - 1 - n0) * (uint32_t)a.in;
+    off[2 + i] = (uint32_t)min(r, a.tokens - 1 - m0) * (uint32_t)a.x.ld;
   }
   auto stage = [&](int s) {
     const int c = 16 * min(4 * s + lc, NC - 1);
-    int8_t* base = lds + (s & (kStages - 1)) * kStageBytes + 32 * wave * 64;
+    const uint32_t base = lds_address(lds) + (s & (kStages - 1)) * kStageBytes + 32 * wave * 64;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      __builtin_amdgcn_global_load_lds(as_global(src[i] + c), as_lds_w(base + (i >> 1) * (kBT * 64) + (i & 1) * 1024), 16, 0, 0);
+    for (int i = 0; i < 4; ++i) load_to_lds(src[i >> 1], off[i] + c, base + (i >> 1) * (kBT * 64) + (i & 1) * 1024);
   };
   i32x4 acc[4][4];
 #pragma unroll
@@ -173,35 +142,57 @@ __global__ __launch_bounds__(256, 2) void gemm_tile_kernel(const GemmSeq a, int 
 #pragma unroll
     for (int t = 0; t < 4; ++t) acc[r][t] = i32x4{0, 0, 0, 0};
 #pragma unroll
-  for (int s = 0; s < kStages - 1; ++s)
+  for (int s = 0; s < kStages; ++s)
     if (s < NS) stage(s);
-  const int fo = j * 64 + 16 * (g ^ ((j >> 2) & 3));   // a fragment's place
-  for (int s = 0; s < NS; ++s) {
-    // this wave's loads of step s have landed (those of the next two stay in flight) and its reads of step s - 1 are
-    // done; after the barrier every wave's
-    if (s + 2 < NS)
-      asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    else if (s + 1 < NS)
-      asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    else
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (s + 3 < NS) stage(s + 3);
+  const int fo = j * 64 + 16 * (g ^ ((j >> 1) & 3));   // a fragment's place
+  i32x4 wv[2][4], xv[2][4];   // fragments of the steps s and s + 1
+  // this wave's loads of step s have landed (those of the `ahead` next stay in flight) and its reads of step s - 1 are
+  // done; after the barrier every wave's
+  auto wait = [&](int ahead) {
+    switch (ahead) {
+#define QH_WAIT(n) case n: asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(4 * n) : "memory"); break;
+      QH_WAIT(0) QH_WAIT(1) QH_WAIT(2) QH_WAIT(3) QH_WAIT(4) QH_WAIT(5) QH_WAIT(6) QH_WAIT(7)
+#undef QH_WAIT
+    }
+  };
+  auto read = [&](int s, i32x4 (&w)[4], i32x4 (&x)[4]) {
     const int8_t* base = lds + (s & (kStages - 1)) * kStageBytes;
-    i32x4 wv[4], xv[4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      wv[t] = *as_lds(reinterpret_cast<const i32x4*>(base + (wr + 16 * t) * 64 + fo));
-      xv[t] = *as_lds(reinterpret_cast<const i32x4*>(base + kBT * 64 + (wt + 16 * t) * 64 + fo));
+      w[t] = *as_lds(reinterpret_cast<const i32x4*>(base + (wr + 16 * t) * 64 + fo));
+      x[t] = *as_lds(reinterpret_cast<const i32x4*>(base + kBT * 64 + (wt + 16 * t) * 64 + fo));
     }
-    if (4 * s + 4 > NC) {   // past the end of the row: nothing
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-        if (4 * s + g >= NC) wv[t] = i32x4{0, 0, 0, 0};
-    }
+  };
+  wait(min(NS - 1, kStages - 1));
+  read(0, wv[0], xv[0]);
+  auto mul = [&](const i32x4 (&w)[4], const i32x4 (&x)[4]) {
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
-      for (int t = 0; t < 4; ++t) acc[r][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv[r], xv[t], acc[r][t], 0, 0, 0);
+      for (int t = 0; t < 4; ++t) acc[r][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[r], x[t], acc[r][t], 0, 0, 0);
+  };
+  int s = 0;
+  for (; s + 1 + kStages < NS; s += 2) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      wait(kStages - 2);
+      stage(s + u + kStages);   // (into the place of step s + u, whose fragments every wave holds)
+      read(s + u + 1, wv[1 - u], xv[1 - u]);
+      mul(wv[u], xv[u]);
+    }
+  }
+  for (; s < NS; ++s) {
+    if (4 * s + 4 > NC) {   // past the end of the row: nothing
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+        if (4 * s + g >= NC) wv[0][t] = i32x4{0, 0, 0, 0};
+    }
+    mul(wv[0], xv[0]);
+    if (s + 1 < NS) {
+      wait(min(NS - 2 - s, kStages - 2));
+      if (s + kStages < NS) stage(s + kStages);
+      read(s + 1, wv[0], xv[0]);
+    }
   }
   f32x4 sc[4];
   float xs[4];
@@ -217,26 +208,27 @@ __global__ __launch_bounds__(256, 2) void gemm_tile_kernel(const GemmSeq a, int 
       for (int r = 0; r < 4; ++r) put4<BF16>(a, m0 + wt + 16 * t + j, n0 + wr + 16 * r + 4 * g, acc[r][t], xs[t], sc[r], wide);
 }
 
-template <bool BF16, int TT>
-void launch_rows(const GemmSeq& a, hipStream_t s) {
-  const int nt = (a.out + 15) / 16, mt = (a.tokens + 16 * TT - 1) / (16 * TT);
-  if ((int64_t)nt * mt >= 4096)
-    gemm_rows_kernel<BF16, 2, TT, 1><<<dim3((nt + 7) / 8, mt), 256, 0, s>>>(a);
-  else
-    gemm_rows_kernel<BF16, 1, TT, 4><<<dim3(nt, mt), 256, 0, s>>>(a);
-}
-
+// The form, by what was measured (us, weights from the L2s and the MALL).
+// Units of 16, 32 and 64 tokens, for 63 of them: 1024 -> 512 outputs 3.2, 3.8 and 4.8, 3584 -> 1024 5.5, 7.1 and 10.2,
+// 1024 -> 2048 4.1, 3.9 and 4.9, 1024 -> 7168 8.7, 8.0 and 7.4: the smallest that are at most a workgroup for each CU.
+// Units of 64 against tiles: 63 tokens 1024 -> 7168 (448 units) 7.4 and 7.7, 1024 -> 151936 60 and 35; 200 and 300 tokens
+// 1024 -> 2048 (512 and 640) 7.4 and 8.2, 9.2 and 8.3; 300 and 512 tokens 3584 -> 1024 (320 and 512) 16.9 and 17.2, 18.7
+// and 17.5.  Units of 16 against tiles, for 4, 8 and 16 tokens: 1024 -> 16384 (1024 units) 4.9 and 7.2, 5.3 and 7.4, 6.1
+// and 7.4; 1024 -> 32768 8.3 and 7.8, 9.0 and 7.8, 10.5 and 7.9; 1024 -> 151936 27 and 27, 31 and 27, 37 and 28.
 template <bool BF16>
 hipError_t launch(const GemmSeq& a, hipStream_t s) {
-  const int nt = (a.out + kBT - 1) / kBT, mt = (a.tokens + kBT - 1) / kBT;
-  if (a.tokens <= 16)
-    launch_rows<BF16, 1>(a, s);
-  else if (a.tokens <= 32)
-    launch_rows<BF16, 2>(a, s);
-  else if (a.tokens <= 64 || (int64_t)nt * mt < 64)
-    launch_rows<BF16, 4>(a, s);
-  else
+  const int rt = (a.out + 15) / 16;
+  auto units = [&](int tt) { return (int64_t)rt * ((a.tokens + 16 * tt - 1) / (16 * tt)); };
+  if (units(1) <= 256 || (a.tokens <= 16 && (a.tokens <= 4 || rt <= 1024)))
+    gemm_rows_kernel<BF16, 1><<<dim3(rt, (a.tokens + 15) / 16), 256, 0, s>>>(a);
+  else if (units(4) <= 512 && (a.tokens <= 32 || units(2) <= 256))
+    gemm_rows_kernel<BF16, 2><<<dim3(rt, (a.tokens + 31) / 32), 256, 0, s>>>(a);
+  else if (units(4) <= 512 || a.x.ld >= 1 << 24)
+    gemm_rows_kernel<BF16, 4><<<dim3(rt, (a.tokens + 63) / 64), 256, 0, s>>>(a);
+  else {
+    const int nt = (a.out + kBT - 1) / kBT, mt = (a.tokens + kBT - 1) / kBT;
     gemm_tile_kernel<BF16><<<(unsigned)((int64_t)nt * mt), 256, 0, s>>>(a, nt, mt);
+  }
   return hipGetLastError();
 }
 

@@ -65,6 +65,31 @@ def test_gemm(q, torch_cuda, tokens, out, inn, bf16):
     assert (got[tokens:] == 7).all() and (got[:, out:] == 7).all()
 
 
+@pytest.mark.parametrize("tokens,out,inn", [
+    (9, 16500, 16), (5, 16400, 80), (70, 4200, 48), (130, 2800, 208), (300, 2000, 272), (129, 2800, 336), (600, 1030, 400),
+    (16, 16390, 528), (24, 4100, 1008), (66, 2050, 96), (257, 100, 1040)])
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+def test_gemm_forms(q, torch_cuda, tokens, out, inn, bf16):
+    """Tiles whose inner dimension is shorter than the loads ahead or ends inside a step, few tokens among them; units
+    of 16, 32 and 64 tokens of both types."""
+    test_gemm(q, torch_cuda, tokens, out, inn, bf16)
+
+
+def test_gemm_rows_far_apart(q, torch_cuda):
+    """Activations' rows 16 MB apart and the last one behind 2^32 bytes."""
+    torch = torch_cuda
+    g, tokens, out, inn, ld = gen(torch, 5), 300, 2000, 48, 1 << 24
+    w = torch.randint(-127, 128, (out, inn), generator=g, dtype=torch.int8).cuda()
+    x = torch.randint(-127, 128, (tokens, inn), generator=g, dtype=torch.int8).cuda()
+    sw, sx = torch.rand(out, generator=g).cuda(), torch.rand(tokens, generator=g).cuda()
+    far = torch.empty((tokens - 1) * ld + inn, dtype=torch.int8, device="cuda").as_strided((tokens, inn), (ld, 1))
+    far.copy_(x)
+    y, want = torch.empty(tokens, out, device="cuda"), torch.empty(tokens, out, device="cuda")
+    q.gemm_i8_w8a8(want, w, sw, x, sx)
+    q.gemm_i8_w8a8(y, w, sw, far, sx)
+    assert torch.equal(y, want)
+
+
 def test_gemm_is_the_one_token_op(q, torch_cuda):
     torch = torch_cuda
     g = gen(torch, 3)
