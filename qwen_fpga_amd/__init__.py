@@ -519,39 +519,44 @@ def _type(t, what: str) -> int:
     raise TypeError(f"{what}: dtype {t.dtype}, expected float32 or bfloat16")
 
 
-def _r3(t, dt, shape, what: str):
-    """(address, row stride, head stride) of an operand [rows, heads, dim] of the given dtype and shape."""
+def _here(t) -> int:
+    """The current device if t is a tensor there, else a device that no tensor has (the checks below then look closer)."""
+    d = t.get_device() if t.__class__ is _Short.tensor else -1
+    return d if d >= 0 and (_Short.device is None or d == _Short.device()) else -2
+
+
+def _same(t, dt, shape, what: str, dev: int):
+    """Refuses all but a tensor on the current device (dev, from _here) of the given dtype and shape."""
+    if t.__class__ is _Short.tensor and t.dtype is dt and t.shape == shape and t.get_device() == dev:
+        return
     _on(t, what)
     if t.dtype is not dt:
         raise TypeError(f"{what}: dtype {t.dtype}, expected {dt}")
     if tuple(t.shape) != shape:
         raise ValueError(f"{what}: shape {tuple(t.shape)}, expected {shape}")
+
+
+def _r3(t, dt, shape, what: str, dev: int):
+    """(address, row stride, head stride) of an operand [rows, heads, dim] of the given dtype and shape."""
+    _same(t, dt, shape, what, dev)
     ld, hs, one = t.stride()
     if one != 1 and shape[2] > 1:
         raise ValueError(f"{what}: the last dimension has stride {one}, expected 1")
     return t.data_ptr(), ld, hs
 
 
-def _r2(t, dt, shape, what: str):
+def _r2(t, dt, shape, what: str, dev: int):
     """(address, row stride) of an operand [rows, dim]."""
-    _on(t, what)
-    if t.dtype is not dt:
-        raise TypeError(f"{what}: dtype {t.dtype}, expected {dt}")
-    if tuple(t.shape) != shape:
-        raise ValueError(f"{what}: shape {tuple(t.shape)}, expected {shape}")
+    _same(t, dt, shape, what, dev)
     ld, one = t.stride()
     if one != 1 and shape[1] > 1:
         raise ValueError(f"{what}: the last dimension has stride {one}, expected 1")
     return t.data_ptr(), ld
 
 
-def _c(t, dt, shape, what: str) -> int:
+def _c(t, dt, shape, what: str, dev: int) -> int:
     """Address of a contiguous tensor of the given dtype and shape."""
-    _on(t, what)
-    if t.dtype is not dt:
-        raise TypeError(f"{what}: dtype {t.dtype}, expected {dt}")
-    if tuple(t.shape) != shape:
-        raise ValueError(f"{what}: shape {tuple(t.shape)}, expected {shape}")
+    _same(t, dt, shape, what, dev)
     if not t.is_contiguous():
         raise ValueError(f"{what}: tensor is not contiguous")
     return t.data_ptr()
@@ -580,11 +585,12 @@ def gemm_i8_w8a8(y, w, scale, xq, sx, stream=None):
     float32 (gemv_i8_w8a8's bits) or bfloat16; xq and y may be slices of wider rows."""
     lib = _op("qh_gemm_i8_w8a8")
     tokens, out = _dims(y, 2, "y")
+    dev = _here(y)
     in_ = _dims(w, 2, "w")[1]
-    yp, ldy = _r2(y, y.dtype, (tokens, out), "y")
-    xp, ldx = _r2(xq, _Short.i8, (tokens, in_), "xq")
-    st = lib(yp, ldy, _type(y, "y"), _c(w, _Short.i8, (out, in_), "w"), _c(scale, _Short.f32, (out,), "scale"), xp, ldx,
-             _c(sx, _Short.f32, (tokens,), "sx"), tokens, out, in_, _st(stream))
+    yp, ldy = _r2(y, y.dtype, (tokens, out), "y", dev)
+    xp, ldx = _r2(xq, _Short.i8, (tokens, in_), "xq", dev)
+    st = lib(yp, ldy, _type(y, "y"), _c(w, _Short.i8, (out, in_), "w", dev), _c(scale, _Short.f32, (out,), "scale", dev), xp, ldx,
+             _c(sx, _Short.f32, (tokens,), "sx", dev), tokens, out, in_, _st(stream))
     if st:
         _check(st, "qh_gemm_i8_w8a8")
 
@@ -609,12 +615,12 @@ def delta_rule_seq(out, q, k, v, g, beta, S, cu, workspace, max_len: int, stream
     tokens, heads, _ = _dims(v, 3, "v")
     kh = _dims(k, 3, "k")[1]
     n = _dims(S, 4, "S")[0]
-    dt, ty = v.dtype, _type(v, "v")
-    gp, ldg = _r2(g, _Short.f32, (tokens, heads), "g")
-    bp, ldb = _r2(beta, _Short.f32, (tokens, heads), "beta")
-    st = lib(*_r3(out, dt, (tokens, heads, LV), "out"), *_r3(q, dt, (tokens, kh, LK), "q"), *_r3(k, dt, (tokens, kh, LK), "k"),
-             *_r3(v, dt, (tokens, heads, LV), "v"), ty, gp, ldg, bp, ldb, _c(S, _Short.f32, (n, heads, LK, LV), "S"),
-             _c(cu, _Short.i32, (n + 1,), "cu"), n, tokens, int(max_len), kh, heads, *_ws(workspace), _st(stream))
+    dt, ty, dev = v.dtype, _type(v, "v"), _here(v)
+    gp, ldg = _r2(g, _Short.f32, (tokens, heads), "g", dev)
+    bp, ldb = _r2(beta, _Short.f32, (tokens, heads), "beta", dev)
+    st = lib(*_r3(out, dt, (tokens, heads, LV), "out", dev), *_r3(q, dt, (tokens, kh, LK), "q", dev), *_r3(k, dt, (tokens, kh, LK), "k", dev),
+             *_r3(v, dt, (tokens, heads, LV), "v", dev), ty, gp, ldg, bp, ldb, _c(S, _Short.f32, (n, heads, LK, LV), "S", dev),
+             _c(cu, _Short.i32, (n + 1,), "cu", dev), n, tokens, int(max_len), kh, heads, *_ws(workspace), _st(stream))
     if st:
         _check(st, "qh_delta_rule_seq")
 
@@ -642,10 +648,10 @@ def attention_seq(out, q, k, v, cu_q, k_start, k_len, workspace, max_q: int, max
     rows, heads, d = _dims(q, 3, "q")
     krows, kvh, _ = _dims(k, 3, "k")
     n = _dims(k_len, 1, "k_len")[0]
-    dt, ty = q.dtype, _type(q, "q")
-    st = lib(*_r3(out, dt, (rows, heads, d), "out"), *_r3(q, dt, (rows, heads, d), "q"), *_r3(k, dt, (krows, kvh, d), "k"),
-             *_r3(v, dt, (krows, kvh, d), "v"), ty, _c(cu_q, _Short.i32, (n + 1,), "cu_q"), _c(k_start, _Short.i64, (n,), "k_start"),
-             _c(k_len, _Short.i32, (n,), "k_len"), n, rows, krows, int(max_q), int(max_k), heads, kvh, d,
+    dt, ty, dev = q.dtype, _type(q, "q"), _here(q)
+    st = lib(*_r3(out, dt, (rows, heads, d), "out", dev), *_r3(q, dt, (rows, heads, d), "q", dev), *_r3(k, dt, (krows, kvh, d), "k", dev),
+             *_r3(v, dt, (krows, kvh, d), "v", dev), ty, _c(cu_q, _Short.i32, (n + 1,), "cu_q", dev), _c(k_start, _Short.i64, (n,), "k_start", dev),
+             _c(k_len, _Short.i32, (n,), "k_len", dev), n, rows, krows, int(max_q), int(max_k), heads, kvh, d,
              float(d ** -0.5 if scale is None else scale), *_ws(workspace), _st(stream))
     if st:
         _check(st, "qh_attention_seq")
