@@ -422,16 +422,19 @@ __global__ __launch_bounds__(1024) void attn_join_kernel(const AttnSeq a) {
 
 // The work of the form for prompts.  A tile is TILE rows of a sequence (tokens x query heads of one kv head) over all
 // the keys they see.  The keys of a tile that sees more than `chunk` of them are split into equal units of at most a
-// chunk, whose sums meet in the workspace; the other tiles are a unit each.  The chunk is about the keys of all tiles
-// over the CUs (but at least min_tile_chunk, and a 64th of the sequence), so that no unit is much longer than a CU's
-// share.  Units start in order, unit b on XCD b % 8: so the longest come first, and neighbours are about equally long.
+// chunk, whose sums meet in the workspace; the other tiles are a unit each.  The chunk is the keys of all tiles over 192
+// CUs, in fp32 over those that half a unit a tile leaves if they are more (but at least min_tile_chunk, and a 64th of
+// the sequence).  The units then come to at most about one for each CU: a few more would start when the first ones end
+// and take as long again (1500 tokens of fp32: 250 units 121 us, 294 units 165).  fp32, whose units are long, over 192
+// and over what is left: 512 tokens behind 7488 keys 347 and 279 us, 1500 tokens 122 and 116; bfloat16 66 and 72 for
+// 512 behind 7488, 53 and 61 for 256 behind 7744 (more units to join).  Units start in order, unit b on XCD b % 8: so
+// the longest come first, and neighbours are about equally long.
 // The workgroups of an XCD then walk the keys of one head side by side and find them in its L2: shares cut to the same
 // length anywhere in the tiles missed it for 38% of the reads and took 450 us, not 390, for 16k packed tokens (8 / 2
 // heads of 256).
 // Split and whole, bfloat16: one sequence of 8000 tokens 307 and 350 us, 4096 106 and 165, 1024 44 and 55, 512 36 and
-// 36; two of 8000 478 and 498; those 16k tokens 383 and 390.  Chunks of a 256th instead of a 192nd of the work: 410 us
-// for the 16k, 165 instead of 127 for 1500 tokens of fp32 (units beyond the CUs start when the first ones end).
-constexpr int kTileFill = 192, kMaxTileSplits = 64;
+// 36; two of 8000 478 and 498; those 16k tokens 383 and 390.
+constexpr int kCUs = 256, kMaxTileSplits = 64;
 constexpr int min_tile_chunk(bool bf16) { return bf16 ? 256 : 128; }
 struct TileUnit {
   SeqSpan sp;
@@ -459,15 +462,17 @@ __device__ __forceinline__ bool find_tile_unit(const AttnSeq& a, int b, TileUnit
     return nt * past + (nt + 1) * min(k, (int64_t)sp.len) / 2;
   };
   load(0);
-  int64_t all = nt > 0 ? work() : 0;
+  int64_t all = nt > 0 ? work() : 0, tiles = nt;
   for (int s0 = 64; s0 < a.n_seq; s0 += 64) {
     load(s0);
     all += nt > 0 ? work() : 0;
+    tiles += nt;
   }
   if (a.n_seq > 64) load(0);
 #pragma unroll
-  for (int d = 1; d < 64; d *= 2) all += __shfl_xor(all, d);
-  const int64_t share = max((all * a.kv_heads + kTileFill - 1) / kTileFill, (int64_t)min_tile_chunk(a.bf16));
+  for (int d = 1; d < 64; d *= 2) all += __shfl_xor(all, d), tiles += __shfl_xor(tiles, d);
+  const int fill = kCUs - (a.bf16 ? kCUs / 4 : (int)min(tiles * a.kv_heads / 2, (int64_t)kCUs / 4));
+  const int64_t share = max((all * a.kv_heads + fill - 1) / fill, (int64_t)min_tile_chunk(a.bf16));
   int base = 0, slots = 0;   // of the next sequence: units (JOIN: split tiles), the split tiles' units
   for (int s0 = 0; s0 < a.n_seq; s0 += 64) {
     if (s0 > 0) load(s0);
@@ -529,8 +534,8 @@ constexpr size_t tile_part_floats(int tile, int D) { return (size_t)tile * (D + 
 // rarely rescaled.
 // bfloat16: at full load the card's power bounds it (1.85 GHz): 930 to 1100 TFLOP/s at 256 elements and long prompts,
 // 830 at 128.  With 64 rows a wave, 128 elements took 301 us for 8000 tokens of 8 heads, and 32 rows take 190.
-// fp32: the fp32 MFMAs bound it, 89% of their cycles at 2.15 GHz; 1500 tokens 206 us in the form for few rows, 127 in
-// this, of which the join takes 10 and a CU has work for 84; 4096 tokens 98 TFLOP/s.
+// fp32: the fp32 MFMAs bound it, 89% of their cycles at 2.15 GHz; 1500 tokens 159 us in the form for few rows, 116 in
+// this, of which the join takes 10 and a CU has work for 84; 512 tokens behind 7488 keys 116 TFLOP/s.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 
@@ -886,7 +891,7 @@ AttnForm attn_seq_form(int64_t q_rows, int n_seq, int max_q, int max_k, int head
     // two workspace places a CU: the chunks are such that more are hardly ever taken
     if (max_k > min_tile_chunk(bf16)) {
       const int64_t splits = max_k / min_tile_chunk(bf16) + 1;
-      f.limit = (int)std::min<int64_t>(2 * kTileFill, tiles * std::min<int64_t>(splits, kMaxTileSplits));
+      f.limit = (int)std::min<int64_t>(2 * kCUs, tiles * std::min<int64_t>(splits, kMaxTileSplits));
     }
     f.bytes = (size_t)f.limit * tile_part_floats(f.tile, dim) * sizeof(float);
   } else if (max_k > kMinChunk) {
