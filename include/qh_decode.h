@@ -251,7 +251,8 @@ int qh_gemm_i8_w8a8(void* y, int64_t ldy, int type, const int8_t* w, const float
 /* The gated delta rule (qh_delta_rule_layer) along each sequence: q, k [tokens][k_heads][128], v, out
  * [tokens][heads][128] of `type`, g (the log of the decay, at most 0) and beta [tokens][heads] fp32 with rows ldg and
  * ldb apart (any alignment), state [n_seq][heads][128][128] fp32 read and updated in place.  Value head h takes key
- * head h / (heads / k_heads).  q and k as the caller normalised them.  An empty sequence keeps its state. */
+ * head h / (heads / k_heads).  q and k as the caller normalised them.  An empty sequence keeps its state.
+ * n_seq * heads: up to 900000. */
 size_t qh_delta_rule_seq_workspace(int tokens, int n_seq, int heads, int k_heads, int type, int max_len);
 int qh_delta_rule_seq(void* out, int64_t ldo, int64_t hso, const void* q, int64_t ldq, int64_t hsq, const void* k, int64_t ldk,
                       int64_t hsk, const void* v, int64_t ldv, int64_t hsv, int type, const float* g, int64_t ldg,
@@ -263,7 +264,7 @@ int qh_delta_rule_seq(void* out, int64_t ldo, int64_t hso, const void* q, int64_
  * cache of several), the new tokens' own among them: row r of q_len sees the first r + 1 + k_len - q_len.
  * out = softmax(scale q k^T) v over those; 0 for a row that sees none; NaN for the rows of a sequence whose keys
  * do not lie inside the array.  Keys a row does not see have no influence on it, whatever they hold.
- * Query head h takes kv head h / (heads / kv_heads). */
+ * Query head h takes kv head h / (heads / kv_heads).  q_rows * heads + 16 * n_seq * kv_heads: up to 64 million. */
 size_t qh_attention_seq_workspace(int q_rows, int n_seq, int max_q, int max_k, int heads, int kv_heads, int head_dim,
                                   int type);
 int qh_attention_seq(void* out, int64_t ldo, int64_t hso, const void* q, int64_t ldq, int64_t hsq, const void* k, int64_t ldk,

@@ -22,7 +22,6 @@ namespace qh {
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -83,15 +82,6 @@ __device__ __forceinline__ void store1(void* p, int64_t at, float v) {
     as_global_w(static_cast<float*>(p))[at] = v;
 }
 
-template <bool BF16>
-__device__ __forceinline__ f32x4 load4(const void* p, int64_t at) {
-  if constexpr (BF16) {
-    const bf16x4 t = *as_global(reinterpret_cast<const bf16x4*>(static_cast<const __bf16*>(p) + at));
-    return f32x4{(float)t[0], (float)t[1], (float)t[2], (float)t[3]};
-  } else {
-    return *as_global(reinterpret_cast<const f32x4*>(static_cast<const float*>(p) + at));
-  }
-}
 __device__ __forceinline__ bool finite(float v) { return (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u; }
 __device__ __forceinline__ f32x4 mfma4(f32x4 x, f32x4 y, f32x4 c) {   // four depths
 #pragma unroll

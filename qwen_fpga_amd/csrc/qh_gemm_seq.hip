@@ -112,7 +112,7 @@ __global__ __launch_bounds__(256) void gemm_rows_kernel(const GemmSeq a) {
 constexpr int kBT = 128, kStages = 4, kStageBytes = 2 * kBT * 64;
 
 template <bool BF16>
-__global__ __launch_bounds__(256, 2) void gemm_tile_kernel(const GemmSeq a, int nt, int mt) {
+__global__ __launch_bounds__(256, 2) void gemm_tile_kernel(const GemmSeq a, int mt) {
   __shared__ __attribute__((aligned(16))) int8_t lds[kStages * kStageBytes];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, j = lane & 15;
@@ -227,7 +227,7 @@ hipError_t launch(const GemmSeq& a, hipStream_t s) {
     gemm_rows_kernel<BF16, 4><<<dim3(rt, (a.tokens + 63) / 64), 256, 0, s>>>(a);
   else {
     const int nt = (a.out + kBT - 1) / kBT, mt = (a.tokens + kBT - 1) / kBT;
-    gemm_tile_kernel<BF16><<<(unsigned)((int64_t)nt * mt), 256, 0, s>>>(a, nt, mt);
+    gemm_tile_kernel<BF16><<<(unsigned)((int64_t)nt * mt), 256, 0, s>>>(a, mt);
   }
   return hipGetLastError();
 }

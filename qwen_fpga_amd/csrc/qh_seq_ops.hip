@@ -12,8 +12,11 @@ namespace {
 hipStream_t S(void* s) { return reinterpret_cast<hipStream_t>(s); }
 
 constexpr int64_t kMaxStride = (int64_t)1 << 40;   // elements; keeps every offset inside 64 bits
-constexpr int64_t kMaxUnits = 0x7fffffff;          // workgroups, and rows times heads
+constexpr int64_t kMaxUnits = 0x7fffffff;          // rows times heads
 constexpr int kMaxGridY = 65535;
+// A grid's threads in one direction stay below 2^32.
+constexpr int64_t kMaxStates = 900000;             // sequences times heads: 8 workgroups of 576 each
+constexpr int64_t kMaxTiles = 4000000;             // tiles of 16 rows and a kv head: a workgroup of 1024 each
 
 // An operand [rows][heads][dim] with its element size, to check it and to compare it with another.
 struct View {
@@ -87,7 +90,7 @@ int qh_gemm_i8_w8a8(void* y, int64_t ldy, int type, const int8_t* w, const float
 }
 
 size_t qh_delta_rule_seq_workspace(int tokens, int n_seq, int heads, int k_heads, int type, int max_len) {
-  if (tokens <= 0 || n_seq <= 0 || heads <= 0 || k_heads <= 0 || !type_ok(type) || (int64_t)n_seq * heads * 8 > kMaxUnits ||
+  if (tokens <= 0 || n_seq <= 0 || heads <= 0 || k_heads <= 0 || !type_ok(type) || (int64_t)n_seq * heads > kMaxStates ||
       (int64_t)tokens * heads > kMaxUnits)
     return 0;
   return delta_seq_workspace(tokens, n_seq, heads, k_heads, type == QH_BF16, max_len);
@@ -100,7 +103,7 @@ int qh_delta_rule_seq(void* out, int64_t ldo, int64_t hso, const void* q, int64_
   if (!type_ok(type) || n_seq < 0 || tokens < 0 || max_len < 0 || k_heads <= 0 || heads <= 0 || heads % k_heads != 0)
     return QH_EINVAL;
   if (tokens == 0 || n_seq == 0) return QH_OK;
-  if ((int64_t)n_seq * heads * 8 > kMaxUnits || (int64_t)tokens * heads > kMaxUnits || heads > kMaxGridY) return QH_ERANGE;
+  if ((int64_t)n_seq * heads > kMaxStates || (int64_t)tokens * heads > kMaxUnits || heads > kMaxGridY) return QH_ERANGE;
   const int eb = type == QH_BF16 ? 2 : 4;
   const View vo{out, tokens, heads, QH_LV, ldo, hso, eb}, vq{q, tokens, k_heads, QH_LK, ldq, hsq, eb},
       vk{k, tokens, k_heads, QH_LK, ldk, hsk, eb}, vv{v, tokens, heads, QH_LV, ldv, hsv, eb};
@@ -137,8 +140,8 @@ int qh_delta_rule_seq(void* out, int64_t ldo, int64_t hso, const void* q, int64_
 }
 
 size_t qh_attention_seq_workspace(int q_rows, int n_seq, int max_q, int max_k, int heads, int kv_heads, int head_dim, int type) {
-  if (!type_ok(type) || q_rows <= 0 || n_seq <= 0 || max_q < 0 || max_k < 0 || max_k > kMaxKeys || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 ||
-      (head_dim != 128 && head_dim != 256) || (int64_t)q_rows * heads > kMaxUnits)
+  if (!type_ok(type) || q_rows <= 0 || n_seq <= 0 || max_q < 0 || max_k < 0 || max_k > kMaxKeys || heads <= 0 || kv_heads <= 0 ||
+      heads % kv_heads != 0 || (head_dim != 128 && head_dim != 256) || (int64_t)q_rows * heads > kMaxUnits)
     return 0;
   return attn_seq_form(q_rows, n_seq, max_q, max_k, heads, kv_heads, head_dim, type == QH_BF16).bytes;
 }
@@ -151,7 +154,8 @@ int qh_attention_seq(void* out, int64_t ldo, int64_t hso, const void* q, int64_t
       heads % kv_heads != 0 || (head_dim != 128 && head_dim != 256) || !std::isfinite(scale))
     return QH_EINVAL;
   if (q_rows == 0 || n_seq == 0) return QH_OK;
-  if (max_k > kMaxKeys || (int64_t)q_rows * heads > kMaxUnits || (int64_t)n_seq * heads > kMaxUnits || k_rows >= kMaxStride)
+  if (max_k > kMaxKeys || (int64_t)q_rows * heads > kMaxUnits || k_rows >= kMaxStride ||
+      seq_tiles_max((int64_t)q_rows * (heads / kv_heads), n_seq, 16) * kv_heads > kMaxTiles)
     return QH_ERANGE;
   const int eb = type == QH_BF16 ? 2 : 4;
   const View vo{out, q_rows, heads, head_dim, ldo, hso, eb}, vq{q, q_rows, heads, head_dim, ldq, hsq, eb},

@@ -595,6 +595,51 @@ def test_attention_of_many_sequences(q, torch_cuda, bf16, max_q):
     attn_check(torch, got, attn_oracle(torch, qq, kk, vv, lens, ctx, at_k, 1 / math.sqrt(128)), bf16)
 
 
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+def test_prompt_forms_captured(q, torch_cuda, bf16):
+    """Chunks of the delta rule and split tiles of attention in one graph, replayed with other bounds, key ranges and
+    inputs on the device and eager calls between; every replay against the eager result."""
+    torch = torch_cuda
+    rows, h, kvh, d, dt = 700, 8, 2, 128, torch.bfloat16 if bf16 else torch.float32
+    g = gen(torch, 12)
+    rnd = lambda *s: torch.randn(*s, generator=g).to(dt).cuda()
+    qq, kk, vv, out = rnd(rows, h, d), rnd(2000, kvh, d), rnd(2000, kvh, d), torch.empty(rows, h, d, dtype=dt, device="cuda")
+    dk, dv, dout = torch.nn.functional.normalize(rnd(rows, 4, 128).float(), dim=-1).to(dt), rnd(rows, h, 128), rnd(rows, h, 128)
+    lg, be = -torch.rand(rows, h, generator=g).cuda(), torch.rand(rows, h, generator=g).cuda()
+    S0 = torch.randn(3, h, 128, 128, generator=g).cuda()
+    S = S0.clone()
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    cu, ks, kl = i32([0, 500, 500, 700]), torch.tensor([0, 0, 900], dtype=torch.int64, device="cuda"), i32([1500, 0, 300])
+    aw = torch.empty(q.attention_seq_workspace(rows, 3, rows, 2000, h, kvh, d), dtype=torch.uint8, device="cuda")
+    dw = torch.empty(q.delta_rule_seq_workspace(rows, 3, h, rows, k_heads=4, dtype=q.BF16 if bf16 else q.F32), dtype=torch.uint8, device="cuda")
+
+    def step():
+        q.attention_seq(out, qq, kk, vv, cu, ks, kl, aw, 4096, 2000)
+        q.delta_rule_seq(dout, dk, dk, dv, lg, be, S, cu, dw, rows)
+
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for bounds, at, n in (([0, 500, 500, 700], [0, 0, 900], [1500, 0, 300]), ([0, 3, 690, 700], [100, 0, 1990], [1800, 687, 10]),
+                          ([0, 0, 1, 1], [0, 5, 0], [0, 2000, 0])):
+        cu.copy_(i32(bounds))
+        ks.copy_(torch.tensor(at, device="cuda"))
+        kl.copy_(i32(n))
+        qq.copy_(rnd(rows, h, d))
+        want = []
+        for run in (step, graph.replay, graph.replay):
+            S.copy_(S0)
+            out.fill_(7.0), dout.fill_(7.0)
+            run()
+            torch.cuda.synchronize()
+            want.append([x.clone() for x in (out, dout, S)])
+        for got in want[1:]:     # (the last sequence's keys end behind the array: NaN, in every run)
+            assert all(((x == y) | (x.isnan() & y.isnan())).all() for x, y in zip(got, want[0]))
+        assert torch.isnan(want[0][0]).any() == (n[1] == 2000) and torch.isfinite(want[0][1]).all()
+        assert (want[0][0][bounds[-1]:] == 7).all() and (want[0][1][bounds[-1]:] == 7).all()
+
+
 # ------------------------------------------------------------------ calls that cannot be answered
 
 def test_refused_tensors(q, torch_cuda):

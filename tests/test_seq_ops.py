@@ -170,6 +170,12 @@ def test_attention_nothing_to_do_ranges_and_workspace(q, args):
     assert q.attention_seq_workspace(0, 1, 1, 100000, 2, 1, 128) == 0
 
 
+def test_more_workgroups_than_a_grid_has(q, args):
+    assert args.delta(n_seq=450001) == q.QH_ERANGE
+    assert q.delta_rule_seq_workspace(1000, 450001, 2, 1000, k_heads=1) == 0
+    assert args.attn(q_rows=33000000) == q.QH_ERANGE and args.attn(q_rows=4100000, n_seq=4100000) == q.QH_ERANGE
+
+
 def test_interleaved_slices_are_no_overlap(q, args):
     """Columns of one buffer: refused where they meet, taken (as far as the next refusal) where they do not."""
     at = args.at(0)
