@@ -227,7 +227,8 @@ int qh_mlp_layer_w8a8(float* out, const float* x, const qh_tensor* gate_w, const
  * Sequences stand one after another: sequence i has the rows cu[i] .. cu[i + 1]
  * (cu [n_seq + 1] int32, on the device).  Empty sequences are allowed; rows
  * outside every sequence are left as they were; a sequence whose bounds are out
- * of order or outside the array is taken as empty.  max_len, max_q and max_k
+ * of order or outside the array is taken as empty (and rows that two sequences
+ * then share hold nothing in particular).  max_len, max_q and max_k
  * are the caller's bounds on the lengths: they choose the form of the kernels
  * and the size of the workspace, longer sequences are computed all the same.
  *
