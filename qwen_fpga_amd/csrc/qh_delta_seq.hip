@@ -245,9 +245,11 @@ __device__ __forceinline__ void put_operand(float* to, int lane, const f32x4& x,
 }
 
 // T, P and the row factors of one chunk, for the value heads of one key head.  Wave i forms the tiles (i, j <= i) of
-// K K^T and Q K^T once; every head scales them.
+// K K^T and Q K^T once; every head scales them.  A head's inputs are brought while the products of the one before run.
+// What bounds it: for one sequence of 1500 tokens (384 workgroups, all at once, 21 us) k and q's way from memory, 7 us, and
+// a chain of short steps; for 7.2k packed tokens of 32 heads 78 us, three workgroups a CU (two: 82).
 template <bool BF16>
-__global__ __launch_bounds__(256) void delta_chunk_kernel(const DeltaSeq a) {
+__global__ __launch_bounds__(256, BF16 ? 3 : 2) void delta_chunk_kernel(const DeltaSeq a) {
   constexpr int LD = kC + 4, NP = Parts<BF16>::NP;
   __shared__ __attribute__((aligned(256))) char kl[NP * kPart < kC * LD * 4 ? kC * LD * 4 : NP * kPart];
   __shared__ __attribute__((aligned(16))) float al[kC * LD];   // A
@@ -262,16 +264,37 @@ __global__ __launch_bounds__(256) void delta_chunk_kernel(const DeltaSeq a) {
   const int hk = blockIdx.y, rep = a.heads / a.k_heads;
   const int t0 = at.sp.start + kC * at.tile, n = min(kC, at.sp.start + at.sp.len - t0);   // n >= 1 tokens
   bool bad = false;
+  // a value head's inputs, brought while the products before it run
+  constexpr int NV = kC * kD / 8 / 256;
+  Raw8<BF16> vr[NV];
+  float gv = 0.0f, be0 = 0.0f;
+  auto load_head = [&](int h) {
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+      const int e = 256 * u + threadIdx.x;
+      vr[u] = raw8<BF16>(a.v.p, (int64_t)(t0 + min(e >> 4, n - 1)) * a.v.ld + h * a.v.hs + 8 * (e & 15));
+    }
+    if (wave == 0) {
+      gv = as_global(a.g)[(int64_t)(t0 + min(lane, n - 1)) * a.ldg + h];
+      be0 = as_global(a.beta)[(int64_t)(t0 + min(lane, n - 1)) * a.ldb + h];
+    }
+  };
   f32x4 G[4], P[4];   // tile (wave, jj): lane's token t = 16 wave + l % 16, tokens j = 16 jj + 4 (l / 16) ..
   {
     const int64_t r = t0 + min(16 * wave + j, n - 1);
     Parts<BF16> kp[4], qp[4];
+    Raw8<BF16> kr[4], qr[4];   // (all on their way before the first store, which no load may pass)
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-      const Raw8<BF16> kr = raw8<BF16>(a.k.p, r * a.k.ld + hk * a.k.hs + 32 * s + 8 * g), qr = raw8<BF16>(a.q.p, r * a.q.ld + hk * a.q.hs + 32 * s + 8 * g);
-      bad |= any_non_finite<BF16>(kr) || any_non_finite<BF16>(qr);
-      kp[s] = parts<BF16>(kr);
-      qp[s] = parts<BF16>(qr);
+      kr[s] = raw8<BF16>(a.k.p, r * a.k.ld + hk * a.k.hs + 32 * s + 8 * g);
+      qr[s] = raw8<BF16>(a.q.p, r * a.q.ld + hk * a.q.hs + 32 * s + 8 * g);
+    }
+    load_head(hk * rep);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      bad |= any_non_finite<BF16>(kr[s]) || any_non_finite<BF16>(qr[s]);
+      kp[s] = parts<BF16>(kr[s]);
+      qp[s] = parts<BF16>(qr[s]);
 #pragma unroll
       for (int p = 0; p < NP; ++p) {
         const int at_k = p * kPart + key_at(16 * wave + j, 4 * s + g);
@@ -302,14 +325,13 @@ __global__ __launch_bounds__(256) void delta_chunk_kernel(const DeltaSeq a) {
     bad = bad_qk;
     if (wave == 0) {
       // a log decay below -1e5 is 0 as a factor like any below -104, and finite in the sums
-      float gv = 0.0f, be = 0.0f;
+      float gl = 0.0f, be = 0.0f;
       if (lane < n) {
-        gv = as_global(a.g)[(t0 + lane) * a.ldg + h];
-        be = as_global(a.beta)[(t0 + lane) * a.ldb + h];
-        if (gv < -1e5f) gv = -1e5f;
-        bad |= !finite(gv) || !finite(be);
+        gl = gv < -1e5f ? -1e5f : gv;
+        be = be0;
+        bad |= !finite(gl) || !finite(be);
       }
-      double c = gv;
+      double c = gl;
 #pragma unroll
       for (int d = 1; d < kC; d *= 2) {
         const double t = __shfl_up(c, d);
@@ -326,10 +348,8 @@ __global__ __launch_bounds__(256) void delta_chunk_kernel(const DeltaSeq a) {
       if (lane == kC - 1) ws[kOffFlag + 1] = ec;
     }
 #pragma unroll
-    for (int u = 0; u < kC * kD / 8 / 256; ++u) {
-      const int e = 256 * u + threadIdx.x;
-      bad |= any_non_finite<BF16>(raw8<BF16>(a.v.p, (int64_t)(t0 + min(e >> 4, n - 1)) * a.v.ld + h * a.v.hs + 8 * (e & 15)));
-    }
+    for (int u = 0; u < NV; ++u) bad |= any_non_finite<BF16>(vr[u]);
+    if (h + 1 < (hk + 1) * rep) load_head(h + 1);
     const uint64_t any = __ballot(bad);
     if (lane == 0) bad_in[wave] = any != 0;
     __syncthreads();
