@@ -640,6 +640,43 @@ def test_prompt_forms_captured(q, torch_cuda, bf16):
         assert (want[0][0][bounds[-1]:] == 7).all() and (want[0][1][bounds[-1]:] == 7).all()
 
 
+def apart(torch, x, ld):
+    """x's rows `ld` elements apart, the last ones behind 2^32 bytes."""
+    far = torch.empty((x.shape[0] - 1) * ld + x[0].numel(), dtype=x.dtype, device="cuda")
+    far = far.as_strided(x.shape, (ld, x.stride(1), 1))
+    far.copy_(x)
+    return far
+
+
+@pytest.mark.parametrize("ld", [1 << 21, 1 << 24])     # (from 2^24 on: the form for few rows)
+@pytest.mark.parametrize("max_q", [1, 4096])
+def test_attention_rows_far_apart(q, torch_cuda, ld, max_q):
+    torch = torch_cuda
+    rows = 1100 if ld == 1 << 21 else 300
+    lens, ctx = [40, 1, 200], [rows, 250, rows - 60]
+    qq, kk, vv, _ = attn_inputs(torch, 13, lens, [rows], 4, 2, 128, True)
+    at_k = [0, rows - 250, 60]
+    want = attn_oracle(torch, qq, kk, vv, lens, ctx, at_k, 1 / math.sqrt(128))
+    far = [apart(torch, x.cuda(), ld) for x in (kk, vv)]
+    attn_check(torch, attn_run(q, torch, qq.cuda(), *far, lens, ctx, at_k, max_q=max_q), want, True)
+
+
+@pytest.mark.parametrize("max_len", [1, 1100])
+def test_delta_rows_far_apart(q, torch_cuda, max_len):
+    torch = torch_cuda
+    g, t, h, ld = gen(torch, 14), 1100, 2, 1 << 20
+    n = lambda *s: torch.randn(*s, generator=g).cuda()
+    qq, kk, vv = (torch.nn.functional.normalize(n(t, h, 128), dim=-1) for _ in range(3))
+    lg, be, cu = -torch.rand(t, h, generator=g).cuda(), torch.rand(t, h, generator=g).cuda(), torch.tensor([0, 70, 1100], dtype=torch.int32, device="cuda")
+    ws = torch.empty(q.delta_rule_seq_workspace(t, 2, h, max_len), dtype=torch.uint8, device="cuda")
+    res = []
+    for f in (lambda x: x, lambda x: apart(torch, x, ld)):
+        S, out = torch.ones(2, h, 128, 128, device="cuda"), f(torch.empty_like(vv))
+        q.delta_rule_seq(out, f(qq), f(kk), f(vv), lg, be, S, cu, ws, max_len)
+        res.append((out.contiguous(), S))
+    assert torch.equal(res[0][0], res[1][0]) and torch.equal(res[0][1], res[1][1])
+
+
 # ------------------------------------------------------------------ calls that cannot be answered
 
 def test_refused_tensors(q, torch_cuda):
@@ -676,6 +713,39 @@ def test_refused_tensors(q, torch_cuda):
         q.attention_seq(z(4, 2, 64), z(4, 2, 64), z(9, 1, 64), z(9, 1, 64), cu, ks, kl, None, 4, 9)
     with pytest.raises(q.QHError):
         q.attention_seq(a, a, z(9, 1, 128), z(9, 1, 128), cu, ks, kl, None, 4, 9)
+
+
+def test_tensors_elsewhere(q, torch_cuda, monkeypatch):
+    """Operands in host memory or on another device than the current one are refused, each of them; module parameters
+    are tensors like others; a workspace that is too small is refused."""
+    torch = torch_cuda
+    z = lambda *s, dt=torch.float32: torch.zeros(*s, dtype=dt, device="cuda")
+    i8 = torch.int8
+    ops = [z(4, 32), z(32, 64, dt=i8), z(32), z(4, 64, dt=i8), z(4)]
+    for i in range(5):
+        with pytest.raises(TypeError):
+            q.gemm_i8_w8a8(*[x.cpu() if k == i else x for k, x in enumerate(ops)])
+    q.gemm_i8_w8a8(*[torch.nn.Parameter(x, requires_grad=False) for x in ops])
+    a, kv, cu, ks, kl = z(4, 2, 128), z(9, 1, 128), z(2, dt=torch.int32), z(1, dt=torch.int64), z(1, dt=torch.int32)
+    d, S, g = z(4, 2, 128), z(1, 2, 128, 128), z(4, 2)
+    attn = [z(4, 2, 128), a, kv, z(9, 1, 128), cu, ks, kl]
+    delta = [d, a, z(4, 2, 128), z(4, 2, 128), g, z(4, 2), S, cu]
+    for i in range(len(attn)):
+        with pytest.raises(TypeError):
+            q.attention_seq(*[x.cpu() if k == i else x for k, x in enumerate(attn)], None, 4, 9)
+    for i in range(len(delta)):
+        with pytest.raises(TypeError):
+            q.delta_rule_seq(*[x.cpu() if k == i else x for k, x in enumerate(delta)], None, 4)
+    with pytest.raises(TypeError):
+        q.attention_seq(*attn, torch.empty(64, dtype=torch.uint8), 4, 9)
+    with pytest.raises(q.QHError):
+        q.attention_seq(*attn, torch.empty(256, dtype=torch.uint8, device="cuda"), 4, 1000)
+    with pytest.raises(q.QHError):
+        q.delta_rule_seq(*delta, torch.empty(256, dtype=torch.uint8, device="cuda"), 1000)
+    monkeypatch.setattr(q._Short, "device", lambda: 1)
+    for call in (lambda: q.gemm_i8_w8a8(*ops), lambda: q.attention_seq(*attn, None, 4, 9), lambda: q.delta_rule_seq(*delta, None, 4)):
+        with pytest.raises(ValueError):
+            call()
 
 
 # ------------------------------------------------------------------ streams, graphs, together
