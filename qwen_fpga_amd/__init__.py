@@ -508,7 +508,6 @@ def _on(t, what: str):
         raise TypeError(f"{what}: expected a torch CUDA tensor, got {getattr(t, 'device', type(t).__name__)}")
     if _Short.device is not None and t.get_device() != _Short.device():
         raise ValueError(f"{what}: tensor is on {t.device}, the current device is {_Short.device()}")
-    return t
 
 
 def _type(t, what: str) -> int:
@@ -520,46 +519,24 @@ def _type(t, what: str) -> int:
 
 
 def _here(t) -> int:
-    """The current device if t is a tensor there, else a device that no tensor has (the checks below then look closer)."""
+    """The current device if t is a tensor there, else a device that no tensor has."""
     d = t.get_device() if t.__class__ is _Short.tensor else -1
     return d if d >= 0 and (_Short.device is None or d == _Short.device()) else -2
 
 
-def _same(t, dt, shape, what: str, dev: int):
-    """Refuses all but a tensor on the current device (dev, from _here) of the given dtype and shape."""
-    if t.__class__ is _Short.tensor and t.dtype is dt and t.shape == shape and t.get_device() == dev:
-        return
+# The calls below compare all operands in one expression, which is most of what they cost the host; where it
+# does not hold, _operand looks at each (and raises what is wrong with it, or takes a tensor of another class).
+def _operand(t, dt, shape, what: str, rows: bool = False):
     _on(t, what)
     if t.dtype is not dt:
         raise TypeError(f"{what}: dtype {t.dtype}, expected {dt}")
-    if tuple(t.shape) != shape:
-        raise ValueError(f"{what}: shape {tuple(t.shape)}, expected {shape}")
-
-
-def _r3(t, dt, shape, what: str, dev: int):
-    """(address, row stride, head stride) of an operand [rows, heads, dim] of the given dtype and shape."""
-    _same(t, dt, shape, what, dev)
-    ld, hs, one = t.stride()
-    if one != 1 and shape[2] > 1:
-        raise ValueError(f"{what}: the last dimension has stride {one}, expected 1")
-    return t.data_ptr(), ld, hs
-
-
-def _r2(t, dt, shape, what: str, dev: int):
-    """(address, row stride) of an operand [rows, dim]."""
-    _same(t, dt, shape, what, dev)
-    ld, one = t.stride()
-    if one != 1 and shape[1] > 1:
-        raise ValueError(f"{what}: the last dimension has stride {one}, expected 1")
-    return t.data_ptr(), ld
-
-
-def _c(t, dt, shape, what: str, dev: int) -> int:
-    """Address of a contiguous tensor of the given dtype and shape."""
-    _same(t, dt, shape, what, dev)
-    if not t.is_contiguous():
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what}: shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if rows:
+        if t.stride()[-1] != 1 and shape[-1] > 1:
+            raise ValueError(f"{what}: the last dimension has stride {t.stride()[-1]}, expected 1")
+    elif not t.is_contiguous():
         raise ValueError(f"{what}: tensor is not contiguous")
-    return t.data_ptr()
 
 
 def _ws(t):
@@ -569,7 +546,7 @@ def _ws(t):
     _on(t, "workspace")
     if not t.is_contiguous():
         raise ValueError("workspace: tensor is not contiguous")
-    return t.data_ptr() or None, t.numel() * t.element_size()
+    return t.data_ptr() or None, t.nbytes
 
 
 def _dims(t, n: int, what: str):
@@ -583,14 +560,24 @@ def gemm_i8_w8a8(y, w, scale, xq, sx, stream=None):
 
     xq int8 [tokens, in] (quant_rows makes it and sx, a row a token), w int8 [out, in], y [tokens, out]
     float32 (gemv_i8_w8a8's bits) or bfloat16; xq and y may be slices of wider rows."""
-    lib = _op("qh_gemm_i8_w8a8")
-    tokens, out = _dims(y, 2, "y")
-    dev = _here(y)
-    in_ = _dims(w, 2, "w")[1]
-    yp, ldy = _r2(y, y.dtype, (tokens, out), "y", dev)
-    xp, ldx = _r2(xq, _Short.i8, (tokens, in_), "xq", dev)
-    st = lib(yp, ldy, _type(y, "y"), _c(w, _Short.i8, (out, in_), "w", dev), _c(scale, _Short.f32, (out,), "scale", dev), xp, ldx,
-             _c(sx, _Short.f32, (tokens,), "sx", dev), tokens, out, in_, _st(stream))
+    fn = _op("qh_gemm_i8_w8a8")
+    tokens, out = ny = _dims(y, 2, "y")
+    nw = _dims(w, 2, "w")
+    in_, T, dev, ty = nw[1], _Short.tensor, _here(y), _type(y, "y")
+    ly, lx = y.stride(), xq.stride() if xq.__class__ is T else ()
+    if not (w.__class__ is T and xq.__class__ is T and scale.__class__ is T and sx.__class__ is T
+            and w.dtype is _Short.i8 and xq.dtype is _Short.i8 and scale.dtype is _Short.f32 and sx.dtype is _Short.f32
+            and nw[0] == out and xq.shape == (tokens, in_) and scale.shape == (out,) and sx.shape == (tokens,)
+            and ly[1] == 1 and lx[1] == 1 and w.is_contiguous() and scale.is_contiguous() and sx.is_contiguous()
+            and dev == w.get_device() == xq.get_device() == scale.get_device() == sx.get_device()):
+        _operand(y, y.dtype, ny, "y", rows=True)
+        _operand(xq, _Short.i8, (tokens, in_), "xq", rows=True)
+        _operand(w, _Short.i8, (out, in_), "w")
+        _operand(scale, _Short.f32, (out,), "scale")
+        _operand(sx, _Short.f32, (tokens,), "sx")
+        lx = xq.stride()
+    st = fn(y.data_ptr(), ly[0], ty, w.data_ptr(), scale.data_ptr(), xq.data_ptr(), lx[0], sx.data_ptr(), tokens, out,
+            in_, _st(stream))
     if st:
         _check(st, "qh_gemm_i8_w8a8")
 
@@ -611,16 +598,33 @@ def delta_rule_seq(out, q, k, v, g, beta, S, cu, workspace, max_len: int, stream
     strides), g, beta float32 [tokens, heads], S float32 [n_seq, heads, 128, 128] (updated in place), cu
     int32 [n_seq + 1] on the device: sequence i has the rows cu[i] .. cu[i + 1].  max_len bounds the
     sequences' lengths (it chooses the kernels' form); workspace: delta_rule_seq_workspace(...) bytes."""
-    lib = _op("qh_delta_rule_seq")
-    tokens, heads, _ = _dims(v, 3, "v")
-    kh = _dims(k, 3, "k")[1]
-    n = _dims(S, 4, "S")[0]
-    dt, ty, dev = v.dtype, _type(v, "v"), _here(v)
-    gp, ldg = _r2(g, _Short.f32, (tokens, heads), "g", dev)
-    bp, ldb = _r2(beta, _Short.f32, (tokens, heads), "beta", dev)
-    st = lib(*_r3(out, dt, (tokens, heads, LV), "out", dev), *_r3(q, dt, (tokens, kh, LK), "q", dev), *_r3(k, dt, (tokens, kh, LK), "k", dev),
-             *_r3(v, dt, (tokens, heads, LV), "v", dev), ty, gp, ldg, bp, ldb, _c(S, _Short.f32, (n, heads, LK, LV), "S", dev),
-             _c(cu, _Short.i32, (n + 1,), "cu", dev), n, tokens, int(max_len), kh, heads, *_ws(workspace), _st(stream))
+    fn = _op("qh_delta_rule_seq")
+    nv, nk, ns = _dims(v, 3, "v"), _dims(k, 3, "k"), _dims(S, 4, "S")
+    tokens, heads, kh, n, T, dev, dt, ty = nv[0], nv[1], nk[1], ns[0], _Short.tensor, _here(v), v.dtype, _type(v, "v")
+    if not (out.__class__ is T and q.__class__ is T and k.__class__ is T and g.__class__ is T and beta.__class__ is T
+            and S.__class__ is T and cu.__class__ is T
+            and out.dtype is dt and q.dtype is dt and k.dtype is dt and g.dtype is _Short.f32 and beta.dtype is _Short.f32
+            and S.dtype is _Short.f32 and cu.dtype is _Short.i32
+            and nv[2] == LV and out.shape == nv and nk == (tokens, kh, LK) and q.shape == nk and g.shape == (tokens, heads)
+            and beta.shape == (tokens, heads) and ns == (n, heads, LK, LV) and cu.shape == (n + 1,)
+            and S.is_contiguous() and cu.is_contiguous()
+            and dev == out.get_device() == q.get_device() == k.get_device() == g.get_device() == beta.get_device()
+            == S.get_device() == cu.get_device()):
+        for t, shape, what in ((out, (tokens, heads, LV), "out"), (q, (tokens, kh, LK), "q"), (k, (tokens, kh, LK), "k"),
+                               (v, (tokens, heads, LV), "v")):
+            _operand(t, dt, shape, what, rows=True)
+        _operand(g, _Short.f32, (tokens, heads), "g", rows=True)
+        _operand(beta, _Short.f32, (tokens, heads), "beta", rows=True)
+        _operand(S, _Short.f32, (n, heads, LK, LV), "S")
+        _operand(cu, _Short.i32, (n + 1,), "cu")
+    (lo, ho, o1), (lq, hq, q1), (lk, hk, k1), (lv, hv, v1), (lg, g1), (lb, b1) = (
+        out.stride(), q.stride(), k.stride(), v.stride(), g.stride(), beta.stride())
+    if not o1 == q1 == k1 == v1 == 1 == g1 == b1:
+        for t, what in ((out, "out"), (q, "q"), (k, "k"), (v, "v"), (g, "g"), (beta, "beta")):
+            _operand(t, t.dtype, t.shape, what, rows=True)
+    st = fn(out.data_ptr(), lo, ho, q.data_ptr(), lq, hq, k.data_ptr(), lk, hk, v.data_ptr(), lv, hv, ty,
+            g.data_ptr(), lg, beta.data_ptr(), lb, S.data_ptr(), cu.data_ptr(), n, tokens, int(max_len), kh,
+            heads, *_ws(workspace), _st(stream))
     if st:
         _check(st, "qh_delta_rule_seq")
 
@@ -644,15 +648,30 @@ def attention_seq(out, q, k, v, cu_q, k_start, k_len, workspace, max_q: int, max
     q_len sees the first r + 1 + k_len - q_len (0 comes out where it sees none).  scale: 1 / sqrt(dim) if
     None.  max_q and max_k bound the sequences' rows and keys (they choose the kernels' form); workspace:
     attention_seq_workspace(...) bytes."""
-    lib = _op("qh_attention_seq")
-    rows, heads, d = _dims(q, 3, "q")
-    krows, kvh, _ = _dims(k, 3, "k")
-    n = _dims(k_len, 1, "k_len")[0]
-    dt, ty, dev = q.dtype, _type(q, "q"), _here(q)
-    st = lib(*_r3(out, dt, (rows, heads, d), "out", dev), *_r3(q, dt, (rows, heads, d), "q", dev), *_r3(k, dt, (krows, kvh, d), "k", dev),
-             *_r3(v, dt, (krows, kvh, d), "v", dev), ty, _c(cu_q, _Short.i32, (n + 1,), "cu_q", dev), _c(k_start, _Short.i64, (n,), "k_start", dev),
-             _c(k_len, _Short.i32, (n,), "k_len", dev), n, rows, krows, int(max_q), int(max_k), heads, kvh, d,
-             float(d ** -0.5 if scale is None else scale), *_ws(workspace), _st(stream))
+    fn = _op("qh_attention_seq")
+    nq, nk, n = _dims(q, 3, "q"), _dims(k, 3, "k"), _dims(k_len, 1, "k_len")[0]
+    (rows, heads, d), (krows, kvh, _) = nq, nk
+    T, dev, dt, ty = _Short.tensor, _here(q), q.dtype, _type(q, "q")
+    if not (out.__class__ is T and k.__class__ is T and v.__class__ is T and cu_q.__class__ is T and k_start.__class__ is T
+            and k_len.__class__ is T
+            and out.dtype is dt and k.dtype is dt and v.dtype is dt and cu_q.dtype is _Short.i32 and k_start.dtype is _Short.i64
+            and k_len.dtype is _Short.i32
+            and out.shape == nq and nk[2] == d and v.shape == nk and cu_q.shape == (n + 1,) and k_start.shape == (n,)
+            and cu_q.is_contiguous() and k_start.is_contiguous() and k_len.is_contiguous()
+            and dev == out.get_device() == k.get_device() == v.get_device() == cu_q.get_device() == k_start.get_device()
+            == k_len.get_device()):
+        for t, shape, what in ((out, nq, "out"), (q, nq, "q"), (k, (krows, kvh, d), "k"), (v, (krows, kvh, d), "v")):
+            _operand(t, dt, shape, what, rows=True)
+        _operand(cu_q, _Short.i32, (n + 1,), "cu_q")
+        _operand(k_start, _Short.i64, (n,), "k_start")
+        _operand(k_len, _Short.i32, (n,), "k_len")
+    (lo, ho, o1), (lq, hq, q1), (lk, hk, k1), (lv, hv, v1) = out.stride(), q.stride(), k.stride(), v.stride()
+    if not o1 == q1 == k1 == v1 == 1:
+        for t, what in ((out, "out"), (q, "q"), (k, "k"), (v, "v")):
+            _operand(t, dt, t.shape, what, rows=True)
+    st = fn(out.data_ptr(), lo, ho, q.data_ptr(), lq, hq, k.data_ptr(), lk, hk, v.data_ptr(), lv, hv, ty,
+            cu_q.data_ptr(), k_start.data_ptr(), k_len.data_ptr(), n, rows, krows, int(max_q), int(max_k), heads, kvh,
+            d, float(d ** -0.5 if scale is None else scale), *_ws(workspace), _st(stream))
     if st:
         _check(st, "qh_attention_seq")
 
