@@ -53,8 +53,7 @@ __device__ __forceinline__ bool find_unit(const AttnSeq& a, int b, Unit& o) {
       work += (int64_t)tiles * max(kl, 0);
     }
     if (a.n_seq > 64) load(0);
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) work += __shfl_xor(work, d);
+    work = sum_all(work);
     const int64_t c = (work * a.kv_heads + kFill - 1) / kFill;
     chunk = (int)min(max((c + 63) / 64 * 64, (int64_t)kMinChunk), (int64_t)kMaxKeys);
   }
@@ -62,12 +61,7 @@ __device__ __forceinline__ bool find_unit(const AttnSeq& a, int b, Unit& o) {
   for (int s0 = 0; s0 < a.n_seq; s0 += 64) {
     if (s0 > 0) load(s0);
     const int ns = max(seq_tiles(max(kl, 0), chunk), 1);
-    int iu = tiles * ns, it = tiles;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const int tu = __shfl_up(iu, d), tt = __shfl_up(it, d);
-      if (lane >= d) iu += tu, it += tt;
-    }
+    const int iu = sum_up_to(tiles * ns), it = sum_up_to(tiles);
     const uint64_t past = __ballot(base + (JOIN ? it : iu) > b);
     if (past != 0) {
       const int l = __builtin_ctzll(past);
@@ -471,8 +465,8 @@ __device__ __forceinline__ bool find_tile_unit(const AttnSeq& a, int b, TileUnit
     tiles += nt;
   }
   if (a.n_seq > 64) load(0);
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) all += __shfl_xor(all, d), tiles += __shfl_xor(tiles, d);
+  all = sum_all(all);
+  tiles = sum_all(tiles);
   const int fill = kCUs - (a.bf16 ? kCUs / 4 : (int)min(tiles * a.kv_heads / 2, (int64_t)kCUs / 4));
   const int64_t share = max((all * a.kv_heads + fill - 1) / fill, (int64_t)min_tile_chunk(a.bf16));
   int base = 0, slots = 0;   // of the next sequence: units (JOIN: split tiles), the split tiles' units

@@ -5,6 +5,23 @@
 
 namespace qh {
 
+// The sum over this lane and those before it, by DPP (within rows of 16 lanes, then the row before and the half before).
+__device__ __forceinline__ int sum_up_to(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);   // row_shr:1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);   // row_bcast:15, rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);   // row_bcast:31, rows 2 and 3
+  return v;
+}
+// The sum over all lanes of values from 0 to 2^48 (larger ones count as that).
+__device__ __forceinline__ int64_t sum_all(int64_t v) {
+  v = min(v, (int64_t)1 << 48);
+  const uint32_t lo = __builtin_amdgcn_readlane(sum_up_to((int)(v & 0xffffff)), 63), hi = __builtin_amdgcn_readlane(sum_up_to((int)(v >> 24)), 63);
+  return ((int64_t)hi << 24) + lo;
+}
+
 // The sequence and the tile in it of row tile b (tiles of `tile` rows; a token is `mult` rows).
 struct TileAt {
   int seq, tile;
@@ -18,12 +35,7 @@ __device__ __forceinline__ bool find_tile(const int32_t* cu, int n_seq, int rows
     SeqSpan sp = {0, 0};
     if (i < n_seq) sp = seq_span(as_global(cu)[i], as_global(cu)[i + 1], rows);
     const int n = seq_tiles(sp.len * mult, tile);
-    int inc = n;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const int t = __shfl_up(inc, d);
-      if (lane >= d) inc += t;
-    }
+    const int inc = sum_up_to(n);
     const uint64_t past = __ballot(base + inc > b);
     if (past != 0) {
       const int l = __builtin_ctzll(past);
