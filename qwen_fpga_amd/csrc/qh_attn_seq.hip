@@ -469,54 +469,57 @@ __device__ __forceinline__ bool find_tile_unit(const AttnSeq& a, int b, TileUnit
   tiles = sum_all(tiles);
   const int fill = kCUs - (a.bf16 ? kCUs / 4 : (int)min(tiles * a.kv_heads / 2, (int64_t)kCUs / 4));
   const int64_t share = max((all * a.kv_heads + fill - 1) / fill, (int64_t)min_tile_chunk(a.bf16));
-  int base = 0, slots = 0;   // of the next sequence: units (JOIN: split tiles), the split tiles' units
+  int base = 0, slots = 0;   // of the next 64 sequences: units (JOIN: split tiles), the split tiles' units
   bool found = false;
   for (int s0 = 0; s0 < a.n_seq; s0 += 64) {
     if (s0 > 0) load(s0);
     // the longest first: place `rank` is this lane's sequence's
     const int n = min(a.n_seq - s0, 64), len = nt > 0 ? max(kl, 0) : -1;
-    int rank = 0;
+    int rank = lane < n ? 0 : lane;
     for (int l = 0; l < n; ++l) {
       const int other = __builtin_amdgcn_readlane(len, l);
-      rank += other > len || (other == len && l < lane);
+      rank += lane < n && (other > len || (other == len && l < lane));
     }
     const int64_t c64 = (max(share, (int64_t)(max(kl, 0) / kMaxTileSplits + 1)) + 31) / 32 * 32;
     const int chunk = a.limit > 0 ? (int)min(c64, (int64_t)kMaxKeys) : kMaxKeys;
-    int splits = 0;   // units of the split tiles
-    for (int k = 1, c; __ballot((c = tiles_past(sp.len, kl, G, TILE, nt, (int64_t)k * chunk)) > 0) != 0; ++k) splits += k == 1 ? 2 * c : c;
-    for (int r = 0; r < n; ++r) {
-      const int l = __builtin_ctzll(__ballot(rank == r && lane < n));
+    const int big = tiles_past(sp.len, kl, G, TILE, nt, chunk);
+    int su = 2 * big;   // units of the split tiles
+    for (int k = 2, c; __ballot((c = tiles_past(sp.len, kl, G, TILE, nt, (int64_t)k * chunk)) > 0) != 0; ++k) su += c;
+    // in the order of the places
+    auto place = [&](int v) { return __builtin_amdgcn_ds_permute(4 * rank, v); };
+    const int who = place(lane), su_at = place(su), big_at = place(big), past = sum_up_to(su_at);
+    const bool split = su_at > 0 && ((int64_t)slots + past) * a.kv_heads <= a.limit;   // (there is place for it)
+    const int m = JOIN ? (split ? big_at : 0) : place(nt) + (split ? su_at - big_at : 0), upto = base + sum_up_to(m);
+    const uint64_t reach = __ballot(upto > b);
+    if (!found && reach != 0) {
+      const int r = __builtin_ctzll(reach), l = __builtin_amdgcn_readlane(who, r);
       auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
-      const int t = of(nt), kn = of(kl), step = of(chunk), su = of(splits);
-      const int len_q = of(sp.len);
-      const bool split = su > 0 && (slots + (int64_t)su) * a.kv_heads <= a.limit;   // (there is place for it)
-      const int big = split ? tiles_past(len_q, kn, G, TILE, t, step) : 0, m = JOIN ? big : t - big + (split ? su : 0);
-      if (b >= base && b < base + m) {
-        o.ks = (int64_t)((uint64_t)(uint32_t)of((int)(ks >> 32)) << 32 | (uint32_t)of((int)ks));
-        o.sp = {of(sp.start), len_q};
-        o.kl = kn;
-        int in = b - base, past = 0, first = slots;   // tiles of more than k splits; the units of those
-        for (int k = split ? seq_tiles(kn, step) : 1;; --k) {
-          const int c = k > 1 ? tiles_past(len_q, kn, G, TILE, t, (int64_t)(k - 1) * step) - past : t - past;   // of k
-          const int u = JOIN ? c : c * k;
-          if (in < u || k == 1) {
-            o.nsplit = k;
-            o.split = k > 1 && !JOIN ? in / c : 0;
-            in -= o.split * c;
-            o.tile = t - 1 - past - in;
-            o.slot = first + in * k + o.split;
-            found = o.tile >= 0 && o.tile < t;
-            break;
-          }
-          in -= u;
-          past += c;
-          first += c * k;
+      auto at = [&](int v) { return __builtin_amdgcn_readlane(v, r); };
+      const int t = of(nt), step = of(chunk), to = at(split);
+      o.sp = {of(sp.start), of(sp.len)};
+      o.ks = (int64_t)((uint64_t)(uint32_t)of((int)(ks >> 32)) << 32 | (uint32_t)of((int)ks));
+      o.kl = of(kl);
+      int in = b - at(upto) + at(m), before = 0, first = slots + at(past) - at(su_at);   // tiles of more than k splits; the units of those
+      for (int k = to ? seq_tiles(o.kl, step) : 1;; --k) {
+        const int c = k > 1 ? tiles_past(o.sp.len, o.kl, G, TILE, t, (int64_t)(k - 1) * step) - before : t - before;   // of k
+        const int u = JOIN ? c : c * k;
+        if (in < u || k == 1) {
+          o.nsplit = k;
+          o.split = k > 1 && !JOIN ? in / c : 0;
+          in -= o.split * c;
+          o.tile = t - 1 - before - in;
+          o.slot = first + in * k + o.split;
+          found = o.tile >= 0 && o.tile < t;
+          break;
         }
-        if (!JOIN) return found;
+        in -= u;
+        before += c;
+        first += c * k;
       }
-      base += m;
-      slots += split ? su : 0;
+      if (!JOIN) return found;
     }
+    base = __builtin_amdgcn_readlane(upto, 63);
+    slots = min(slots + __builtin_amdgcn_readlane(past, 63), kMaxKeys);   // (past the limit: none has place any more)
   }
   o.all = base;
   return found;
