@@ -582,6 +582,18 @@ def test_prompt_form_bad_ranges(prompts, q, torch_cuda, bf16):
 
 
 @pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+@pytest.mark.parametrize("max_k", [129, 300, 700, 20000])
+def test_prompt_form_places_in_the_workspace(q, torch_cuda, bf16, max_k):
+    """max_k is a bound on what the workspace holds, not on the keys: what finds no place there is not split.  Long keys
+    and short ones in turn, and the longest sequence last."""
+    torch = torch_cuda
+    lens, ctx = [70, 3, 0, 129, 64, 1, 70, 2, 300], [900, 3, 10, 1500, 64, 2500, 400, 2, 3000]
+    qq, kk, vv, at_k = attn_inputs(torch, 15, lens, ctx, 4, 2, 128, bf16)
+    want = attn_oracle(torch, qq, kk, vv, lens, ctx, at_k, 1 / math.sqrt(128))
+    attn_check(torch, attn_run(q, torch, qq.cuda(), kk.cuda(), vv.cuda(), lens, ctx, at_k, max_q=4096, max_k=max_k), want, bf16)
+
+
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
 @pytest.mark.parametrize("max_q", [1, 4096])
 def test_attention_of_many_sequences(q, torch_cuda, bf16, max_q):
     """More than the 64 sequences that a wave looks at together; long ones among empty and short ones."""
