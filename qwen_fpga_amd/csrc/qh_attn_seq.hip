@@ -427,8 +427,8 @@ __global__ __launch_bounds__(1024) void attn_join_kernel(const AttnSeq a) {
 // The workgroups of an XCD then walk the keys of one head side by side and find them in its L2: shares cut to the same
 // length anywhere in the tiles missed it for 38% of the reads and took 450 us, not 390, for 16k packed tokens (8 / 2
 // heads of 256).
-// Split and whole, bfloat16: one sequence of 8000 tokens 307 and 350 us, 4096 106 and 165, 1024 44 and 55, 512 36 and
-// 36; two of 8000 478 and 498; those 16k tokens 383 and 390.
+// Split and whole, bfloat16: one sequence of 8000 tokens 317 and 359 us, 4096 114 and 170, 1024 42 and 56, 512 35 and
+// 36; two of 8000 509 and 520; those 16k tokens 420 and 452 (one call behind another without a pause).
 constexpr int kCUs = 256, kMaxTileSplits = 64;
 constexpr int min_tile_chunk(bool bf16) { return bf16 ? 256 : 128; }
 struct TileUnit {
@@ -894,10 +894,10 @@ AttnForm attn_seq_form(int64_t q_rows, int n_seq, int max_q, int max_k, int head
   const int G = heads / kv_heads;
   AttnForm f = {0, 0, 0};
   // Prompts, or many short ones that see many keys.  8 / 2 heads of 256, us in this form and in the one for few rows:
-  // fp32   one of 256 tokens 49 and 31, of 512 55 and 60, of 1500 123 and 162, of 4096 700 and 820; 128 tokens behind
-  //        1500 keys 57 and 44, behind 8000 121 and 117; 16 of 128 tokens 49 and 41, behind 8000 keys 1021 and 1367
-  // bf16   one of 128 tokens 23 and 15, of 256 27 and 27, of 512 34 and 46, of 4096 112 and 378; 128 tokens behind
-  //        1500 keys 36 and 33, behind 8000 50 and 61; 16 of 128 tokens 27 and 26, behind 8000 keys 169 and 599
+  // fp32   one of 256 tokens 49 and 29, of 512 56 and 56, of 1500 116 and 157, of 4096 714 and 817; 128 tokens behind
+  //        1372 keys 58 and 44, behind 7872 113 and 121; 16 of 128 tokens 47 and 40, behind 7872 keys 1018 and 1386
+  // bf16   one of 128 tokens 24 and 11, of 256 27 and 26, of 512 35 and 43, of 4096 115 and 369; 128 tokens behind
+  //        1372 keys 37 and 32, behind 7872 49 and 61; 16 of 128 tokens 24 and 25, behind 7872 keys 169 and 598
   const int64_t seen = q_rows * heads * std::max(max_k, 1);
   if ((int64_t)max_q * G >= (bf16 ? 1024 : 2048) || ((int64_t)max_q * G >= 128 && seen >= 5000000)) {
     f.tile = tile_rows(bf16);
