@@ -64,6 +64,45 @@ def test_index_rules(tmp_path):
     assert r.returncode == 0, r.stdout + r.stderr
 
 
+PAST = r"""
+#include <cstdio>
+#include <initializer_list>
+#include "qh_seq.hpp"
+using namespace qh;
+// tiles_past counts the tiles whose last row sees more than `keys` keys: against each tile in turn
+int main() {
+  for (int len : {0, 1, 2, 31, 33, 64, 127, 300})
+    for (int k : {-1, 0, 1, 5, 64, 200, 299, 300, 301, 1000, kMaxKeys})
+      for (int G : {1, 2, 3, 4, 7, 32})
+        for (int tile : {128, 256}) {
+          const int nt = seq_tiles(len * G, tile);
+          for (int64_t keys : {(int64_t)0, (int64_t)1, (int64_t)31, (int64_t)32, (int64_t)64, (int64_t)128, (int64_t)299, (int64_t)300,
+                               (int64_t)999, (int64_t)1000, (int64_t)kMaxKeys, (int64_t)64 * kMaxKeys}) {
+            int n = 0;
+            for (int t = 0; t < nt; ++t) {
+              const int last = ((t + 1) * tile < len * G ? (t + 1) * tile : len * G) - 1;
+              n += keys_seen(last / G, len, k) > keys;
+            }
+            if (tiles_past(len, k, G, tile, nt, keys) != n) {
+              std::printf("len %d keys %d G %d tile %d past %d: %d, not %d\n", len, k, G, tile, (int)keys, tiles_past(len, k, G, tile, nt, keys), n);
+              return 1;
+            }
+          }
+        }
+  return 0;
+}
+"""
+
+
+def test_tiles_past(tmp_path):
+    src, exe = tmp_path / "t.cpp", tmp_path / "t"
+    src.write_text(PAST)
+    subprocess.run(["g++", "-std=c++17", "-Wall", "-Wextra", "-Werror", "-ftrapv", "-I",
+                    os.path.join(ROOT, "qwen_fpga_amd", "csrc"), "-o", str(exe), str(src)], check=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert r.returncode == 0, r.stdout + r.stderr
+
+
 class Args:
     """A call's arguments by name: good ones (host addresses that no kernel reads, since every call here is
     refused or has nothing to do), and the ones that a case changes."""
