@@ -103,73 +103,75 @@ __global__ __launch_bounds__(256) void gemm_rows_kernel(const GemmSeq a) {
   if (m < a.tokens) put4<BF16>(a, m, o, s, as_global(a.sx)[m], scale4(a, o), a.wide && o + 4 <= a.out);
 }
 
-// Many tokens: a workgroup takes 128 rows and 128 tokens, in steps of 64 through a ring of four LDS stages that
-// global -> LDS loads fill three steps ahead; a wave multiplies 64 x 64, and reads the fragments of a step beside the
-// products of the one before.  A row's 16-byte chunk c stands at chunk c ^ (row / 2 % 4) of its 64 bytes, so that eight
-// rows of a fragment, which are read at once, lie in all banks.  4096 tokens of 3584 -> 1024: 23.4 us, the loop 16.8 of
-// them (1.8 POP/s at 1.95 GHz; LDS and MFMA pipes are busy for 65 and 45% of it); 1500 tokens of 1024 -> 7168: 26.5 us,
-// two rounds of workgroups, each 8 us of loop and 5 of start and of writing 43 MB of fp32 outputs.
-constexpr int kBT = 128, kStages = 4, kStageBytes = 2 * kBT * 64;
+// Many tokens: a workgroup takes kBT (128 or 64) rows and kBT tokens, in steps of 64 through a ring of four LDS stages
+// that global -> LDS loads fill three steps ahead; a wave multiplies a quarter, and reads the fragments of a step beside
+// the products of the one before.  A row's 16-byte chunk c stands at chunk c ^ (row / 2 % 4) of its 64 bytes, so that
+// eight rows of a fragment, which are read at once, lie in all banks.  4096 tokens of 3584 -> 1024: 23 us, the loop 16.8
+// of them (1.8 POP/s at 1.95 GHz; LDS and MFMA pipes are busy for 65 and 45% of it); 1500 tokens of 1024 -> 7168: 26 us,
+// two rounds of workgroups, each 8 us of loop and 5 of start and of writing 43 MB of fp32 outputs.  Tiles of 64 are for
+// products with fewer tiles than CUs, which the way of one tile bounds: 1024 tokens of 3584 -> 1024 11 us, not 18.
+constexpr int kStages = 4;
 
-template <bool BF16>
+template <bool BF16, int kBT>
 __global__ __launch_bounds__(256, 2) void gemm_tile_kernel(const GemmSeq a, int mt) {
+  constexpr int F = kBT / 32, NL = kBT / 64, kStageBytes = 2 * kBT * 64;   // fragments of a wave; loads of w's and of x's rows
   __shared__ __attribute__((aligned(16))) int8_t lds[kStages * kStageBytes];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, j = lane & 15;
   const int b = blockIdx.x;
   const int n0 = (b / mt) * kBT, m0 = (b % mt) * kBT;
-  const int wr = 64 * (wave & 1), wt = 64 * (wave >> 1);
+  const int wr = 16 * F * (wave & 1), wt = 16 * F * (wave >> 1);
   const int NC = a.in >> 4, NS = (NC + 3) >> 2;
-  // a wave's loads of a step: 2 x 16 rows of w, 2 x 16 of x; lane l brings chunk (l % 4) ^ (row / 2 % 4) of row l / 4
+  // a wave's loads of a step: NL x 16 rows of w, NL x 16 of x; lane l brings chunk (l % 4) ^ (row / 2 % 4) of row l / 4
   const int lr = lane >> 2, lc = (lane & 3) ^ ((lr >> 1) & 3);
   const char* src[2] = {reinterpret_cast<const char*>(a.w) + (size_t)n0 * a.in, static_cast<const char*>(a.x.p) + (int64_t)m0 * a.x.ld};
-  uint32_t off[4];   // (below 128 rows of less than 2^24 bytes: the launch's rule)
+  uint32_t off[2 * NL];   // (below 128 rows of less than 2^24 bytes: the launch's rule)
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int r = 32 * wave + 16 * i + lr;
+  for (int i = 0; i < NL; ++i) {
+    const int r = 16 * (NL * wave + i) + lr;
     off[i] = (uint32_t)min(r, a.out - 1 - n0) * (uint32_t)a.in;
-    off[2 + i] = (uint32_t)min(r, a.tokens - 1 - m0) * (uint32_t)a.x.ld;
+    off[NL + i] = (uint32_t)min(r, a.tokens - 1 - m0) * (uint32_t)a.x.ld;
   }
   auto stage = [&](int s) {
     const int c = 16 * min(4 * s + lc, NC - 1);
-    const uint32_t base = lds_address(lds) + (s & (kStages - 1)) * kStageBytes + 32 * wave * 64;
+    const uint32_t base = lds_address(lds) + (s & (kStages - 1)) * kStageBytes + 16 * NL * wave * 64;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) load_to_lds(src[i >> 1], off[i] + c, base + (i >> 1) * (kBT * 64) + (i & 1) * 1024);
+    for (int i = 0; i < 2 * NL; ++i) load_to_lds(src[i / NL], off[i] + c, base + i / NL * (kBT * 64) + i % NL * 1024);
   };
-  i32x4 acc[4][4];
+  i32x4 acc[F][F];
 #pragma unroll
-  for (int r = 0; r < 4; ++r)
+  for (int r = 0; r < F; ++r)
 #pragma unroll
-    for (int t = 0; t < 4; ++t) acc[r][t] = i32x4{0, 0, 0, 0};
+    for (int t = 0; t < F; ++t) acc[r][t] = i32x4{0, 0, 0, 0};
 #pragma unroll
   for (int s = 0; s < kStages; ++s)
     if (s < NS) stage(s);
   const int fo = j * 64 + 16 * (g ^ ((j >> 1) & 3));   // a fragment's place
-  i32x4 wv[2][4], xv[2][4];   // fragments of the steps s and s + 1
+  i32x4 wv[2][F], xv[2][F];   // fragments of the steps s and s + 1
   // this wave's loads of step s have landed (those of the `ahead` next stay in flight) and its reads of step s - 1 are
   // done; after the barrier every wave's
   auto wait = [&](int ahead) {
     switch (ahead) {
-#define QH_WAIT(n) case n: asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(4 * n) : "memory"); break;
+#define QH_WAIT(n) case n: asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * NL * n) : "memory"); break;
       QH_WAIT(0) QH_WAIT(1) QH_WAIT(2) QH_WAIT(3) QH_WAIT(4) QH_WAIT(5) QH_WAIT(6) QH_WAIT(7)
 #undef QH_WAIT
     }
   };
-  auto read = [&](int s, i32x4 (&w)[4], i32x4 (&x)[4]) {
+  auto read = [&](int s, i32x4 (&w)[F], i32x4 (&x)[F]) {
     const int8_t* base = lds + (s & (kStages - 1)) * kStageBytes;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
+    for (int t = 0; t < F; ++t) {
       w[t] = *as_lds(reinterpret_cast<const i32x4*>(base + (wr + 16 * t) * 64 + fo));
       x[t] = *as_lds(reinterpret_cast<const i32x4*>(base + kBT * 64 + (wt + 16 * t) * 64 + fo));
     }
   };
   wait(min(NS - 1, kStages - 1));
   read(0, wv[0], xv[0]);
-  auto mul = [&](const i32x4 (&w)[4], const i32x4 (&x)[4]) {
+  auto mul = [&](const i32x4 (&w)[F], const i32x4 (&x)[F]) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
+    for (int r = 0; r < F; ++r)
 #pragma unroll
-      for (int t = 0; t < 4; ++t) acc[r][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[r], x[t], acc[r][t], 0, 0, 0);
+      for (int t = 0; t < F; ++t) acc[r][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[r], x[t], acc[r][t], 0, 0, 0);
   };
   int s = 0;
   for (; s + 1 + kStages < NS; s += 2) {
@@ -184,7 +186,7 @@ __global__ __launch_bounds__(256, 2) void gemm_tile_kernel(const GemmSeq a, int 
   for (; s < NS; ++s) {
     if (4 * s + 4 > NC) {   // past the end of the row: nothing
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
+      for (int t = 0; t < F; ++t)
         if (4 * s + g >= NC) wv[0][t] = i32x4{0, 0, 0, 0};
     }
     mul(wv[0], xv[0]);
@@ -194,41 +196,42 @@ __global__ __launch_bounds__(256, 2) void gemm_tile_kernel(const GemmSeq a, int 
       read(s + 1, wv[0], xv[0]);
     }
   }
-  f32x4 sc[4];
-  float xs[4];
+  f32x4 sc[F];
+  float xs[F];
 #pragma unroll
-  for (int r = 0; r < 4; ++r) sc[r] = scale4(a, n0 + wr + 16 * r + 4 * g);
+  for (int r = 0; r < F; ++r) sc[r] = scale4(a, n0 + wr + 16 * r + 4 * g);
 #pragma unroll
-  for (int t = 0; t < 4; ++t) xs[t] = as_global(a.sx)[min(m0 + wt + 16 * t + j, a.tokens - 1)];
+  for (int t = 0; t < F; ++t) xs[t] = as_global(a.sx)[min(m0 + wt + 16 * t + j, a.tokens - 1)];
   const bool wide = a.wide && n0 + kBT <= a.out;
 #pragma unroll
-  for (int t = 0; t < 4; ++t)
+  for (int t = 0; t < F; ++t)
     if (m0 + wt + 16 * t + j < a.tokens)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) put4<BF16>(a, m0 + wt + 16 * t + j, n0 + wr + 16 * r + 4 * g, acc[r][t], xs[t], sc[r], wide);
+      for (int r = 0; r < F; ++r) put4<BF16>(a, m0 + wt + 16 * t + j, n0 + wr + 16 * r + 4 * g, acc[r][t], xs[t], sc[r], wide);
 }
 
 // The form, by what was measured (us, weights from the L2s and the MALL).
-// Units of 16, 32 and 64 tokens, for 63 of them: 1024 -> 512 outputs 3.2, 3.8 and 4.8, 3584 -> 1024 5.5, 7.1 and 10.2,
-// 1024 -> 2048 4.1, 3.9 and 4.9, 1024 -> 7168 8.7, 8.0 and 7.4: the smallest that are at most a workgroup for each CU.
-// Units of 64 against tiles: 63 tokens 1024 -> 7168 (448 units) 7.4 and 7.7, 1024 -> 151936 60 and 35; 200 and 300 tokens
-// 1024 -> 2048 (512 and 640) 7.4 and 8.2, 9.2 and 8.3; 300 and 512 tokens 3584 -> 1024 (320 and 512) 16.9 and 17.2, 18.7
-// and 17.5.  Units of 16 against tiles, for 4, 8 and 16 tokens: 1024 -> 16384 (1024 units) 4.9 and 7.2, 5.3 and 7.4, 6.1
-// and 7.4; 1024 -> 32768 8.3 and 7.8, 9.0 and 7.8, 10.5 and 7.9; 1024 -> 151936 27 and 27, 31 and 27, 37 and 28.
+// Units of 16 and 32 tokens and tiles of 64: 63 tokens 3584 -> 1024 5.5, 7.1 and 9.3, 1024 -> 512 3.2, 3.8 and 4.9, 1024 ->
+// 2048 (512 and 256 units) 4.1, 3.8 and 4.8, 1024 -> 7168 (1792 and 896) 8.7, 8.0 and 5.2; 200 tokens 3584 -> 1024 (832 and
+// 448) 14, 12 and 9.5: the smallest units that are at most a workgroup for each CU, else tiles.  Units of 16 and tiles
+// for 16 tokens: 1024 -> 7168 (448 units) 4.0 and 4.5, 1024 -> 16384 (1024) 5.9 and 5.3, 1024 -> 151936 37 and 28; for 4
+// tokens there 27 and 27.
+// Tiles of 128 and of 64, by the number of the former: 3584 -> 1024 64 17.9 and 10.9, 96 19.3 and 16.4, 128 19.5 and 17.8;
+// 4096 -> 4096 64 20.5 and 17.1, 128 22.2 and 23.9; 2048 -> 2048 128 13.7 and 11.8, 192 14.4 and 15.8; 1024 -> 7168 112
+// 8.9 and 7.1, 224 10.3 and 15.0.
 template <bool BF16>
 hipError_t launch(const GemmSeq& a, hipStream_t s) {
   const int rt = (a.out + 15) / 16;
   auto units = [&](int tt) { return (int64_t)rt * ((a.tokens + 16 * tt - 1) / (16 * tt)); };
-  if (units(1) <= 256 || (a.tokens <= 16 && (a.tokens <= 4 || rt <= 1024)))
+  auto tiles = [&](int t) { return (int64_t)((a.out + t - 1) / t) * ((a.tokens + t - 1) / t); };
+  if (units(1) <= 256 || a.tokens <= 4 || (a.tokens <= 16 && rt <= 512))
     gemm_rows_kernel<BF16, 1><<<dim3(rt, (a.tokens + 15) / 16), 256, 0, s>>>(a);
-  else if (units(4) <= 512 && (a.tokens <= 32 || units(2) <= 256))
+  else if (units(2) <= 256 || a.x.ld >= 1 << 24)
     gemm_rows_kernel<BF16, 2><<<dim3(rt, (a.tokens + 31) / 32), 256, 0, s>>>(a);
-  else if (units(4) <= 512 || a.x.ld >= 1 << 24)
-    gemm_rows_kernel<BF16, 4><<<dim3(rt, (a.tokens + 63) / 64), 256, 0, s>>>(a);
-  else {
-    const int nt = (a.out + kBT - 1) / kBT, mt = (a.tokens + kBT - 1) / kBT;
-    gemm_tile_kernel<BF16><<<(unsigned)((int64_t)nt * mt), 256, 0, s>>>(a, mt);
-  }
+  else if (tiles(128) <= 128)
+    gemm_tile_kernel<BF16, 64><<<(unsigned)tiles(64), 256, 0, s>>>(a, (a.tokens + 63) / 64);
+  else
+    gemm_tile_kernel<BF16, 128><<<(unsigned)tiles(128), 256, 0, s>>>(a, (a.tokens + 127) / 128);
   return hipGetLastError();
 }
 
