@@ -265,6 +265,9 @@ int qh_delta_rule_seq(void* out, int64_t ldo, int64_t hso, const void* q, int64_
  * cache of several), the new tokens' own among them: row r of q_len sees the first r + 1 + k_len - q_len.
  * out = softmax(scale q k^T) v over those; 0 for a row that sees none; NaN for the rows of a sequence whose keys
  * do not lie inside the array.  Keys a row does not see have no influence on it, whatever they hold.
+ * Scores, the softmax and sums are fp32.  With QH_BF16 the probabilities' product with v takes them in two bfloat16 parts
+ * (off by 2^-14 of sum p |v| at most) in the form for few rows and rounded to bfloat16 once (2^-8) in the one for
+ * prompts; the output is rounded once in both.
  * Query head h takes kv head h / (heads / kv_heads).  q_rows * heads + 16 * n_seq * kv_heads: up to 64 million. */
 size_t qh_attention_seq_workspace(int q_rows, int n_seq, int max_q, int max_k, int heads, int kv_heads, int head_dim,
                                   int type);

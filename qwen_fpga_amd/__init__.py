@@ -647,7 +647,8 @@ def attention_seq(out, q, k, v, cu_q, k_start, k_len, workspace, max_q: int, max
     sequence i's keys are the rows k_start[i] .. + k_len[i], the new tokens' own among them, and row r of
     q_len sees the first r + 1 + k_len - q_len (0 comes out where it sees none).  scale: 1 / sqrt(dim) if
     None.  max_q and max_k bound the sequences' rows and keys (they choose the kernels' form); workspace:
-    attention_seq_workspace(...) bytes."""
+    attention_seq_workspace(...) bytes.  bfloat16: the form for prompts rounds the probabilities to bfloat16 for
+    their product with v (2^-8 of sum p |v|), the one for few rows takes them in two parts (2^-14)."""
     fn = _op("qh_attention_seq")
     nq, nk, n = _dims(q, 3, "q"), _dims(k, 3, "k"), _dims(k_len, 1, "k_len")[0]
     (rows, heads, d), (krows, kvh, _) = nq, nk
