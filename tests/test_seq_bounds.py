@@ -74,6 +74,23 @@ def test_bounds_see_how_probabilities_are_rounded(lens, ctx):
     assert not within(plain_attention(torch, args, once), few)
 
 
+@pytest.mark.parametrize("m,lost,p_rounding", [(5000, 32, PROMPTS), (2500, 16, PROMPTS), (5000, 32, FEW), (2500, 16, FEW)])
+def test_bounds_see_a_lost_step(m, lost, p_rounding):
+    """One step of one wave of the smallest work, among thousands of keys."""
+    import torch
+    qq, kk, vv, at_k = ops.attn_inputs(torch, m, [1], [m], 8, 2, 256, True)
+    args = (qq, kk, vv, [1], [m], at_k, 1 / 16.0)
+    limit = attn_limit(torch, args, True, p_rounding)
+
+    def without(p):
+        p = p.clone()
+        p[:, 640:640 + lost] = 0
+        return p
+
+    assert within(plain_attention(torch, args, once if p_rounding == PROMPTS else two_parts), limit)
+    assert not within(plain_attention(torch, args, without), limit)
+
+
 FORMS = [  # lens, keys, heads, kv heads, dim: P's rounding shows where few keys cancel, a lost step where there are many
     ([1, 1, 1], [7, 300, 33], 8, 2, 256), ([1], [5000], 8, 2, 256), ([16, 3], [200, 90], 4, 1, 128), ([1, 1], [2500, 15], 4, 4, 128),
     ([260, 1], [261, 900], 2, 1, 256), ([130], [700], 6, 2, 128),
