@@ -6,6 +6,14 @@ Attention, bfloat16.  A product with P adds to the fp32 bound (tests/test_gpu_se
 few rows multiplies V with P in two bfloat16 parts, the first cut (p - hi < 2^-7 p) and the second rounded (2^-8 of itself) and moved
 up by 2^-18 p, 2^-14 sum p |v| in all; the form for prompts rounds each probability once, 2^-8 sum p |v|.  Both round the output
 once, 2^-8 of it.
+
+Delta rule.  Every rounding is taken as independent, half a step u = 2^-24 of the value at most, and carried through the
+recursion in 64 bits as a covariance over the state's rows (summed over its columns): a token's sums of 128 products
+are off by sqrt(128) u of the root of the products' squares, its delta and the state by u of themselves, the decay by
+u (1 + |g|); later tokens pass an error on as they pass the state on, e^g (I - beta k k^T).  An output is off by what its query reads
+of that, and by its own sum.  The norms over a head's columns may be three times that deviation (they scatter by
+a few per cent).  In chunks the kernel sums in another order, of the same length; what its parts of bfloat16 leave out of a
+product, 2^-21, is 0.7 u sqrt(128) of a sum in the same sense.
 """
 import math
 
@@ -124,3 +132,145 @@ def test_infinite_value_that_every_row_sees(q, torch_cuda, max_q, bf16):
         assert (got[:, :, 3] == math.inf).all() and (got[:, :, 9] == -math.inf).all()
         got[:, :, 3], got[:, :, 9] = clean[:, :, 3], clean[:, :, 9]
         assert torch.equal(got, clean)
+
+
+# ------------------------------------------------------------------ delta rule
+
+DEVIATIONS = 3
+
+
+def delta_bound(torch, qq, kk, vv, g, beta, S, lens):
+    """64-bit outputs and states, and the deviations of a token's (head's) and of a state's norms."""
+    qq, kk, vv, g, beta, S = (x.double() for x in (qq, kk, vv, g, beta, S))
+    rep, h = vv.shape[1] // kk.shape[1], vv.shape[1]
+    out, S, at, u2 = torch.zeros_like(vv), S.clone(), 0, U * U
+    dev_out, dev_S = torch.zeros(vv.shape[:2], dtype=torch.float64), torch.zeros(S.shape[:2], dtype=torch.float64)
+    for i, n in enumerate(lens):
+        s, C = S[i], torch.zeros(h, 128, 128, dtype=torch.float64)
+        for t in range(at, at + n):
+            k, q, b, e = kk[t].repeat_interleave(rep, 0), qq[t].repeat_interleave(rep, 0), beta[t], torch.exp(g[t])
+            s = s * e[:, None, None]
+            rows = s.square().sum(-1)
+            x = torch.einsum("hkv,hk->hv", s, k)
+            d = (vv[t] - x) * b[:, None]
+            var = u2 * (b * b * (128 * (k * k * rows).sum(-1) + x.square().sum(-1) + vv[t].square().sum(-1)) + d.square().sum(-1))
+            Ck = torch.einsum("hij,hj->hi", C, k)
+            kk2 = k[:, :, None] * k[:, None, :]
+            C = C - b[:, None, None] * (k[:, :, None] * Ck[:, None, :] + Ck[:, :, None] * k[:, None, :])
+            C = (C + (b * b * (Ck * k).sum(-1))[:, None, None] * kk2) * (e * e)[:, None, None] + var[:, None, None] * kk2
+            s = s + k[:, :, None] * d[:, None, :]
+            now = s.square().sum(-1)
+            C = C + torch.diag_embed(u2 * ((1 + g[t].square())[:, None].clamp(max=4) * rows + now))
+            out[t] = torch.einsum("hkv,hk->hv", s, q)
+            dev_out[t] = torch.sqrt(torch.einsum("hi,hij,hj->h", q, C, q) + u2 * (128 * (q * q * now).sum(-1) + out[t].square().sum(-1)))
+        S[i], dev_S[i] = s, torch.sqrt(torch.diagonal(C, dim1=-2, dim2=-1).sum(-1))
+        at += n
+    return out, S, dev_out, dev_S
+
+
+def delta_excess(out, S, bound, bf16):
+    """The largest part of what the bound allows that an output's and a state's norm are off by."""
+    want, wS, dev_out, dev_S = bound
+    eo = (out.double().cpu()[:want.shape[0]] - want).norm(dim=-1)
+    lo = DEVIATIONS * dev_out + (BF * (want.norm(dim=-1) + DEVIATIONS * dev_out) if bf16 else 0)
+    eS = (S.double().cpu() - wS).flatten(2).norm(dim=-1)
+    part = lambda e, lim: (e / lim.clamp(min=1e-300)).masked_fill(e == 0, 0.0)
+    top = lambda x: x.max().item() if x.numel() else 0.0
+    return top(part(eo, lo)), top(part(eS, DEVIATIONS * dev_S))
+
+
+def cut(torch, x):
+    """A float as the sum of three bfloat16."""
+    parts, x = [], x.float().contiguous()
+    for _ in range(3):
+        p = (x.view(torch.int32) & -65536).view(torch.float32)
+        parts.append(p.double())
+        x = x - p
+    return parts
+
+
+def delta_in_chunks(torch, qq, kk, vv, g, beta, S, lens, lost=None):
+    """The chunked form with products of three parts, rounded to fp32 once; `lost`: the product without its third parts."""
+    qq, kk, vv, g, beta, S = (x.float() for x in (qq, kk, vv, g, beta, S))
+    out, S, rep, at = torch.zeros_like(vv), S.clone(), vv.shape[1] // kk.shape[1], 0
+
+    def mul(name, x, y):
+        a, b = cut(torch, x), cut(torch, y)
+        return sum(a[i] @ b[j] for i in range(3) for j in range(3) if i + j <= (1 if name == lost else 2)).float()
+
+    for i, n in enumerate(lens):
+        for h in range(vv.shape[1]):
+            s = S[i, h]
+            for a in range(at, at + n, 64):
+                z = min(a + 64, at + n)
+                q, k, v, b = qq[a:z, h // rep], kk[a:z, h // rep], vv[a:z, h], beta[a:z, h, None]
+                c = torch.cumsum(g[a:z, h].double(), 0)
+                e, ec, rest = torch.exp(c[:, None] - c[None, :]).float(), torch.exp(c).float()[:, None], torch.exp(c[-1] - c).float()[:, None]
+                A = torch.tril(b * e * mul("K K^T", k, k.t()), -1)
+                P = torch.tril(e * mul("Q K^T", q, k.t()))
+                T = torch.linalg.solve_triangular(torch.eye(z - a) + A, torch.eye(z - a), upper=False)
+                d = mul("T R", T, b * v - b * ec * mul("K S", k, s))
+                out[a:z, h] = mul("Q S", q, s) * ec + mul("P d", P, d)
+                s = s * ec[-1] + mul("K^T d", k.t(), d * rest)
+            S[i, h] = s
+        at += n
+    return out, S
+
+
+PRODUCTS = ["K K^T", "Q K^T", "K S", "T R", "K^T d", "Q S", "P d"]
+
+
+def host_inputs(monkeypatch, *args, **kw):
+    import torch
+    with monkeypatch.context() as m:
+        m.setattr(torch.Tensor, "cuda", lambda x: x)
+        return ops.delta_inputs(torch, *args, **kw)[0]
+
+
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+def test_delta_bounds_see_lost_parts(monkeypatch, bf16):
+    """The chunked form passes, each of its products without third parts fails, as do operands cut to bfloat16."""
+    import torch
+    lens = [200, 1, 0, 70]
+    host = host_inputs(monkeypatch, 7, lens, 1, 2, bf16, decay=0.05)
+    bound = delta_bound(torch, *host, lens)
+    off = lambda *a: max(delta_excess(*a, bound, False))      # (before the outputs' own rounding)
+    assert off(*delta_in_chunks(torch, *host, lens)) <= 0.5
+    for lost in PRODUCTS if not bf16 else ["K S", "T R", "K^T d", "Q S", "P d"]:      # (bfloat16 q and k have one part)
+        assert off(*delta_in_chunks(torch, *host, lens, lost=lost)) > 1, lost
+    if not bf16:
+        for i in range(3):
+            cutoff = list(host)
+            cutoff[i] = cut(torch, host[i])[0].float()
+            assert off(*delta_in_chunks(torch, *cutoff, lens)) > 100
+
+
+def test_delta_bounds_hold_for_the_recursion(monkeypatch):
+    """Token by token in fp32, whatever the decay, within the bound."""
+    import torch
+    for lens, decay in (([130], 1.0), ([15, 1, 17], 1.0), ([150], 30.0), ([160], 0.0)):
+        host = host_inputs(monkeypatch, 3, lens, 1, 2, False, decay=decay)
+        qq, kk, vv, g, beta, S = (x.clone() for x in host)
+        out, at = torch.zeros_like(vv), 0
+        for i, n in enumerate(lens):
+            for t in range(at, at + n):
+                k, q = kk[t].expand(2, 128), qq[t].expand(2, 128)
+                s = S[i] * torch.exp(g[t])[:, None, None]
+                d = (vv[t] - (s * k[:, :, None]).sum(1)) * beta[t][:, None]
+                S[i] = s + k[:, :, None] * d[:, None, :]
+                out[t] = (S[i] * q[:, :, None]).sum(1)
+            at += n
+        assert max(delta_excess(out, S, delta_bound(torch, *host, lens), False)) <= 0.5
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("decay", [1.0, 0.05])
+@pytest.mark.parametrize("max_len", [None, 1], ids=["", "steps"])
+@pytest.mark.parametrize("lens,kh,h", ops.DELTA, ids=str)
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+def test_delta_precision(q, torch_cuda, lens, kh, h, bf16, max_len, decay):
+    torch = torch_cuda
+    host, dev = ops.delta_inputs(torch, 3 * sum(lens) + h, lens, kh, h, bf16, decay=decay)
+    S = host[5].cuda()
+    out = ops.delta_run(q, torch, dev, S, lens, max_len=max_len)
+    assert max(delta_excess(out, S, delta_bound(torch, *host, lens), bf16)) <= 1
