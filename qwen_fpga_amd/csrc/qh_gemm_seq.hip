@@ -210,28 +210,19 @@ __global__ __launch_bounds__(256, 2) void gemm_tile_kernel(const GemmSeq a, int 
       for (int r = 0; r < F; ++r) put4<BF16>(a, m0 + wt + 16 * t + j, n0 + wr + 16 * r + 4 * g, acc[r][t], xs[t], sc[r], wide);
 }
 
-// The form, by what was measured (us, weights from the L2s and the MALL).
-// Units of 16 and 32 tokens and tiles of 64: 63 tokens 3584 -> 1024 5.5, 7.1 and 9.3, 1024 -> 512 3.2, 3.8 and 4.9, 1024 ->
-// 2048 (512 and 256 units) 4.1, 3.8 and 4.8, 1024 -> 7168 (1792 and 896) 8.7, 8.0 and 5.2; 200 tokens 3584 -> 1024 (832 and
-// 448) 14, 12 and 9.5: the smallest units that are at most a workgroup for each CU, else tiles.  Units of 16 and tiles
-// for 16 tokens: 1024 -> 7168 (448 units) 4.0 and 4.5, 1024 -> 16384 (1024) 5.9 and 5.3, 1024 -> 151936 37 and 28; for 4
-// tokens there 27 and 27.
-// Tiles of 128 and of 64, by the number of the former: 3584 -> 1024 64 17.9 and 10.9, 96 19.3 and 16.4, 128 19.5 and 17.8;
-// 4096 -> 4096 64 20.5 and 17.1, 128 22.2 and 23.9; 2048 -> 2048 128 13.7 and 11.8, 192 14.4 and 15.8; 1024 -> 7168 112
-// 8.9 and 7.1, 224 10.3 and 15.0.
 template <bool BF16>
 hipError_t launch(const GemmSeq& a, hipStream_t s) {
-  const int rt = (a.out + 15) / 16;
-  auto units = [&](int tt) { return (int64_t)rt * ((a.tokens + 16 * tt - 1) / (16 * tt)); };
-  auto tiles = [&](int t) { return (int64_t)((a.out + t - 1) / t) * ((a.tokens + t - 1) / t); };
-  if (units(1) <= 256 || a.tokens <= 4 || (a.tokens <= 16 && rt <= 512))
+  const GemmForm f = gemm_form(a.tokens, a.out, a.x.ld);
+  const unsigned rt = (a.out + 15) / 16;
+  auto tiles = [&]() { return (unsigned)((a.out + f.tile - 1) / f.tile) * ((a.tokens + f.tile - 1) / f.tile); };
+  if (f.unit == 16)
     gemm_rows_kernel<BF16, 1><<<dim3(rt, (a.tokens + 15) / 16), 256, 0, s>>>(a);
-  else if (units(2) <= 256 || a.x.ld >= 1 << 24)
+  else if (f.unit == 32)
     gemm_rows_kernel<BF16, 2><<<dim3(rt, (a.tokens + 31) / 32), 256, 0, s>>>(a);
-  else if (tiles(128) <= 128)
-    gemm_tile_kernel<BF16, 64><<<(unsigned)tiles(64), 256, 0, s>>>(a, (a.tokens + 63) / 64);
+  else if (f.tile == 64)
+    gemm_tile_kernel<BF16, 64><<<tiles(), 256, 0, s>>>(a, (a.tokens + 63) / 64);
   else
-    gemm_tile_kernel<BF16, 128><<<(unsigned)tiles(128), 256, 0, s>>>(a, (a.tokens + 127) / 128);
+    gemm_tile_kernel<BF16, 128><<<tiles(), 256, 0, s>>>(a, (a.tokens + 127) / 128);
   return hipGetLastError();
 }
 

@@ -51,6 +51,28 @@ QH_SEQ_FN int tiles_past(int q_len, int k_len, int G, int tile, int nt, int64_t 
   return tok <= 0 ? nt : nt - (int)(tok * G / tile);
 }
 
+// The form of the int8 product: units of 16 rows and `unit` tokens straight from memory, or tiles of tile x tile.  By what
+// was measured (us, weights from the L2s and the MALL).
+// Units of 16 and 32 tokens and tiles of 64: 63 tokens 3584 -> 1024 5.5, 7.1 and 9.3, 1024 -> 512 3.2, 3.8 and 4.9, 1024 ->
+// 2048 (512 and 256 units) 4.1, 3.8 and 4.8, 1024 -> 7168 (1792 and 896) 8.7, 8.0 and 5.2; 200 tokens 3584 -> 1024 (832 and
+// 448) 14, 12 and 9.5: the smallest units that are at most a workgroup for each CU, else tiles.  Units of 16 and tiles
+// for 16 tokens: 1024 -> 7168 (448 units) 4.0 and 4.5, 1024 -> 16384 (1024) 5.9 and 5.3, 1024 -> 151936 37 and 28; for 4
+// tokens there 27 and 27.
+// Tiles of 128 and of 64, by the number of the former: 3584 -> 1024 64 17.9 and 10.9, 96 19.3 and 16.4, 128 19.5 and 17.8;
+// 4096 -> 4096 64 20.5 and 17.1, 128 22.2 and 23.9; 2048 -> 2048 128 13.7 and 11.8, 192 14.4 and 15.8; 1024 -> 7168 112
+// 8.9 and 7.1, 224 10.3 and 15.0.
+struct GemmForm {
+  int unit, tile;   // one of them 0
+};
+inline GemmForm gemm_form(int tokens, int out, int64_t ldx) {
+  const int64_t rt = (out + 15) / 16;
+  auto units = [&](int t) { return rt * ((tokens + t - 1) / t); };
+  auto tiles = [&](int t) { return (int64_t)((out + t - 1) / t) * ((tokens + t - 1) / t); };
+  if (units(16) <= 256 || tokens <= 4 || (tokens <= 16 && rt <= 512)) return {16, 0};
+  if (units(32) <= 256 || ldx >= 1 << 24) return {32, 0};   // (tiles: 32-bit offsets)
+  return {0, tiles(128) <= 128 ? 64 : 128};
+}
+
 }  // namespace qh
 
 #if defined(__HIPCC__)

@@ -16,10 +16,13 @@ a few per cent).  In chunks the kernel sums in another order, of the same length
 product, 2^-21, is 0.7 u sqrt(128) of a sum in the same sense.
 """
 import math
+import os
+import subprocess
 
 import pytest
 
 import test_gpu_seq_ops as ops
+from conftest import ROOT
 
 U, BF = ops.U, ops.BF
 FEW, PROMPTS = 2.0 ** -14, BF      # what P's rounding takes, of sum p |v|
@@ -274,3 +277,55 @@ def test_delta_precision(q, torch_cuda, lens, kh, h, bf16, max_len, decay):
     S = host[5].cuda()
     out = ops.delta_run(q, torch, dev, S, lens, max_len=max_len)
     assert max(delta_excess(out, S, delta_bound(torch, *host, lens), bf16)) <= 1
+
+
+# ------------------------------------------------------------------ int8 matrix product
+
+# both forms and both sizes of each in several units or tiles along both sides, the last ones ragged and whole; inner
+# dimensions that end inside a step of 64, inside the loads ahead and far behind them
+GEMM_TILES = [
+    (257, 8321, 1040), (1500, 1540, 1024), (1100, 2049, 3584), (640, 4096, 1024), (130, 8324, 272), (258, 8192, 32), (384, 7040, 64),
+    (300, 2048, 1040), (256, 2048, 1008), (513, 1028, 3584), (193, 1344, 208), (130, 517, 1008),
+    (47, 1000, 1040), (64, 1024, 512), (100, 800, 2064), (33, 68, 4096), (100, 130, 1040), (129, 68, 80),
+]
+
+
+def test_every_form_of_the_product_is_reached(tmp_path):
+    """By the launch's own rule, each form with several units or tiles of tokens and of rows, ragged and whole, beyond its
+    loads ahead, and with outputs in one store of four and not."""
+    src, exe = tmp_path / "t.cpp", tmp_path / "t"
+    src.write_text('#include <cstdio>\n#include <cstdlib>\n#include "qh_seq.hpp"\nint main(int n, char** v) { for (int i = 1; i + 1 < n; i += 2) { '
+                   'auto f = qh::gemm_form(atoi(v[i]), atoi(v[i + 1]), 4096); std::printf("%d %d\\n", f.unit, f.tile); } }')
+    subprocess.run(["g++", "-std=c++17", "-Wall", "-Wextra", "-Werror", "-I", os.path.join(ROOT, "qwen_fpga_amd", "csrc"), "-o", str(exe), str(src)],
+                   check=True)
+    r = subprocess.run([str(exe)] + [str(x) for t, o, _ in GEMM_TILES for x in (t, o)], capture_output=True, text=True, check=True)
+    forms = [tuple(map(int, line.split())) for line in r.stdout.split("\n") if line]
+    assert set(forms) == {(16, 0), (32, 0), (0, 64), (0, 128)}
+    for form in set(forms):
+        of = [s for s, f in zip(GEMM_TILES, forms) if f == form]
+        tok, row = form[0] or form[1], form[1] or 16
+        many = [(t, o, k) for t, o, k in of if t > tok and o > row]
+        assert any(t % tok for t, _, _ in many) and any(o % row for _, o, _ in many), form
+        assert any(k > 1000 and k % 64 for _, _, k in many) and any(o % 4 == 0 for _, o, _ in many), form
+        if form[1]:
+            assert any(t % tok == 0 and o % row == 0 for t, o, _ in many), form
+            assert any(t % tok > tok // 2 or t % tok == 0 for t, _, _ in many), form      # (the waves of a tile's second half)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens,out,inn", GEMM_TILES)
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+@pytest.mark.parametrize("wide", [False, True], ids=["rows", "contiguous"])
+def test_gemm_tiles(q, torch_cuda, tokens, out, inn, bf16, wide):
+    """Equal bits; contiguous outputs (one store for four where out is a multiple of 4) and inside wider rows."""
+    torch = torch_cuda
+    if not wide:
+        return ops.test_gemm(q, torch_cuda, tokens, out, inn, bf16)
+    g = ops.gen(torch, tokens + out + inn)
+    w = torch.randint(-128, 128, (out, inn), generator=g, dtype=torch.int8)
+    x = torch.randint(-128, 128, (tokens, inn), generator=g, dtype=torch.int8)
+    sw, sx = torch.rand(out, generator=g) * 1e-2, torch.rand(tokens, generator=g)
+    want = (x.double() @ w.double().t()).float() * sx[:, None] * sw[None, :]
+    y = torch.full((tokens, out), 7.0, dtype=torch.bfloat16 if bf16 else torch.float32, device="cuda")
+    q.gemm_i8_w8a8(y, w.cuda(), sw.cuda(), x.cuda(), sx.cuda())
+    assert torch.equal(y.cpu(), want.to(y.dtype))
