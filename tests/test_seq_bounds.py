@@ -15,6 +15,7 @@ of that, and by its own sum.  The norms over a head's columns may be three times
 a few per cent).  In chunks the kernel sums in another order, of the same length; what its parts of bfloat16 leave out of a
 product, 2^-21, is 0.7 u sqrt(128) of a sum in the same sense.
 """
+import functools
 import math
 import os
 import subprocess
@@ -329,3 +330,57 @@ def test_gemm_tiles(q, torch_cuda, tokens, out, inn, bf16, wide):
     y = torch.full((tokens, out), 7.0, dtype=torch.bfloat16 if bf16 else torch.float32, device="cuda")
     q.gemm_i8_w8a8(y, w.cuda(), sw.cuda(), x.cuda(), sx.cuda())
     assert torch.equal(y.cpu(), want.to(y.dtype))
+
+
+# ------------------------------------------------------------------ delta rule: what is not finite
+
+@functools.lru_cache(None)
+def many_heads(bf16):
+    import torch
+    lens = [150, 70]
+    host, _ = ops.delta_inputs(torch, 14, lens, 16, 64, bf16, decay=0.05, fused=False)
+    return lens, host, delta_bound(torch, *host, lens)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+@pytest.mark.parametrize("which", ["q", "k", "v", "g", "beta", "S"])
+@pytest.mark.parametrize("bad", [math.nan, math.inf], ids=str)
+def test_delta_non_finite_inputs_of_many_heads(q, torch_cuda, bf16, which, bad):
+    """Enough heads for two column tiles a workgroup in bfloat16, key heads with four value heads each: a value that is not
+    finite (in a whole chunk's middle, of one value head or one key head) reaches that head's later tokens only, and the other
+    heads' and sequences' states and outputs keep the bound."""
+    torch = torch_cuda
+    lens, clean, bound = many_heads(bf16)
+    h, hit, at, host = 64, 22, 75, [x.clone() for x in clean]
+    i = ["q", "k", "v", "g", "beta", "S"].index(which)
+    if which == "S":
+        host[5][0, hit, :, 9] = bad
+    elif which in ("q", "k"):
+        host[i][at, hit // 4, 5] = bad
+    else:
+        host[i][(at, hit) if which != "v" else (at, hit, 37)] = bad
+    S = host[5].cuda()
+    out = ops.delta_run(q, torch, [x.cuda() for x in host[:5]], S, lens).cpu()
+    S = S.cpu()
+    heads = [hit] if which not in ("q", "k") else list(range(hit // 4 * 4, hit // 4 * 4 + 4))
+    rest = [x for x in range(h) if x not in heads]
+    first = 0 if which == "S" else at
+    pick = lambda o, s, a, b, hh: delta_excess(o[a:b][:, hh], s[:0], (bound[0][a:b][:, hh], bound[1][:0], bound[2][a:b][:, hh], bound[3][:0]), bf16)[0]
+    states = lambda i, hh: delta_excess(out[:0], S[i:i + 1, hh], (bound[0][:0], bound[1][i:i + 1, hh], bound[2][:0], bound[3][i:i + 1, hh]), bf16)[1]
+    assert pick(out, S, 0, 220, rest) <= 1 and states(0, rest) <= 1 and states(1, list(range(h))) <= 1
+    assert pick(out, S, 150, 220, heads) <= 1
+    if first:
+        assert pick(out, S, 0, first, heads) <= 1
+    if which == "q":
+        assert not torch.isfinite(out[at, heads]).any() and pick(out, S, at + 1, 150, heads) <= 1 and states(0, heads) <= 1
+    elif which == "S":
+        assert not torch.isfinite(S[0, hit, :, 9]).any() and not torch.isfinite(out[:150, hit, 9]).any()
+        keep = [c for c in range(128) if c != 9]
+        assert torch.isfinite(S[0, hit][:, keep]).all() and torch.isfinite(out[:150, hit][:, keep]).all()
+    elif which == "v":      # one column
+        keep = [c for c in range(128) if c != 37]
+        assert not torch.isfinite(S[0, hit, :, 37]).any() and torch.isfinite(S[0, hit][:, keep]).all()
+        assert not torch.isfinite(out[at:150, hit, 37]).any() and torch.isfinite(out[:150, hit][:, keep]).all()
+    else:
+        assert not torch.isfinite(S[0, heads]).all()
