@@ -11,7 +11,7 @@
 //
 // The products run on the matrix cores at fp32 precision.  A float is the sum of three bfloat16 exactly (its 24 bits
 // cut into three eights, by masking), so an fp32 product is the six largest of the nine partial products (what is
-// left out is below 2^-22 of the largest), and one with a bfloat16 operand is three: 6 and 3 MFMAs of 16 cycles do
+// left out, the second times the third part twice over, is below 2^-21 of the product), and one with a bfloat16 operand is three: 6 and 3 MFMAs of 16 cycles do
 // what takes eight of 32 in v_mfma_f32_16x16x4_f32.  That one stays for the small triangular products with T and P.
 // In all of them lane l has row l % 16 of the left and column l % 16 of the right operand, at the depths of lane group
 // l / 16, and ends with rows 4 (l / 16) .. + 3 of column l % 16: what a lane holds of a result is what it has to
@@ -162,13 +162,10 @@ __global__ __launch_bounds__(256) void delta_step_kernel(const DeltaSeq a) {
 __device__ __forceinline__ float exp_of(double x) { return __builtin_amdgcn_exp2f((float)(x * 1.4426950408889634)); }
 // Two floats as pairs of bfloat16: the top eight bits of each, the next eight, the last eight.
 __device__ __forceinline__ void cut2(float x, float y, uint32_t& hi, uint32_t& mid, uint32_t& lo) {
-  const uint32_t xu = __float_as_uint(x), yu = __float_as_uint(y);
-  hi = __builtin_amdgcn_perm(yu, xu, 0x07060302u);
-  const float x1 = x - __uint_as_float(xu & 0xffff0000u), y1 = y - __uint_as_float(yu & 0xffff0000u);
-  const uint32_t x1u = __float_as_uint(x1), y1u = __float_as_uint(y1);
-  mid = __builtin_amdgcn_perm(y1u, x1u, 0x07060302u);
-  const float x2 = x1 - __uint_as_float(x1u & 0xffff0000u), y2 = y1 - __uint_as_float(y1u & 0xffff0000u);
-  lo = __builtin_amdgcn_perm(__float_as_uint(y2), __float_as_uint(x2), 0x07060302u);
+  const Cut a = cut_float(x), b = cut_float(y);
+  hi = __builtin_amdgcn_perm(b.p[0], a.p[0], 0x07060302u);
+  mid = __builtin_amdgcn_perm(b.p[1], a.p[1], 0x07060302u);
+  lo = __builtin_amdgcn_perm(b.p[2], a.p[2], 0x07060302u);
 }
 // Eight elements as NP parts: a bfloat16 input as it is, fp32 in three.
 template <bool BF16>

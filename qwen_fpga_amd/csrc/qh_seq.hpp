@@ -51,6 +51,21 @@ QH_SEQ_FN int tiles_past(int q_len, int k_len, int G, int tile, int nt, int64_t 
   return tok <= 0 ? nt : nt - (int)(tok * G / tile);
 }
 
+// A float as the sum of three bfloat16, eight bits of it each: the upper halves of p[0], p[1], p[2].
+struct Cut {
+  uint32_t p[3];
+};
+QH_SEQ_FN Cut cut_float(float x) {
+  Cut c;
+  auto next = [&]() {
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    x -= __builtin_bit_cast(float, u & 0xffff0000u);
+    return u;
+  };
+  c.p[0] = next(), c.p[1] = next(), c.p[2] = next();
+  return c;
+}
+
 // The form of the int8 product: units of 16 rows and `unit` tokens straight from memory, or tiles of tile x tile.  By what
 // was measured (us, weights from the L2s and the MALL).
 // Units of 16 and 32 tokens and tiles of 64: 63 tokens 3584 -> 1024 5.5, 7.1 and 9.3, 1024 -> 512 3.2, 3.8 and 4.9, 1024 ->

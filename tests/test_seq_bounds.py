@@ -267,6 +267,48 @@ def test_delta_bounds_hold_for_the_recursion(monkeypatch):
         assert max(delta_excess(out, S, delta_bound(torch, *host, lens), False)) <= 0.5
 
 
+CUT = r"""
+#include <cmath>
+#include <cstdio>
+#include "qh_seq.hpp"
+using namespace qh;
+// the three parts come to the float, and the partial products that are left out to less than 2^-21 of a product
+int main() {
+  uint64_t r = 88172645463325252ull;
+  double most = 0;
+  for (int i = 0; i < 4000000; ++i) {
+    float f[2];
+    double p[2][3];
+    for (int j = 0; j < 2; ++j) {
+      r ^= r << 13, r ^= r >> 7, r ^= r << 17;
+      // any significand, half of them with long runs of ones; exponents whose parts are normal numbers
+      uint32_t u = (uint32_t)(r >> 20) & 0x807fffffu;
+      if (r & 1) u |= 0x007fffffu >> (r >> 60);
+      u |= (uint32_t)(100 + (r >> 8) % 50) << 23;
+      if (i == 0) u = 0x3f80ffffu;   // below 1 + 2^-7
+      f[j] = __builtin_bit_cast(float, u);
+      const Cut c = cut_float(f[j]);
+      for (int k = 0; k < 3; ++k) p[j][k] = __builtin_bit_cast(float, c.p[k] & 0xffff0000u);
+      if (p[j][0] + p[j][1] + p[j][2] != (double)f[j] || (c.p[2] & 0xffffu) != 0) return std::printf("%a is not its parts\n", f[j]), 1;
+    }
+    const double left = p[0][1] * p[1][2] + p[0][2] * p[1][1] + p[0][2] * p[1][2], of = std::fabs(left / ((double)f[0] * f[1]));
+    if (of > most) most = of;
+  }
+  std::printf("%a\n", most);
+  return most < 0x1p-21 && most > 0x1p-22 ? 0 : 2;
+}
+"""
+
+
+def test_cut_of_a_float(tmp_path):
+    src, exe = tmp_path / "t.cpp", tmp_path / "t"
+    src.write_text(CUT)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Wextra", "-Werror", "-I", os.path.join(ROOT, "qwen_fpga_amd", "csrc"),
+                    "-o", str(exe), str(src)], check=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert r.returncode == 0, r.stdout + r.stderr
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("decay", [1.0, 0.05])
 @pytest.mark.parametrize("max_len", [None, 1], ids=["", "steps"])
