@@ -151,10 +151,12 @@ __global__ __launch_bounds__(256, 2) void gemm_tile_kernel(const GemmSeq a, int 
   // this wave's loads of step s have landed (those of the `ahead` next stay in flight) and its reads of step s - 1 are
   // done; after the barrier every wave's
   auto wait = [&](int ahead) {
+    static_assert(kStages == 4, "a case for each number of stages ahead");
     switch (ahead) {
 #define QH_WAIT(n) case n: asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * NL * n) : "memory"); break;
-      QH_WAIT(0) QH_WAIT(1) QH_WAIT(2) QH_WAIT(3) QH_WAIT(4) QH_WAIT(5) QH_WAIT(6) QH_WAIT(7)
+      QH_WAIT(1) QH_WAIT(2) QH_WAIT(3)
 #undef QH_WAIT
+      default: asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     }
   };
   auto read = [&](int s, i32x4 (&w)[F], i32x4 (&x)[F]) {
