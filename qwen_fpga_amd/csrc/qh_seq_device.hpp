@@ -74,13 +74,11 @@ __device__ __forceinline__ __attribute__((address_space(3))) T* lds_at(uint32_t 
 }
 
 // 16 bytes per lane from base + off (base the same for the wave) to LDS at `to` + 16 lane (`to` the same for the
-// wave).  In assembly, so that the caller counts the loads in flight itself (s_waitcnt vmcnt before the barrier that
-// hands a stage over): the compiler waits for every such load before any transposing LDS read.  Nothing is
-// returned to a register.
+// wave, in m0, which the compiler sets as the operand that it is).  In assembly, so that the caller counts the loads in
+// flight itself (s_waitcnt vmcnt before the barrier that hands a stage over): the compiler waits for every such load
+// before any transposing LDS read.  Nothing is returned to a register.
 __device__ __forceinline__ void load_to_lds(const char* base, uint32_t off, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-               :: "s"(__builtin_amdgcn_readfirstlane(to)), "v"(off), "s"(base)
-               : "memory", "m0");
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"{m0}"(__builtin_amdgcn_readfirstlane(to)), "v"(off), "s"(base) : "memory");
 }
 
 }  // namespace qh
