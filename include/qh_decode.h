@@ -222,7 +222,9 @@ int qh_mlp_layer_w8a8(float* out, const float* x, const qh_tensor* gate_w, const
  * projection and head-major tensors need no copy).  Pointers and strides are
  * multiples of 16 bytes where not said otherwise; the stride of a dimension with
  * one entry does not count.  Inputs may repeat rows (a stride of 0), outputs may
- * not; an output that shares memory with an input is QH_EINVAL.
+ * not; an output that shares memory with an input is QH_EINVAL.  Disjoint columns
+ * of rows of one length share none, nor do disjoint parts of each head (the query
+ * and gate halves of a projection); other interleavings are taken as sharing.
  *
  * Sequences stand one after another: sequence i has the rows cu[i] .. cu[i + 1]
  * (cu [n_seq + 1] int32, on the device).  Empty sequences are allowed; rows

@@ -4,6 +4,7 @@
 
 #include "qh_common.hpp"
 #include "qh_seq.hpp"
+#include "qh_seq_view.hpp"
 
 using namespace qh;
 
@@ -11,52 +12,11 @@ namespace {
 
 hipStream_t S(void* s) { return reinterpret_cast<hipStream_t>(s); }
 
-constexpr int64_t kMaxStride = (int64_t)1 << 40;   // elements; keeps every offset inside 64 bits
 constexpr int64_t kMaxUnits = 0x7fffffff;          // rows times heads
 constexpr int kMaxGridY = 65535;
 // A grid's threads in one direction stay below 2^32.
 constexpr int64_t kMaxStates = 900000;             // sequences times heads: 8 workgroups of 576 each
 constexpr int64_t kMaxTiles = 4000000;             // tiles of 16 rows and a kv head: a workgroup of 1024 each
-
-// An operand [rows][heads][dim] with its element size, to check it and to compare it with another.
-struct View {
-  const void* p;
-  int64_t rows, heads, dim, ld, hs;
-  int eb;
-  uintptr_t at() const { return reinterpret_cast<uintptr_t>(p); }
-  int64_t width() const { return ((heads > 1 ? (heads - 1) * hs : 0) + dim) * eb; }             // bytes of a row's span
-  int64_t bytes() const { return (rows > 1 ? (rows - 1) * ld * eb : 0) + width(); }
-  // 16-byte pieces: pointer and strides (those of dimensions with one entry do not count)
-  bool readable() const {
-    return p && aligned16(p) && (rows <= 1 || (ld >= 0 && ld < kMaxStride && ld * eb % 16 == 0)) &&
-           (heads <= 1 || (hs >= 0 && hs < kMaxStride && hs * eb % 16 == 0));
-  }
-  // and no two elements in one place
-  bool writable() const {
-    if (!readable()) return false;
-    if (rows > 1 && heads > 1)
-      return (hs >= dim && ld >= (heads - 1) * hs + dim) || (ld >= dim && hs / rows >= ld && hs >= (rows - 1) * ld + dim);
-    return (rows <= 1 || ld >= dim) && (heads <= 1 || hs >= dim);
-  }
-};
-
-View flat(const void* p, int64_t n, int eb) { return {p, 1, 1, n, 0, 0, eb}; }
-
-// Whether two operands share memory: their spans meet, and they are not disjoint columns of rows of one length.
-bool overlap(const View& a, const View& b) {
-  if (a.at() >= b.at() + b.bytes() || b.at() >= a.at() + a.bytes()) return false;
-  const int64_t la = a.ld * a.eb, lb = b.ld * b.eb;
-  if (a.rows > 1 && b.rows > 1 && la == lb && a.width() <= la && b.width() <= la) {
-    int64_t d = (int64_t)(b.at() - a.at()) % la;
-    if (d < 0) d += la;
-    return d < a.width() || d + b.width() > la;
-  }
-  return true;
-}
-template <class... V>
-bool overlap_any(const View& a, const V&... v) {
-  return (overlap(a, v) || ...);
-}
 
 bool type_ok(int type) { return type == QH_F32 || type == QH_BF16; }
 

@@ -426,3 +426,87 @@ def test_delta_non_finite_inputs_of_many_heads(q, torch_cuda, bf16, which, bad):
         assert not torch.isfinite(out[at:150, hit, 37]).any() and torch.isfinite(out[:150, hit][:, keep]).all()
     else:
         assert not torch.isfinite(S[0, heads]).all()
+
+
+# ------------------------------------------------------------------ operands in one buffer
+
+VIEWS = r"""
+#include <cstdio>
+#include <map>
+#include <random>
+#include "qh_seq_view.hpp"
+using namespace qh;
+// against every byte in turn: an answer of "apart" is always right, and so is "writable"; the layouts that are used in
+// earnest are known for what they are
+int main() {
+  std::mt19937 g(5);
+  auto pick = [&](std::initializer_list<int> v) { return *(v.begin() + g() % v.size()); };
+  const uintptr_t base = 1 << 20;
+  long apart = 0, write = 0;
+  for (int it = 0; it < 200000; ++it) {
+    View v[2];
+    std::map<uintptr_t, int> bytes[2];
+    bool twice[2] = {false, false};
+    const int ld = 8 * pick({0, 1, 2, 3, 4, 6, 8, 12}), hs = 8 * pick({0, 1, 2, 3, 4, 9});
+    for (int i = 0; i < 2; ++i) {
+      v[i] = {nullptr, pick({1, 2, 3, 4}), pick({1, 2, 3}), 8 * pick({1, 1, 2}), g() % 3 ? ld : 8 * pick({1, 2, 4, 5, 8, 16}),
+              g() % 3 ? hs : 8 * pick({1, 2, 3, 8, 16}), 2};
+      v[i].p = reinterpret_cast<const void*>(base + 16 * (g() % 12));
+      for (int r = 0; r < v[i].rows; ++r)
+        for (int h = 0; h < v[i].heads; ++h)
+          for (int d = 0; d < v[i].dim * 2; ++d) twice[i] |= ++bytes[i][v[i].at() + 2 * (r * v[i].ld + h * v[i].hs) + d] > 1;
+      if (v[i].writable()) {
+        ++write;
+        if (twice[i]) return std::printf("%d rows %d heads of %d, %d and %d apart, taken as writable\n", (int)v[i].rows, (int)v[i].heads,
+                                         (int)v[i].dim, (int)v[i].ld, (int)v[i].hs), 1;
+      }
+    }
+    if (overlap(v[0], v[1]) != overlap(v[1], v[0])) return std::printf("not symmetric\n"), 1;
+    if (!overlap(v[0], v[1])) {
+      ++apart;
+      for (auto& b : bytes[0])
+        if (bytes[1].count(b.first)) return std::printf("%d: taken as apart\n", it), 1;
+    }
+  }
+  if (apart < 10000 || write < 10000) return std::printf("%ld apart, %ld writable\n", apart, write), 1;
+  auto at = [&](int64_t el) { return reinterpret_cast<const void*>(base + 2 * el); };
+  const View out{at(128), 40, 8, 128, 8 * 256, 256, 2}, q{at(0), 40, 8, 128, 8 * 256, 256, 2};   // halves of each head
+  if (overlap(out, q) || !overlap(View{at(64), 40, 8, 128, 8 * 256, 256, 2}, q)) return std::printf("halves\n"), 1;
+  const View odd{at(0), 3, 4, 128, 2 * 128, 5 * 128, 2};   // every other row of head-major rows, five a head
+  if (!odd.writable()) return std::printf("every other row\n"), 1;
+  return 0;
+}
+"""
+
+
+def test_views(tmp_path):
+    src, exe = tmp_path / "t.cpp", tmp_path / "t"
+    src.write_text(VIEWS)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Wextra", "-Werror", "-ftrapv", "-I", os.path.join(ROOT, "qwen_fpga_amd", "csrc"),
+                    "-o", str(exe), str(src)], check=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert r.returncode == 0, r.stdout + r.stderr
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+def test_outputs_beside_their_inputs(q, torch_cuda, bf16):
+    """Outputs in the gate halves of the projection whose query halves are read, and in every other row of head-major
+    rows of odd number: as elsewhere, and the rest of the buffer as it was."""
+    torch = torch_cuda
+    lens, ctx, h, kvh, d = [40, 1, 0, 30], [40, 90, 3, 31], 4, 2, 128
+    qq, kk, vv, at_k = ops.attn_inputs(torch, 5, lens, ctx, h, kvh, d, bf16)
+    t, dev = sum(lens), [x.cuda() for x in (qq, kk, vv)]
+    want = ops.attn_run(q, torch, *dev, lens, ctx, at_k)
+    both = torch.cat([dev[0], torch.full_like(dev[0], 7.0)], -1)
+    ops.attn_run(q, torch, both[:, :, :d], *dev[1:], lens, ctx, at_k, out=both[:, :, d:])
+    assert torch.equal(both[:, :, d:], want) and torch.equal(both[:, :, :d], dev[0])
+    rows = torch.full((h, 2 * t - 1, d), 7.0, dtype=qq.dtype, device="cuda")
+    ops.attn_run(q, torch, *dev, lens, ctx, at_k, out=rows[:, ::2].transpose(0, 1))
+    assert torch.equal(rows[:, ::2].transpose(0, 1), want) and (rows[:, 1::2] == 7).all()
+    host, dd = ops.delta_inputs(torch, 8, lens, 4, 4, bf16, fused=False)
+    S, S2 = host[5].cuda(), host[5].cuda()
+    want = ops.delta_run(q, torch, dd, S, lens)
+    both = torch.cat([dd[2], torch.full_like(dd[2], 7.0)], -1)
+    ops.delta_run(q, torch, dd[:2] + [both[:, :, :128]] + dd[3:], S2, lens, out=both[:, :, 128:])
+    assert torch.equal(both[:, :, 128:], want) and torch.equal(both[:, :, :128], dd[2]) and torch.equal(S, S2)
