@@ -35,6 +35,7 @@ int qh_gemm_i8_w8a8(void* y, int64_t ldy, int type, const int8_t* w, const float
   if (!vx.readable()) return QH_EINVAL;
   // y is written element by element: any row stride of at least a row
   if (!y || (reinterpret_cast<uintptr_t>(y) % eb) != 0 || (tokens > 1 && (ldy < out || ldy >= kMaxStride))) return QH_EINVAL;
+  if (!all_countable(vx, vy)) return QH_ERANGE;
   if (overlap_any(vy, vx, flat(w, (int64_t)out * in, 1), flat(scale, out, 4), flat(sx, tokens, 4))) return QH_EINVAL;
   GemmSeq a;
   a.y = {y, ldy, 0};
@@ -72,6 +73,7 @@ int qh_delta_rule_seq(void* out, int64_t ldo, int64_t hso, const void* q, int64_
   if (tokens > 1 && (ldg < 0 || ldb < 0 || ldg >= kMaxStride || ldb >= kMaxStride)) return QH_EINVAL;
   const View vg{g, tokens, 1, heads, ldg, 0, 4}, vb{beta, tokens, 1, heads, ldb, 0, 4},
       vs = flat(state, (int64_t)n_seq * heads * QH_LK * QH_LV, 4), vc = flat(cu, n_seq + 1, 4);
+  if (!all_countable(vo, vq, vk, vv, vg, vb)) return QH_ERANGE;
   if (overlap_any(vo, vq, vk, vv, vg, vb, vs, vc) || overlap_any(vs, vq, vk, vv, vg, vb, vc)) return QH_EINVAL;
   const size_t need = qh_delta_rule_seq_workspace(tokens, n_seq, heads, k_heads, type, max_len);
   if (need > 0) {
@@ -122,7 +124,7 @@ int qh_attention_seq(void* out, int64_t ldo, int64_t hso, const void* q, int64_t
       vk{k, k_rows, kv_heads, head_dim, ldk, hsk, eb}, vv{v, k_rows, kv_heads, head_dim, ldv, hsv, eb};
   if (!vo.writable() || !vq.readable()) return QH_EINVAL;
   if (k_rows > 0 && (!vk.readable() || !vv.readable())) return QH_EINVAL;
-  if (k_rows > 1 && (ldk > INT64_MAX / 8 / k_rows || ldv > INT64_MAX / 8 / k_rows)) return QH_ERANGE;
+  if (!all_countable(vo, vq) || (k_rows > 0 && !all_countable(vk, vv))) return QH_ERANGE;
   if (!cu_q || !k_start || !k_len) return QH_EINVAL;
   const View vc = flat(cu_q, n_seq + 1, 4), vt = flat(k_start, n_seq, 8), vl = flat(k_len, n_seq, 4);
   if (overlap_any(vo, vq, vc, vt, vl) || (k_rows > 0 && overlap_any(vo, vk, vv))) return QH_EINVAL;

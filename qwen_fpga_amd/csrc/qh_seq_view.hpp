@@ -7,6 +7,7 @@
 namespace qh {
 
 constexpr int64_t kMaxStride = (int64_t)1 << 40;   // elements
+constexpr int64_t kMaxSpan = (int64_t)1 << 61;     // bytes that a dimension may go over: every offset fits 64 bits
 
 inline bool aligned_to_16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
@@ -23,6 +24,10 @@ struct View {
     return p && aligned_to_16(p) && (rows <= 1 || (ld >= 0 && ld < kMaxStride && ld * eb % 16 == 0)) &&
            (heads <= 1 || (hs >= 0 && hs < kMaxStride && hs * eb % 16 == 0));
   }
+  // and width() and bytes() can be counted
+  bool countable() const {
+    return (rows <= 1 || ld <= kMaxSpan / eb / (rows - 1)) && (heads <= 1 || hs <= kMaxSpan / eb / (heads - 1)) && dim <= kMaxSpan / eb;
+  }
   // and no two elements in one place
   bool writable() const {
     if (!readable()) return false;
@@ -34,7 +39,7 @@ struct View {
 
 inline View flat(const void* p, int64_t n, int eb) { return {p, 1, 1, n, 0, 0, eb}; }
 
-// Whether two operands share memory, as far as their spans and strides tell: they share none if the spans do
+// Whether two operands (countable ones) share memory, as far as their spans and strides tell: they share none if the spans do
 // not meet, or are disjoint columns of rows of one length, or if all their strides have a common divisor of which
 // the one's pieces of `dim` elements and the other's take different parts (halves of each head, interleaved).
 inline bool overlap(const View& a, const View& b) {
@@ -53,6 +58,10 @@ inline bool overlap(const View& a, const View& b) {
     if (v->heads > 1) step = std::gcd(step, v->hs * v->eb);
   }
   return !(step > 0 && apart(step, a.dim * a.eb, b.dim * b.eb));
+}
+template <class... V>
+bool all_countable(const V&... v) {
+  return (v.countable() && ...);
 }
 template <class... V>
 bool overlap_any(const View& a, const V&... v) {

@@ -23,6 +23,7 @@ import subprocess
 import pytest
 
 import test_gpu_seq_ops as ops
+import test_seq_ops as seq_ops
 from conftest import ROOT
 
 U, BF = ops.U, ops.BF
@@ -455,6 +456,7 @@ int main() {
       for (int r = 0; r < v[i].rows; ++r)
         for (int h = 0; h < v[i].heads; ++h)
           for (int d = 0; d < v[i].dim * 2; ++d) twice[i] |= ++bytes[i][v[i].at() + 2 * (r * v[i].ld + h * v[i].hs) + d] > 1;
+      if (!v[i].countable()) return std::printf("not countable\n"), 1;
       if (v[i].writable()) {
         ++write;
         if (twice[i]) return std::printf("%d rows %d heads of %d, %d and %d apart, taken as writable\n", (int)v[i].rows, (int)v[i].heads,
@@ -474,6 +476,8 @@ int main() {
   if (overlap(out, q) || !overlap(View{at(64), 40, 8, 128, 8 * 256, 256, 2}, q)) return std::printf("halves\n"), 1;
   const View odd{at(0), 3, 4, 128, 2 * 128, 5 * 128, 2};   // every other row of head-major rows, five a head
   if (!odd.writable()) return std::printf("every other row\n"), 1;
+  if (View{at(0), 1 << 30, 4, 128, (int64_t)1 << 39, 128, 4}.countable() || View{at(0), 4, 1 << 30, 128, 128, (int64_t)1 << 39, 4}.countable())
+    return std::printf("too far\n"), 1;
   return 0;
 }
 """
@@ -486,6 +490,15 @@ def test_views(tmp_path):
                     "-o", str(exe), str(src)], check=True)
     r = subprocess.run([str(exe)], capture_output=True, text=True)
     assert r.returncode == 0, r.stdout + r.stderr
+
+
+def test_strides_too_far_to_count(q):
+    """Refused before a span is counted (the products would not fit 64 bits)."""
+    a, far = seq_ops.Args(q), (1 << 40) - 16
+    assert a.delta(tokens=1 << 29, heads=2, ldo=far) == q.QH_ERANGE
+    assert a.delta(tokens=1 << 29, heads=2, ldo=256, ldb=far) == q.QH_ERANGE
+    assert a.attn(q_rows=1 << 24, ldq=far) == q.QH_ERANGE
+    assert a.attn(k_rows=1 << 30, ldv=far) == q.QH_ERANGE
 
 
 @pytest.mark.gpu
