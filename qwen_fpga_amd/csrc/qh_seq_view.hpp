@@ -26,13 +26,14 @@ struct View {
   }
   // and width() and bytes() can be counted
   bool countable() const {
-    return (rows <= 1 || ld <= kMaxSpan / eb / (rows - 1)) && (heads <= 1 || hs <= kMaxSpan / eb / (heads - 1)) && dim <= kMaxSpan / eb;
+    auto span = [&](int64_t n, int64_t stride) { return n <= 1 || (__int128)(n - 1) * stride * eb <= kMaxSpan; };
+    return span(rows, ld) && span(heads, hs) && span(2, dim);
   }
   // and no two elements in one place
   bool writable() const {
     if (!readable()) return false;
     if (rows > 1 && heads > 1)
-      return hs >= dim && ld >= dim && ((ld - dim) / (heads - 1) >= hs || (hs - dim) / (rows - 1) >= ld);
+      return hs >= dim && ld >= dim && ((__int128)(heads - 1) * hs <= ld - dim || (__int128)(rows - 1) * ld <= hs - dim);
     return (rows <= 1 || ld >= dim) && (heads <= 1 || hs >= dim);
   }
 };
