@@ -549,6 +549,15 @@ def _ws(t):
     return t.data_ptr() or None, t.nbytes
 
 
+_INT_MAX = 0x7fffffff
+
+
+def _sizes(what: str, *n):
+    """Refuses sizes that the C ABI's ints do not hold (ctypes would pass their low 32 bits)."""
+    if max(n) > _INT_MAX or min(n) < -_INT_MAX:
+        raise QHError(QH_ERANGE, what)
+
+
 def _dims(t, n: int, what: str):
     if getattr(t, "ndim", None) != n:
         raise ValueError(f"{what}: expected a tensor with {n} dimensions")
@@ -564,6 +573,8 @@ def gemm_i8_w8a8(y, w, scale, xq, sx, stream=None):
     tokens, out = ny = _dims(y, 2, "y")
     nw = _dims(w, 2, "w")
     in_, T, dev, ty = nw[1], _Short.tensor, _here(y), _type(y, "y")
+    if tokens > _INT_MAX or out > _INT_MAX or in_ > _INT_MAX:
+        _sizes("qh_gemm_i8_w8a8", tokens, out, in_)
     ly, lx = y.stride(), xq.stride() if xq.__class__ is T else ()
     if not (w.__class__ is T and xq.__class__ is T and scale.__class__ is T and sx.__class__ is T
             and w.dtype is _Short.i8 and xq.dtype is _Short.i8 and scale.dtype is _Short.f32 and sx.dtype is _Short.f32
@@ -588,7 +599,9 @@ def delta_rule_seq_workspace(tokens: int, n_seq: int, heads: int, max_len: int, 
     dtype BF16, less is enough: pass them, or take what serves both types and any k_heads."""
     f = _lib().qh_delta_rule_seq_workspace
     f.restype = ctypes.c_size_t
-    return int(f(int(tokens), int(n_seq), int(heads), int(heads if k_heads is None else k_heads), int(dtype), int(max_len)))
+    n = (int(tokens), int(n_seq), int(heads), int(heads if k_heads is None else k_heads), int(dtype), int(max_len))
+    _sizes("qh_delta_rule_seq_workspace", *n)
+    return int(f(*n))
 
 
 def delta_rule_seq(out, q, k, v, g, beta, S, cu, workspace, max_len: int, stream=None):
@@ -601,6 +614,9 @@ def delta_rule_seq(out, q, k, v, g, beta, S, cu, workspace, max_len: int, stream
     fn = _op("qh_delta_rule_seq")
     nv, nk, ns = _dims(v, 3, "v"), _dims(k, 3, "k"), _dims(S, 4, "S")
     tokens, heads, kh, n, T, dev, dt, ty = nv[0], nv[1], nk[1], ns[0], _Short.tensor, _here(v), v.dtype, _type(v, "v")
+    max_len = int(max_len)
+    if tokens > _INT_MAX or n >= _INT_MAX or max_len > _INT_MAX or max_len < 0 or heads > _INT_MAX or kh > _INT_MAX:
+        _sizes("qh_delta_rule_seq", tokens, n + 1, heads, kh, max_len)
     if not (out.__class__ is T and q.__class__ is T and k.__class__ is T and g.__class__ is T and beta.__class__ is T
             and S.__class__ is T and cu.__class__ is T
             and out.dtype is dt and q.dtype is dt and k.dtype is dt and g.dtype is _Short.f32 and beta.dtype is _Short.f32
@@ -623,7 +639,7 @@ def delta_rule_seq(out, q, k, v, g, beta, S, cu, workspace, max_len: int, stream
         for t, what in ((out, "out"), (q, "q"), (k, "k"), (v, "v"), (g, "g"), (beta, "beta")):
             _operand(t, t.dtype, t.shape, what, rows=True)
     st = fn(out.data_ptr(), lo, ho, q.data_ptr(), lq, hq, k.data_ptr(), lk, hk, v.data_ptr(), lv, hv, ty,
-            g.data_ptr(), lg, beta.data_ptr(), lb, S.data_ptr(), cu.data_ptr(), n, tokens, int(max_len), kh,
+            g.data_ptr(), lg, beta.data_ptr(), lb, S.data_ptr(), cu.data_ptr(), n, tokens, max_len, kh,
             heads, *_ws(workspace), _st(stream))
     if st:
         _check(st, "qh_delta_rule_seq")
@@ -635,6 +651,7 @@ def attention_seq_workspace(q_rows: int, n_seq: int, max_q: int, max_k: int, hea
     f = _lib().qh_attention_seq_workspace
     f.restype = ctypes.c_size_t
     n = (int(q_rows), int(n_seq), int(max_q), int(max_k), int(heads), int(kv_heads), int(head_dim))
+    _sizes("qh_attention_seq_workspace", *n)
     return max(int(f(*n, t)) for t in ((F32, BF16) if dtype is None else (int(dtype),)))
 
 
@@ -653,6 +670,9 @@ def attention_seq(out, q, k, v, cu_q, k_start, k_len, workspace, max_q: int, max
     nq, nk, n = _dims(q, 3, "q"), _dims(k, 3, "k"), _dims(k_len, 1, "k_len")[0]
     (rows, heads, d), (krows, kvh, _) = nq, nk
     T, dev, dt, ty = _Short.tensor, _here(q), q.dtype, _type(q, "q")
+    max_q, max_k = int(max_q), int(max_k)
+    if rows > _INT_MAX or n >= _INT_MAX or not 0 <= max_q <= _INT_MAX or not 0 <= max_k <= _INT_MAX or heads > _INT_MAX or kvh > _INT_MAX:
+        _sizes("qh_attention_seq", rows, n + 1, heads, kvh, max_q, max_k)
     if not (out.__class__ is T and k.__class__ is T and v.__class__ is T and cu_q.__class__ is T and k_start.__class__ is T
             and k_len.__class__ is T
             and out.dtype is dt and k.dtype is dt and v.dtype is dt and cu_q.dtype is _Short.i32 and k_start.dtype is _Short.i64
@@ -671,7 +691,7 @@ def attention_seq(out, q, k, v, cu_q, k_start, k_len, workspace, max_q: int, max
         for t, what in ((out, "out"), (q, "q"), (k, "k"), (v, "v")):
             _operand(t, dt, t.shape, what, rows=True)
     st = fn(out.data_ptr(), lo, ho, q.data_ptr(), lq, hq, k.data_ptr(), lk, hk, v.data_ptr(), lv, hv, ty,
-            cu_q.data_ptr(), k_start.data_ptr(), k_len.data_ptr(), n, rows, krows, int(max_q), int(max_k), heads, kvh,
+            cu_q.data_ptr(), k_start.data_ptr(), k_len.data_ptr(), n, rows, krows, max_q, max_k, heads, kvh,
             d, float(d ** -0.5 if scale is None else scale), *_ws(workspace), _st(stream))
     if st:
         _check(st, "qh_attention_seq")

@@ -501,6 +501,40 @@ def test_strides_too_far_to_count(q):
     assert a.attn(k_rows=1 << 30, ldv=far) == q.QH_ERANGE
 
 
+def test_sizes_beyond_an_int(q, monkeypatch):
+    """Refused, where the C ABI would be given their low 32 bits: by the calls, with tensors that hold no memory, and by
+    the workspaces' queries."""
+    import torch
+    monkeypatch.setattr(q, "_on", lambda t, what: None)
+    monkeypatch.setattr(q, "_op", lambda name: lambda *a: pytest.fail(f"{name} was called with {a}"))
+    f32, i8, i32, i64 = torch.float32, torch.int8, torch.int32, torch.int64
+
+    def z(*shape, dt=f32, many=None):      # a dimension of `many` entries in one place
+        t = torch.empty([1 if i == many else n for i, n in enumerate(shape)], dtype=dt, device="meta")
+        return t.expand(*shape) if many is not None else t
+
+    def refused(call, *args):
+        with pytest.raises(q.QHError) as e:
+            call(*args)
+        assert e.value.status == q.QH_ERANGE
+
+    for big in ((1 << 32) + 4, 1 << 32, 1 << 31):
+        refused(q.gemm_i8_w8a8, z(big, 16), z(16, 32, dt=i8), z(16), z(big, 32, dt=i8, many=0), z(big))
+        refused(q.gemm_i8_w8a8, z(4, big), z(big, 32, dt=i8), z(big), z(4, 32, dt=i8), z(4))
+        a, k = z(big, 2, 128, many=0), z(9, 1, 128)
+        refused(q.delta_rule_seq, a, a, a, a, z(big, 2), z(big, 2), z(1, 2, 128, 128), z(2, dt=i32), None, 4)
+        refused(q.attention_seq, a, a, k, k, z(2, dt=i32), z(1, dt=i64), z(1, dt=i32), None, 4, 9)
+        refused(q.attention_seq, z(4, 2, 128), z(4, 2, 128), k, k, z(big + 1, dt=i32), z(big, dt=i64), z(big, dt=i32), None, 4, 9)
+        a, g = z(4, 2, 128), z(4, 2)
+        refused(q.delta_rule_seq, a, a, a, a, g, g, z(1, 2, 128, 128), z(2, dt=i32), None, big)
+        refused(q.attention_seq, a, a, k, k, z(2, dt=i32), z(1, dt=i64), z(1, dt=i32), None, 4, big)
+        refused(q.attention_seq, a, a, k, k, z(2, dt=i32), z(1, dt=i64), z(1, dt=i32), None, big, 9)
+        refused(q.delta_rule_seq_workspace, big, 1, 2, 100)
+        refused(q.delta_rule_seq_workspace, 100, 1, 2, big)
+        refused(q.attention_seq_workspace, big, 1, 4, 9, 2, 1, 128)
+        refused(q.attention_seq_workspace, 4, 1, 4, big, 2, 1, 128)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
 def test_outputs_beside_their_inputs(q, torch_cuda, bf16):
