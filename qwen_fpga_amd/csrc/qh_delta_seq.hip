@@ -34,7 +34,7 @@ constexpr int kC = 64;                       // tokens of a chunk
 // A chunk's and head's part of the workspace, in floats: T and P in parts of bfloat16, as the operands that the wave of
 // the tokens 16 w .. + 15 takes (depth 32 kk: kk = 0, and 1 for the waves 2 and 3; part by part, 16 bytes a lane: row
 // l % 16, columns 32 kk + 4 (l / 16) .. and + 16); the tokens' factors beta, beta e^c, e^{c_63 - c} and e^c; whether an
-// input is not finite, e^{c_63}.  (The factors in arrays of their own: a lane that loads what it does not use reuses
+// input is large or not finite, e^{c_63}.  (The factors in arrays of their own: a lane that loads what it does not use reuses
 // those registers at once, and waits for the load before it.)
 constexpr int kOperand = 3 * 256, kOffP = 6 * kOperand, kOffRow = 2 * kOffP, kOffFlag = kOffRow + 4 * kC, kChunkFloats = kOffFlag + 64;
 __device__ __forceinline__ constexpr int operand(int w, int kk) { return w + (w == 3) + kk; }
@@ -82,7 +82,6 @@ __device__ __forceinline__ void store1(void* p, int64_t at, float v) {
     as_global_w(static_cast<float*>(p))[at] = v;
 }
 
-__device__ __forceinline__ bool finite(float v) { return (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u; }
 __device__ __forceinline__ f32x4 mfma4(f32x4 x, f32x4 y, f32x4 c) {   // four depths
 #pragma unroll
   for (int r = 0; r < 4; ++r) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[r], y[r], c, 0, 0, 0);
@@ -200,15 +199,17 @@ __device__ __forceinline__ Parts<BF16> parts(const Raw8<BF16>& r) {
   }
   return o;
 }
+// Whether an element is not finite, or so large (2^56) that a sum of products of finite ones may overflow.
+constexpr uint32_t kLarge = (127 + 56) << 7;
 template <bool BF16>
-__device__ __forceinline__ bool any_non_finite(const Raw8<BF16>& r) {
+__device__ __forceinline__ bool any_large(const Raw8<BF16>& r) {
   bool bad = false;
 #pragma unroll
   for (int q = 0; q < (BF16 ? 1 : 2); ++q)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      bad |= (r.v[q][e] & 0x7f800000u) == 0x7f800000u;
-      if constexpr (BF16) bad |= (r.v[q][e] & 0x7f80u) == 0x7f80u;
+      bad |= (r.v[q][e] & 0x7f800000u) >= kLarge << 16;
+      if constexpr (BF16) bad |= (r.v[q][e] & 0x7f80u) >= kLarge;
     }
   return bad;
 }
@@ -291,7 +292,7 @@ __global__ __launch_bounds__(256, BF16 ? 3 : 2) void delta_chunk_kernel(const De
     load_head(hk * rep);
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-      bad |= any_non_finite<BF16>(kr[s]) || any_non_finite<BF16>(qr[s]);
+      bad |= any_large<BF16>(kr[s]) || any_large<BF16>(qr[s]);
       kp[s] = parts<BF16>(kr[s]);
       qp[s] = parts<BF16>(qr[s]);
 #pragma unroll
@@ -328,7 +329,7 @@ __global__ __launch_bounds__(256, BF16 ? 3 : 2) void delta_chunk_kernel(const De
       if (lane < n) {
         gl = gv < -1e5f ? -1e5f : gv;
         be = be0;
-        bad |= !finite(gl) || !finite(be);
+        bad |= !(gl <= 0.5f) || !(__builtin_fabsf(be) < 0x1p56f);   // (64 tokens of 1/2: e^32)
       }
       double c = gl;
 #pragma unroll
@@ -347,7 +348,7 @@ __global__ __launch_bounds__(256, BF16 ? 3 : 2) void delta_chunk_kernel(const De
       if (lane == kC - 1) ws[kOffFlag + 1] = ec;
     }
 #pragma unroll
-    for (int u = 0; u < NV; ++u) bad |= any_non_finite<BF16>(vr[u]);
+    for (int u = 0; u < NV; ++u) bad |= any_large<BF16>(vr[u]);
     if (h + 1 < (hk + 1) * rep) load_head(h + 1);
     const uint64_t any = __ballot(bad);
     if (lane == 0) bad_in[wave] = any != 0;
@@ -518,8 +519,8 @@ __global__ __launch_bounds__(576, 2) void delta_scan_kernel(const DeltaSeq a) {
       for (int e = 0; e < 8; ++e) s[n][e] = as_global(Sp)[(32 * w + 8 * g + e) * kD + 16 * n];
     while (c < nc) {
       if (flagged(c) != 0.0f) {
-        // an input that is not finite: the products below would carry it to tokens before it (0 times it is not
-        // 0), so the chunk runs token by token, in all four waves alike (lane: rows 32 w + 8 (l / 16) .. + 7 of all w)
+        // an input that is not finite, or from which a sum may overflow: the products below would carry it to tokens
+        // before it (0 times infinity is not 0), so the chunk runs token by token, in all four waves alike (lane: rows 32 w + 8 (l / 16) .. + 7 of all w)
         float* x0 = reinterpret_cast<float*>(xl);
 #pragma unroll
         for (int n = 0; n < NB; ++n)

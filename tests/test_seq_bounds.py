@@ -429,6 +429,31 @@ def test_delta_non_finite_inputs_of_many_heads(q, torch_cuda, bf16, which, bad):
         assert not torch.isfinite(S[0, heads]).all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+@pytest.mark.parametrize("which", ["v", "q", "k", "beta", "g"])
+def test_delta_overflow_of_finite_inputs(q, torch_cuda, bf16, which):
+    """A finite value from which a token's delta, state or output overflows has no influence on the tokens before it."""
+    torch = torch_cuda
+    lens, at = [100, 80], 75
+    host, _ = ops.delta_inputs(torch, 21, lens, 2, 2, bf16, decay=0.05, fused=False)
+    bound = delta_bound(torch, *host, lens)
+    big = [x.clone() for x in host]
+    if which == "v":            # the second delta is -2 * 3e38, the first and all inputs are finite
+        big[1][at + 1, 0] = big[1][at, 0]
+        big[2][at, 0], big[2][at + 1, 0] = 3e38, -3e38
+        big[3][at:at + 2, 0], big[4][at:at + 2, 0] = 0.0, 1.0
+    else:
+        big[["q", "k", "", "g", "beta"].index(which)][at, 0] = 150.0 if which == "g" else 3e38
+    S = host[5].cuda()
+    out = ops.delta_run(q, torch, [x.cuda() for x in big[:5]], S, lens).cpu()
+    assert not torch.isfinite(out[at:100, 0]).all()
+    for rows, heads in ((slice(0, at), [0, 1]), (slice(0, 100), [1]), (slice(100, 180), [0, 1])):
+        part = (bound[0][rows][:, heads], bound[1][:0], bound[2][rows][:, heads], bound[3][:0])
+        assert delta_excess(out[rows][:, heads], S[:0], part, bf16)[0] <= 1
+    assert delta_excess(out[:0], S[1:], (bound[0][:0], bound[1][1:], bound[2][:0], bound[3][1:]), bf16)[1] <= 1
+
+
 # ------------------------------------------------------------------ operands in one buffer
 
 VIEWS = r"""
