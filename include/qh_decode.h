@@ -229,8 +229,10 @@ int qh_mlp_layer_w8a8(float* out, const float* x, const qh_tensor* gate_w, const
  * Sequences stand one after another: sequence i has the rows cu[i] .. cu[i + 1]
  * (cu [n_seq + 1] int32, on the device).  Empty sequences are allowed; rows
  * outside every sequence are left as they were; a sequence whose bounds are out
- * of order or outside the array is taken as empty (and rows that two sequences
- * then share hold nothing in particular).  max_len, max_q and max_k
+ * of order or outside the array is taken as empty.  Sequences may not share rows:
+ * where those that are left do (bounds that go back), the call ends like any other
+ * and writes nothing outside their rows and states, but what it writes there, in
+ * other sequences' too, holds nothing in particular.  max_len, max_q and max_k
  * are the caller's bounds on the lengths: they choose the form of the kernels
  * and the size of the workspace, longer sequences are computed all the same.
  *

@@ -496,7 +496,8 @@ def quant_rows(q, scale, w, rows: int, cols: int, stream=None):
 
 # ---------------------------------------------------------------- packed sequences
 # Tensors carry their own sizes and strides here: operands are [rows, heads, dim] with a unit last stride,
-# the other two as the caller has them.  Every tensor has to be on the current device, whose stream the call
+# the other two as the caller has them.  Sequences may not share rows (include/qh_decode.h: what bounds that are
+# no bounds give).  Every tensor has to be on the current device, whose stream the call
 # takes.
 
 F32, BF16 = 0, 1

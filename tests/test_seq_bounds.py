@@ -582,3 +582,35 @@ def test_outputs_beside_their_inputs(q, torch_cuda, bf16):
     both = torch.cat([dd[2], torch.full_like(dd[2], 7.0)], -1)
     ops.delta_run(q, torch, dd[:2] + [both[:, :, :128]] + dd[3:], S2, lens, out=both[:, :, 128:])
     assert torch.equal(both[:, :, 128:], want) and torch.equal(both[:, :, :128], dd[2]) and torch.equal(S, S2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+@pytest.mark.parametrize("cu", [[0, 300, 0, 300, 0, 310], [0, 310, 5, 200, 90, 310], [0, 70, 70, 10, 250, 250]], ids=str)
+def test_sequences_that_share_rows(q, torch_cuda, bf16, cu):
+    """Bounds that go back: the calls end, and leave alone what lies around their outputs, states and workspaces."""
+    torch = torch_cuda
+    t, h, kvh, n, dt = 320, 4, 2, len(cu) - 1, torch.bfloat16 if bf16 else torch.float32
+    g = ops.gen(torch, 3)
+    rnd = lambda *s: torch.randn(*s, generator=g).to(dt).cuda()
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    qq, kk, vv = rnd(t, h, 128), rnd(2000, kvh, 128), rnd(2000, kvh, 128)
+    dk = torch.nn.functional.normalize(rnd(t, kvh, 128).float(), dim=-1).to(dt)
+
+    def room(need):      # a workspace inside a larger array of one value
+        buf = torch.full((need + 1024,), 0x5A, dtype=torch.uint8, device="cuda")
+        return buf, buf[512:512 + need] if need else None
+
+    for max_q, max_k in ((1, 1), (1, 2000), (320, 2000), (4096, 2000), (4096, 300)):
+        buf, ws = room(q.attention_seq_workspace(t, n, max_q, max_k, h, kvh, 128))
+        out = torch.full((t + 2, h, 128), 7.0, dtype=dt, device="cuda")
+        q.attention_seq(out[1:-1], qq, kk, vv, i32(cu), torch.arange(n, device="cuda") * 10, i32([1900] * n), ws, max_q, max_k)
+        assert (out[0] == 7).all() and (out[-1] == 7).all() and (out[311:] == 7).all()
+        assert (buf[:512] == 0x5A).all() and (buf[-512:] == 0x5A).all()
+    for max_len in (1, 320):
+        buf, ws = room(q.delta_rule_seq_workspace(t, n, h, max_len, k_heads=kvh, dtype=q.BF16 if bf16 else q.F32))
+        S, out = torch.full((n + 2, h, 128, 128), 0.5, device="cuda"), torch.full((t + 2, h, 128), 7.0, dtype=dt, device="cuda")
+        q.delta_rule_seq(out[1:-1], dk, dk, qq, torch.full((t, h), -0.1, device="cuda"), torch.full((t, h), 0.5, device="cuda"), S[1:-1], i32(cu),
+                         ws, max_len)
+        assert (out[0] == 7).all() and (out[-1] == 7).all() and (out[311:] == 7).all()
+        assert (S[0] == 0.5).all() and (S[-1] == 0.5).all() and (buf[:512] == 0x5A).all() and (buf[-512:] == 0x5A).all()
