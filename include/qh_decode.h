@@ -239,7 +239,13 @@ int qh_mlp_layer_w8a8(float* out, const float* x, const qh_tensor* gate_w, const
  * Nothing is allocated; scratch is the caller's workspace (256-byte aligned, at
  * least the bytes its query names, NULL allowed for 0; nothing in it lasts from
  * one call to the next).  Calls that can run at the same time, captured graphs
- * among them, need a workspace each.
+ * among them, need a workspace each.  Its size: the delta rule in chunks takes, for
+ * every 64 tokens and once more a sequence, 37 KB a head and (fp32) 96 KB or (bfloat16)
+ * 32 KB a key head: 52 MB for 1500 fp32 tokens of 16 heads, none for short sequences;
+ * attention of prompts takes up to 512 units' sums, (bfloat16) 256 or (fp32) 128 rows
+ * of head_dim + 2 floats each (135 MB at most for bfloat16 heads of 256, 14 MB for a
+ * prompt of 512 tokens), and of few rows 16 such rows for every 16 rows (tokens times query
+ * heads of a kv head) and kv head, and for 512 units more.
  * ==================================================================== */
 #define QH_F32 0
 #define QH_BF16 1
