@@ -436,10 +436,11 @@ __global__ __launch_bounds__(1024) void attn_join_kernel(const AttnSeq a) {
 // 512 behind 7488, 53 and 61 for 256 behind 7744 (more units to join).  Units start in order, unit b on XCD b % 8: so
 // the longest come first, and neighbours are about equally long.
 // The workgroups of an XCD then walk the keys of one head side by side and find them in its L2: shares cut to the same
-// length anywhere in the tiles missed it for 38% of the reads and took 450 us, not 390, for 16k packed tokens (8 / 2
-// heads of 256).
-// Split and whole, bfloat16: one sequence of 8000 tokens 317 and 359 us, 4096 114 and 170, 1024 42 and 56, 512 35 and
-// 36; two of 8000 509 and 520; those 16k tokens 420 and 452 (one call behind another without a pause).
+// length anywhere in the tiles missed it for 38% of the reads and took 15% longer for 16k packed tokens (8 / 2 heads of
+// 256).  (Each pair of figures here is of one run, the two timed side by side; runs differ by some per cent.)
+// Split and whole, bfloat16, calls one behind another over the same operands: one sequence of 512 tokens 34 and 36 us, 1024
+// 43 and 54, 1500 47 and 70, 4096 109 and 163, 8000 290 and 316; 128 tokens behind 7872 keys 47 and 298; where there are
+// tiles for all CUs without it, splitting costs a little: two of 8000 tokens 454 and 435, those 16k 361 and 354.
 constexpr int kCUs = 256, kMaxTileSplits = 64;
 constexpr int min_tile_chunk(bool bf16) { return bf16 ? 256 : 128; }
 struct TileUnit {
@@ -549,7 +550,7 @@ constexpr size_t tile_part_floats(int tile, int D) { return (size_t)tile * (D + 
 // rarely rescaled.
 // bfloat16: at full load the card's power bounds it (1.85 GHz): 930 to 1100 TFLOP/s at 256 elements and long prompts,
 // 830 at 128.  With 64 rows a wave, 128 elements took 301 us for 8000 tokens of 8 heads, and 32 rows take 190.
-// fp32: the fp32 MFMAs bound it, 89% of their cycles at 2.15 GHz; 1500 tokens 159 us in the form for few rows, 116 in
+// fp32: the fp32 MFMAs bound it, 89% of their cycles at 2.15 GHz; 1500 tokens 163 us in the form for few rows, 119 in
 // this, of which the join takes 10 and a CU has work for 84; 512 tokens behind 7488 keys 116 TFLOP/s.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
@@ -713,7 +714,7 @@ __global__ __launch_bounds__(512, 2) void attn_tile_kernel(const AttnSeq a) {
     bool bad = false;   // (see attn_split_kernel: what is not finite in V goes only to the rows that see it)
     if constexpr (BF16) {
       // P rounded to bfloat16 once, 2^-8 of sum p |V|.  Two parts, as in the form for few rows, would be half as many
-      // products again: 8000 tokens 304 -> 427 us, 16k packed 370 -> 540, 1024 44 -> 50.
+      // products again: 8000 tokens 304 -> 427 us, 1024 44 -> 50.
       u32x4 pf[2];
 #pragma unroll
       for (int r = 0; r < 16; r += 2) {
@@ -906,11 +907,12 @@ hipError_t launch(const AttnSeq& a, hipStream_t s) {
 AttnForm attn_seq_form(int64_t q_rows, int n_seq, int max_q, int max_k, int heads, int kv_heads, int dim, bool bf16) {
   const int G = heads / kv_heads;
   AttnForm f = {0, 0, 0};
-  // Prompts, or many short ones that see many keys.  8 / 2 heads of 256, us in this form and in the one for few rows:
-  // fp32   one of 256 tokens 49 and 29, of 512 56 and 56, of 1500 116 and 157, of 4096 714 and 817; 128 tokens behind
-  //        1372 keys 58 and 44, behind 7872 113 and 121; 16 of 128 tokens 47 and 40, behind 7872 keys 1018 and 1386
-  // bf16   one of 128 tokens 24 and 11, of 256 27 and 26, of 512 35 and 43, of 4096 115 and 369; 128 tokens behind
-  //        1372 keys 37 and 32, behind 7872 49 and 61; 16 of 128 tokens 24 and 25, behind 7872 keys 169 and 598
+  // Prompts, or many short ones that see many keys.  8 / 2 heads of 256, us in this form and in the one for few rows (calls
+  // one behind another over the same operands):
+  // fp32   one of 128 tokens 41 and 15, of 256 49 and 30, of 512 56 and 57, of 1500 119 and 163, of 4096 705 and 811; 128
+  //        behind 1372 keys 55 and 41, behind 7872 108 and 119; 16 of 128 tokens 49 and 42, behind 7872 keys 1006 and 1379
+  // bf16   one of 128 tokens 22 and 11, of 256 27 and 26, of 512 34 and 42, of 4096 109 and 371; 128 behind 1372 keys
+  //        35 and 31, behind 7872 47 and 61; 16 of 128 tokens 25 and 27, behind 7872 keys 162 and 589
   const int64_t seen = q_rows * heads * std::max(max_k, 1);
   if ((int64_t)max_q * G >= (bf16 ? 1024 : 2048) || ((int64_t)max_q * G >= 128 && seen >= 5000000)) {
     f.tile = tile_rows(bf16);
