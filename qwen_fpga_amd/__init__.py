@@ -664,7 +664,8 @@ def attention_seq(out, q, k, v, cu_q, k_start, k_len, workspace, max_q: int, max
     and head strides); cu_q int32 [n_seq + 1], k_start int64 [n_seq] and k_len int32 [n_seq] on the device:
     sequence i's keys are the rows k_start[i] .. + k_len[i], the new tokens' own among them, and row r of
     q_len sees the first r + 1 + k_len - q_len (0 comes out where it sees none).  scale: 1 / sqrt(dim) if
-    None.  max_q and max_k bound the sequences' rows and keys (they choose the kernels' form); workspace:
+    None.  Up to 65536 sequences; the search for each workgroup's rows grows with their number (4096 single tokens
+    take 5.7 ms).  max_q and max_k bound the sequences' rows and keys (they choose the kernels' form); workspace:
     attention_seq_workspace(...) bytes.  bfloat16: the form for prompts rounds the probabilities to bfloat16 for
     their product with v (2^-8 of sum p |v|), the one for few rows takes them in two parts (2^-14)."""
     fn = _op("qh_attention_seq")

@@ -102,7 +102,7 @@ int qh_delta_rule_seq(void* out, int64_t ldo, int64_t hso, const void* q, int64_
 }
 
 size_t qh_attention_seq_workspace(int q_rows, int n_seq, int max_q, int max_k, int heads, int kv_heads, int head_dim, int type) {
-  if (!type_ok(type) || q_rows <= 0 || n_seq <= 0 || max_q < 0 || max_k < 0 || max_k > kMaxKeys || heads <= 0 || kv_heads <= 0 ||
+  if (!type_ok(type) || q_rows <= 0 || n_seq <= 0 || n_seq > QH_ATTN_MAX_SEQ || max_q < 0 || max_k < 0 || max_k > kMaxKeys || heads <= 0 || kv_heads <= 0 ||
       heads % kv_heads != 0 || (head_dim != 128 && head_dim != 256) || (int64_t)q_rows * heads > kMaxUnits)
     return 0;
   return attn_seq_form(q_rows, n_seq, max_q, max_k, heads, kv_heads, head_dim, type == QH_BF16).bytes;
@@ -116,7 +116,7 @@ int qh_attention_seq(void* out, int64_t ldo, int64_t hso, const void* q, int64_t
       heads % kv_heads != 0 || (head_dim != 128 && head_dim != 256) || !std::isfinite(scale))
     return QH_EINVAL;
   if (q_rows == 0 || n_seq == 0) return QH_OK;
-  if (max_k > kMaxKeys || (int64_t)q_rows * heads > kMaxUnits || k_rows >= kMaxStride ||
+  if (n_seq > QH_ATTN_MAX_SEQ || max_k > kMaxKeys || (int64_t)q_rows * heads > kMaxUnits || k_rows >= kMaxStride ||
       seq_tiles_max((int64_t)q_rows * (heads / kv_heads), n_seq, 16) * kv_heads > kMaxTiles)
     return QH_ERANGE;
   const int eb = type == QH_BF16 ? 2 : 4;

@@ -526,6 +526,13 @@ def test_strides_too_far_to_count(q):
     assert a.attn(k_rows=1 << 30, ldv=far) == q.QH_ERANGE
 
 
+def test_more_sequences_than_a_search_is_for(q):
+    """Every workgroup looks through all of them: a million would take minutes."""
+    a = seq_ops.Args(q)
+    assert a.attn(n_seq=65537, q_rows=70000) == q.QH_ERANGE and a.attn(n_seq=1 << 20, q_rows=1 << 20) == q.QH_ERANGE
+    assert q.attention_seq_workspace(70000, 65537, 1, 1000, 2, 1, 128) == 0 < q.attention_seq_workspace(70000, 65536, 1, 1000, 2, 1, 128)
+
+
 def test_sizes_beyond_an_int(q, monkeypatch):
     """Refused, where the C ABI would be given their low 32 bits: by the calls, with tensors that hold no memory, and by
     the workspaces' queries."""
@@ -614,3 +621,19 @@ def test_sequences_that_share_rows(q, torch_cuda, bf16, cu):
                          ws, max_len)
         assert (out[0] == 7).all() and (out[-1] == 7).all() and (out[311:] == 7).all()
         assert (S[0] == 0.5).all() and (S[-1] == 0.5).all() and (buf[:512] == 0x5A).all() and (buf[-512:] == 0x5A).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("max_k", [100, 400])
+def test_attention_of_thousands_of_sequences(q, torch_cuda, max_k):
+    """One token each; empty ones and long ones among them."""
+    torch = torch_cuda
+    lens = [i % 7 != 3 for i in range(2500)]
+    ctx = [1 + (37 * i) % 90 for i in range(2500)]
+    for i in (0, 64, 1000, 2499):
+        lens[i], ctx[i] = 1, 390
+    lens = [int(n) for n in lens]
+    qq, kk, vv, at_k = ops.attn_inputs(torch, 17, lens, ctx, 2, 1, 128, True)
+    got = ops.attn_run(q, torch, qq.cuda(), kk.cuda(), vv.cuda(), lens, ctx, at_k, max_k=max_k)
+    want, lim = attn_limit(torch, (qq, kk, vv, lens, ctx, at_k, 1 / math.sqrt(128)), True, FEW)
+    assert ((got.cpu().double() - want).abs() <= lim).all()
