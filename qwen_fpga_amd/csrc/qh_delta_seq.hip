@@ -246,8 +246,9 @@ __device__ __forceinline__ void put_operand(float* to, int lane, const f32x4& x,
 
 // T, P and the row factors of one chunk, for the value heads of one key head.  Wave i forms the tiles (i, j <= i) of
 // K K^T and Q K^T once; every head scales them.  A head's inputs are brought while the products of the one before run.
-// What bounds it: for one sequence of 1500 tokens (384 workgroups, all at once, 21 us) k and q's way from memory, 7 us, and
-// a chain of short steps; for 7.2k packed tokens of 32 heads 78 us, three workgroups a CU (two: 82).
+// What bounds it is mostly its traffic: for one sequence of 1500 fp32 tokens of 16 heads (384 workgroups, all at once, 21
+// us) 37 MB of inputs and 52 MB of workspace, 18 us at the rate of a large copy; for 7.2k packed bfloat16 tokens of 32
+// heads (77 us, three workgroups a CU; two: 82) 120 and 210 MB, 66 us.
 template <bool BF16>
 __global__ __launch_bounds__(256, BF16 ? 3 : 2) void delta_chunk_kernel(const DeltaSeq a) {
   constexpr int LD = kC + 4, NP = Parts<BF16>::NP;
