@@ -637,3 +637,62 @@ def test_attention_of_thousands_of_sequences(q, torch_cuda, max_k):
     got = ops.attn_run(q, torch, qq.cuda(), kk.cuda(), vv.cuda(), lens, ctx, at_k, max_k=max_k)
     want, lim = attn_limit(torch, (qq, kk, vv, lens, ctx, at_k, 1 / math.sqrt(128)), True, FEW)
     assert ((got.cpu().double() - want).abs() <= lim).all()
+
+
+# ------------------------------------------------------------------ calls beside one another
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+def test_calls_at_the_same_time(q, torch_cuda, bf16):
+    """Two streams, each with outputs, states and workspaces of its own, over the same inputs, in both forms; and the two
+    captured and replayed beside each other: every result that of a call alone."""
+    torch = torch_cuda
+    lens, ctx, at_k = [260, 1, 130], [2000, 900, 1500], [0, 1000, 500]      # (keys that sequences share)
+    t, h, kvh = sum(lens), 8, 2
+    qq, kk, vv, _ = ops.attn_inputs(torch, 19, lens, [2000], h, kvh, 128, bf16)
+    host, dev = ops.delta_inputs(torch, 19, lens, 2, h, bf16, fused=False)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    args = [x.cuda() for x in (qq, kk, vv)] + [i32(ops.starts(lens)), torch.tensor(at_k, device="cuda"), i32(ctx)]
+    S0, cu = host[5].cuda(), i32(ops.starts(lens))
+
+    class Call:
+        def __init__(self, max_q, max_len):
+            u8 = lambda n: torch.empty(n, dtype=torch.uint8, device="cuda")
+            self.max_q, self.max_len, self.S = max_q, max_len, S0.clone()
+            self.out, self.do = torch.empty_like(args[0]), torch.empty_like(dev[2])
+            self.w1, self.w2 = u8(q.attention_seq_workspace(t, 3, max_q, 2000, h, kvh, 128)), u8(q.delta_rule_seq_workspace(t, 3, h, max_len))
+
+        def run(self):
+            self.S.copy_(S0)
+            q.attention_seq(self.out, *args, self.w1, self.max_q, 2000)
+            q.delta_rule_seq(self.do, *dev, self.S, cu, self.w2, self.max_len)
+
+        def all(self):
+            return [self.out, self.do, self.S]
+
+    for max_q, max_len in ((1, 260), (4096, 260), (260, 1)):
+        calls, streams = [Call(max_q, max_len), Call(max_q, max_len)], [torch.cuda.Stream(), torch.cuda.Stream()]
+        calls[0].run()
+        want = [x.clone() for x in calls[0].all()]
+        graphs = []
+        for c in calls:
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                c.run()
+            graphs.append(g)
+        for replay in (False, True, True):
+            for c in calls:
+                for x in c.all():
+                    x.zero_()
+            torch.cuda.synchronize()
+            for _ in range(3):
+                for c, s, g in zip(calls, streams, graphs):
+                    with torch.cuda.stream(s):
+                        g.replay() if replay else c.run()
+            torch.cuda.synchronize()
+            for c in calls:
+                assert all(torch.equal(x, y) for x, y in zip(c.all(), want))
+    scale = 1 / math.sqrt(128)
+    wo, lim = attn_limit(torch, (qq, kk, vv, lens, ctx, at_k, scale), bf16, PROMPTS)
+    assert ((want[0].cpu().double() - wo).abs() <= lim).all()
+    assert max(delta_excess(want[1], want[2], delta_bound(torch, *host, lens), bf16)) <= 1
