@@ -548,8 +548,9 @@ constexpr size_t tile_part_floats(int tile, int D) { return (size_t)tile * (D + 
 // and c ^ 4 (r % 4) of V's in bfloat16 (four keys of 32 elements do, as the transposing read takes them).  The running
 // maximum moves only when a score passes it by more than 8 (a factor of 256, exact in the sums), so that the sums are
 // rarely rescaled.
-// bfloat16: at full load the card's power bounds it (1.85 GHz): 930 to 1100 TFLOP/s at 256 elements and long prompts,
-// 830 at 128.  With 64 rows a wave, 128 elements took 301 us for 8000 tokens of 8 heads, and 32 rows take 190.
+// bfloat16: at full load the card's power bounds it (1.85 GHz): one and two sequences of 8000 tokens and 8 heads of 256
+// elements 900 and 1150 TFLOP/s, of 128 elements (the same softmax for half the products) 680 and 910.  With 64 rows a
+// wave, 128 elements took 301 us for 8000 tokens, and 32 rows take 190.
 // fp32: the fp32 MFMAs bound it, 89% of their cycles at 2.15 GHz; 1500 tokens 163 us in the form for few rows, 119 in
 // this, of which the join takes 10 and a CU has work for 84; 512 tokens behind 7488 keys 116 TFLOP/s.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
