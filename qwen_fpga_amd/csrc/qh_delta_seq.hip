@@ -11,7 +11,8 @@
 //
 // The products run on the matrix cores at fp32 precision.  A float is the sum of three bfloat16 exactly (its 24 bits
 // cut into three eights, by masking), so an fp32 product is the six largest of the nine partial products (what is
-// left out, the second times the third part twice over, is below 2^-21 of the product), and one with a bfloat16 operand is three: 6 and 3 MFMAs of 16 cycles do
+// left out, the second times the third part twice over, is below 2^-21 of the product), and one with a bfloat16
+// operand is three: 6 and 3 MFMAs of 16 cycles do
 // what takes eight of 32 in v_mfma_f32_16x16x4_f32.  That one stays for the small triangular products with T and P.
 // In all of them lane l has row l % 16 of the left and column l % 16 of the right operand, at the depths of lane group
 // l / 16, and ends with rows 4 (l / 16) .. + 3 of column l % 16: what a lane holds of a result is what it has to
@@ -521,7 +522,8 @@ __global__ __launch_bounds__(576, 2) void delta_scan_kernel(const DeltaSeq a) {
     while (c < nc) {
       if (flagged(c) != 0.0f) {
         // an input that is not finite, or from which a sum may overflow: the products below would carry it to tokens
-        // before it (0 times infinity is not 0), so the chunk runs token by token, in all four waves alike (lane: rows 32 w + 8 (l / 16) .. + 7 of all w)
+        // before it (0 times infinity is not 0), so the chunk runs token by token, in all four waves alike (lane: rows
+        // 32 w + 8 (l / 16) .. + 7 of all w)
         float* x0 = reinterpret_cast<float*>(xl);
 #pragma unroll
         for (int n = 0; n < NB; ++n)

@@ -51,8 +51,7 @@ inline bool overlap(const View& a, const View& b) {
     if (d < 0) d += period;
     return d >= wa && d + wb <= period;
   };
-  const int64_t la = a.ld * a.eb, lb = b.ld * b.eb;
-  if (a.rows > 1 && b.rows > 1 && la == lb && la > 0 && apart(la, a.width(), b.width())) return false;
+  if (a.rows > 1 && b.rows > 1 && a.ld * a.eb == b.ld * b.eb && a.ld > 0 && apart(a.ld * a.eb, a.width(), b.width())) return false;
   int64_t step = 0;
   for (const View* v : {&a, &b}) {
     if (v->rows > 1) step = std::gcd(step, v->ld * v->eb);

@@ -469,7 +469,7 @@ int main() {
   auto pick = [&](std::initializer_list<int> v) { return *(v.begin() + g() % v.size()); };
   const uintptr_t base = 1 << 20;
   long apart = 0, write = 0;
-  for (int it = 0; it < 200000; ++it) {
+  for (int it = 0; it < 60000; ++it) {
     View v[2];
     std::map<uintptr_t, int> bytes[2];
     bool twice[2] = {false, false};
@@ -495,12 +495,15 @@ int main() {
         if (bytes[1].count(b.first)) return std::printf("%d: taken as apart\n", it), 1;
     }
   }
-  if (apart < 10000 || write < 10000) return std::printf("%ld apart, %ld writable\n", apart, write), 1;
+  if (apart < 5000 || write < 5000) return std::printf("%ld apart, %ld writable\n", apart, write), 1;
   auto at = [&](int64_t el) { return reinterpret_cast<const void*>(base + 2 * el); };
   const View out{at(128), 40, 8, 128, 8 * 256, 256, 2}, q{at(0), 40, 8, 128, 8 * 256, 256, 2};   // halves of each head
   if (overlap(out, q) || !overlap(View{at(64), 40, 8, 128, 8 * 256, 256, 2}, q)) return std::printf("halves\n"), 1;
   const View odd{at(0), 3, 4, 128, 2 * 128, 5 * 128, 2};   // every other row of head-major rows, five a head
   if (!odd.writable()) return std::printf("every other row\n"), 1;
+  // (strides of dimensions with one entry do not count, whatever they are)
+  const View one{at(0), 1, 1, 128, INT64_MAX, INT64_MIN, 2}, next{at(128), 1, 1, 128, INT64_MIN, INT64_MAX, 2};
+  if (!one.writable() || !one.countable() || overlap(one, next) || !overlap(one, one) || !overlap(one, q)) return std::printf("one entry\n"), 1;
   if (View{at(0), 1 << 30, 4, 128, (int64_t)1 << 39, 128, 4}.countable() || View{at(0), 4, 1 << 30, 128, 128, (int64_t)1 << 39, 4}.countable())
     return std::printf("too far\n"), 1;
   return 0;
@@ -511,7 +514,7 @@ int main() {
 def test_views(tmp_path):
     src, exe = tmp_path / "t.cpp", tmp_path / "t"
     src.write_text(VIEWS)
-    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Wextra", "-Werror", "-ftrapv", "-I", os.path.join(ROOT, "qwen_fpga_amd", "csrc"),
+    subprocess.run(["g++", "-std=c++17", "-O0", "-Wall", "-Wextra", "-Werror", "-ftrapv", "-I", os.path.join(ROOT, "qwen_fpga_amd", "csrc"),
                     "-o", str(exe), str(src)], check=True)
     r = subprocess.run([str(exe)], capture_output=True, text=True)
     assert r.returncode == 0, r.stdout + r.stderr
