@@ -242,6 +242,11 @@ _OPS = {
     "qh_gemm_i8_w8a8": [_V, _L, _I] + [_V] * 3 + [_L, _V] + [_I] * 3 + [_V],
     "qh_delta_rule_seq": [_V, _L, _L] * 4 + [_I, _V, _L, _V, _L, _V, _V] + [_I] * 5 + [_V, ctypes.c_size_t, _V],
     "qh_attention_seq": [_V, _L, _L] * 4 + [_I, _V, _V, _V, _I, _I, _L] + [_I] * 5 + [_FL, _V, ctypes.c_size_t, _V],
+    "qh_qk_norm_rope_seq": [_V, _L, _L] * 4 + [_I, _V, _V, _V] + [_I] * 5 + [ctypes.c_double, _FL, _V],
+    "qh_kv_cache_write_i8": [_V, _L, _L] * 6 + [_I, _V, _L] + [_I] * 3 + [_V],
+    "qh_kv_cache_read_i8": [_V, _L, _L] * 2 + [_I] + [_V, _L, _L] * 4 + [_V, _L] + [_I] * 3 + [_V],
+    "qh_attention_seq_i8": [_V, _L, _L] * 2 + [_I] + [_V, _L, _L] * 4 + [_V, _V, _V, _I, _I, _L] + [_I] * 5
+                           + [_FL, _V, ctypes.c_size_t, _V],
 }
 for _n in ("deltanet", "attention", "mlp"):
     _OPS[f"qh_{_n}_layer_w8a8"] = _OPS[f"qh_{_n}_layer"]
@@ -527,7 +532,7 @@ def _here(t) -> int:
 
 # The calls below compare all operands in one expression, which is most of what they cost the host; where it
 # does not hold, _operand looks at each (and raises what is wrong with it, or takes a tensor of another class).
-def _operand(t, dt, shape, what: str, rows: bool = False):
+def _operand(t, dt, shape, what: str, rows: bool = False, free: bool = False):
     _on(t, what)
     if t.dtype is not dt:
         raise TypeError(f"{what}: dtype {t.dtype}, expected {dt}")
@@ -536,7 +541,7 @@ def _operand(t, dt, shape, what: str, rows: bool = False):
     if rows:
         if t.stride()[-1] != 1 and shape[-1] > 1:
             raise ValueError(f"{what}: the last dimension has stride {t.stride()[-1]}, expected 1")
-    elif not t.is_contiguous():
+    elif not free and not t.is_contiguous():
         raise ValueError(f"{what}: tensor is not contiguous")
 
 
@@ -697,6 +702,152 @@ def attention_seq(out, q, k, v, cu_q, k_start, k_len, workspace, max_q: int, max
             d, float(d ** -0.5 if scale is None else scale), *_ws(workspace), _st(stream))
     if st:
         _check(st, "qh_attention_seq")
+
+
+# ---------------------------------------------------------------- an int8 K/V cache
+# Codes kq, vq int8 [rows, kv_heads, dim] (dim 128 or 256, a unit last stride) and a scale for each row and head,
+# ks, vs float32 [rows, kv_heads] (any strides): an element is code * scale.
+
+def qk_norm_rope_seq(q_out, k_out, q, k, q_norm, k_norm, pos, rope_dim: int = 64, theta: float = 1e7, eps: float = EPS,
+                     stream=None):
+    """The norms of queries and keys for each head (rmsnorm, weights 1 + q_norm and 1 + k_norm), then the position
+    rotation of each head's first rope_dim elements (rope_cos_sin and apply_rope for 64 of them), in one pass.
+
+    q, q_out [tokens, heads, dim], k, k_out [tokens, kv_heads, dim] (float32 or bfloat16, dim 128 or 256, any row and
+    head strides), q_norm, k_norm float32 [dim], pos int32 [tokens] on the device, rope_dim a multiple of 16 (0: norms
+    only).  q_out and k_out may be q and k themselves.  Angles are formed in 64 bits."""
+    fn = _op("qh_qk_norm_rope_seq")
+    nq, nk = _dims(q, 3, "q"), _dims(k, 3, "k")
+    (tokens, heads, d), kvh = nq, nk[1]
+    T, dev, dt, ty, rope_dim = _Short.tensor, _here(q), q.dtype, _type(q, "q"), int(rope_dim)
+    if tokens > _INT_MAX or heads > _INT_MAX or kvh > _INT_MAX or not -_INT_MAX <= rope_dim <= _INT_MAX:
+        _sizes("qh_qk_norm_rope_seq", tokens, heads, kvh, rope_dim)
+    if not (q_out.__class__ is T and k_out.__class__ is T and k.__class__ is T and q_norm.__class__ is T and k_norm.__class__ is T
+            and pos.__class__ is T
+            and q_out.dtype is dt and k_out.dtype is dt and k.dtype is dt and q_norm.dtype is _Short.f32
+            and k_norm.dtype is _Short.f32 and pos.dtype is _Short.i32
+            and q_out.shape == nq and nk == (tokens, kvh, d) and k_out.shape == nk and q_norm.shape == (d,)
+            and k_norm.shape == (d,) and pos.shape == (tokens,)
+            and q_norm.is_contiguous() and k_norm.is_contiguous() and pos.is_contiguous()
+            and dev == q_out.get_device() == k_out.get_device() == k.get_device() == q_norm.get_device() == k_norm.get_device()
+            == pos.get_device()):
+        for t, shape, what in ((q_out, nq, "q_out"), (k_out, (tokens, kvh, d), "k_out"), (q, nq, "q"), (k, (tokens, kvh, d), "k")):
+            _operand(t, dt, shape, what, rows=True)
+        _operand(q_norm, _Short.f32, (d,), "q_norm")
+        _operand(k_norm, _Short.f32, (d,), "k_norm")
+        _operand(pos, _Short.i32, (tokens,), "pos")
+    (l0, h0, e0), (l1, h1, e1), (l2, h2, e2), (l3, h3, e3) = q_out.stride(), k_out.stride(), q.stride(), k.stride()
+    if not e0 == e1 == e2 == e3 == 1:
+        for t, what in ((q_out, "q_out"), (k_out, "k_out"), (q, "q"), (k, "k")):
+            _operand(t, dt, t.shape, what, rows=True)
+    st = fn(q_out.data_ptr(), l0, h0, k_out.data_ptr(), l1, h1, q.data_ptr(), l2, h2, k.data_ptr(), l3, h3, ty, q_norm.data_ptr(),
+            k_norm.data_ptr(), pos.data_ptr(), tokens, heads, kvh, d, rope_dim, float(theta), float(eps), _st(stream))
+    if st:
+        _check(st, "qh_qk_norm_rope_seq")
+
+
+def _cache_operands(name: str, kq, ks, vq, vs, k, v, slot):
+    """The operands of a call over rows of the cache, checked: (type, the C call's strided cache operands, k's and
+    v's, and its slots and sizes)."""
+    nk, nc = _dims(k, 3, "k"), _dims(kq, 3, "kq")
+    (tokens, kvh, d), rows = nk, nc[0]
+    T, dev, dt, ty = _Short.tensor, _here(k), k.dtype, _type(k, "k")
+    if tokens > _INT_MAX or kvh > _INT_MAX or d > _INT_MAX:
+        _sizes(name, tokens, kvh, d)
+    if not (kq.__class__ is T and ks.__class__ is T and vq.__class__ is T and vs.__class__ is T and v.__class__ is T
+            and slot.__class__ is T
+            and kq.dtype is _Short.i8 and vq.dtype is _Short.i8 and ks.dtype is _Short.f32 and vs.dtype is _Short.f32
+            and v.dtype is dt and slot.dtype is _Short.i64
+            and nc == (rows, kvh, d) and vq.shape == nc and ks.shape == (rows, kvh) and vs.shape == (rows, kvh) and v.shape == nk
+            and slot.shape == (tokens,) and slot.is_contiguous()
+            and dev == kq.get_device() == ks.get_device() == vq.get_device() == vs.get_device() == v.get_device()
+            == slot.get_device()):
+        _operand(k, dt, nk, "k", rows=True)
+        _operand(v, dt, nk, "v", rows=True)
+        _operand(kq, _Short.i8, (rows, kvh, d), "kq", rows=True)
+        _operand(vq, _Short.i8, (rows, kvh, d), "vq", rows=True)
+        for t, what in ((ks, "ks"), (vs, "vs")):
+            _operand(t, _Short.f32, (rows, kvh), what, free=True)
+        _operand(slot, _Short.i64, (tokens,), "slot")
+    (l0, h0, e0), (l1, h1), (l2, h2, e2), (l3, h3), (l4, h4, e4), (l5, h5, e5) = (
+        kq.stride(), ks.stride(), vq.stride(), vs.stride(), k.stride(), v.stride())
+    if not e0 == e2 == e4 == e5 == 1:
+        for t, what in ((kq, "kq"), (vq, "vq"), (k, "k"), (v, "v")):
+            _operand(t, t.dtype, t.shape, what, rows=True)
+    return (ty, (kq.data_ptr(), l0, h0, ks.data_ptr(), l1, h1, vq.data_ptr(), l2, h2, vs.data_ptr(), l3, h3),
+            (k.data_ptr(), l4, h4, v.data_ptr(), l5, h5), (slot.data_ptr(), rows, tokens, kvh, d))
+
+
+def kv_cache_write_i8(kq, ks, vq, vs, k, v, slot, stream=None):
+    """Keys and values quantised into rows of the cache: token t of k, v [tokens, kv_heads, dim] (float32 or bfloat16,
+    any row and head strides) goes to row slot[t] (int64 on the device; one outside the cache, such as -1, is skipped).
+    quant_rows of each head's row, bit for bit: scale = largest magnitude / 127, and NaN where the row is not finite.
+    Two tokens may not name the same row."""
+    ty, cache, new, where = _cache_operands("qh_kv_cache_write_i8", kq, ks, vq, vs, k, v, slot)
+    st = _op("qh_kv_cache_write_i8")(*cache, *new, ty, *where, _st(stream))
+    if st:
+        _check(st, "qh_kv_cache_write_i8")
+
+
+def kv_cache_read_i8(k, v, kq, ks, vq, vs, slot, stream=None):
+    """Rows of the cache as the values that they stand for: k, v [tokens, kv_heads, dim] (float32 or bfloat16), token t
+    from row slot[t] (int64 on the device; one outside the cache leaves the token's rows of k and v as they were)."""
+    ty, cache, new, where = _cache_operands("qh_kv_cache_read_i8", kq, ks, vq, vs, k, v, slot)
+    st = _op("qh_kv_cache_read_i8")(*new, ty, *cache, *where, _st(stream))
+    if st:
+        _check(st, "qh_kv_cache_read_i8")
+
+
+def attention_seq_i8_workspace(q_rows: int, n_seq: int, max_q: int, max_k: int, heads: int, kv_heads: int, head_dim: int,
+                               dtype: Optional[int] = None) -> int:
+    """Bytes of device scratch attention_seq_i8 takes from its caller (dtype F32 or BF16; None: enough for both)."""
+    f = _lib().qh_attention_seq_i8_workspace
+    f.restype = ctypes.c_size_t
+    n = (int(q_rows), int(n_seq), int(max_q), int(max_k), int(heads), int(kv_heads), int(head_dim))
+    _sizes("qh_attention_seq_i8_workspace", *n)
+    return max(int(f(*n, t)) for t in ((F32, BF16) if dtype is None else (int(dtype),)))
+
+
+def attention_seq_i8(out, q, kq, ks, vq, vs, cu_q, k_start, k_len, workspace, max_q: int, max_k: int,
+                     scale: Optional[float] = None, stream=None):
+    """attention_seq over an int8 cache (kv_cache_write_i8's): q, out [q_rows, heads, dim] (float32 or bfloat16, any row
+    and head strides), kq, vq int8 [k_rows, kv_heads, dim], ks, vs float32 [k_rows, kv_heads]; sequences, key ranges,
+    bounds and workspace (attention_seq_i8_workspace(...) bytes) as there.  A row that sees a scale that is not finite
+    gives NaN.  A query row takes part as whole numbers, off by 2^-16 of its largest element at most (bfloat16) or 2^-24
+    (float32)."""
+    fn = _op("qh_attention_seq_i8")
+    nq, nk, n = _dims(q, 3, "q"), _dims(kq, 3, "kq"), _dims(k_len, 1, "k_len")[0]
+    (rows, heads, d), (krows, kvh, _) = nq, nk
+    T, dev, dt, ty = _Short.tensor, _here(q), q.dtype, _type(q, "q")
+    max_q, max_k = int(max_q), int(max_k)
+    if rows > _INT_MAX or n >= _INT_MAX or not 0 <= max_q <= _INT_MAX or not 0 <= max_k <= _INT_MAX or heads > _INT_MAX or kvh > _INT_MAX:
+        _sizes("qh_attention_seq_i8", rows, n + 1, heads, kvh, max_q, max_k)
+    if not (out.__class__ is T and kq.__class__ is T and ks.__class__ is T and vq.__class__ is T and vs.__class__ is T
+            and cu_q.__class__ is T and k_start.__class__ is T and k_len.__class__ is T
+            and out.dtype is dt and kq.dtype is _Short.i8 and vq.dtype is _Short.i8 and ks.dtype is _Short.f32
+            and vs.dtype is _Short.f32 and cu_q.dtype is _Short.i32 and k_start.dtype is _Short.i64 and k_len.dtype is _Short.i32
+            and out.shape == nq and nk[2] == d and vq.shape == nk and ks.shape == (krows, kvh) and vs.shape == (krows, kvh)
+            and cu_q.shape == (n + 1,) and k_start.shape == (n,)
+            and cu_q.is_contiguous() and k_start.is_contiguous() and k_len.is_contiguous()
+            and dev == out.get_device() == kq.get_device() == ks.get_device() == vq.get_device() == vs.get_device()
+            == cu_q.get_device() == k_start.get_device() == k_len.get_device()):
+        for t, t_dt, shape, what in ((out, dt, nq, "out"), (q, dt, nq, "q"), (kq, _Short.i8, (krows, kvh, d), "kq"),
+                                     (vq, _Short.i8, (krows, kvh, d), "vq")):
+            _operand(t, t_dt, shape, what, rows=True)
+        for t, what in ((ks, "ks"), (vs, "vs")):
+            _operand(t, _Short.f32, (krows, kvh), what, free=True)
+        _operand(cu_q, _Short.i32, (n + 1,), "cu_q")
+        _operand(k_start, _Short.i64, (n,), "k_start")
+        _operand(k_len, _Short.i32, (n,), "k_len")
+    (lo, ho, o1), (lq, hq, q1), (lk, hk, k1), (lv, hv, v1) = out.stride(), q.stride(), kq.stride(), vq.stride()
+    if not o1 == q1 == k1 == v1 == 1:
+        for t, what in ((out, "out"), (q, "q"), (kq, "kq"), (vq, "vq")):
+            _operand(t, t.dtype, t.shape, what, rows=True)
+    st = fn(out.data_ptr(), lo, ho, q.data_ptr(), lq, hq, ty, kq.data_ptr(), lk, hk, ks.data_ptr(), *ks.stride(), vq.data_ptr(), lv, hv,
+            vs.data_ptr(), *vs.stride(), cu_q.data_ptr(), k_start.data_ptr(), k_len.data_ptr(), n, rows, krows, max_q, max_k, heads,
+            kvh, d, float(d ** -0.5 if scale is None else scale), *_ws(workspace), _st(stream))
+    if st:
+        _check(st, "qh_attention_seq_i8")
 
 
 # ---------------------------------------------------------------- layout / synthetic weights

@@ -51,6 +51,16 @@ QH_SEQ_FN int tiles_past(int q_len, int k_len, int G, int tile, int nt, int64_t 
   return tok <= 0 ? nt : nt - (int)(tok * G / tile);
 }
 
+// Whether a token has a place in a cache of `rows` rows; one that has none is skipped.
+QH_SEQ_FN bool has_slot(int64_t slot, int64_t rows) { return slot >= 0 && slot < rows; }
+
+// The scale of a row of int8 codes whose largest magnitude is `top`: top / 127, 1 for a row of zeros, and at least the
+// smallest number, so that no value is divided by 0.
+QH_SEQ_FN float code_scale(float top) {
+  const float s = top / 127.0f;
+  return !(top > 0.0f) ? 1.0f : s > 0.0f ? s : 0x1p-149f;
+}
+
 // A float as the sum of three bfloat16, eight bits of it each: the upper halves of p[0], p[1], p[2].
 struct Cut {
   uint32_t p[3];
@@ -143,6 +153,46 @@ struct AttnSeq {
   int limit = 0;                  // places in the workspace (few rows: 1: the keys may be split)
 };
 
+// Norms of queries and keys for each head, with the position rotation.
+struct NormRope {
+  SeqOut qo, ko;                  // [tokens][heads][dim], [tokens][kv_heads][dim]
+  SeqIn q, k;                     // of the same type; q (k) may be qo (ko) itself
+  const float* qw = nullptr;      // [dim]
+  const float* kw = nullptr;
+  const int32_t* pos = nullptr;   // [tokens]
+  int tokens = 0, heads = 0, kv_heads = 0, dim = 0, rot = 0;
+  float eps = 0.0f;
+  int bf16 = 0;
+  double turns[128];              // of the angle i of a pair for each position: theta^(-2 i / rot) / (2 pi)
+};
+
+// A cache of int8 rows: codes [rows][heads][dim], a scale for each row and head.
+struct CacheSide {
+  int8_t* q = nullptr;            // codes, element (r, h, d) at q + r * ld + h * hs + d
+  int64_t ld = 0, hs = 0;
+  float* s = nullptr;             // scales, (r, h) at s + r * lds + h * hss
+  int64_t lds = 0, hss = 0;
+};
+struct CacheSeq {
+  CacheSide c[2];                 // keys, values
+  const void* x[2] = {};          // new keys and values, or where the read ones go (written then): [tokens][heads][dim]
+  int64_t ld[2] = {}, hs[2] = {};
+  const int64_t* slot = nullptr;  // [tokens]
+  int64_t rows = 0;
+  int tokens = 0, heads = 0, dim = 0;
+  int bf16 = 0;
+};
+
+// Attention over such a cache: k and v of AttnSeq are the codes.
+struct AttnI8 : AttnSeq {
+  const float *ks = nullptr, *vs = nullptr;   // scales, (r, h) at ks + r * ldks + h * hsks
+  int64_t ldks = 0, hsks = 0, ldvs = 0, hsvs = 0;
+};
+
+hipError_t launch_attn_i8(const AttnI8& a, hipStream_t s);
+hipError_t launch_norm_rope(const NormRope& a, hipStream_t s);
+hipError_t launch_cache_write(const CacheSeq& a, hipStream_t s);
+hipError_t launch_cache_read(const CacheSeq& a, hipStream_t s);
 hipError_t launch_gemm_seq(const GemmSeq& a, hipStream_t s);
 hipError_t launch_delta_seq(const DeltaSeq& a, hipStream_t s);
 hipError_t launch_attn_seq(const AttnSeq& a, hipStream_t s);
@@ -159,6 +209,7 @@ struct AttnForm {
   int tile, limit;
   size_t bytes;
 };
+AttnForm attn_i8_form(int64_t q_rows, int n_seq, int max_q, int max_k, int heads, int kv_heads, int dim, bool bf16);
 AttnForm attn_seq_form(int64_t q_rows, int n_seq, int max_q, int max_k, int heads, int kv_heads, int dim, bool bf16);
 
 }  // namespace qh

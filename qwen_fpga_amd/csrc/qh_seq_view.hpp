@@ -29,15 +29,24 @@ struct View {
     auto span = [&](int64_t n, int64_t stride) { return n <= 1 || (__int128)(n - 1) * stride * eb <= kMaxSpan; };
     return span(rows, ld) && span(heads, hs) && span(2, dim);
   }
-  // and no two elements in one place
-  bool writable() const {
-    if (!readable()) return false;
+  // rows and heads any distance apart
+  bool strided() const {
+    return p && at() % eb == 0 && (rows <= 1 || (ld >= 0 && ld < kMaxStride)) && (heads <= 1 || (hs >= 0 && hs < kMaxStride));
+  }
+  // no two elements in one place
+  bool writable() const { return readable() && distinct(); }
+  bool distinct() const {
     if (rows > 1 && heads > 1)
       return hs >= dim && ld >= dim && ((__int128)(heads - 1) * hs <= ld - dim || (__int128)(rows - 1) * ld <= hs - dim);
     return (rows <= 1 || ld >= dim) && (heads <= 1 || hs >= dim);
   }
 };
 
+// One and the same operand.
+inline bool same(const View& a, const View& b) {
+  return a.p == b.p && a.rows == b.rows && a.heads == b.heads && a.dim == b.dim && a.eb == b.eb && (a.rows <= 1 || a.ld == b.ld) &&
+         (a.heads <= 1 || a.hs == b.hs);
+}
 inline View flat(const void* p, int64_t n, int eb) { return {p, 1, 1, n, 0, 0, eb}; }
 
 // Whether two operands (countable ones) share memory, as far as their spans and strides tell: they share none if the spans do

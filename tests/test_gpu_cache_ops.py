@@ -1,0 +1,820 @@
+"""Operators around an int8 K/V cache on the device, against plain 64-bit implementations.
+
+Tolerances.  u = 2^-24 is half a step of fp32, 2^-8 of bfloat16 (finfo.eps / 2).
+  qk_norm_rope_seq   a sum of up to 256 squares, 8 in a lane and then pairs: 13 roundings at most, so 13 u of it, 6.5 u of
+                     its root; the mean, eps, root and reciprocal 4 u, the two products and 1 + w 3 u: 14 u of a normalised element,
+                     taken as 16.  A rotated one is x cos - y sin: the angle in turns, at most half a one, is rounded to
+                     fp32 once (2^-25 of a turn, 3.2 u of a radian), sine and cosine are off by up to 2 u more, products and
+                     the sum by 2 u: (16 + 8) u (|x| + |y|).  bfloat16: rounded once more.
+  kv_cache_*         the quotient and the scale are IEEE divisions and everything else is exact: equal bits.
+  attention_seq_i8   an element of q is off by half a unit, 1 / 2 of its row's largest over 32639 (bfloat16) or 8355711 (fp32),
+                     a score so by that times |scale| sum |k|; the sum itself is exact, its conversions and the products with the
+                     row's unit (itself three roundings) and K's scale take 10 u of the score.  The largest of
+                     a row's errors counts twice, in the numerator and in the sum.  exp2 and its argument, sums over n keys
+                     and their joins (16 + sqrt(n)) u, V's scale u, of sum p |v|; bfloat16: P in two parts, 2^-16 of it, and the output rounded once
+                     more.  A part of P below 2^-126, the smallest normal number, may count as 0 in the matrix instruction: each of
+                     at most three parts of n keys then takes up to 2^-126 times a code of 128 from a sum that is divided by
+                     at least 1 (the largest probability's term): n 3 2^-119 in all, whatever the output's size.
+"""
+import functools
+import math
+import sys
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+BF = 2.0 ** -8
+
+
+def gen(torch, seed):
+    g = torch.Generator()
+    g.manual_seed(seed)
+    return g
+
+
+def starts(lens):
+    return [0] + np.cumsum(lens).tolist()
+
+
+# ------------------------------------------------------------------ norms and rotation
+
+def rope_oracle(torch, x, w, pos, rot, theta=1e7, eps=1e-6):
+    """float64 on the CPU: (out, bound)."""
+    x = x.double()
+    y = x / torch.sqrt(x.square().mean(-1, keepdim=True) + eps) * (1.0 + w.double())
+    half, out, tol = rot // 2, y.clone(), 16 * U * y.abs()
+    if half:
+        ang = pos.double()[:, None] * torch.tensor([theta ** (-2.0 * i / rot) for i in range(half)], dtype=torch.float64)
+        c, s = torch.cos(ang)[:, None], torch.sin(ang)[:, None]
+        a, b = y[..., :half], y[..., half:rot]
+        out[..., :half], out[..., half:rot] = a * c - b * s, b * c + a * s
+        both = 24 * U * (a.abs() + b.abs())
+        tol[..., :half], tol[..., half:rot] = both, both
+    return out, tol
+
+
+def rope_check(torch, got, want, bf16):
+    wo, tol = want
+    err = (got.cpu().double() - wo).abs()
+    lim = tol + (BF * (wo.abs() + tol) if bf16 else U * wo.abs())
+    assert (err <= lim).all(), (err.max().item(), (err / lim.clamp(min=1e-30)).max().item())
+
+
+ROPE = [  # tokens, heads, kv heads, dim, rotated
+    (1, 8, 2, 256, 64), (1, 1, 1, 128, 128), (2, 3, 1, 256, 256), (5, 6, 2, 128, 32), (7, 16, 4, 128, 16), (33, 8, 2, 256, 0),
+    (64, 32, 1, 256, 64), (65, 2, 2, 128, 64), (300, 8, 8, 128, 96), (1000, 8, 2, 256, 48), (3, 1, 40, 256, 240),
+]
+
+
+@pytest.mark.parametrize("tokens,h,kvh,d,rot", ROPE)
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+def test_norm_rope(q, torch_cuda, tokens, h, kvh, d, rot, bf16):
+    torch = torch_cuda
+    g, dt = gen(torch, tokens + h + rot), torch.bfloat16 if bf16 else torch.float32
+    qk = (torch.randn(tokens, h, 2 * d, generator=g) * 3).to(dt)      # query and gate halves
+    kk = (torch.randn(tokens, kvh, d, generator=g) * 0.2).to(dt)
+    qw, kw = torch.randn(d, generator=g) * 0.3, torch.randn(d, generator=g) * 0.3
+    pos = torch.randint(0, 131072, (tokens,), generator=g, dtype=torch.int32)
+    pos[0] = 0 if tokens > 1 else 131071
+    wide = torch.full((tokens + 1, (h + kvh) * d + 16), 7.0, dtype=dt, device="cuda")
+    qo, ko = wide[:tokens, :h * d].view(tokens, h, d), wide[:tokens, h * d:(h + kvh) * d].view(tokens, kvh, d)
+    dev = [qk.cuda()[:, :, :d], kk.cuda(), qw.cuda(), kw.cuda(), pos.cuda()]
+    q.qk_norm_rope_seq(qo, ko, *dev, rot)
+    rope_check(torch, qo, rope_oracle(torch, qk[:, :, :d], qw, pos, rot), bf16)
+    rope_check(torch, ko, rope_oracle(torch, kk, kw, pos, rot), bf16)
+    assert (wide[tokens:] == 7).all() and (wide[:, (h + kvh) * d:] == 7).all()
+    # head-major, and in place: the same bits
+    q2, k2 = dev[0].transpose(0, 1).contiguous().transpose(0, 1), kk.cuda()
+    q.qk_norm_rope_seq(q2, k2, q2, k2, *dev[2:], rot)
+    assert torch.equal(q2, qo) and torch.equal(k2, ko)
+
+
+def test_norm_rope_is_the_one_token_ops(q, torch_cuda):
+    """rmsnorm, rope_cos_sin and apply_rope of each head, near enough: their angles are rounded to fp32, so positions are small."""
+    torch = torch_cuda
+    g, d = gen(torch, 1), 256
+    x, kk, w = torch.randn(4, 2, d, generator=g).cuda(), torch.randn(4, 1, d, generator=g).cuda(), torch.randn(d, generator=g).cuda()
+    pos = torch.tensor([0, 1, 7, 40], dtype=torch.int32)
+    qo, ko = torch.empty_like(x), torch.empty_like(kk)
+    q.qk_norm_rope_seq(qo, ko, x, kk, w, w, pos.cuda())
+    c, s, y = torch.empty(64, device="cuda"), torch.empty(64, device="cuda"), torch.empty(d, device="cuda")
+    for t in range(4):
+        q.rope_cos_sin(int(pos[t]), c, s)
+        for got, src in ((qo[t, 0], x[t, 0]), (qo[t, 1], x[t, 1]), (ko[t, 0], kk[t, 0])):
+            q.rmsnorm(y, src.contiguous(), w, d)
+            q.apply_rope(y, c, s)
+            # 24 u (|x| + |y|) on either side, and the angle's rounding: 2 u of 40
+            assert (got - y).abs().max().item() <= (48 + 80) * U * 2 * y.abs().max().item()
+
+
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+def test_norm_rope_far_positions_and_bases(q, torch_cuda, bf16):
+    torch = torch_cuda
+    g, d, dt = gen(torch, 2), 128, torch.bfloat16 if bf16 else torch.float32
+    pos = torch.tensor([0, 1, -1, 2 ** 31 - 1, -2 ** 31, 1 << 20, 131071, 99999999], dtype=torch.int32)
+    x, kk = torch.randn(8, 2, d, generator=g).to(dt), torch.randn(8, 1, d, generator=g).to(dt)
+    w = torch.zeros(d)
+    for theta, rot, eps in ((1e7, 128, 1e-6), (1e4, 64, 1e-5), (2.0, 16, 0.0), (1.0, 32, 1.0), (5e8, 64, 1e-6)):
+        qo, ko = torch.empty_like(x, device="cuda"), torch.empty_like(kk, device="cuda")
+        q.qk_norm_rope_seq(qo, ko, x.cuda(), kk.cuda(), w.cuda(), w.cuda(), pos.cuda(), rot, theta, eps)
+        # positions of 2^31 turn 2^31 / (2 pi) times at most: what 64 bits leave of that, 2^-53 2^29 of a turn, four times over
+        far = 4 * 2.0 ** -24 * 2 * math.pi * 2
+        for got, src in ((qo, x), (ko, kk)):
+            wo, tol = rope_oracle(torch, src, w, pos, rot, theta, eps)
+            rope_check(torch, got, (wo, tol + far * src.double().abs().amax(-1, keepdim=True) / torch.sqrt(src.double().square().mean(-1, keepdim=True) + eps)), bf16)
+
+
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+def test_norm_rope_rows_on_their_own(q, torch_cuda, bf16):
+    """A row of zeros stays one, a row with a NaN or an infinity is its own affair."""
+    torch = torch_cuda
+    g, dt = gen(torch, 3), torch.bfloat16 if bf16 else torch.float32
+    x, kk = torch.randn(6, 3, 256, generator=g).to(dt).cuda(), torch.randn(6, 2, 256, generator=g).to(dt).cuda()
+    w, pos = torch.randn(256, generator=g).cuda(), torch.arange(6, dtype=torch.int32, device="cuda")
+    run = lambda: (lambda a, b: (q.qk_norm_rope_seq(a, b, x, kk, w, w, pos), a, b)[1:])(torch.empty_like(x), torch.empty_like(kk))
+    a0, b0 = run()
+    x[1, 0] = 0
+    x[2, 1, 5], kk[3, 1, 200] = math.nan, math.inf
+    a, b = run()
+    assert (a[1, 0] == 0).all() and torch.isnan(a[2, 1]).all() and torch.isnan(b[3, 1, 200])
+    a[1, 0], a[2, 1], b[3, 1] = a0[1, 0], a0[2, 1], b0[3, 1]
+    assert torch.equal(a, a0) and torch.equal(b, b0)
+
+
+# ------------------------------------------------------------------ the cache
+
+def code_oracle(torch, x):
+    """(codes, scales) of rows, by fp32 divisions on the CPU, as quant_rows defines them."""
+    x = x.float()
+    top = x.abs().amax(-1)
+    s = torch.where(top > 0, top / 127.0, 1.0)
+    s = torch.where((top > 0) & (s == 0), torch.tensor(2.0 ** -149), s)
+    ok = torch.isfinite(x).all(-1)
+    c = torch.where(ok[..., None], torch.clamp(torch.round(x / s[..., None]), -127, 127), 0.0).to(torch.int8)
+    return c, torch.where(ok, s, math.nan)
+
+
+def same(torch, a, b):
+    return bool(((a == b) | (a.isnan() & b.isnan())).all())
+
+
+def cache_new(torch, rows, kvh, d, layout):
+    """(kq, ks, vq, vs) filled with what no call writes."""
+    i8 = dict(dtype=torch.int8, device="cuda")
+    if layout == "rows":
+        kq, vq = torch.full((rows, kvh, d), -128, **i8), torch.full((rows, kvh, d), -128, **i8)
+        ks, vs = torch.full((rows, kvh), -5.0, device="cuda"), torch.full((rows, kvh), -5.0, device="cuda")
+    elif layout == "heads":          # head-major, scales as well
+        kq, vq = (torch.full((kvh, rows, d), -128, **i8).transpose(0, 1) for _ in range(2))
+        ks, vs = (torch.full((kvh, rows), -5.0, device="cuda").t() for _ in range(2))
+    else:                            # keys and values of a row side by side, scales in odd places
+        both = torch.full((rows, 2, kvh, d + 16), -128, **i8)
+        kq, vq = both[:, 0, :, :d], both[:, 1, :, :d]
+        sc = torch.full((rows, 2 * kvh + 3), -5.0, device="cuda")
+        ks, vs = sc[:, 1:1 + kvh], sc[:, 2 + kvh:2 + 2 * kvh]
+    return kq, ks, vq, vs
+
+
+CACHE = [  # tokens, rows, kv heads, dim
+    (1, 1, 1, 128), (1, 40, 2, 256), (3, 9, 1, 256), (15, 16, 3, 128), (16, 33, 8, 128), (17, 1000, 2, 256), (129, 200, 5, 128),
+    (700, 900, 2, 256), (5, 4000, 40, 256),
+]
+
+
+@pytest.mark.parametrize("tokens,rows,kvh,d", CACHE)
+@pytest.mark.parametrize("layout", ["rows", "heads", "side"])
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+def test_cache_write_and_read(q, torch_cuda, tokens, rows, kvh, d, layout, bf16):
+    torch = torch_cuda
+    g, dt = gen(torch, tokens * 3 + rows + kvh), torch.bfloat16 if bf16 else torch.float32
+    row = (torch.randn(tokens, 2 * kvh * d + 32, generator=g) * torch.exp(torch.randn(tokens, 1, generator=g) * 4)).to(dt)
+    kv = [row[:, a:a + kvh * d].view(tokens, kvh, d) for a in (0, kvh * d + 16)]
+    dev = [row.cuda()[:, a:a + kvh * d].view(tokens, kvh, d) for a in (0, kvh * d + 16)]
+    slot = torch.randperm(rows, generator=g)[:tokens].to(torch.int64)
+    for i, s in ((1, -1), (4, rows), (6, 2 ** 63 - 1), (8, -2 ** 63), (10, rows + 7)):     # no places of the cache
+        if i < tokens:
+            slot[i] = s
+    there = (slot >= 0) & (slot < rows)
+    c = cache_new(torch, rows, kvh, d, layout)
+    q.kv_cache_write_i8(*c, *dev, slot.cuda())
+    out = [torch.full((tokens + 1, kvh, d + 16), 7.0, dtype=dt, device="cuda") for _ in range(2)]
+    o = [x[:tokens, :, :d] for x in out]
+    q.kv_cache_read_i8(*o, *c, slot.cuda())
+    for x, cq, cs, got, full in zip(kv, c[::2], c[1::2], o, out):
+        codes, sc = code_oracle(torch, x)
+        wq, wsc = torch.full((rows, kvh, d), -128, dtype=torch.int8), torch.full((rows, kvh), -5.0)
+        wq[slot[there]], wsc[slot[there]] = codes[there], sc[there]
+        assert torch.equal(cq.cpu(), wq) and torch.equal(cs.cpu(), wsc)
+        want = (codes.float() * sc[..., None]).to(dt)
+        want[~there] = 7.0
+        assert torch.equal(got.cpu(), want) and (full[tokens:] == 7).all() and (full[:, :, d:] == 7).all()
+        # the same codes as the packer's operator gives
+        if layout == "rows" and not bf16:
+            pq, ps = torch.empty(tokens * kvh, d, dtype=torch.int8, device="cuda"), torch.empty(tokens * kvh, device="cuda")
+            q.quant_rows(pq, ps, x.reshape(-1, d).contiguous().cuda(), tokens * kvh, d)
+            assert torch.equal(pq.cpu().view(tokens, kvh, d), codes) and torch.equal(ps.cpu().view(tokens, kvh), sc)
+
+
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+@pytest.mark.parametrize("d", [128, 256])
+def test_cache_odd_rows(q, torch_cuda, bf16, d):
+    """Zeros, halves between two codes, the smallest and the largest numbers, what is not finite."""
+    torch = torch_cuda
+    dt = torch.bfloat16 if bf16 else torch.float32
+    g = gen(torch, d)
+    x = torch.randn(14, 2, d, generator=g)
+    x[0] = 0.0
+    x[1] = torch.arange(d) - 126.5
+    x[1, :, 0] = 127.0                               # scale 1: ties go to the even code
+    x[2] = torch.sign(x[2]) * 2.0 ** -149
+    x[3] *= 2.0 ** -140
+    x[4] *= 2.0 ** -127
+    x[5] *= 1e-36
+    x[6] = torch.sign(x[6]) * 3.3895314e38           # the largest bfloat16
+    x[7] *= 1e30
+    x[8, 0, 3], x[9, 1, d - 1], x[10, 0, 64] = math.nan, math.inf, -math.inf
+    x[11] = -0.0
+    x[12, :, 1:] = 0.0
+    x[13] = 5.0
+    x = x.to(dt)
+    c = cache_new(torch, 14, 2, d, "rows")
+    slot = torch.arange(14).cuda()
+    q.kv_cache_write_i8(*c, x.cuda(), x.flip(0).cuda(), slot)
+    for src, cq, cs in ((x, c[0], c[1]), (x.flip(0), c[2], c[3])):
+        codes, sc = code_oracle(torch, src)
+        assert torch.equal(cq.cpu(), codes) and same(torch, cs.cpu(), sc)
+    o = [torch.empty(14, 2, d, dtype=dt, device="cuda") for _ in range(2)]
+    q.kv_cache_read_i8(*o, *c, slot)
+    codes, sc = code_oracle(torch, x)
+    assert same(torch, o[0].cpu(), (codes.float() * sc[..., None]).to(dt))
+
+
+def test_cache_read_any_codes_many_times(q, torch_cuda):
+    """All codes, -128 among them, and one row named by every token."""
+    torch = torch_cuda
+    g = gen(torch, 4)
+    kq, vq = (torch.randint(-128, 128, (50, 2, 128), generator=g, dtype=torch.int8) for _ in range(2))
+    ks, vs = torch.randn(50, 2, generator=g), torch.rand(50, 2, generator=g)
+    slot = torch.randint(0, 50, (400,), generator=g)
+    slot[:100] = 17
+    for dt in (torch.float32, torch.bfloat16):
+        o = [torch.empty(400, 2, 128, dtype=dt, device="cuda") for _ in range(2)]
+        q.kv_cache_read_i8(*o, kq.cuda(), ks.cuda(), vq.cuda(), vs.cuda(), slot.cuda())
+        assert torch.equal(o[0].cpu(), (kq[slot].float() * ks[slot][..., None]).to(dt))
+        assert torch.equal(o[1].cpu(), (vq[slot].float() * vs[slot][..., None]).to(dt))
+
+
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+def test_cache_rows_far_apart(q, torch_cuda, bf16):
+    """Rows of the cache 16 MB apart, the last behind 2^32 bytes, and a token's rows far from the next."""
+    torch = torch_cuda
+    g, dt, rows, ld = gen(torch, 6), torch.bfloat16 if bf16 else torch.float32, 300, 1 << 24
+    far = torch.zeros((rows - 1) * ld + 512, dtype=torch.int8, device="cuda").as_strided((rows, 2, 256), (ld, 256, 1))
+    vq = torch.zeros(rows, 2, 256, dtype=torch.int8, device="cuda")
+    ks, vs = torch.zeros(rows, 2, device="cuda"), torch.zeros((rows - 1) * (1 << 22) + 2, device="cuda").as_strided((rows, 2), (1 << 22, 1))
+    x = torch.randn(40, 2, 256, generator=g).to(dt)
+    xf = torch.empty(39 * (1 << 26) + 512, dtype=dt, device="cuda").as_strided((40, 2, 256), (1 << 26, 256, 1))
+    xf.copy_(x)
+    slot = torch.randperm(rows, generator=g)[:40]
+    slot[0] = rows - 1
+    q.kv_cache_write_i8(far, ks, vq, vs, xf, xf, slot.cuda())
+    codes, sc = code_oracle(torch, x)
+    for cq, cs in ((far, ks), (vq, vs)):
+        assert torch.equal(cq[slot.cuda()].cpu(), codes) and torch.equal(cs[slot.cuda()].cpu(), sc)
+    o = torch.empty(40, 2, 256, dtype=dt, device="cuda")
+    xf.zero_()
+    q.kv_cache_read_i8(o, xf, far, ks, vq, vs, slot.cuda())
+    want = (codes.float() * sc[..., None]).to(dt)
+    assert torch.equal(o.cpu(), want) and torch.equal(xf.contiguous().cpu(), want)
+
+
+# ------------------------------------------------------------------ attention over the cache
+
+TOP = {False: 8355711.0, True: 32639.0}      # a query row's largest element, in units
+
+
+def attn_oracle(torch, qq, kq, ks, vq, vs, lens, ctx, at_k, scale, bf16):
+    """float64 on the CPU: (out, the bound without the output's rounding)."""
+    h, kvh = qq.shape[1], kq.shape[1]
+    out, tol, at = torch.zeros(qq.shape, dtype=torch.float64), torch.zeros(qq.shape, dtype=torch.float64), 0
+    for n, m, k0 in zip(lens, ctx, at_k):
+        for hh in range(h if n and m else 0):
+            c = hh // (h // kvh)
+            a = qq[at:at + n, hh].double()
+            b, v = (x[k0:k0 + m, c].double() * s[k0:k0 + m, c, None].double() for x, s in ((kq, ks), (vq, vs)))
+            s = a @ b.t() * scale
+            es = abs(scale) * a.abs().amax(-1, keepdim=True) / (2 * TOP[bf16]) * b.abs().sum(-1)[None, :] + 10 * U * s.abs()
+            hide = torch.arange(m)[None, :] > torch.arange(n)[:, None] + (m - n)
+            es = es.masked_fill(hide, 0.0).amax(-1, keepdim=True)
+            none = hide.all(-1, keepdim=True)
+            p = torch.softmax(s.masked_fill(hide, -math.inf).masked_fill(none, 0.0), -1).masked_fill(none, 0.0)
+            out[at:at + n, hh] = p @ v
+            tol[at:at + n, hh] = (2 * es + (17 + math.sqrt(m)) * U + (2.0 ** -16 if bf16 else 0.0)) * (p @ v.abs()) + 3 * m * 2.0 ** -119
+        at += n
+    return out, tol
+
+
+def attn_inputs(torch, seed, lens, ctx, h, kvh, d, bf16, gap=0, qscale=2.0):
+    """(q, kq, ks, vq, vs) and where each sequence's keys begin."""
+    g = gen(torch, seed)
+    at_k, rows = [], 0
+    for m in ctx:
+        rows += gap
+        at_k.append(rows)
+        rows += m
+    rows += gap
+    qq = (torch.randn(sum(lens), h, d, generator=g) * qscale).to(torch.bfloat16 if bf16 else torch.float32)
+    sides = []
+    for _ in range(2):
+        x = torch.randn(rows, kvh, d, generator=g) * torch.exp(torch.randn(rows, kvh, 1, generator=g) * 0.3)
+        sides += code_oracle(torch, x) if rows else (torch.zeros(0, kvh, d, dtype=torch.int8), torch.zeros(0, kvh))
+    return (qq, *sides), at_k
+
+
+def attn_run(q, torch, dev, lens, ctx, at_k, scale=None, max_q=None, max_k=None, out=None):
+    qq, kq = dev[:2]
+    t, h, d = qq.shape
+    if out is None:
+        out = torch.full((t, h, d), 7.0, dtype=qq.dtype, device="cuda")
+    mq, mk = max(lens + [0]) if max_q is None else max_q, max(ctx + [0]) if max_k is None else max_k
+    nb = q.attention_seq_i8_workspace(t, len(lens), mq, mk, h, kq.shape[1], d, q.BF16 if qq.dtype is torch.bfloat16 else q.F32)
+    ws = torch.full((nb,), 0xFF, dtype=torch.uint8, device="cuda")          # NaN bits
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    q.attention_seq_i8(out, *dev, i32(starts(lens)), torch.tensor(at_k, dtype=torch.int64, device="cuda"), i32(ctx), ws, mq, mk, scale)
+    return out
+
+
+def attn_check(torch, got, want, bf16):
+    wo, tol = want
+    err = (got.cpu().double()[:wo.shape[0]] - wo).abs()
+    lim = tol + (BF * (wo.abs() + tol) if bf16 else U * wo.abs())
+    assert (err <= lim).all(), (err.max().item(), (err / lim.clamp(min=1e-30)).max().item())
+
+
+def both(torch, inp, at, lens, ctx, scale, bf16):
+    return [x.cuda() for x in inp], attn_oracle(torch, *inp, lens, ctx, at, scale, bf16)
+
+
+ATTN = [  # lens, keys, heads, kv heads, dim
+    ([1], [1], 1, 1, 128), ([1], [1], 8, 2, 256), ([1, 1, 1], [7, 300, 1], 8, 2, 256), ([1, 1], [2500, 15], 4, 4, 128),
+    ([1], [5000], 8, 2, 256), ([2, 3], [33, 64], 6, 2, 128), ([4], [1000], 16, 1, 128), ([1], [777], 32, 1, 256), ([1], [31], 2, 1, 128),
+    ([1], [32], 2, 1, 256), ([1], [129], 2, 1, 128), ([15, 16, 17], [15, 16, 17], 2, 1, 128), ([64], [64], 2, 2, 256),
+    ([63, 0, 65], [63, 5, 70], 4, 2, 128), ([127, 1], [127, 129], 8, 2, 256), ([129], [400], 2, 1, 256), ([200, 90], [200, 90], 3, 3, 128),
+    ([300], [300], 8, 2, 256), ([33], [2000], 2, 1, 128), ([260], [261], 1, 1, 256), ([520], [520], 4, 1, 128), ([5], [5], 3, 1, 256),
+]
+
+
+@pytest.mark.parametrize("lens,ctx,h,kvh,d", ATTN, ids=str)
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+def test_attention(q, torch_cuda, lens, ctx, h, kvh, d, bf16):
+    torch = torch_cuda
+    inp, at = attn_inputs(torch, sum(lens) + sum(ctx) + h, lens, ctx, h, kvh, d, bf16, gap=3)
+    dev, want = both(torch, inp, at, lens, ctx, 1 / math.sqrt(d), bf16)
+    t = sum(lens)
+    out = torch.full((t + 2, h, d), 7.0, dtype=dev[0].dtype, device="cuda")
+    dev[0] = torch.cat([dev[0], dev[0][:1], dev[0][:1]])            # two rows behind the last sequence
+    attn_check(torch, attn_run(q, torch, dev, lens, ctx, at, out=out), want, bf16)
+    assert (out[t:] == 7).all()
+
+
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+@pytest.mark.parametrize("d", [128, 256])
+def test_attention_rows_without_keys(q, torch_cuda, bf16, d):
+    """More rows than keys: the first rows see none and come out as 0; no key at all."""
+    torch = torch_cuda
+    for lens, ctx in (([70, 3], [9, 0]), ([200], [1]), ([5, 1], [2, 0]), ([2], [0])):
+        inp, at = attn_inputs(torch, 1, lens, ctx, 4, 2, d, bf16, gap=1)
+        dev, want = both(torch, inp, at, lens, ctx, 1 / math.sqrt(d), bf16)
+        got = attn_run(q, torch, dev, lens, ctx, at)
+        attn_check(torch, got, want, bf16)
+        assert (got[:lens[0] - ctx[0]] == 0).all()
+
+
+def test_attention_without_a_cache(q, torch_cuda):
+    torch = torch_cuda
+    inp, _ = attn_inputs(torch, 1, [3], [0], 2, 1, 128, False)
+    assert (attn_run(q, torch, [x.cuda() for x in inp], [3], [0], [0]) == 0).all()
+
+
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+@pytest.mark.parametrize("d", [128, 256])
+@pytest.mark.parametrize("n,m", [(1, 200), (5, 300), (100, 100), (150, 260), (90, 1200)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf, 3e38], ids=str)
+def test_attention_hidden_keys_have_no_influence(q, torch_cuda, bf16, d, n, m, bad):
+    """What stands behind a row's keys (the next tokens, rows of the cache not yet written, another sequence's) may be
+    anything; a scale that is not finite reaches the rows that see it, in the heads that share it."""
+    torch = torch_cuda
+    lens, ctx = [n, 2], [m, 2]
+    inp, at = attn_inputs(torch, 2, lens, ctx, 4, 2, d, bf16, gap=40)
+    clean = attn_run(q, torch, [x.cuda() for x in inp], lens, ctx, at)
+    for codes, sc in (inp[1:3], inp[3:5]):
+        for r in (slice(0, at[0]), slice(at[0] + m, at[1]), slice(at[1] + 2, None)):
+            codes[r], sc[r] = 127, bad
+    hit = at[0] + m - max(n // 3, 1)      # a key that the first rows do not see, and the last ones do
+    finite = math.isfinite(bad)
+    if n > 1 and not finite:
+        inp[2][hit, 0], inp[4][hit, 1] = bad, bad
+    got = attn_run(q, torch, [x.cuda() for x in inp], lens, ctx, at)
+    free = n if n == 1 or finite else n - max(n // 3, 1)
+    assert torch.equal(got[:free], clean[:free]) and torch.equal(got[n:], clean[n:])
+    if free < n:
+        assert torch.isnan(got[free:n, 2:]).all()            # V's scale
+        assert math.isinf(bad) or torch.isnan(got[free:n, :2]).all()   # K's
+
+
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+def test_attention_strides(q, torch_cuda, bf16):
+    """Queries inside a query and gate projection, a cache of slots with keys and values side by side, head-major ones,
+    an output inside wider rows, one row of queries for all (stride 0)."""
+    torch = torch_cuda
+    lens, ctx, h, kvh, d = [40, 1, 70], [40, 90, 71], 4, 2, 128
+    inp, _ = attn_inputs(torch, 5, lens, ctx, h, kvh, d, bf16)
+    src, at, t = starts(ctx), [240, 0, 120], sum(lens)
+    c = cache_new(torch, 360, kvh, d, "side")
+    hm = cache_new(torch, 360, kvh, d, "heads")
+    for i, m in enumerate(ctx):
+        for x, a, b in zip(inp[1:], c, hm):
+            a[at[i]:at[i] + m] = x[src[i]:src[i] + m].cuda()
+            b[at[i]:at[i] + m] = x[src[i]:src[i] + m].cuda()
+    want = attn_oracle(torch, inp[0], *[x.cpu() for x in c], lens, ctx, at, 1 / math.sqrt(d), bf16)
+    gate = torch.full((t, h, 2 * d), 9.0, dtype=inp[0].dtype, device="cuda")
+    gate[:, :, :d] = inp[0].cuda()
+    wide = torch.full((t, h * d + 64), 7.0, dtype=inp[0].dtype, device="cuda")
+    out = wide[:, 32:32 + h * d].view(t, h, d)
+    attn_run(q, torch, [gate[:, :, :d], *c], lens, ctx, at, out=out)
+    attn_check(torch, out, want, bf16)
+    assert (wide[:, :32] == 7).all() and (wide[:, 32 + h * d:] == 7).all()
+    o2 = torch.empty(h, t, d, dtype=inp[0].dtype, device="cuda").transpose(0, 1)
+    attn_run(q, torch, [inp[0].transpose(0, 1).contiguous().cuda().transpose(0, 1), *hm], lens, ctx, at, out=o2)
+    assert torch.equal(o2, out)
+    one = inp[0][:1].expand(t, h, d)
+    want = attn_oracle(torch, one, *[x.cpu() for x in c], lens, ctx, at, 1 / math.sqrt(d), bf16)
+    attn_check(torch, attn_run(q, torch, [inp[0][:1].cuda().expand(t, h, d), *c], lens, ctx, at), want, bf16)
+
+
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+def test_attention_bounds_too_small_or_large(q, torch_cuda, bf16):
+    """max_q and max_k choose the form: any value gives the same within tolerance."""
+    torch = torch_cuda
+    lens, ctx = [1, 90, 3], [900, 90, 500]
+    inp, at = attn_inputs(torch, 6, lens, ctx, 4, 2, 128, bf16)
+    dev, want = both(torch, inp, at, lens, ctx, 1 / math.sqrt(128), bf16)
+    for mq in (0, 1, 4, 90, 5000):
+        for mk in (0, 100, 900, 100000):
+            attn_check(torch, attn_run(q, torch, dev, lens, ctx, at, max_q=mq, max_k=mk), want, bf16)
+
+
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+def test_attention_large_scores(q, torch_cuda, bf16):
+    """Scores far apart (one key takes all), equal scores, a scale of 0 (the mean of the keys), a negative one."""
+    torch = torch_cuda
+    for scale in (4.0, 0.0, -0.3):
+        inp, at = attn_inputs(torch, 7, [20, 1], [30, 400], 2, 1, 128, bf16)
+        dev, want = both(torch, inp, at, [20, 1], [30, 400], scale, bf16)
+        attn_check(torch, attn_run(q, torch, dev, [20, 1], [30, 400], at, scale=scale), want, bf16)
+
+
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+@pytest.mark.parametrize("size", [2.0 ** -140, 2.0 ** -120, 2.0 ** -64, 2.0 ** -62, 1e-3, 1e30])
+def test_attention_queries_of_any_size(q, torch_cuda, bf16, size):
+    """Rows of very small and very large elements beside ordinary ones, rows of zeros, single elements; K's scales make up for it."""
+    torch = torch_cuda
+    lens, ctx, d = [30, 1], [50, 300], 256
+    inp, at = attn_inputs(torch, 8, lens, ctx, 2, 1, d, bf16)
+    inp = list(inp)
+    inp[0] = inp[0] * size
+    inp[0][3] = 0.0
+    inp[0][4, :, 1:] = 0.0
+    inp[0][5] = torch.sign(inp[0][5]) * size
+    inp[2] = inp[2] * min(max(1.0 / size, 1e-30), 1e30)
+    dev, want = both(torch, inp, at, lens, ctx, 1 / math.sqrt(d), bf16)
+    wo, tol = want
+    if size < 2.0 ** -125:     # the row's unit has steps of 2^-149: up to 2^-150 off, times sums of 256 codes of 128 and 30 (scales up to 1e30)
+        tol = tol + 1e-6 * inp[4].abs().max().double() * 127
+    attn_check(torch, attn_run(q, torch, dev, lens, ctx, at), (wo, tol), bf16)
+
+
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+def test_attention_any_codes(q, torch_cuda, bf16):
+    """All codes, -128 among them, and the largest sums that there are."""
+    torch = torch_cuda
+    g = gen(torch, 9)
+    for d in (128, 256):
+        inp, at = attn_inputs(torch, 9, [40], [70], 2, 1, d, bf16)
+        kq, vq = (torch.randint(-128, 128, inp[1].shape, generator=g, dtype=torch.int8) for _ in range(2))
+        kq[7], kq[8], vq[9] = -128, 127, -128
+        inp = (inp[0], kq, torch.full((70, 1), 1e-3), vq, inp[4])
+        inp[0][5] = -2.0
+        inp[0][6] = 2.0
+        dev, want = both(torch, inp, at, [40], [70], 0.1, bf16)
+        attn_check(torch, attn_run(q, torch, dev, [40], [70], at, scale=0.1), want, bf16)
+
+
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+@pytest.mark.parametrize("bad", [math.nan, math.inf], ids=str)
+def test_attention_query_rows_on_their_own(q, torch_cuda, bf16, bad):
+    torch = torch_cuda
+    lens, ctx = [70, 1], [90, 300]
+    inp, at = attn_inputs(torch, 10, lens, ctx, 4, 2, 128, bf16)
+    clean = attn_run(q, torch, [x.cuda() for x in inp], lens, ctx, at)
+    for r, h, e in ((0, 1, 5), (33, 3, 127), (70, 0, 0)):
+        inp[0][r, h, e] = bad
+    got = attn_run(q, torch, [x.cuda() for x in inp], lens, ctx, at)
+    for r, h in ((0, 1), (33, 3), (70, 0)):
+        assert torch.isnan(got[r, h]).all()
+        got[r, h] = clean[r, h]
+    assert torch.equal(got, clean)
+
+
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+@pytest.mark.parametrize("n,m", [(1, 40), (30, 40), (90, 600)])
+def test_attention_bad_ranges(q, torch_cuda, bf16, n, m):
+    """Key ranges outside the array give NaN in that sequence's rows; row bounds out of order leave rows alone."""
+    torch = torch_cuda
+    lens, ctx = [n, n, n], [m, m, m]
+    inp, at = attn_inputs(torch, 8, lens, ctx, 2, 1, 128, bf16)
+    dev, want = both(torch, inp, at, lens, ctx, 1 / math.sqrt(128), bf16)
+    part = lambda a, b: (want[0][a:b], want[1][a:b])
+    for start, length in ((-1, m), (2 * m + 1, m), (m, -1), (1 << 40, m), (0, 3 * m + 1)):
+        k2, c2 = list(at), list(ctx)
+        k2[1], c2[1] = start, length
+        got = attn_run(q, torch, dev, lens, c2, k2, max_k=m)
+        assert torch.isnan(got[n:2 * n]).all()
+        attn_check(torch, got[:n], part(0, n), bf16)
+        attn_check(torch, got[2 * n:], part(2 * n, 3 * n), bf16)
+    out = torch.full((3 * n, 2, 128), 7.0, dtype=dev[0].dtype, device="cuda")
+    ws = torch.empty(q.attention_seq_i8_workspace(3 * n, 3, n, m, 2, 1, 128), dtype=torch.uint8, device="cuda")
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    q.attention_seq_i8(out, *dev, i32([0, n, 3 * n + 1, 3 * n]), torch.tensor(at, dtype=torch.int64, device="cuda"), i32(ctx), ws, n, m)
+    attn_check(torch, out[:n], part(0, n), bf16)
+    assert (out[n:] == 7).all()
+
+
+# The form for prompts, whatever the lengths: max_q is a bound, and a large one asks for it.
+
+@pytest.fixture
+def prompts(monkeypatch):
+    monkeypatch.setattr(sys.modules[__name__], "attn_run", functools.partial(attn_run, max_q=4096))
+
+
+@pytest.mark.parametrize("lens,ctx,h,kvh,d", ATTN + [
+    ([700], [3000], 8, 2, 256), ([130, 1], [4100, 2000], 2, 2, 128), ([40], [9000], 4, 4, 128), ([1023, 0, 513], [1023, 4, 800], 4, 1, 256),
+    ([257], [700], 12, 4, 256)], ids=str)
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+def test_prompt_form(prompts, q, torch_cuda, lens, ctx, h, kvh, d, bf16):
+    test_attention(q, torch_cuda, lens, ctx, h, kvh, d, bf16)
+
+
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+@pytest.mark.parametrize("d", [128, 256])
+def test_prompt_form_rows_without_keys(prompts, q, torch_cuda, bf16, d):
+    test_attention_rows_without_keys(q, torch_cuda, bf16, d)
+
+
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+@pytest.mark.parametrize("n,m", [(1, 200), (5, 300), (100, 100), (150, 260), (90, 1200)])
+@pytest.mark.parametrize("d", [128, 256])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, 3e38], ids=str)
+def test_prompt_form_hidden_keys_have_no_influence(prompts, q, torch_cuda, bf16, d, n, m, bad):
+    test_attention_hidden_keys_have_no_influence(q, torch_cuda, bf16, d, n, m, bad)
+
+
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+def test_prompt_form_strides(prompts, q, torch_cuda, bf16):
+    test_attention_strides(q, torch_cuda, bf16)
+
+
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+def test_prompt_form_large_scores_and_any_codes(prompts, q, torch_cuda, bf16):
+    test_attention_large_scores(q, torch_cuda, bf16)
+    test_attention_any_codes(q, torch_cuda, bf16)
+
+
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+@pytest.mark.parametrize("size", [2.0 ** -140, 2.0 ** -64, 1e30])
+def test_prompt_form_queries_of_any_size(prompts, q, torch_cuda, bf16, size):
+    test_attention_queries_of_any_size(q, torch_cuda, bf16, size)
+
+
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+@pytest.mark.parametrize("bad", [math.nan, math.inf], ids=str)
+def test_prompt_form_query_rows_on_their_own(prompts, q, torch_cuda, bf16, bad):
+    test_attention_query_rows_on_their_own(q, torch_cuda, bf16, bad)
+
+
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+@pytest.mark.parametrize("n,m", [(30, 40), (90, 600)])
+def test_prompt_form_bad_ranges(prompts, q, torch_cuda, bf16, n, m):
+    test_attention_bad_ranges(q, torch_cuda, bf16, n, m)
+
+
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+@pytest.mark.parametrize("max_k", [129, 300, 700, 20000])
+def test_prompt_form_places_in_the_workspace(q, torch_cuda, bf16, max_k):
+    """max_k is a bound on what the workspace holds, not on the keys: what finds no place there is not split."""
+    torch = torch_cuda
+    lens, ctx = [70, 3, 0, 129, 64, 1, 70, 2, 300], [900, 3, 10, 1500, 64, 2500, 400, 2, 3000]
+    inp, at = attn_inputs(torch, 15, lens, ctx, 4, 2, 128, bf16)
+    dev, want = both(torch, inp, at, lens, ctx, 1 / math.sqrt(128), bf16)
+    attn_check(torch, attn_run(q, torch, dev, lens, ctx, at, max_q=4096, max_k=max_k), want, bf16)
+
+
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+@pytest.mark.parametrize("max_q", [1, 4096])
+def test_attention_of_many_sequences(q, torch_cuda, bf16, max_q):
+    """More than the 64 sequences that a wave looks at together; long ones among empty and short ones."""
+    torch = torch_cuda
+    lens = [(5 * i) % 9 for i in range(150)]
+    ctx = [n + (7 * i) % 40 for i, n in enumerate(lens)]
+    for i, n, m in ((3, 140, 900), (64, 1, 1500), (149, 70, 70)):
+        lens[i], ctx[i] = n, m
+    inp, at = attn_inputs(torch, 10, lens, ctx, 4, 2, 128, bf16)
+    dev, want = both(torch, inp, at, lens, ctx, 1 / math.sqrt(128), bf16)
+    attn_check(torch, attn_run(q, torch, dev, lens, ctx, at, max_q=max_q), want, bf16)
+
+
+@pytest.mark.parametrize("ld", [1 << 22, 1 << 25])
+@pytest.mark.parametrize("max_q", [1, 4096])
+def test_attention_rows_far_apart(q, torch_cuda, ld, max_q):
+    """Rows of codes 4 and 32 MB apart, the last ones behind 2^32 bytes; scales 1 MB apart."""
+    torch = torch_cuda
+    rows = 1100 if ld == 1 << 22 else 300
+    lens, ctx, at = [40, 1, 200], [rows, 250, rows - 60], [0, rows - 250, 60]
+    inp, _ = attn_inputs(torch, 13, lens, [rows], 4, 2, 128, True)
+    want = attn_oracle(torch, *inp, lens, ctx, at, 1 / math.sqrt(128), True)
+    dev = [inp[0].cuda()]
+    for x in inp[1:]:
+        step = ld if x.dtype is torch.int8 else 1 << 18
+        far = torch.empty((rows - 1) * step + x[0].numel(), dtype=x.dtype, device="cuda").as_strided(x.shape, (step, *x.stride()[1:]))
+        far.copy_(x)
+        dev.append(far)
+    attn_check(torch, attn_run(q, torch, dev, lens, ctx, at, max_q=max_q), want, True)
+
+
+# ------------------------------------------------------------------ calls that cannot be answered
+
+def test_refused_tensors(q, torch_cuda, monkeypatch):
+    """Other types, shapes and strides; operands in host memory or on another device, each of them; parameters are tensors
+    like others."""
+    torch = torch_cuda
+    z = lambda *s, dt=torch.float32: torch.zeros(*s, dtype=dt, device="cuda")
+    i8, i32, i64 = torch.int8, torch.int32, torch.int64
+    cache = lambda: [z(9, 1, 128, dt=i8), z(9, 1), z(9, 1, 128, dt=i8), z(9, 1)]
+    rope = [z(4, 2, 128), z(4, 1, 128), z(4, 2, 128), z(4, 1, 128), z(128), z(128), z(4, dt=i32)]
+    write = [*cache(), z(4, 1, 128), z(4, 1, 128), torch.arange(4, device="cuda")]
+    read = [z(4, 1, 128), z(4, 1, 128), *cache(), torch.arange(4, device="cuda")]
+    attn = [z(4, 2, 128), z(4, 2, 128), *cache(), z(2, dt=i32), z(1, dt=i64), z(1, dt=i32), None, 4, 9]
+    calls = [(q.qk_norm_rope_seq, rope, 7), (q.kv_cache_write_i8, write, 7), (q.kv_cache_read_i8, read, 7), (q.attention_seq_i8, attn, 9)]
+    for f, ops, n in calls:
+        f(*ops)
+        f(*[torch.nn.Parameter(x, requires_grad=False) if k < n else x for k, x in enumerate(ops)])
+        for i in range(n):
+            put = lambda x: [x if k == i else y for k, y in enumerate(ops)]
+            with pytest.raises(TypeError):
+                f(*put(ops[i].cpu()))
+            with pytest.raises(TypeError):
+                f(*put(ops[i].half() if ops[i].is_floating_point() else ops[i].to(torch.int16)))
+            with pytest.raises(ValueError):
+                f(*put(z(*[s + 1 for s in ops[i].shape], dt=ops[i].dtype)))
+            if ops[i].shape[-1] == 128:
+                with pytest.raises(ValueError):
+                    f(*put(z(*ops[i].shape[:-1], 256, dt=ops[i].dtype)[..., ::2]))
+    for f, ops, _ in calls[1:3]:
+        with pytest.raises(q.QHError):
+            f(*[z(9, 1, 136, dt=i8)[..., 8:] if x.dtype is i8 else x for x in ops])      # 8 bytes off
+    with pytest.raises(q.QHError):
+        q.kv_cache_write_i8(*[z(1, 1, 128, dt=i8).expand(9, 1, 128) if k == 0 else x for k, x in enumerate(write)])   # one row for all
+    with pytest.raises(q.QHError):
+        q.kv_cache_write_i8(*[write[2] if k == 0 else x for k, x in enumerate(write)])   # keys and values in one place
+    with pytest.raises(q.QHError):
+        q.qk_norm_rope_seq(*rope, 24)
+    with pytest.raises(q.QHError):
+        q.qk_norm_rope_seq(*[x[..., :64].contiguous() if x.shape[-1] == 128 else x for x in rope])
+    with pytest.raises(TypeError):
+        q.attention_seq_i8(*attn[:9], torch.empty(64, dtype=torch.uint8), 4, 9)
+    with pytest.raises(q.QHError):
+        q.attention_seq_i8(*attn[:9], torch.empty(256, dtype=torch.uint8, device="cuda"), 4, 1000)
+    with pytest.raises(q.QHError):
+        q.attention_seq_i8(*attn[:10], 4, 1 << 40)
+    monkeypatch.setattr(q._Short, "device", lambda: 1)
+    for f, ops, _ in calls:
+        with pytest.raises(ValueError):
+            f(*ops)
+
+
+# ------------------------------------------------------------------ streams, graphs, together
+
+def test_two_streams(q, torch_cuda):
+    """Calls beside one another on two streams, each with operands and a workspace of its own, over one cache that both read."""
+    torch = torch_cuda
+    lens, ctx = [80, 5], [80, 900]
+    inp, at = attn_inputs(torch, 12, lens, ctx, 8, 2, 256, True)
+    dev, want = both(torch, inp, at, lens, ctx, 1 / 16, True)
+    slot = torch.arange(980, device="cuda")
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    res = []
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(5):
+        for s in streams:
+            with torch.cuda.stream(s):
+                c = cache_new(torch, 980, 2, 256, "rows")
+                o = [torch.empty(980, 2, 256, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+                q.kv_cache_read_i8(*o, *dev[1:], slot)
+                q.kv_cache_write_i8(*c, *o, slot)
+                res.append((attn_run(q, torch, dev, lens, ctx, at), attn_run(q, torch, dev, lens, ctx, at, max_q=4096), o, c))
+    torch.cuda.synchronize()
+    for a, b, o, c in res:
+        attn_check(torch, a, want, True)
+        attn_check(torch, b, want, True)
+        assert torch.equal(a, res[0][0]) and torch.equal(b, res[0][1])
+        assert torch.equal(o[0].cpu(), (inp[1].float() * inp[2][..., None]).bfloat16())
+        assert torch.equal(c[0].cpu(), code_oracle(torch, o[0].cpu())[0])
+
+
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+def test_layer_over_the_cache(q, torch_cuda, bf16):
+    """The operators as a layer chains them: one projection's queries, keys and values normalised, rotated, written into
+    slots of the cache and attended to; prompts of several sequences first, then single tokens from a graph that is replayed with
+    other positions, slots and lengths on the device (some places of the batch unused), eager work between.  Every replay gives the
+    eager call's bits, and each stage its bound against 64 bits on its own inputs."""
+    torch = torch_cuda
+    h, kvh, d, room, n_seq, dt = 8, 2, 128, 200, 4, torch.bfloat16 if bf16 else torch.float32
+    g = gen(torch, 21)
+    lens = [90, 1, 0, 33]
+    qw, kw = (torch.randn(d, generator=g) * 0.2 for _ in range(2))
+    c = cache_new(torch, n_seq * room, kvh, d, "side")
+    for x in c[1::2]:
+        x.fill_(math.nan)                          # rows that were never written hold anything
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    k_start = torch.arange(n_seq, device="cuda") * room
+
+    def stage_check(row, pos, out, qn, kn, vv, cu, ctx):
+        rope_check(torch, qn, rope_oracle(torch, row[:, :h].cpu(), qw, pos, 64), bf16)
+        rope_check(torch, kn, rope_oracle(torch, row[:, h:h + kvh].cpu(), kw, pos, 64), bf16)
+        ln = [b - a for a, b in zip(cu, cu[1:])]
+        n = cu[-1]
+        host = [x.cpu() for x in c]
+        for x in host[1::2]:
+            x[x.isnan()] = 0.0
+        attn_check(torch, out[:n], attn_oracle(torch, qn[:n].cpu(), *host, ln, ctx, k_start.tolist(), 1 / math.sqrt(d), bf16), bf16)
+
+    def step(row, pos, slot, cu, kl, out, ws, mq):
+        t = row.shape[0]
+        qn, kn = torch.empty(t, h, d, dtype=dt, device="cuda"), torch.empty(t, kvh, d, dtype=dt, device="cuda")
+        q.qk_norm_rope_seq(qn, kn, row[:, :h], row[:, h:h + kvh], qw_d, kw_d, pos)
+        q.kv_cache_write_i8(*c, kn, row[:, h + kvh:], slot)
+        q.attention_seq_i8(out, qn, *c, cu, k_start, kl, ws, mq, room)
+        return qn, kn
+
+    qw_d, kw_d = qw.cuda(), kw.cuda()
+    t = sum(lens)
+    row = torch.randn(t, h + 2 * kvh, d, generator=g).to(dt).cuda()
+    pos = torch.cat([torch.arange(n) for n in lens]).to(torch.int32)
+    slot = pos.long() + torch.tensor(sum([[i] * n for i, n in enumerate(lens)], [])) * room
+    out = torch.full((t, h, d), 7.0, dtype=dt, device="cuda")
+    ws = torch.empty(q.attention_seq_i8_workspace(t, n_seq, max(lens), room, h, kvh, d), dtype=torch.uint8, device="cuda")
+    qn, kn = step(row, pos.cuda(), slot.cuda(), i32(starts(lens)), i32(lens), out, ws, max(lens))
+    stage_check(row, pos, out, qn, kn, None, starts(lens), lens)
+    codes, sc = code_oracle(torch, kn.cpu())
+    assert torch.equal(c[0][slot.cuda()].cpu(), codes) and torch.equal(c[1][slot.cuda()].cpu(), sc)
+
+    # single tokens
+    row1, pos1, slot1 = torch.zeros(n_seq, h + 2 * kvh, d, dtype=dt, device="cuda"), i32([0] * n_seq), torch.full((n_seq,), -1, device="cuda")
+    cu1, kl1, out1 = i32([0] * (n_seq + 1)), i32([0] * n_seq), torch.empty(n_seq, h, d, dtype=dt, device="cuda")
+    ws1 = torch.empty(q.attention_seq_i8_workspace(n_seq, n_seq, 1, room, h, kvh, d), dtype=torch.uint8, device="cuda")
+    args = (row1, pos1, slot1, cu1, kl1, out1, ws1, 1)
+    step(*args)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        qn1, kn1 = step(*args)
+    held = list(lens)
+    for it in range(6):
+        live = [i for i in range(n_seq) if (it + i) % 3 != 0]       # the sequences with a token now, at the batch's first places
+        new = torch.randn(n_seq, h + 2 * kvh, d, generator=g).to(dt)
+        row1.copy_(new)
+        p = [held[i] for i in live] + [0] * (n_seq - len(live))
+        pos1.copy_(i32(p))
+        slot1.copy_(torch.tensor([i * room + held[i] for i in live] + [-1] * (n_seq - len(live)), device="cuda"))
+        for i in live:
+            held[i] += 1
+        cu = [0]
+        for i in range(n_seq):
+            cu.append(cu[-1] + (i in live))
+        cu1.copy_(i32(cu)), kl1.copy_(i32(held))
+        before = [x.clone() for x in c]
+        res = []
+        for run in (lambda: step(*args), lambda: (graph.replay(), (qn1, kn1))[1], lambda: (graph.replay(), (qn1, kn1))[1]):
+            for x, b in zip(c, before):
+                x.copy_(b)
+            out1.fill_(7.0)
+            got = run()
+            torch.cuda.synchronize()
+            res.append([x.clone() for x in (out1, *got, *c)])
+        for r in res[1:]:
+            assert all(same(torch, a, b) for a, b in zip(r, res[0]))
+        assert (out1[len(live):] == 7).all()
+        stage_check(row1, pos1.cpu(), out1, res[0][1], res[0][2], None, cu, held)
