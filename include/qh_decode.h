@@ -325,7 +325,9 @@ int qh_kv_cache_read_i8(void* k, int64_t ldk, int64_t hsk, void* v, int64_t ldv,
                         int64_t hsvq, const float* vs, int64_t ldvs, int64_t hsvs, const int64_t* slot, int64_t rows, int tokens,
                         int kv_heads, int head_dim, void* stream);
 
-/* qh_attention_seq over the cache: the same sequences, key ranges, rows without keys, limits and workspace rules; q and
+#define QH_ATTN_I8_MAX_LD (1 << 24)
+
+/* qh_attention_seq over the cache, whose row strides (of codes and of scales) are below QH_ATTN_I8_MAX_LD: the same sequences, key ranges, rows without keys, limits and workspace rules; q and
  * out of `type`.  Codes and scales of keys that a row does not see have no influence on it; a row that sees a
  * scale that is not finite gives NaN.  A query row takes part as whole numbers, its largest magnitude being 32639
  * (QH_BF16: an element is off by 2^-16 of the row's largest at most) or 8355711 (QH_F32: 2^-24), so that sums of products with

@@ -1,6 +1,7 @@
 // Causal attention with grouped heads over packed sequences whose keys and values are rows of an int8 cache, a scale for
 // each row and head:  out = softmax(scale q (s_k K)^T) (s_v V)  over the keys a row sees; 0 without any.
 #include <algorithm>
+#include <type_traits>
 
 #include "qh_attn_device.hpp"
 
@@ -20,17 +21,33 @@ __device__ __forceinline__ uint32_t bytes4(int a, int b, int c, int d) {
   return lo | hi;
 }
 
-// Codes of eight rows as the upper halves of floats: element (byte) c of rows 2 i and 2 i + 1 in dword i.  A code has
-// eight bits, a bfloat16 as well.
-template <typename V>
-__device__ __forceinline__ u32x4 widen(const V (&rows)[8], int c) {
+// Byte B of x, signed, as a float, in one instruction (the compiler takes three).
+template <int B>
+__device__ __forceinline__ uint32_t code_float(uint32_t x) {
+  uint32_t f;
+  if constexpr (B == 0) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_0" : "=v"(f) : "v"(x));
+  if constexpr (B == 1) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_1" : "=v"(f) : "v"(x));
+  if constexpr (B == 2) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_2" : "=v"(f) : "v"(x));
+  if constexpr (B == 3) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_3" : "=v"(f) : "v"(x));
+  return f;
+}
+// Byte C of eight rows as bfloat16, rows 2 i and 2 i + 1 in dword i.  A code has eight bits, a bfloat16 as well: the upper half of
+// the float is all of it.
+template <int C, typename V>
+__device__ __forceinline__ u32x4 widen(const V (&rows)[8]) {
   u32x4 t;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float a = (float)(int8_t)(rows[2 * i][c >> 2] >> (8 * (c & 3))), b = (float)(int8_t)(rows[2 * i + 1][c >> 2] >> (8 * (c & 3)));
-    t[i] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
-  }
+  for (int i = 0; i < 4; ++i)
+    t[i] = __builtin_amdgcn_perm(code_float<C & 3>(rows[2 * i + 1][C >> 2]), code_float<C & 3>(rows[2 * i][C >> 2]), 0x07060302u);
   return t;
+}
+// f(0), f(1) .. f(N - 1) with constants
+template <int N, typename F>
+__device__ __forceinline__ void each(F f) {
+  if constexpr (N > 0) {
+    each<N - 1>(f);
+    f(std::integral_constant<int, N - 1>{});
+  }
 }
 
 // Few query rows: a workgroup takes 16 rows (tokens x query heads of one kv head) and one chunk of the keys, its four
@@ -64,26 +81,33 @@ __global__ __launch_bounds__(256, 2) void attn_i8_split_kernel(const AttnI8 a) {
   const int k0 = at.split * at.chunk, k1 = min(end, at.split + 1 == at.nsplit ? end : k0 + at.chunk);
   if (at.split > 0 && k0 >= end) return;   // (no row of the tile sees it)
 
-  const char* kp = static_cast<const char*>(a.k.p) + ks * a.k.ld + kvh * a.k.hs + 16 * g;
-  const char* vp = static_cast<const char*>(a.v.p) + ks * a.v.ld + kvh * a.v.hs + VB * j;
-  const float* sp = lane < 32 ? a.ks + ks * a.ldks + kvh * a.hsks : a.vs + ks * a.ldvs + kvh * a.hsvs;
-  const int64_t sld = lane < 32 ? a.ldks : a.ldvs;
-  u32x4 kv[2][NS];   // a step's rows; the next step's are loaded as soon as these are used
+  // A step's rows by 32-bit offsets from its first key (the strides are below 2^24: the entry point's rule); the next
+  // step's are loaded as soon as these are used.
+  const uint32_t kld = (uint32_t)a.k.ld, vld = (uint32_t)a.v.ld, sld = (uint32_t)(lane < 32 ? a.ldks : a.ldvs);
+  const char* kp = static_cast<const char*>(a.k.p) + ks * a.k.ld + kvh * a.k.hs;
+  const char* vp = static_cast<const char*>(a.v.p) + ks * a.v.ld + kvh * a.v.hs;
+  const float *ksp = a.ks + ks * a.ldks + kvh * a.hsks, *vsp = a.vs + ks * a.ldvs + kvh * a.hsvs;
+  u32x4 kv[2][NS];
   vrow vv[8];
   float sc = 0.0f;   // of key lane % 32 of the step: K's scale, in the upper half V's
-  auto load_k = [&](int kb) {
-    sc = as_global(sp)[min(kb + (lane & 31), k1 - 1) * sld];
+  auto load_k = [&](int kb) {   // kb: the same for the wave, below k1
+    const int last = k1 - 1 - kb;
+    const float* sp = lane < 32 ? ksp + kb * a.ldks : vsp + kb * a.ldvs;
+    sc = as_global(sp)[__umul24(min(lane & 31, last), sld)];
+    const char* p = kp + kb * a.k.ld;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const char* p = kp + min(kb + 16 * t + j, k1 - 1) * a.k.ld;
+      const uint32_t o = __umul24(min(16 * t + j, last), kld) + 16 * g;
 #pragma unroll
-      for (int s = 0; s < NS; ++s) kv[t][s] = *as_global(reinterpret_cast<const u32x4*>(p + 64 * s));
+      for (int s = 0; s < NS; ++s) kv[t][s] = *as_global(reinterpret_cast<const u32x4*>(p + o + 64 * s));
     }
   };
   auto load_v = [&](int kb) {
+    const int last = k1 - 1 - kb;
+    const char* p = vp + kb * a.v.ld;
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      vv[i] = *as_global(reinterpret_cast<const vrow*>(vp + min(kb + 16 * (i >> 2) + 4 * g + (i & 3), k1 - 1) * a.v.ld));
+      vv[i] = *as_global(reinterpret_cast<const vrow*>(p + (uint32_t)(__umul24(min(16 * (i >> 2) + 4 * g + (i & 3), last), vld) + VB * j)));
   };
   int kb = k0 + 32 * wave;
   if (kb < k1) load_k(kb), load_v(kb);
@@ -156,7 +180,8 @@ __global__ __launch_bounds__(256, 2) void attn_i8_split_kernel(const AttnI8 a) {
     float p[8], mx = kNegInf;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const f32x4 ksc = *as_lds(reinterpret_cast<const f32x4*>(&lsc[wave][16 * t + 4 * g]));
+      f32x4 ksc = *as_lds(reinterpret_cast<const f32x4*>(&lsc[wave][16 * t + 4 * g]));
+      settle(ksc);   // (read by all lanes, not under the condition below)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int key = kb + 16 * t + 4 * g + r;
@@ -168,13 +193,24 @@ __global__ __launch_bounds__(256, 2) void attn_i8_split_kernel(const AttnI8 a) {
     }
     mx = fmaxf(mx, xor_perm<16>(mx));
     mx = fmaxf(mx, xor_perm<32>(mx));
-    const float mn = fmaxf(m, mx), mu = mn == kNegInf ? 0.0f : mn;
-    const float al = __builtin_amdgcn_exp2f(m - mu);
-    m = mn;
+    // the running maximum moves only when a score passes it by more than 8 (a factor of 256, exact in the sums); a row's
+    // own scores decide, so that other rows have no influence on it
+    const bool up = mx > m + 8.0f;
+    if (__ballot(up) != 0) {
+      const float mn = up ? mx : m, al = __builtin_amdgcn_exp2f(m - (mn == kNegInf ? 0.0f : mn));
+      m = mn;
+      l *= al;
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[t][c] *= al;
+    }
+    const float mu = m == kNegInf ? 0.0f : m;
     float ps = 0.0f;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const f32x4 vsc = *as_lds(reinterpret_cast<const f32x4*>(&lsc[wave][32 + 16 * t + 4 * g]));
+      f32x4 vsc = *as_lds(reinterpret_cast<const f32x4*>(&lsc[wave][32 + 16 * t + 4 * g]));
+      settle(vsc);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const float e = __builtin_amdgcn_exp2f(p[4 * t + r] - mu);
@@ -182,11 +218,7 @@ __global__ __launch_bounds__(256, 2) void attn_i8_split_kernel(const AttnI8 a) {
         p[4 * t + r] = kb + 16 * t + 4 * g + r < lim ? e * vsc[r] : 0.0f;   // (a hidden row's scale may be anything)
       }
     }
-    l = l * al + ps;
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int c = 0; c < 4; ++c) acc[t][c] *= al;
+    l += ps;
     u32x4 pb[NP];
 #pragma unroll
     for (int d = 0; d < 4; ++d) {
@@ -202,13 +234,21 @@ __global__ __launch_bounds__(256, 2) void attn_i8_split_kernel(const AttnI8 a) {
       const bf16x2 last = {(__bf16)x, (__bf16)y};
       pb[NP - 1][d] = __builtin_bit_cast(uint32_t, last);
     }
-#pragma unroll
-    for (int c = 0; c < VB; ++c) {
-      const u32x4 t = widen(vv, c);
+    __builtin_amdgcn_sched_barrier(0);   // (the codes are widened where they are used: all at once they would not fit the registers)
+    each<VB>([&](auto C) {
+      const u32x4 t = widen<C>(vv);
 #pragma unroll
       for (int i = NP - 1; i >= 0; --i)
-        acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, t), __builtin_bit_cast(bf16x8, pb[i]), acc[c], 0, 0, 0);
+        acc[C] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, t), __builtin_bit_cast(bf16x8, pb[i]), acc[C], 0, 0, 0);
+    });
+    __builtin_amdgcn_sched_group_barrier(0x2, 24, 0);
+#pragma unroll
+    for (int c = 0; c < VB - 2; ++c) {
+      __builtin_amdgcn_sched_group_barrier(0x8, NP, 0);
+      __builtin_amdgcn_sched_group_barrier(0x2, 12, 0);
     }
+    __builtin_amdgcn_sched_group_barrier(0x8, 2 * NP, 0);
+    __builtin_amdgcn_sched_barrier(0);
     load_v(min(kb + 128, k1 - 1));
   }
   l = l + xor_perm<16>(l);

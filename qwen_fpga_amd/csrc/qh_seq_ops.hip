@@ -283,6 +283,8 @@ int qh_attention_seq_i8(void* out, int64_t ldo, int64_t hso, const void* q, int6
   if (!vo.writable() || !vq_.readable()) return QH_EINVAL;
   if (k_rows > 0 && (!vk.readable() || !vv.readable() || !sk.strided() || !sv.strided())) return QH_EINVAL;
   if (!all_countable(vo, vq_) || (k_rows > 0 && !all_countable(vk, vv, sk, sv))) return QH_ERANGE;
+  for (const int64_t ld : {ldkq, ldvq, ldks, ldvs})   // (the kernels' 32-bit offsets)
+    if (k_rows > 1 && ld >= QH_ATTN_I8_MAX_LD) return QH_ERANGE;
   if (!cu_q || !k_start || !k_len) return QH_EINVAL;
   const View vc = flat(cu_q, n_seq + 1, 4), vt = flat(k_start, n_seq, 8), vl = flat(k_len, n_seq, 4);
   if (overlap_any(vo, vq_, vc, vt, vl) || (k_rows > 0 && overlap_any(vo, vk, vv, sk, sv))) return QH_EINVAL;

@@ -179,6 +179,9 @@ def test_attention_nothing_to_do_ranges_and_workspace(q, args):
     assert args.attn(max_k=(1 << 30) + 1) == q.QH_ERANGE
     assert args.attn(n_seq=65537) == q.QH_ERANGE
     assert args.attn(q_rows=1 << 30, heads=4) == q.QH_ERANGE and args.attn(q_rows=33000000) == q.QH_ERANGE
+    for name in ("ldkq", "ldvq", "ldks", "ldvs"):
+        assert args.attn(**{name: 1 << 24}) == q.QH_ERANGE
+        assert args.attn(k_rows=1, cu_q=None, **{name: 1 << 24}) == q.QH_EINVAL    # (one row has no next one)
     need = q.attention_seq_i8_workspace(3, 1, 1, 100000, 2, 1, 128)   # few rows, many keys: the keys are split
     assert need > 0
     for ws in (dict(ws=None), dict(ws_bytes=need - 1), dict(ws=args.at(10) + 16), dict(ws=args.at(1)), dict(ws=args.at(3) - 256)):

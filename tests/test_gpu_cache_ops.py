@@ -636,10 +636,10 @@ def test_attention_of_many_sequences(q, torch_cuda, bf16, max_q):
     attn_check(torch, attn_run(q, torch, dev, lens, ctx, at, max_q=max_q), want, bf16)
 
 
-@pytest.mark.parametrize("ld", [1 << 22, 1 << 25])
+@pytest.mark.parametrize("ld", [1 << 22, (1 << 24) - 16])
 @pytest.mark.parametrize("max_q", [1, 4096])
 def test_attention_rows_far_apart(q, torch_cuda, ld, max_q):
-    """Rows of codes 4 and 32 MB apart, the last ones behind 2^32 bytes; scales 1 MB apart."""
+    """Rows of codes 4 and 16 MB apart (the largest stride), the last ones behind 2^32 bytes; scales 1 MB apart."""
     torch = torch_cuda
     rows = 1100 if ld == 1 << 22 else 300
     lens, ctx, at = [40, 1, 200], [rows, 250, rows - 60], [0, rows - 250, 60]
@@ -699,6 +699,9 @@ def test_refused_tensors(q, torch_cuda, monkeypatch):
         q.attention_seq_i8(*attn[:9], torch.empty(256, dtype=torch.uint8, device="cuda"), 4, 1000)
     with pytest.raises(q.QHError):
         q.attention_seq_i8(*attn[:10], 4, 1 << 40)
+    far = torch.empty(8 * (1 << 24) + 128, dtype=i8, device="cuda").as_strided((9, 1, 128), (1 << 24, 128, 1))
+    with pytest.raises(q.QHError):
+        q.attention_seq_i8(*[far if k == 2 else x for k, x in enumerate(attn)])
     monkeypatch.setattr(q._Short, "device", lambda: 1)
     for f, ops, _ in calls:
         with pytest.raises(ValueError):
