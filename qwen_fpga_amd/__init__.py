@@ -783,8 +783,9 @@ def kv_cache_write_i8(kq, ks, vq, vs, k, v, slot, stream=None):
     any row and head strides) goes to row slot[t] (int64 on the device; one outside the cache, such as -1, is skipped).
     quant_rows of each head's row, bit for bit: scale = largest magnitude / 127, and NaN where the row is not finite.
     Two tokens may not name the same row."""
+    fn = _op("qh_kv_cache_write_i8")
     ty, cache, new, where = _cache_operands("qh_kv_cache_write_i8", kq, ks, vq, vs, k, v, slot)
-    st = _op("qh_kv_cache_write_i8")(*cache, *new, ty, *where, _st(stream))
+    st = fn(*cache, *new, ty, *where, _st(stream))
     if st:
         _check(st, "qh_kv_cache_write_i8")
 
@@ -792,8 +793,9 @@ def kv_cache_write_i8(kq, ks, vq, vs, k, v, slot, stream=None):
 def kv_cache_read_i8(k, v, kq, ks, vq, vs, slot, stream=None):
     """Rows of the cache as the values that they stand for: k, v [tokens, kv_heads, dim] (float32 or bfloat16), token t
     from row slot[t] (int64 on the device; one outside the cache leaves the token's rows of k and v as they were)."""
+    fn = _op("qh_kv_cache_read_i8")
     ty, cache, new, where = _cache_operands("qh_kv_cache_read_i8", kq, ks, vq, vs, k, v, slot)
-    st = _op("qh_kv_cache_read_i8")(*new, ty, *cache, *where, _st(stream))
+    st = fn(*new, ty, *cache, *where, _st(stream))
     if st:
         _check(st, "qh_kv_cache_read_i8")
 

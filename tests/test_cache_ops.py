@@ -3,6 +3,7 @@ cache a token may name, the scale of a row), the host's refusals and the workspa
 import ctypes
 import os
 import subprocess
+import sys
 
 import pytest
 
@@ -208,3 +209,19 @@ def test_python_checks_need_no_gpu(q):
                            torch.zeros(1, dtype=torch.int32), None, 2, 2)
     with pytest.raises(ValueError, match="dimensions"):
         q.kv_cache_write_i8(*cache(), f(2, 128), f(2, 128), slot)
+
+
+@pytest.mark.parametrize("call", [
+    "qk_norm_rope_seq(f(2, 2, 128), f(2, 1, 128), f(2, 2, 128), f(2, 1, 128), f(128), f(128), torch.zeros(2, dtype=torch.int32))",
+    "kv_cache_write_i8(*c, f(2, 1, 128), f(2, 1, 128), s)",
+    "kv_cache_read_i8(f(2, 1, 128), f(2, 1, 128), *c, s)",
+    "attention_seq_i8(f(2, 2, 128), f(2, 2, 128), *c, s[:0].int(), s[:1], s[:1].int(), None, 2, 2)",
+], ids=lambda c: c.split("(")[0])
+def test_any_operator_may_be_the_first(call):
+    """The library is loaded by the first call, whichever it is: the operands' types are known then (here, that they are not on the GPU)."""
+    code = ("import torch, qwen_fpga_amd as q\n"
+            "f, i8, s = torch.zeros, lambda *n: torch.zeros(*n, dtype=torch.int8), torch.zeros(2, dtype=torch.int64)\n"
+            "c = i8(9, 1, 128), f(9, 1), i8(9, 1, 128), f(9, 1)\n"
+            f"try:\n    q.{call}\nexcept TypeError as e:\n    assert 'CUDA' in str(e), e\nelse:\n    raise SystemExit('taken')\n")
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=ROOT)
+    assert r.returncode == 0, r.stderr
