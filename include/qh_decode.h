@@ -329,10 +329,11 @@ int qh_kv_cache_read_i8(void* k, int64_t ldk, int64_t hsk, void* v, int64_t ldv,
 
 /* qh_attention_seq over the cache, whose row strides (of codes and of scales) are below QH_ATTN_I8_MAX_LD: the same sequences, key ranges, rows without keys, limits and workspace rules; q and
  * out of `type`.  Codes and scales of keys that a row does not see have no influence on it; a row that sees a
- * scale that is not finite gives NaN.  A query row takes part as whole numbers, its largest magnitude being 32639
- * (QH_BF16: an element is off by 2^-16 of the row's largest at most) or 8355711 (QH_F32: 2^-24), so that sums of products with
- * codes are exact; scores, the softmax and sums are fp32, probabilities times V's scales enter the product with the
- * codes in two bfloat16 parts (QH_BF16: off by 2^-16 of sum p |v| at most) or three (QH_F32: exact). */
+ * scale of V that is not finite gives nothing finite, and NaN where that or one of K is NaN.  A query row takes part as whole numbers, its largest magnitude being 32639
+ * (QH_BF16: an element is off by 2^-16 of the row's largest at most) or 8355704 (QH_F32: 2^-24), so that sums of products with
+ * codes are exact; scores, the softmax and sums are fp32.  Probabilities times V's scales enter the product with the
+ * codes exactly for QH_F32; for QH_BF16 in two bfloat16 parts in the form for few rows (off by 2^-16 of sum p |v| at
+ * most) and rounded to bfloat16 once in the one for prompts (2^-8). */
 size_t qh_attention_seq_i8_workspace(int q_rows, int n_seq, int max_q, int max_k, int heads, int kv_heads, int head_dim,
                                      int type);
 int qh_attention_seq_i8(void* out, int64_t ldo, int64_t hso, const void* q, int64_t ldq, int64_t hsq, int type, const int8_t* kq,

@@ -8,17 +8,64 @@
 namespace qh {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
 
 namespace {
 
-// A query row as whole numbers: the row's largest magnitude becomes `top` = 2 or 3 digits of eight bits (the upper one
-// 127), an element the nearest whole number, so that  q k = (sum_i digits_i 256^i k) * unit  and the sums of digit times
+// A query row as whole numbers of two or three digits in base 256, from -128 to 127 each: its largest magnitude becomes
+// `top`, an element the nearest whole number, so that  q k = (sum_i digit_i 256^i k) * unit  and the sums of digit times
 // code are exact in 32 bits.  Two digits leave out 2^-16 of the row's largest element at most, three 2^-24.
-constexpr int kTop2 = 127 * 256 + 127, kTop3 = kTop2 * 256 + 127;
-// digit i of four whole numbers, as bytes
-__device__ __forceinline__ uint32_t bytes4(int a, int b, int c, int d) {
-  const uint32_t lo = __builtin_amdgcn_perm((uint32_t)b, (uint32_t)a, 0x0c0c0400u), hi = __builtin_amdgcn_perm((uint32_t)d, (uint32_t)c, 0x04000c0cu);
-  return lo | hi;
+template <bool BF16>
+struct Row {
+  static constexpr int NP = BF16 ? 2 : 3;
+  static constexpr float kTop = BF16 ? 127 * 256 + 127 : 127 * 65536 + 127 * 256 + 120;   // (a rounding above it has the same digits)
+  float unit, up, to;   // (to * up may overflow: a row of very small elements is moved up first)
+  // top: the largest of the magnitudes' bits (infinities and NaN are above all numbers; the row is NaN then)
+  __device__ __forceinline__ explicit Row(uint32_t top) {
+    up = top < 0x20000000u ? 0x1p64f : 1.0f;   // below 2^-63
+    const float big = __uint_as_float(top) * up;
+    unit = top >= 0x7f800000u ? __builtin_nanf("") : big / kTop / up;
+    to = big > 0.0f ? kTop / big : 0.0f;
+  }
+  // The digits of 16 elements, the highest first: bytes of x + 0x80 (0x8080), of which all but the highest are 0x80 off.
+  __device__ __forceinline__ void digits(const float (&q)[16], u32x4 (&o)[NP]) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t y[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float v = q[4 * i + e] * up * to;
+        if constexpr (BF16)
+          y[e] = __float_as_uint(v + (12582912.0f + 128.0f));   // 1.5 * 2^23: the whole number stands in the lowest bits
+        else
+          y[e] = (uint32_t)((int)__builtin_rintf(v) + 0x8080);
+      }
+#pragma unroll
+      for (int p = 0; p < NP; ++p) {
+        const uint32_t sel = NP - 1 - p, two = 0x0c0c0000u | (sel + 4) << 8 | sel;
+        const uint32_t t = __builtin_amdgcn_perm(__builtin_amdgcn_perm(y[3], y[2], two), __builtin_amdgcn_perm(y[1], y[0], two), 0x05040100u);
+        o[p][i] = p == 0 ? t : t ^ 0x80808080u;
+      }
+    }
+  }
+};
+__device__ __forceinline__ uint32_t larger_bits(uint32_t top, float x) { return max(top, __float_as_uint(x) & 0x7fffffffu); }
+// 16 neighbours of a row of queries
+template <bool BF16>
+__device__ __forceinline__ void load16(const char* p, float (&x)[16]) {
+#pragma unroll
+  for (int i = 0; i < (BF16 ? 2 : 4); ++i) {
+    const u32x4 v = *as_global(reinterpret_cast<const u32x4*>(p) + i);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      if constexpr (BF16)
+        x[8 * i + 2 * c] = __uint_as_float(v[c] << 16), x[8 * i + 2 * c + 1] = __uint_as_float(v[c] & 0xffff0000u);
+      else
+        x[4 * i + c] = __uint_as_float(v[c]);
+    }
+  }
 }
 
 // Byte B of x, signed, as a float, in one instruction (the compiler takes three).
@@ -56,7 +103,7 @@ __device__ __forceinline__ void each(F f) {
 // out 2^-16 of it at most (bfloat16), or three, which leave out nothing (fp32).  V's codes are widened in registers, 1.5 instructions an element.
 template <bool BF16, int D>
 __global__ __launch_bounds__(256, 2) void attn_i8_split_kernel(const AttnI8 a) {
-  constexpr int NP = BF16 ? 2 : 3;        // digits of Q, parts of P
+  constexpr int NP = Row<BF16>::NP;       // digits of Q, parts of P
   constexpr int NS = D / 64;              // 16-byte pieces of a K row in a lane
   constexpr int VB = D / 16;              // bytes of a V row in a lane
   constexpr int NT = D / 16, E = BF16 ? 2 : 4;
@@ -114,22 +161,11 @@ __global__ __launch_bounds__(256, 2) void attn_i8_split_kernel(const AttnI8 a) {
 
   // Q's digits: wave s forms those of elements 64 s + 16 g .. of row j
   float qv[16];
-  uint32_t top = 0;   // of the magnitudes' bits: infinities and NaN are the largest
+  uint32_t top = 0;
   if (wave < NS) {
-    const char* qp = static_cast<const char*>(a.q.p) + ((at.sp.start + tok) * a.q.ld + hq * a.q.hs + 64 * wave + 16 * g) * E;
+    load16<BF16>(static_cast<const char*>(a.q.p) + ((at.sp.start + tok) * a.q.ld + hq * a.q.hs + 64 * wave + 16 * g) * E, qv);
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-      const u32x4 v = *as_global(reinterpret_cast<const u32x4*>(qp) + i);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        if constexpr (BF16)
-          qv[8 * i + 2 * c] = __uint_as_float(v[c] << 16), qv[8 * i + 2 * c + 1] = __uint_as_float(v[c] & 0xffff0000u);
-        else
-          qv[4 * i + c] = __uint_as_float(v[c]);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(qv[i]) & 0x7fffffffu);
+    for (int i = 0; i < 16; ++i) top = larger_bits(top, qv[i]);
     top = max(top, (uint32_t)xor_perm_i<16>((int)top));
     top = max(top, (uint32_t)xor_perm_i<32>((int)top));
     if (g == 0) ltop[wave][j] = top;
@@ -137,23 +173,12 @@ __global__ __launch_bounds__(256, 2) void attn_i8_split_kernel(const AttnI8 a) {
   __syncthreads();
 #pragma unroll
   for (int s = 0; s < NS; ++s) top = max(top, ltop[s][j]);
-  constexpr int kTop = BF16 ? kTop2 : kTop3;
-  // (a row of very small elements is moved up first: kTop / its largest would overflow)
-  const float up = top < 0x20000000u ? 0x1p64f : 1.0f, big = __uint_as_float(top) * up;   // 0x20000000: 2^-63
-  const float unit = top >= 0x7f800000u ? __builtin_nanf("") : big / (float)kTop / up, to = big > 0.0f ? (float)kTop / big : 0.0f;
+  const Row<BF16> qr(top);
   if (wave < NS) {
-    int x[16];
+    u32x4 v[NP];
+    qr.digits(qv, v);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = (int)__builtin_rintf(fminf(fmaxf(qv[i] * up * to, -(float)kTop), (float)kTop));
-#pragma unroll
-    for (int p = NP - 1; p >= 0; --p) {   // the lowest digit first; what is left is a multiple of 256
-      u32x4 v;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = bytes4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
-      lq[wave][p][lane] = v;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] = (x[i] + 128) >> 8;
-    }
+    for (int p = 0; p < NP; ++p) lq[wave][p][lane] = v[p];
   }
   __syncthreads();
 
@@ -161,7 +186,7 @@ __global__ __launch_bounds__(256, 2) void attn_i8_split_kernel(const AttnI8 a) {
 #pragma unroll
   for (int t = 0; t < NT; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   float m = kNegInf, l = 0.0f;
-  const float fac = unit * (a.scale * kLog2e);
+  const float fac = qr.unit * (a.scale * kLog2e);
   const int lim = min(seen, k1);
   for (; kb < k1; kb += 128) {
     lsc[wave][lane] = sc;
@@ -230,7 +255,6 @@ __global__ __launch_bounds__(256, 2) void attn_i8_split_kernel(const AttnI8 a) {
         x -= __uint_as_float(u & 0xffff0000u);
         y -= __uint_as_float(w & 0xffff0000u);
       }
-      typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
       const bf16x2 last = {(__bf16)x, (__bf16)y};
       pb[NP - 1][d] = __builtin_bit_cast(uint32_t, last);
     }
@@ -307,9 +331,336 @@ __global__ __launch_bounds__(256, 2) void attn_i8_split_kernel(const AttnI8 a) {
   }
 }
 
+// 4 bytes per lane from base + off to LDS at `to` + 4 lane (see load_to_lds)
+__device__ __forceinline__ void load_word_to_lds(const float* base, uint32_t off, uint32_t to) {
+  asm volatile("s_nop 0\n\tglobal_load_lds_dword %1, %2" ::"{m0}"(__builtin_amdgcn_readfirstlane(to)), "v"(off), "s"(base) : "memory");
+}
+
+// Prompts: a workgroup takes 256 rows (fp32: 128; tokens x query heads of one kv head) over all the keys they see, 32
+// (16) rows a wave, with the products of the form for few rows.  Keys come 8 KB of codes at a time (a stage: 32 keys of 256
+// elements, 64 of 128) by global -> LDS loads, three stages ahead.  K's codes stay codes; V's are widened to bfloat16 once a
+// workgroup, one stage ahead, by the wave that loaded them.  16-byte chunk c of K's row r stands at chunk c ^ (r % 16) (128
+// elements: c ^ (r / 2 % 8)), so that 16 keys of one chunk lie in all banks, and chunk c of V's widened row r at c ^ (4 (r % 4) + 2 (r / 4 % 2)),
+// as the transposing reads take four keys of 32 elements or eight of 16.  P (times V's scales) is rounded to bfloat16 once for
+// bfloat16 (2^-8 of sum p |v|) and taken in three parts for fp32 (exact).
+template <bool BF16, int D>
+__global__ __launch_bounds__(512, 2) void attn_i8_tile_kernel(const AttnI8 a) {
+  constexpr int E = BF16 ? 2 : 4, kTile = tile_rows(BF16), NR = kTile / 8, NP = Row<BF16>::NP;
+  constexpr int SK = 8192 / D, CH = D / 16, kRing = 4;    // keys of a stage; 16-byte chunks of a row of codes
+  constexpr int kWide = 16384, kScales = 512;             // bytes of a stage's widened V, of its scales (K's, V's 256 bytes on)
+  constexpr int LR = 64 / NR, FB = 16 * LR;               // lanes of a row; its elements in a fragment of K and Q
+  constexpr int NF = D / FB, NT = D / NR, VW = BF16 ? 16 : 4, MT = 32 / NR;   // fragments; accumulators, their elements; of 32 keys
+  constexpr int NQ = NT * VW / 4, PP = BF16 ? 1 : 3;      // quads of a lane's output; parts of P
+  constexpr bool kChain = BF16 && D == 256;               // one digit's sums after the other's in the same registers (K read twice)
+  typedef std::conditional_t<BF16, f32x16, f32x4> fvec;
+  typedef std::conditional_t<BF16, i32x16, i32x4> ivec;
+  __shared__ __attribute__((aligned(256))) char lds[kRing * 16384 + 2 * kWide + kRing * kScales];
+  constexpr int kRaw = kRing * 8192, kV = 2 * kRaw, kS = kV + 2 * kWide;      // V's codes, widened V, scales
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int h = lane / NR, j = lane % NR;
+  const int G = a.heads / a.kv_heads;
+  const int kvh = (int)blockIdx.x % a.kv_heads;
+  TileUnit at;
+  if (!find_tile_unit<false, kTile>(a, (int)blockIdx.x / a.kv_heads, at)) return;
+  const int rows = at.sp.len * G, r0 = kTile * at.tile, w0 = r0 + NR * wave;
+  auto all = [&](int row) { return keys_seen(min(row, rows - 1) / G, at.sp.len, at.kl); };
+  const int piece = unit_keys(all(r0 + kTile - 1), at.nsplit), k0 = at.split * piece;   // keys are counted from here
+  auto sees = [&](int row) { return all(row) - k0; };
+  const int end = min(sees(r0 + kTile - 1), piece), wend = w0 < rows ? min(sees(w0 + NR - 1), end) : 0;
+  if (at.split > 0 && end <= 0) return;   // (a unit of no key that the tile sees)
+
+  // A thread's place in a stage is row tid / CH, chunk tid % CH.  (What follows from the thread's number alone is formed where it
+  // is used, by tid_here: held over the loop it would not fit the registers.)
+  const char* kp = static_cast<const char*>(a.k.p) + (at.ks + k0) * a.k.ld + kvh * a.k.hs;
+  const char* vp = static_cast<const char*>(a.v.p) + (at.ks + k0) * a.v.ld + kvh * a.v.hs;
+  const uint32_t kld = (uint32_t)a.k.ld, vld = (uint32_t)a.v.ld;   // (below 2^24: the entry point's rule)
+  const uint32_t lds0 = lds_address(lds);
+  const bool scales = wave < 2;   // wave 0 brings K's scales, wave 1 V's
+  const float* sp = wave == 0 ? a.ks + (at.ks + k0) * a.ldks + kvh * a.hsks : a.vs + (at.ks + k0) * a.ldvs + kvh * a.hsvs;
+  const int64_t sld = wave == 0 ? a.ldks : a.ldvs;
+  auto stage = [&](int it) {
+    const int t = tid_here(), pr = t / CH, pc = t % CH, last = end - 1 - SK * it, slot = it & (kRing - 1);   // last: the last row that is there
+    const uint32_t r = min(pr, last), kc = 16 * (pc ^ (D == 256 ? pr & 15 : (pr >> 1) & 7)), vc = 16 * pc;
+    load_to_lds(kp + (int64_t)it * SK * a.k.ld, __umul24(r, kld) + kc, lds0 + slot * 8192 + 1024 * wave);
+    load_to_lds(vp + (int64_t)it * SK * a.v.ld, __umul24(r, vld) + vc, lds0 + kRaw + slot * 8192 + 1024 * wave);
+    if (scales)
+      load_word_to_lds(sp + it * SK * sld, 4 * __umul24(min(t % SK, last), (uint32_t)sld), lds0 + kS + slot * kScales + 256 * wave);
+  };
+  const int n = seq_tiles(end, SK);
+#pragma unroll
+  for (int i = 0; i < kRing - 1; ++i)
+    if (i < n) stage(i);
+
+  // Q's digits: a lane has elements FB s + 16 h .. of row j
+  const int row = min(w0 + j, rows - 1), tok = row / G, hq = kvh * G + row % G;
+  const int seen = sees(row);
+  u32x4 qf[NF][NP];
+  float fac;
+  {
+    const char* qp = static_cast<const char*>(a.q.p) + ((at.sp.start + tok) * a.q.ld + hq * a.q.hs + 16 * h) * E;
+    uint32_t top = 0;
+#pragma unroll
+    for (int s = 0; s < NF; ++s) {
+      float x[16];
+      load16<BF16>(qp + FB * E * s, x);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = larger_bits(top, x[i]);
+    }
+    if constexpr (!BF16) top = max(top, (uint32_t)xor_perm_i<16>((int)top));
+    top = max(top, (uint32_t)xor_perm_i<32>((int)top));
+    Row<BF16> qr(top);
+    fac = qr.unit * (fabsf(a.scale) * kLog2e);
+    if (a.scale < 0.0f) qr.to = -qr.to;   // (-q) k |scale|: a maximum stays one
+#pragma unroll
+    for (int s = 0; s < NF; ++s) {        // (read again: held over the maximum they would not fit the registers)
+      float x[16];
+      load16<BF16>(qp + FB * E * s, x);
+      qr.digits(x, qf[s]);
+    }
+  }
+
+  fvec acc[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) acc[t] = fvec{};
+  float m = kNegInf, l = 0.0f;
+  // this wave's loads of stage `it` have landed (those of the next `after` stages stay in flight)
+  auto landed = [&](int after) {
+    if (after >= 2) {
+      if (scales) asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
+      else asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+    } else if (after == 1) {
+      if (scales) asm volatile("s_waitcnt vmcnt(3)" ::: "memory");
+      else asm volatile("s_waitcnt vmcnt(2)" ::: "memory");
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+  };
+  auto widen_stage = [&](int it) {
+    const int tid = tid_here(), pr = tid / CH, pc = tid % CH;
+    const uint32_t vw = lds0 + kV + pr * D * 2 + ((32 * pc) ^ (64 * (pr & 3) + 32 * ((pr >> 2) & 1)));
+    const u32x4 x = *lds_at<u32x4>(lds0 + kRaw + (it & (kRing - 1)) * 8192 + 16 * tid);
+    u32x4 o[2];
+    each<8>([&](auto I) {
+      constexpr int i = I, d = i / 2, b = 2 * (i % 2);
+      o[i / 4][i % 4] = __builtin_amdgcn_perm(code_float<b + 1>(x[d]), code_float<b>(x[d]), 0x07060302u);
+    });
+    *lds_at<u32x4>(vw + (it & 1) * kWide) = o[0];
+    *lds_at<u32x4>(vw + (it & 1) * kWide + 16) = o[1];
+  };
+  auto barrier = [&]() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+
+  // a lane holds four neighbours of its row from place(i) on, i below NQ
+  auto place = [&](int i) { return BF16 ? 32 * (i >> 2) + 8 * (i & 3) + 4 * h : 16 * i + 4 * h; };
+  // 32 keys, from key 32 u of stage `it` on.  PART: some row may see them only in part.
+  auto step = [&](int it, int u, auto PART) {
+    constexpr bool part = decltype(PART)::value;
+    const int kb = SK * it + 32 * u;
+    const int t6 = tid_here() & 63, h = t6 / NR, j = t6 % NR;
+    const uint32_t kl = lds0 + (it & (kRing - 1)) * 8192 + (32 * u + j) * D + 16 * (h ^ (D == 256 ? j & 15 : (j >> 1) & 7));
+    const uint32_t sl = lds0 + kS + (it & (kRing - 1)) * kScales + 128 * u + 16 * h;
+    // Fragments are on their way ahead of the products they are for, and no more of them than fit the registers.
+    ivec dg[kChain ? 1 : NP][MT] = {};
+    auto k_frag = [&](int s, int t) { return *lds_at<i32x4>((kl ^ (FB * s)) + 16 * D * t); };
+    auto product = [&](const i32x4& k, const u32x4& q, ivec& o) {
+      if constexpr (BF16)
+        o = __builtin_amdgcn_mfma_i32_32x32x32_i8(k, __builtin_bit_cast(i32x4, q), o, 0, 0, 0);
+      else
+        o = __builtin_amdgcn_mfma_i32_16x16x64_i8(k, __builtin_bit_cast(i32x4, q), o, 0, 0, 0);
+    };
+    if constexpr (kChain) {
+#pragma unroll
+      for (int p = 0; p < NP; ++p) {
+        if (p > 0) dg[0][0] *= 256;
+#pragma unroll
+        for (int s = 0; s < NF; ++s) product(k_frag(s, 0), qf[s][p], dg[0][0]);
+        __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
+#pragma unroll
+        for (int i = 0; i < NF - 3; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x8, 3, 0);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    } else {
+#pragma unroll
+      for (int s = 0; s < NF; ++s)
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+          const i32x4 kf = k_frag(s, t);
+#pragma unroll
+          for (int p = 0; p < NP; ++p) product(kf, qf[s][p], dg[p][t]);
+        }
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+#pragma unroll
+      for (int i = 0; i < NF * MT - 2; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x8, NP, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x8, 2 * NP, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    // score 4 i + r is of key 8 i + 4 h + r (fp32: 16 i + 4 h + r)
+    constexpr int NK = BF16 ? 4 : 2, KS = 32 / NK;
+    float st[4 * NK];
+#pragma unroll
+    for (int i = 0; i < NK; ++i) {
+      const f32x4 ks = *lds_at<f32x4>(sl + 4 * KS * i);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        auto d = [&](int p) { return BF16 ? dg[kChain ? 0 : p][0][4 * i + r] : dg[kChain ? 0 : p][i % MT][r]; };
+        // (the row's unit first: a sum of digits times a large scale could overflow)
+        float x = (float)(kChain ? d(0) : d(0) * 256 + d(1)) * (BF16 ? fac : 256.0f * fac);   // of a whole number below 2^30
+        if constexpr (!BF16) x = __builtin_fmaf((float)d(NP - 1), fac, x);
+        st[4 * i + r] = x * ks[r];
+        if (part && kb + KS * i + 4 * h + r >= seen) st[4 * i + r] = kNegInf;
+      }
+    }
+    float mt = st[0];
+#pragma unroll
+    for (int r = 1; r < 4 * NK; ++r) mt = fmaxf(mt, st[r]);
+    if constexpr (!BF16) mt = fmaxf(mt, xor_perm<16>(mt));
+    mt = fmaxf(mt, xor_perm<32>(mt));
+    const bool up = mt > m + 8.0f;                       // (as in the form for few rows)
+    if (__ballot(up) != 0) {
+      const float mn = up ? mt : m, al = __builtin_amdgcn_exp2f(m - (mn == kNegInf ? 0.0f : mn));
+      m = mn;
+      l *= al;
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < VW; ++r) acc[t][r] *= al;
+    }
+    const float mu = m == kNegInf ? 0.0f : m;
+    float ps = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NK; ++i) {
+      const f32x4 vs = *lds_at<f32x4>(sl + 256 + 4 * KS * i);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float p = __builtin_amdgcn_exp2f(st[4 * i + r] - mu);
+        const bool hidden = part && kb + KS * i + 4 * h + r >= seen;
+        ps += p;
+        st[4 * i + r] = hidden ? 0.0f : p * vs[r];   // (a hidden row's scale may be anything)
+      }
+    }
+    l += ps;
+    u32x4 pf[PP][NK / 2];
+#pragma unroll
+    for (int d = 0; d < 2 * NK; ++d) {
+      float x = st[2 * d], y = st[2 * d + 1];
+#pragma unroll
+      for (int p = 0; p < PP - 1; ++p) {   // cut: what is left is exact
+        const uint32_t u0 = __float_as_uint(x), u1 = __float_as_uint(y);
+        pf[p][d >> 2][d & 3] = __builtin_amdgcn_perm(u1, u0, 0x07060302u);
+        x -= __uint_as_float(u0 & 0xffff0000u);
+        y -= __uint_as_float(u1 & 0xffff0000u);
+      }
+      const bf16x2 lastp = {(__bf16)x, (__bf16)y};
+      pf[PP - 1][d >> 2][d & 3] = __builtin_bit_cast(uint32_t, lastp);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    const int t7 = tid_here() & 63, vh = t7 / NR, vx = (t7 & 15) >> 2;   // vx: the key of four that this lane's transposing read brings
+    const uint32_t vl = lds0 + kV + (it & 1) * kWide + (32 * u + 4 * vh + vx) * D * 2 +
+                        ((BF16 ? 32 * ((t7 >> 4) & 1) : 0) ^ (64 * vx + 32 * (vh & 1))) + 16 * ((t7 & 3) >> 1) + 8 * (t7 & 1);
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int kk = 0; kk < NK / 2; ++kk) {
+        // bfloat16: keys 16 kk + 4 h .., + 8 of element 32 t + lane % 32; fp32: 4 h .., + 16 of 16 t + lane % 16
+        const uint32_t p = (BF16 ? (vl ^ (64 * (t & 3))) + 256 * (t >> 2) : (vl ^ (32 * (t & 7))) + 256 * (t >> 3)) + 32 * D * kk;
+        union {
+          i16x4 q[2];
+          bf16x8 v;
+        } w;
+#pragma unroll
+        for (int q = 0; q < 2; ++q) w.q[q] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_at<i16x4>(p + (BF16 ? 16 : 32) * D * q));
+#pragma unroll
+        for (int i = PP - 1; i >= 0; --i) {
+          if constexpr (BF16)
+            acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w.v, __builtin_bit_cast(bf16x8, pf[i][kk]), acc[t], 0, 0, 0);
+          else
+            acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.v, __builtin_bit_cast(bf16x8, pf[i][kk]), acc[t], 0, 0, 0);
+        }
+      }
+    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+    for (int i = 0; i < NT * NK / 2 - 2; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x8, PP, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x8, 2 * PP, 0);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto ahead = [&](int it) {
+    if (it + 1 < n) {
+      landed(min(n - 2 - it, 1));
+      widen_stage(it + 1);
+    }
+    if (it + kRing - 1 < n) stage(it + kRing - 1);   // (where stage it - 1 was, which every wave is done with)
+  };
+  const int full = max(min(sees(r0), end), 0) / SK;  // stages that every row sees whole
+  if (n > 0) {
+    landed(min(n - 1, 2));
+    widen_stage(0);
+    barrier();
+  }
+  int it = 0;
+  for (; it < full; ++it) {
+    ahead(it);
+#pragma unroll
+    for (int u = 0; u < SK / 32; ++u) step(it, u, std::false_type{});
+    barrier();
+  }
+  for (; it < n; ++it) {
+    ahead(it);
+#pragma unroll
+    for (int u = 0; u < SK / 32; ++u)
+      if (SK * it + 32 * u < wend) step(it, u, std::true_type{});
+    barrier();
+  }
+  if constexpr (!BF16) l = l + xor_perm<16>(l);
+  l = l + xor_perm<32>(l);
+  if (w0 + j >= rows) return;
+  auto quad = [&](int i) {
+    if constexpr (BF16)
+      return f32x4{acc[i >> 2][4 * (i & 3)], acc[i >> 2][4 * (i & 3) + 1], acc[i >> 2][4 * (i & 3) + 2], acc[i >> 2][4 * (i & 3) + 3]};
+    else
+      return acc[i];
+  };
+  if (at.nsplit > 1) {
+    float* pp = a.part + ((size_t)at.slot * a.kv_heads + kvh) * tile_part_floats(kTile, D);
+    const int rr = row - r0;
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) *as_global_w(reinterpret_cast<f32x4*>(pp + rr * D + place(i))) = quad(i);
+    if (h == 0) pp[kTile * D + rr] = m, pp[kTile * D + kTile + rr] = l;
+    return;
+  }
+  const float inv = at.kl < 0 ? __builtin_nanf("") : seen <= 0 ? 0.0f : 1.0f / l;
+  char* op = static_cast<char*>(a.out.p) + ((at.sp.start + tok) * a.out.ld + hq * a.out.hs) * E;
+#pragma unroll
+  for (int i = 0; i < NQ; ++i) {
+    const f32x4 o = quad(i) * inv;
+    if constexpr (BF16)
+      *as_global_w(reinterpret_cast<bf16x4*>(op + place(i) * 2)) = bf16x4{(__bf16)o[0], (__bf16)o[1], (__bf16)o[2], (__bf16)o[3]};
+    else
+      *as_global_w(reinterpret_cast<f32x4*>(op + place(i) * 4)) = o;
+  }
+}
+
 template <bool BF16, int D>
 hipError_t launch(const AttnI8& a, hipStream_t s) {
-  const unsigned tiles = (unsigned)(seq_tiles_max((int64_t)a.q_rows * (a.heads / a.kv_heads), a.n_seq, 16) * a.kv_heads);
+  const int64_t rows = (int64_t)a.q_rows * (a.heads / a.kv_heads);
+  if (a.tile > 0) {
+    const int64_t t = seq_tiles_max(rows, a.n_seq, a.tile) * a.kv_heads;
+    attn_i8_tile_kernel<BF16, D><<<(unsigned)(t + a.limit), 512, 0, s>>>(a);
+    if (a.limit > 0) {
+      const int64_t split = std::min<int64_t>(t, a.limit / 2);
+      attn_tile_join_kernel<BF16, D><<<dim3((unsigned)split, (unsigned)std::clamp<int64_t>(1024 / split, 8, a.tile / 4)), 256, 0, s>>>(a);
+    }
+    return hipGetLastError();
+  }
+  const unsigned tiles = (unsigned)(seq_tiles_max(rows, a.n_seq, 16) * a.kv_heads);
   attn_i8_split_kernel<BF16, D><<<a.limit > 0 ? tiles + kFill : tiles, 256, 0, s>>>(a);
   if (a.limit > 0) attn_join_kernel<BF16, D><<<dim3(tiles, 4), 1024, 0, s>>>(a);
   return hipGetLastError();
@@ -318,10 +669,21 @@ hipError_t launch(const AttnI8& a, hipStream_t s) {
 }  // namespace
 
 AttnForm attn_i8_form(int64_t q_rows, int n_seq, int max_q, int max_k, int heads, int kv_heads, int dim, bool bf16) {
+  const int G = heads / kv_heads;
   AttnForm f = {0, 0, 0};
-  if (max_k > kMinChunk) {
+  const int64_t seen = q_rows * heads * std::max(max_k, 1);
+  if ((int64_t)max_q * G >= (bf16 ? 1024 : 2048) || ((int64_t)max_q * G >= 128 && seen >= 5000000)) {
+    f.tile = tile_rows(bf16);
+    const int64_t tiles = seq_tiles_max(q_rows * G, n_seq, f.tile) * kv_heads;
+    // two workspace places a CU: the chunks are such that more are hardly ever taken
+    if (max_k > min_tile_chunk(bf16)) {
+      const int64_t splits = max_k / min_tile_chunk(bf16) + 1;
+      f.limit = (int)std::min<int64_t>(2 * kCUs, tiles * std::min<int64_t>(splits, kMaxTileSplits));
+    }
+    f.bytes = (size_t)f.limit * tile_part_floats(f.tile, dim) * sizeof(float);
+  } else if (max_k > kMinChunk) {
     f.limit = 1;
-    f.bytes = (size_t)(seq_tiles_max(q_rows * (heads / kv_heads), n_seq, 16) * kv_heads + kFill) * part_floats(dim) * sizeof(float);
+    f.bytes = (size_t)(seq_tiles_max(q_rows * G, n_seq, 16) * kv_heads + kFill) * part_floats(dim) * sizeof(float);
   }
   return f;
 }
