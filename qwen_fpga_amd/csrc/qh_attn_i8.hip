@@ -88,9 +88,14 @@ __device__ __forceinline__ u32x4 widen(const V (&rows)[8]) {
     t[i] = __builtin_amdgcn_perm(code_float<C & 3>(rows[2 * i + 1][C >> 2]), code_float<C & 3>(rows[2 * i][C >> 2]), 0x07060302u);
   return t;
 }
+// Lane C's value of each 16 lanes (a modifier of the instruction that takes it).
+template <int C>
+__device__ __forceinline__ float lane_of_16(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x150 + C, 0xf, 0xf, true));   // row_newbcast
+}
 // f(0), f(1) .. f(N - 1) with constants
 template <int N, typename F>
-__device__ __forceinline__ void each(F f) {
+__device__ __forceinline__ void each(F&& f) {
   if constexpr (N > 0) {
     each<N - 1>(f);
     f(std::integral_constant<int, N - 1>{});
@@ -331,11 +336,6 @@ __global__ __launch_bounds__(256, 2) void attn_i8_split_kernel(const AttnI8 a) {
   }
 }
 
-// 4 bytes per lane from base + off to LDS at `to` + 4 lane (see load_to_lds)
-__device__ __forceinline__ void load_word_to_lds(const float* base, uint32_t off, uint32_t to) {
-  asm volatile("s_nop 0\n\tglobal_load_lds_dword %1, %2" ::"{m0}"(__builtin_amdgcn_readfirstlane(to)), "v"(off), "s"(base) : "memory");
-}
-
 // Prompts: a workgroup takes 256 rows (fp32: 128; tokens x query heads of one kv head) over all the keys they see, 32
 // (16) rows a wave, with the products of the form for few rows.  Keys come 8 KB of codes at a time (a stage: 32 keys of 256
 // elements, 64 of 128) by global -> LDS loads, three stages ahead.  K's codes stay codes; V's are widened to bfloat16 once a
@@ -349,12 +349,12 @@ __global__ __launch_bounds__(512, 2) void attn_i8_tile_kernel(const AttnI8 a) {
   constexpr int SK = 8192 / D, CH = D / 16, kRing = 4;    // keys of a stage; 16-byte chunks of a row of codes
   constexpr int kWide = 16384, kScales = 512;             // bytes of a stage's widened V, of its scales (K's, V's 256 bytes on)
   constexpr int LR = 64 / NR, FB = 16 * LR;               // lanes of a row; its elements in a fragment of K and Q
-  constexpr int NF = D / FB, NT = D / NR, VW = BF16 ? 16 : 4, MT = 32 / NR;   // fragments; accumulators, their elements; of 32 keys
+  constexpr int NF = D / FB, NT = D / NR, VW = BF16 ? 16 : 4;   // fragments; accumulators, their elements
+  constexpr int NM = SK / NR, NK = SK / (2 * LR) / 2;     // tiles of a stage's scores; quads of scores of a lane
   constexpr int NQ = NT * VW / 4, PP = BF16 ? 1 : 3;      // quads of a lane's output; parts of P
-  constexpr bool kChain = BF16 && D == 256;               // one digit's sums after the other's in the same registers (K read twice)
   typedef std::conditional_t<BF16, f32x16, f32x4> fvec;
   typedef std::conditional_t<BF16, i32x16, i32x4> ivec;
-  __shared__ __attribute__((aligned(256))) char lds[kRing * 16384 + 2 * kWide + kRing * kScales];
+  __shared__ __attribute__((aligned(256))) char lds[kRing * 16384 + 2 * kWide + 2 * kRing * kScales];
   constexpr int kRaw = kRing * 8192, kV = 2 * kRaw, kS = kV + 2 * kWide;      // V's codes, widened V, scales
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int h = lane / NR, j = lane % NR;
@@ -366,7 +366,7 @@ __global__ __launch_bounds__(512, 2) void attn_i8_tile_kernel(const AttnI8 a) {
   auto all = [&](int row) { return keys_seen(min(row, rows - 1) / G, at.sp.len, at.kl); };
   const int piece = unit_keys(all(r0 + kTile - 1), at.nsplit), k0 = at.split * piece;   // keys are counted from here
   auto sees = [&](int row) { return all(row) - k0; };
-  const int end = min(sees(r0 + kTile - 1), piece), wend = w0 < rows ? min(sees(w0 + NR - 1), end) : 0;
+  const int end = min(sees(r0 + kTile - 1), piece);
   if (at.split > 0 && end <= 0) return;   // (a unit of no key that the tile sees)
 
   // A thread's place in a stage is row tid / CH, chunk tid % CH.  (What follows from the thread's number alone is formed where it
@@ -378,13 +378,13 @@ __global__ __launch_bounds__(512, 2) void attn_i8_tile_kernel(const AttnI8 a) {
   const bool scales = wave < 2;   // wave 0 brings K's scales, wave 1 V's
   const float* sp = wave == 0 ? a.ks + (at.ks + k0) * a.ldks + kvh * a.hsks : a.vs + (at.ks + k0) * a.ldvs + kvh * a.hsvs;
   const int64_t sld = wave == 0 ? a.ldks : a.ldvs;
-  auto stage = [&](int it) {
-    const int t = tid_here(), pr = t / CH, pc = t % CH, last = end - 1 - SK * it, slot = it & (kRing - 1);   // last: the last row that is there
-    const uint32_t r = min(pr, last), kc = 16 * (pc ^ (D == 256 ? pr & 15 : (pr >> 1) & 7)), vc = 16 * pc;
+  auto stage = [&](int it) __attribute__((always_inline)) {
+    const int last = end - 1 - SK * it, slot = it & (kRing - 1);   // last: the last row that is there
+    const uint32_t t = tid_here(), pr = t / CH, pc = t % CH, r = min(pr, (uint32_t)last), kc = 16 * (pc ^ (D == 256 ? pr & 15 : (pr >> 1) & 7)), vc = 16 * pc;
     load_to_lds(kp + (int64_t)it * SK * a.k.ld, __umul24(r, kld) + kc, lds0 + slot * 8192 + 1024 * wave);
     load_to_lds(vp + (int64_t)it * SK * a.v.ld, __umul24(r, vld) + vc, lds0 + kRaw + slot * 8192 + 1024 * wave);
     if (scales)
-      load_word_to_lds(sp + it * SK * sld, 4 * __umul24(min(t % SK, last), (uint32_t)sld), lds0 + kS + slot * kScales + 256 * wave);
+      load_word_to_lds(sp + it * SK * sld, 4 * __umul24(min(t % SK, (uint32_t)last), (uint32_t)sld), lds0 + kS + (it & (2 * kRing - 1)) * kScales + 256 * wave);
   };
   const int n = seq_tiles(end, SK);
 #pragma unroll
@@ -393,7 +393,7 @@ __global__ __launch_bounds__(512, 2) void attn_i8_tile_kernel(const AttnI8 a) {
 
   // Q's digits: a lane has elements FB s + 16 h .. of row j
   const int row = min(w0 + j, rows - 1), tok = row / G, hq = kvh * G + row % G;
-  const int seen = sees(row);
+  const int seen = min(sees(row), end);   // (a unit may end inside a stage)
   u32x4 qf[NF][NP];
   float fac;
   {
@@ -424,7 +424,7 @@ __global__ __launch_bounds__(512, 2) void attn_i8_tile_kernel(const AttnI8 a) {
   for (int t = 0; t < NT; ++t) acc[t] = fvec{};
   float m = kNegInf, l = 0.0f;
   // this wave's loads of stage `it` have landed (those of the next `after` stages stay in flight)
-  auto landed = [&](int after) {
+  auto landed = [&](int after) __attribute__((always_inline)) {
     if (after >= 2) {
       if (scales) asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
       else asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
@@ -435,92 +435,115 @@ __global__ __launch_bounds__(512, 2) void attn_i8_tile_kernel(const AttnI8 a) {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
   };
-  auto widen_stage = [&](int it) {
-    const int tid = tid_here(), pr = tid / CH, pc = tid % CH;
-    const uint32_t vw = lds0 + kV + pr * D * 2 + ((32 * pc) ^ (64 * (pr & 3) + 32 * ((pr >> 2) & 1)));
-    const u32x4 x = *lds_at<u32x4>(lds0 + kRaw + (it & (kRing - 1)) * 8192 + 16 * tid);
-    u32x4 o[2];
-    each<8>([&](auto I) {
-      constexpr int i = I, d = i / 2, b = 2 * (i % 2);
-      o[i / 4][i % 4] = __builtin_amdgcn_perm(code_float<b + 1>(x[d]), code_float<b>(x[d]), 0x07060302u);
-    });
-    *lds_at<u32x4>(vw + (it & 1) * kWide) = o[0];
-    *lds_at<u32x4>(vw + (it & 1) * kWide + 16) = o[1];
-  };
   auto barrier = [&]() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
 
   // a lane holds four neighbours of its row from place(i) on, i below NQ
   auto place = [&](int i) { return BF16 ? 32 * (i >> 2) + 8 * (i & 3) + 4 * h : 16 * i + 4 * h; };
-  // 32 keys, from key 32 u of stage `it` on.  PART: some row may see them only in part.
-  auto step = [&](int it, int u, auto PART) {
-    constexpr bool part = decltype(PART)::value;
-    const int kb = SK * it + 32 * u;
-    const int t6 = tid_here() & 63, h = t6 / NR, j = t6 % NR;
-    const uint32_t kl = lds0 + (it & (kRing - 1)) * 8192 + (32 * u + j) * D + 16 * (h ^ (D == 256 ? j & 15 : (j >> 1) & 7));
-    const uint32_t sl = lds0 + kS + (it & (kRing - 1)) * kScales + 128 * u + 16 * h;
-    // Fragments are on their way ahead of the products they are for, and no more of them than fit the registers.
-    ivec dg[kChain ? 1 : NP][MT] = {};
-    auto k_frag = [&](int s, int t) { return *lds_at<i32x4>((kl ^ (FB * s)) + 16 * D * t); };
-    auto product = [&](const i32x4& k, const u32x4& q, ivec& o) {
-      if constexpr (BF16)
-        o = __builtin_amdgcn_mfma_i32_32x32x32_i8(k, __builtin_bit_cast(i32x4, q), o, 0, 0, 0);
-      else
-        o = __builtin_amdgcn_mfma_i32_16x16x64_i8(k, __builtin_bit_cast(i32x4, q), o, 0, 0, 0);
+  constexpr int KS = 4 * LR;   // a lane's quad i of scores is of the keys KS i + 4 h ..
+  // A turn at the matrix pipe: O^T += V^T P^T of stage it - 1 (not in the FIRST turn), and S^T of stage it, digit by digit, if
+  // there is one (not in the LAST); between the products the thread's 16 codes of stage it of V are widened.  The
+  // fragments of V and K come from LDS kAhead products before they are used: the order is the program's, which the
+  // compiler left to itself does not keep (it waited for each fragment right after asking for it).
+  constexpr int kAhead = 3, NV = NT * NK / 2, NKF = NF * NM;
+  ivec dg[NP][NM];
+  u32x4 pf[PP][NK / 2];
+  auto matrix = [&](int it, auto FIRST, auto LAST) __attribute__((always_inline)) {
+    constexpr bool first = decltype(FIRST)::value, last = decltype(LAST)::value;
+    constexpr int i0 = first ? NV : 0, i1 = last ? NV : NV + NKF;
+    const uint32_t tid = tid_here(), ln = tid & 63, h = ln / NR, j = ln % NR, vx = (ln & 15) >> 2;   // vx: the key of four that this lane's transposing read brings
+    const uint32_t kl = lds0 + (it & (kRing - 1)) * 8192 + j * D + 16 * (h ^ (D == 256 ? j & 15 : (j >> 1) & 7));
+    const uint32_t vl = lds0 + kV + ((it - 1) & 1) * kWide + (4 * h + vx) * D * 2 +
+                        ((BF16 ? 32 * ((ln >> 4) & 1) : 0) ^ (64 * vx + 32 * (h & 1))) + 16 * ((ln & 3) >> 1) + 8 * (ln & 1);
+    u32x4 f[kAhead], codes, o;
+    auto ask = [&](auto I, u32x4& to) __attribute__((always_inline)) {
+      constexpr int i = I;
+      if constexpr (i < NV) {
+        // tile t of the elements, keys 16 kk + 4 h .., + 8 of element 32 t + lane % 32 (fp32: 32 kk + 4 h .., + 16 of 16 t + lane % 16)
+        constexpr int t = i / (NK / 2), kk = i % (NK / 2);
+        const uint32_t p = (BF16 ? (vl ^ (64 * (t & 3))) + 256 * (t >> 2) : (vl ^ (32 * (t & 7))) + 256 * (t >> 3)) + 4 * KS * D * kk;
+        union {
+          i16x4 q[2];
+          u32x4 v;
+        } w;
+        w.q[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_at<i16x4>(p));
+        w.q[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_at<i16x4>(p + 2 * KS * D));
+        to = w.v;
+      } else {
+        constexpr int s = (i - NV) / NM, t = (i - NV) % NM;
+        to = *lds_at<u32x4>((kl ^ (FB * s)) + NR * D * t);
+      }
     };
-    if constexpr (kChain) {
-#pragma unroll
-      for (int p = 0; p < NP; ++p) {
-        if (p > 0) dg[0][0] *= 256;
-#pragma unroll
-        for (int s = 0; s < NF; ++s) product(k_frag(s, 0), qf[s][p], dg[0][0]);
-        __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
-#pragma unroll
-        for (int i = 0; i < NF - 3; ++i) {
-          __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-        }
-        __builtin_amdgcn_sched_group_barrier(0x8, 3, 0);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    } else {
-#pragma unroll
-      for (int s = 0; s < NF; ++s)
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-          const i32x4 kf = k_frag(s, t);
-#pragma unroll
-          for (int p = 0; p < NP; ++p) product(kf, qf[s][p], dg[p][t]);
-        }
-      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-#pragma unroll
-      for (int i = 0; i < NF * MT - 2; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x8, NP, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      }
-      __builtin_amdgcn_sched_group_barrier(0x8, 2 * NP, 0);
-    }
+    if constexpr (!last) codes = *lds_at<u32x4>(lds0 + kRaw + (it & (kRing - 1)) * 8192 + 16 * tid);
+    each<kAhead>([&](auto I) { ask(std::integral_constant<int, i0 + I>{}, f[(i0 + I) % kAhead]); });
+    const uint32_t pr = tid / CH, pc = tid % CH;
+    const uint32_t vw = lds0 + kV + (it & 1) * kWide + pr * D * 2 + ((32 * pc) ^ (64 * (pr & 3) + 32 * ((pr >> 2) & 1)));
     __builtin_amdgcn_sched_barrier(0);
-    // score 4 i + r is of key 8 i + 4 h + r (fp32: 16 i + 4 h + r)
-    constexpr int NK = BF16 ? 4 : 2, KS = 32 / NK;
-    float st[4 * NK];
+    each<i1 - i0>([&](auto I) {
+      constexpr int i = i0 + I;
+      u32x4& x = f[i % kAhead];
+      if constexpr (i < NV) {
+        constexpr int t = i / (NK / 2), kk = i % (NK / 2);
 #pragma unroll
-    for (int i = 0; i < NK; ++i) {
-      const f32x4 ks = *lds_at<f32x4>(sl + 4 * KS * i);
+        for (int p = PP - 1; p >= 0; --p) {
+          if constexpr (BF16)
+            acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, pf[p][kk]), acc[t], 0, 0, 0);
+          else
+            acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, pf[p][kk]), acc[t], 0, 0, 0);
+        }
+      } else {
+        constexpr int s = (i - NV) / NM, t = (i - NV) % NM;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        auto d = [&](int p) { return BF16 ? dg[kChain ? 0 : p][0][4 * i + r] : dg[kChain ? 0 : p][i % MT][r]; };
-        // (the row's unit first: a sum of digits times a large scale could overflow)
-        float x = (float)(kChain ? d(0) : d(0) * 256 + d(1)) * (BF16 ? fac : 256.0f * fac);   // of a whole number below 2^30
-        if constexpr (!BF16) x = __builtin_fmaf((float)d(NP - 1), fac, x);
-        st[4 * i + r] = x * ks[r];
-        if (part && kb + KS * i + 4 * h + r >= seen) st[4 * i + r] = kNegInf;
+        for (int p = 0; p < NP; ++p) {
+          const ivec c = s == 0 ? ivec{} : dg[p][t];
+          if constexpr (BF16)
+            dg[p][t] = __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4, x), __builtin_bit_cast(i32x4, qf[s][p]), c, 0, 0, 0);
+          else
+            dg[p][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, x), __builtin_bit_cast(i32x4, qf[s][p]), c, 0, 0, 0);
+        }
       }
-    }
+      if constexpr (i + kAhead < i1) ask(std::integral_constant<int, i + kAhead>{}, x);
+      // a dword of widened codes after a product, four to a store
+      constexpr int d = I - (first ? 0 : 3);
+      static_assert(last || i1 - i0 >= (first ? 8 : 11), "a product for each dword");
+      if constexpr (!last && d >= 0 && d < 8) {
+        constexpr int b = 2 * (d % 2);
+        o[d % 4] = __builtin_amdgcn_perm(code_float<b + 1>(codes[d / 2]), code_float<b>(codes[d / 2]), 0x07060302u);
+        if constexpr (d % 4 == 3) *lds_at<u32x4>(vw + 16 * (d / 4)) = o;
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  };
+  // The scales of a stage: each 16 lanes hold those of their scores, lane c of them score 16 q + c's in register q.
+  constexpr int NSC = (NK + 3) / 4;
+  float ksc[NSC], vsc[NSC];
+  auto scales_of = [&](int it) __attribute__((always_inline)) {
+    const uint32_t t8 = tid_here() & 63, c = t8 & 15;
+    const uint32_t sl = lds0 + kS + (it & (2 * kRing - 1)) * kScales + 16 * (t8 / NR) + 4 * (KS * ((c >> 2) % NK) + (c & 3));
+#pragma unroll
+    for (int q = 0; q < NSC; ++q) ksc[q] = *lds_at<float>(sl + 16 * KS * q), vsc[q] = *lds_at<float>(sl + 256 + 16 * KS * q);
+  };
+  // P^T of a stage's keys from its scores.  PART: some row may see them only in part.
+  auto softmax = [&](int it, auto PART) __attribute__((always_inline)) {
+    constexpr bool part = decltype(PART)::value;
+    const int h = (uint32_t)(tid_here() & 63) / NR, kb = SK * it + 4 * h;
+    float st[4 * NK];
+    each<NK>([&](auto I) {
+      each<4>([&](auto R) {
+        constexpr int i = I, r = R;
+        auto d = [&](int p) { return BF16 ? dg[p][i / 4][4 * (i % 4) + r] : dg[p][i % NM][r]; };
+        float x = (float)(d(0) * 256 + d(1));   // a whole number below 2^30
+        // (fp32: the row's unit first, a sum of three digits times a large scale could overflow)
+        if constexpr (!BF16) x = __builtin_fmaf(x, 256.0f * fac, (float)d(NP - 1) * fac);
+        st[4 * i + r] = x * lane_of_16<(4 * i + r) % 16>(ksc[(4 * i + r) / 16]);
+        if (part && kb + KS * i + r >= seen) st[4 * i + r] = kNegInf;
+      });
+    });
     float mt = st[0];
 #pragma unroll
     for (int r = 1; r < 4 * NK; ++r) mt = fmaxf(mt, st[r]);
     if constexpr (!BF16) mt = fmaxf(mt, xor_perm<16>(mt));
     mt = fmaxf(mt, xor_perm<32>(mt));
+    if constexpr (BF16) mt = mt == kNegInf ? kNegInf : mt * fac;   // (0 times it is not it)
     const bool up = mt > m + 8.0f;                       // (as in the form for few rows)
     if (__ballot(up) != 0) {
       const float mn = up ? mt : m, al = __builtin_amdgcn_exp2f(m - (mn == kNegInf ? 0.0f : mn));
@@ -533,19 +556,18 @@ __global__ __launch_bounds__(512, 2) void attn_i8_tile_kernel(const AttnI8 a) {
     }
     const float mu = m == kNegInf ? 0.0f : m;
     float ps = 0.0f;
-#pragma unroll
-    for (int i = 0; i < NK; ++i) {
-      const f32x4 vs = *lds_at<f32x4>(sl + 256 + 4 * KS * i);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float p = __builtin_amdgcn_exp2f(st[4 * i + r] - mu);
-        const bool hidden = part && kb + KS * i + 4 * h + r >= seen;
+    each<NK>([&](auto I) {
+      each<4>([&](auto R) {
+        constexpr int i = I, r = R;
+        const bool hidden = part && kb + KS * i + r >= seen;
+        float p = __builtin_amdgcn_exp2f(BF16 ? __builtin_fmaf(st[4 * i + r], fac, -mu) : st[4 * i + r] - mu);
+        if (BF16 && hidden) p = 0.0f;   // (a unit of 0)
         ps += p;
-        st[4 * i + r] = hidden ? 0.0f : p * vs[r];   // (a hidden row's scale may be anything)
-      }
-    }
+        const float v = p * lane_of_16<(4 * i + r) % 16>(vsc[(4 * i + r) / 16]);
+        st[4 * i + r] = hidden ? 0.0f : v;   // (a hidden row's scale may be anything)
+      });
+    });
     l += ps;
-    u32x4 pf[PP][NK / 2];
 #pragma unroll
     for (int d = 0; d < 2 * NK; ++d) {
       float x = st[2 * d], y = st[2 * d + 1];
@@ -556,68 +578,41 @@ __global__ __launch_bounds__(512, 2) void attn_i8_tile_kernel(const AttnI8 a) {
         x -= __uint_as_float(u0 & 0xffff0000u);
         y -= __uint_as_float(u1 & 0xffff0000u);
       }
-      const bf16x2 lastp = {(__bf16)x, (__bf16)y};
-      pf[PP - 1][d >> 2][d & 3] = __builtin_bit_cast(uint32_t, lastp);
+      const bf16x2 last = {(__bf16)x, (__bf16)y};
+      pf[PP - 1][d >> 2][d & 3] = __builtin_bit_cast(uint32_t, last);
     }
     __builtin_amdgcn_sched_barrier(0);
-    const int t7 = tid_here() & 63, vh = t7 / NR, vx = (t7 & 15) >> 2;   // vx: the key of four that this lane's transposing read brings
-    const uint32_t vl = lds0 + kV + (it & 1) * kWide + (32 * u + 4 * vh + vx) * D * 2 +
-                        ((BF16 ? 32 * ((t7 >> 4) & 1) : 0) ^ (64 * vx + 32 * (vh & 1))) + 16 * ((t7 & 3) >> 1) + 8 * (t7 & 1);
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int kk = 0; kk < NK / 2; ++kk) {
-        // bfloat16: keys 16 kk + 4 h .., + 8 of element 32 t + lane % 32; fp32: 4 h .., + 16 of 16 t + lane % 16
-        const uint32_t p = (BF16 ? (vl ^ (64 * (t & 3))) + 256 * (t >> 2) : (vl ^ (32 * (t & 7))) + 256 * (t >> 3)) + 32 * D * kk;
-        union {
-          i16x4 q[2];
-          bf16x8 v;
-        } w;
-#pragma unroll
-        for (int q = 0; q < 2; ++q) w.q[q] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_at<i16x4>(p + (BF16 ? 16 : 32) * D * q));
-#pragma unroll
-        for (int i = PP - 1; i >= 0; --i) {
-          if constexpr (BF16)
-            acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w.v, __builtin_bit_cast(bf16x8, pf[i][kk]), acc[t], 0, 0, 0);
-          else
-            acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.v, __builtin_bit_cast(bf16x8, pf[i][kk]), acc[t], 0, 0, 0);
-        }
-      }
-    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
-#pragma unroll
-    for (int i = 0; i < NT * NK / 2 - 2; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x8, PP, 0);
-      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-    }
-    __builtin_amdgcn_sched_group_barrier(0x8, 2 * PP, 0);
-    __builtin_amdgcn_sched_barrier(0);
   };
-  auto ahead = [&](int it) {
-    if (it + 1 < n) {
-      landed(min(n - 2 - it, 1));
-      widen_stage(it + 1);
-    }
-    if (it + kRing - 1 < n) stage(it + kRing - 1);   // (where stage it - 1 was, which every wave is done with)
-  };
-  const int full = max(min(sees(r0), end), 0) / SK;  // stages that every row sees whole
+  // The two waves of a SIMD (w and w + 4) take turns at the matrix pipe: while the one forms stage it - 1's outputs and stage
+  // it's scores, the other turns its scores into probabilities, and a barrier ends each turn.  In turn t = 0, 1 .. the first four
+  // waves are at the matrix pipe when t is even, with it = t / 2, and at the probabilities of stage (t - 1) / 2 when t is odd; the
+  // last four are one turn behind.  In its turn at the matrix pipe a wave also widens its part of stage it (in turn 2 it or 2 it + 1;
+  // read from turn 2 it + 2 on; the place held stage it - 2, last read in turn 2 it - 1), sends for its part of stage it + 3
+  // (in the place of stage it - 1, whose K was last read in turn 2 it - 1; the scales, read until turn 2 it, have places of
+  // their own) and waits for its part of stage it + 1 (read from turn 2 it + 2 on).
+  const int second = wave >> 2;
   if (n > 0) {
     landed(min(n - 1, 2));
-    widen_stage(0);
     barrier();
-  }
-  int it = 0;
-  for (; it < full; ++it) {
-    ahead(it);
-#pragma unroll
-    for (int u = 0; u < SK / 32; ++u) step(it, u, std::false_type{});
-    barrier();
-  }
-  for (; it < n; ++it) {
-    ahead(it);
-#pragma unroll
-    for (int u = 0; u < SK / 32; ++u)
-      if (SK * it + 32 * u < wend) step(it, u, std::true_type{});
-    barrier();
+    if (second) barrier();
+    const int full = max(min(sees(r0), end), 0) / SK;  // stages that every row sees whole
+    auto turns = [&](int it, auto FIRST, auto PART) __attribute__((always_inline)) {
+      __builtin_amdgcn_s_setprio(2);   // (before the other wave's vector instructions: 2.79 -> 2.58 us a stage)
+      if (it + kRing - 1 < n) stage(it + kRing - 1);
+      matrix(it, FIRST, std::false_type{});
+      __builtin_amdgcn_s_setprio(0);
+      if (it + 1 < n) landed(min(n - 2 - it, 2));
+      barrier();
+      scales_of(it);
+      softmax(it, PART);
+      barrier();
+    };
+    turns(0, std::true_type{}, std::true_type{});
+    int it = 1;
+    for (; it < full; ++it) turns(it, std::false_type{}, std::false_type{});
+    for (; it < n; ++it) turns(it, std::false_type{}, std::true_type{});
+    matrix(n, std::false_type{}, std::true_type{});
+    if (!second) barrier();
   }
   if constexpr (!BF16) l = l + xor_perm<16>(l);
   l = l + xor_perm<32>(l);
