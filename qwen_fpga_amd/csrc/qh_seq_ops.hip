@@ -230,8 +230,10 @@ int qh_qk_norm_rope_seq(void* q_out, int64_t ldqo, int64_t hsqo, void* k_out, in
   a.rot = rope_dim;
   a.eps = eps;
   a.bf16 = type == QH_BF16;
-  const double half_turns = 0.15915494309189533577;   // 1 / (2 pi)
-  for (int i = 0; i < rope_dim / 2; ++i) a.turns[i] = std::pow(theta, -2.0 * i / rope_dim) * half_turns;
+  // (a product for each pair in more than 64 bits: a power each took 1.3 us of the call)
+  long double turn = 0.159154943091895335768883763372514362L;   // 1 / (2 pi)
+  const long double step = rope_dim > 0 ? std::pow((long double)theta, -2.0L / rope_dim) : 1.0L;
+  for (int i = 0; i < rope_dim / 2; ++i, turn *= step) a.turns[i] = (double)turn;
   return hip_status(launch_norm_rope(a, S(stream)));
 }
 
