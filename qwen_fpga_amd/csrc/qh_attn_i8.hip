@@ -29,18 +29,27 @@ struct Row {
     unit = top >= 0x7f800000u ? __builtin_nanf("") : big / kTop / up;
     to = big > 0.0f ? kTop / big : 0.0f;
   }
-  // The digits of 16 elements, the highest first: bytes of x + 0x80 (0x8080), of which all but the highest are 0x80 off.
-  __device__ __forceinline__ void digits(const float (&q)[16], u32x4 (&o)[NP]) const {
+  // The digits of 16 elements as they were loaded, the highest first: bytes of x + 0x80 (0x8080), of which all but the
+  // highest are 0x80 off.
+  template <bool UP>
+  __device__ __forceinline__ void digits(const u32x4 (&q)[BF16 ? 2 : 4], u32x4 (&o)[NP]) const {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       uint32_t y[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float v = q[4 * i + e] * up * to;
+        float v;
+        if constexpr (BF16) {
+          const uint32_t two = q[i / 2][2 * (i % 2) + e / 2];
+          v = __uint_as_float(e % 2 ? two & 0xffff0000u : two << 16);
+        } else {
+          v = __uint_as_float(q[i][e]);
+        }
+        if constexpr (UP) v *= up;
         if constexpr (BF16)
-          y[e] = __float_as_uint(v + (12582912.0f + 128.0f));   // 1.5 * 2^23: the whole number stands in the lowest bits
+          y[e] = __float_as_uint(__builtin_fmaf(v, to, 12582912.0f + 128.0f));   // 1.5 * 2^23: the whole number stands in the lowest bits
         else
-          y[e] = (uint32_t)((int)__builtin_rintf(v) + 0x8080);
+          y[e] = (uint32_t)((int)__builtin_rintf(v * to) + 0x8080);
       }
 #pragma unroll
       for (int p = 0; p < NP; ++p) {
@@ -51,21 +60,31 @@ struct Row {
     }
   }
 };
-__device__ __forceinline__ uint32_t larger_bits(uint32_t top, float x) { return max(top, __float_as_uint(x) & 0x7fffffffu); }
-// 16 neighbours of a row of queries
+// 16 neighbours of a row of queries, and the largest of `top` and their magnitudes' bits (bfloat16: in each half of `top`)
 template <bool BF16>
-__device__ __forceinline__ void load16(const char* p, float (&x)[16]) {
+__device__ __forceinline__ void load16(const char* p, u32x4 (&q)[BF16 ? 2 : 4]) {
 #pragma unroll
-  for (int i = 0; i < (BF16 ? 2 : 4); ++i) {
-    const u32x4 v = *as_global(reinterpret_cast<const u32x4*>(p) + i);
+  for (int i = 0; i < (BF16 ? 2 : 4); ++i) q[i] = *as_global(reinterpret_cast<const u32x4*>(p) + i);
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t larger_of(uint32_t top, const u32x4 (&q)[BF16 ? 2 : 4]) {
+#pragma unroll
+  for (int i = 0; i < (BF16 ? 2 : 4); ++i)
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      if constexpr (BF16)
-        x[8 * i + 2 * c] = __uint_as_float(v[c] << 16), x[8 * i + 2 * c + 1] = __uint_as_float(v[c] & 0xffff0000u);
-      else
-        x[4 * i + c] = __uint_as_float(v[c]);
+      if constexpr (BF16) {
+        typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+        top = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, top), __builtin_bit_cast(u16x2, q[i][c] & 0x7fff7fffu)));
+      } else {
+        top = max(top, q[i][c] & 0x7fffffffu);
+      }
     }
-  }
+  return top;
+}
+// that as the bits of one float
+template <bool BF16>
+__device__ __forceinline__ uint32_t largest(uint32_t top) {
+  return BF16 ? max(top & 0xffff0000u, top << 16) : top;
 }
 
 // Byte B of x, signed, as a float, in one instruction (the compiler takes three).
@@ -165,12 +184,11 @@ __global__ __launch_bounds__(256, 2) void attn_i8_split_kernel(const AttnI8 a) {
   if (kb < k1) load_k(kb), load_v(kb);
 
   // Q's digits: wave s forms those of elements 64 s + 16 g .. of row j
-  float qv[16];
+  u32x4 qv[BF16 ? 2 : 4];
   uint32_t top = 0;
   if (wave < NS) {
     load16<BF16>(static_cast<const char*>(a.q.p) + ((at.sp.start + tok) * a.q.ld + hq * a.q.hs + 64 * wave + 16 * g) * E, qv);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) top = larger_bits(top, qv[i]);
+    top = largest<BF16>(larger_of<BF16>(0, qv));
     top = max(top, (uint32_t)xor_perm_i<16>((int)top));
     top = max(top, (uint32_t)xor_perm_i<32>((int)top));
     if (g == 0) ltop[wave][j] = top;
@@ -181,7 +199,7 @@ __global__ __launch_bounds__(256, 2) void attn_i8_split_kernel(const AttnI8 a) {
   const Row<BF16> qr(top);
   if (wave < NS) {
     u32x4 v[NP];
-    qr.digits(qv, v);
+    qr.template digits<true>(qv, v);
 #pragma unroll
     for (int p = 0; p < NP; ++p) lq[wave][p][lane] = v[p];
   }
@@ -398,24 +416,24 @@ __global__ __launch_bounds__(512, 2) void attn_i8_tile_kernel(const AttnI8 a) {
   float fac;
   {
     const char* qp = static_cast<const char*>(a.q.p) + ((at.sp.start + tok) * a.q.ld + hq * a.q.hs + 16 * h) * E;
+    u32x4 x[NF][BF16 ? 2 : 4];
+#pragma unroll
+    for (int s = 0; s < NF; ++s) load16<BF16>(qp + FB * E * s, x[s]);
     uint32_t top = 0;
 #pragma unroll
-    for (int s = 0; s < NF; ++s) {
-      float x[16];
-      load16<BF16>(qp + FB * E * s, x);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) top = larger_bits(top, x[i]);
-    }
+    for (int s = 0; s < NF; ++s) top = larger_of<BF16>(top, x[s]);
+    top = largest<BF16>(top);
     if constexpr (!BF16) top = max(top, (uint32_t)xor_perm_i<16>((int)top));
     top = max(top, (uint32_t)xor_perm_i<32>((int)top));
     Row<BF16> qr(top);
     fac = qr.unit * (fabsf(a.scale) * kLog2e);
     if (a.scale < 0.0f) qr.to = -qr.to;   // (-q) k |scale|: a maximum stays one
+    if (__ballot(qr.up != 1.0f) == 0) {
 #pragma unroll
-    for (int s = 0; s < NF; ++s) {        // (read again: held over the maximum they would not fit the registers)
-      float x[16];
-      load16<BF16>(qp + FB * E * s, x);
-      qr.digits(x, qf[s]);
+      for (int s = 0; s < NF; ++s) qr.template digits<false>(x[s], qf[s]);
+    } else {
+#pragma unroll
+      for (int s = 0; s < NF; ++s) qr.template digits<true>(x[s], qf[s]);
     }
   }
 
