@@ -28,8 +28,14 @@ struct Unit {
   int first;    // unit (before kv heads) of the tile's first split
 };
 constexpr int kFill = 512, kMinChunk = 128;
-// Unit b of the split kernel, or (JOIN) the units of row tile b.
-template <bool JOIN>
+// Keys that the longest unsplit tile may hold more than a chunk, before splitting it (writing sums, a second kernel, more
+// of it with more tiles) is worth it.  attention_seq_i8, bfloat16, 8 / 2 heads of 256, whole and split: 512 tokens 13
+// and 17 us, 1024 24 and 28, 512 behind 1488 29 and 32, 100 single tokens of 1500 keys each 44 and 52, one of 500 12
+// and 13; where it splits, 256 tokens behind 7744 95 and 62, 16 single tokens of 900 23 and 17.
+__host__ __device__ __forceinline__ int few_whole(int64_t tiles) { return 384 + (int)(tiles > 192 ? 1536 : 8 * tiles); }
+// Unit b of the split kernel, or (JOIN) the units of row tile b.  WHOLE: no tile is split where that
+// would save no more than joining costs (few_whole).
+template <bool JOIN, bool WHOLE = false>
 __device__ __forceinline__ bool find_unit(const AttnSeq& a, int b, Unit& o) {
   const int lane = threadIdx.x & 63, G = a.heads / a.kv_heads;
   SeqSpan sp;   // of sequence s0 + lane, as of its keys and tiles
@@ -46,14 +52,19 @@ __device__ __forceinline__ bool find_unit(const AttnSeq& a, int b, Unit& o) {
   load(0);
   if (a.limit > 0) {
     int64_t work = (int64_t)tiles * max(kl, 0);   // keys of all row tiles
+    int64_t all = tiles;
+    int longest = tiles > 0 ? kl : 0;
     for (int s0 = 64; s0 < a.n_seq; s0 += 64) {
       load(s0);
       work += (int64_t)tiles * max(kl, 0);
+      all += tiles;
+      if (tiles > 0) longest = max(longest, kl);
     }
     if (a.n_seq > 64) load(0);
     work = sum_all(work);
     const int64_t c = (work * a.kv_heads + kFill - 1) / kFill;
     chunk = (int)min(max((c + 63) / 64 * 64, (int64_t)kMinChunk), (int64_t)kMaxKeys);
+    if (WHOLE && __ballot(longest - chunk > few_whole(sum_all(all) * a.kv_heads)) == 0) chunk = kMaxKeys;
   }
   int base = 0, first = 0;   // of the next 64 sequences: tiles (JOIN) or units, units
   for (int s0 = 0; s0 < a.n_seq; s0 += 64) {
@@ -86,7 +97,7 @@ constexpr size_t part_floats(int D) { return 16 * D + 32; }
 
 // Joins the splits of a tile's rows, every fourth row in a workgroup: sixteen waves take every sixteenth split, four
 // in flight, each with a running maximum of its own.
-template <bool BF16, int D>
+template <bool BF16, int D, bool WHOLE = false>
 __global__ __launch_bounds__(1024) void attn_join_kernel(const AttnSeq a) {
   constexpr int W = D / 64, NW = 16, U = 4;   // elements of a lane; waves; splits in flight
   typedef float vec __attribute__((ext_vector_type(W)));
@@ -96,13 +107,13 @@ __global__ __launch_bounds__(1024) void attn_join_kernel(const AttnSeq a) {
   const int G = a.heads / a.kv_heads;
   const int kvh = (int)blockIdx.x % a.kv_heads;
   Unit at;
-  if (!find_unit<true>(a, (int)blockIdx.x / a.kv_heads, at)) return;
+  if (!find_unit<true, WHOLE>(a, (int)blockIdx.x / a.kv_heads, at)) return;
   if (at.nsplit == 1) return;   // written by the split kernel
   if (at.first < 0 || (int64_t)(at.first + at.nsplit) * a.kv_heads > (int64_t)gridDim.x + kFill) return;   // past its grid
   const int rows = at.sp.len * G;
   const size_t step = part_floats(D) * a.kv_heads;
   const float* pp = a.part + ((size_t)at.first * a.kv_heads + kvh) * part_floats(D);
-  for (int j = blockIdx.y; j < 16 && 16 * at.tile + j < rows; j += 4) {
+  for (int j = blockIdx.y; j < 16 && 16 * at.tile + j < rows; j += gridDim.y) {
     const int row = 16 * at.tile + j, tok = row / G, hq = kvh * G + row % G;
     const int seen = keys_seen(tok, at.sp.len, at.kl);
     const int ns = min(seq_tiles(seen, at.chunk), at.nsplit);   // splits that this row sees (the rest hold no key of it)

@@ -142,7 +142,7 @@ __global__ __launch_bounds__(256, 2) void attn_i8_split_kernel(const AttnI8 a) {
   const int G = a.heads / a.kv_heads;
   const int kvh = (int)blockIdx.x % a.kv_heads;
   Unit at;
-  if (!find_unit<false>(a, (int)blockIdx.x / a.kv_heads, at)) return;
+  if (!find_unit<false, true>(a, (int)blockIdx.x / a.kv_heads, at)) return;
   const int64_t ks = at.ks;
   const int kl = at.kl;
   const int rows = at.sp.len * G, r0 = 16 * at.tile;
@@ -675,7 +675,9 @@ hipError_t launch(const AttnI8& a, hipStream_t s) {
   }
   const unsigned tiles = (unsigned)(seq_tiles_max(rows, a.n_seq, 16) * a.kv_heads);
   attn_i8_split_kernel<BF16, D><<<a.limit > 0 ? tiles + kFill : tiles, 256, 0, s>>>(a);
-  if (a.limit > 0) attn_join_kernel<BF16, D><<<dim3(tiles, 4), 1024, 0, s>>>(a);
+  // rows of a tile side by side where there are few tiles (4 tokens behind 29996 keys: 16 workgroups 23 us, 4 36), few
+  // workgroups where there are many, most of which find nothing to join (16 x 128 behind 1872: 4 106 us, 1 97)
+  if (a.limit > 0) attn_join_kernel<BF16, D, true><<<dim3(tiles, tiles >= 256 ? 1 : tiles >= 64 ? 4 : 16), 1024, 0, s>>>(a);
   return hipGetLastError();
 }
 
@@ -684,8 +686,14 @@ hipError_t launch(const AttnI8& a, hipStream_t s) {
 AttnForm attn_i8_form(int64_t q_rows, int n_seq, int max_q, int max_k, int heads, int kv_heads, int dim, bool bf16) {
   const int G = heads / kv_heads;
   AttnForm f = {0, 0, 0};
-  const int64_t seen = q_rows * heads * std::max(max_k, 1);
-  if ((int64_t)max_q * G >= (bf16 ? 1024 : 2048) || ((int64_t)max_q * G >= 128 && seen >= 5000000)) {
+  // Pairs of a query row and a key it sees, about (where there is one sequence, or several of equal length).  The form for
+  // prompts takes a workgroup of 512 threads a CU and 2 us for every 32 keys however few rows there are, the one for few
+  // rows takes half as long again where there is work for all CUs.  few / prompts, bfloat16, 8 / 2 heads of 256: 1024
+  // tokens 24 / 47 us, 1500 41 / 50, 2000 59 / 59, 6000 382 / 210, 512 behind 1488 29 / 47, 512 behind 3488 75 / 54, 300
+  // behind 15700 160 / 79, 64 behind 31936 59 / 75; 8 / 8 heads of 128: 1500 27 / 39, 2000 40 / 46, 6000 261 / 148; fp32,
+  // 8 / 2 heads of 256: 1500 47 / 51, 2000 67 / 68, 6000 425 / 353, 512 behind 3488 78 / 56.
+  const int64_t pairs = q_rows * heads * (std::max(max_k, max_q) - max_q / 2);
+  if ((int64_t)max_q * G > 256 && pairs >= 15000000) {
     f.tile = tile_rows(bf16);
     const int64_t tiles = seq_tiles_max(q_rows * G, n_seq, f.tile) * kv_heads;
     // two workspace places a CU: the chunks are such that more are hardly ever taken
@@ -694,7 +702,7 @@ AttnForm attn_i8_form(int64_t q_rows, int n_seq, int max_q, int max_k, int heads
       f.limit = (int)std::min<int64_t>(2 * kCUs, tiles * std::min<int64_t>(splits, kMaxTileSplits));
     }
     f.bytes = (size_t)f.limit * tile_part_floats(f.tile, dim) * sizeof(float);
-  } else if (max_k > kMinChunk) {
+  } else if (max_k > kMinChunk + few_whole((q_rows * G + 15) / 16 * kv_heads)) {
     f.limit = 1;
     f.bytes = (size_t)(seq_tiles_max(q_rows * G, n_seq, 16) * kv_heads + kFill) * part_floats(dim) * sizeof(float);
   }

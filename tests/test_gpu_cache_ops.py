@@ -294,6 +294,7 @@ def test_cache_rows_far_apart(q, torch_cuda, bf16):
 
 TOP = {False: 8355704.0, True: 32639.0}      # a query row's largest element, in units
 MAX_Q = None                                 # the bound that a call is given; None: the longest sequence
+LARGE = 1 << 26                              # a bound that asks for the form for prompts
 
 
 def p_rounding(lens, G, bf16):
@@ -339,6 +340,7 @@ def attn_inputs(torch, seed, lens, ctx, h, kvh, d, bf16, gap=0, qscale=2.0):
     return (qq, *sides), at_k
 
 
+
 def attn_run(q, torch, dev, lens, ctx, at_k, scale=None, max_q=None, max_k=None, out=None):
     qq, kq = dev[:2]
     t, h, d = qq.shape
@@ -370,6 +372,7 @@ ATTN = [  # lens, keys, heads, kv heads, dim
     ([1], [32], 2, 1, 256), ([1], [129], 2, 1, 128), ([15, 16, 17], [15, 16, 17], 2, 1, 128), ([64], [64], 2, 2, 256),
     ([63, 0, 65], [63, 5, 70], 4, 2, 128), ([127, 1], [127, 129], 8, 2, 256), ([129], [400], 2, 1, 256), ([200, 90], [200, 90], 3, 3, 128),
     ([300], [300], 8, 2, 256), ([33], [2000], 2, 1, 128), ([260], [261], 1, 1, 256), ([520], [520], 4, 1, 128), ([5], [5], 3, 1, 256),
+    ([200, 1], [1400, 900], 8, 2, 256), ([1] * 70, [1500 - 20 * i for i in range(70)], 4, 1, 128), ([100, 7], [3000, 100], 4, 2, 128),
 ]
 
 
@@ -466,11 +469,11 @@ def test_attention_strides(q, torch_cuda, bf16):
 def test_attention_bounds_too_small_or_large(q, torch_cuda, monkeypatch, bf16):
     """max_q and max_k choose the form: any value gives the same within tolerance."""
     torch = torch_cuda
-    monkeypatch.setattr(sys.modules[__name__], "MAX_Q", 5000)      # (the bound of the form for prompts)
+    monkeypatch.setattr(sys.modules[__name__], "MAX_Q", LARGE)      # (the bound of the form for prompts)
     lens, ctx = [1, 90, 3], [900, 90, 500]
     inp, at = attn_inputs(torch, 6, lens, ctx, 4, 2, 128, bf16)
     dev, want = both(torch, inp, at, lens, ctx, 1 / math.sqrt(128), bf16)
-    for mq in (0, 1, 4, 90, 5000):
+    for mq in (0, 1, 4, 90, 5000, LARGE):
         for mk in (0, 100, 900, 100000):
             attn_check(torch, attn_run(q, torch, dev, lens, ctx, at, max_q=mq, max_k=mk), want, bf16)
 
@@ -561,11 +564,11 @@ def test_attention_bad_ranges(q, torch_cuda, bf16, n, m):
     assert (out[n:] == 7).all()
 
 
-# The form for prompts, whatever the lengths: max_q is a bound, and a large one asks for it.
+# The form for prompts, whatever the lengths.
 
 @pytest.fixture
 def prompts(monkeypatch):
-    monkeypatch.setattr(sys.modules[__name__], "MAX_Q", 4096)
+    monkeypatch.setattr(sys.modules[__name__], "MAX_Q", LARGE)
 
 
 @pytest.mark.parametrize("lens,ctx,h,kvh,d", ATTN + [
@@ -627,11 +630,11 @@ def test_prompt_form_places_in_the_workspace(q, torch_cuda, prompts, bf16, max_k
     lens, ctx = [70, 3, 0, 129, 64, 1, 70, 2, 300], [900, 3, 10, 1500, 64, 2500, 400, 2, 3000]
     inp, at = attn_inputs(torch, 15, lens, ctx, 4, 2, 128, bf16)
     dev, want = both(torch, inp, at, lens, ctx, 1 / math.sqrt(128), bf16)
-    attn_check(torch, attn_run(q, torch, dev, lens, ctx, at, max_q=4096, max_k=max_k), want, bf16)
+    attn_check(torch, attn_run(q, torch, dev, lens, ctx, at, max_q=LARGE, max_k=max_k), want, bf16)
 
 
 @pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
-@pytest.mark.parametrize("max_q", [1, 4096])
+@pytest.mark.parametrize("max_q", [1, LARGE])
 def test_attention_of_many_sequences(q, torch_cuda, monkeypatch, bf16, max_q):
     """More than the 64 sequences that a wave looks at together; long ones among empty and short ones."""
     torch = torch_cuda
@@ -646,7 +649,7 @@ def test_attention_of_many_sequences(q, torch_cuda, monkeypatch, bf16, max_q):
 
 
 @pytest.mark.parametrize("ld", [1 << 22, (1 << 24) - 16])
-@pytest.mark.parametrize("max_q", [1, 4096])
+@pytest.mark.parametrize("max_q", [1, LARGE])
 def test_attention_rows_far_apart(q, torch_cuda, monkeypatch, ld, max_q):
     """Rows of codes 4 and 16 MB apart (the largest stride), the last ones behind 2^32 bytes; scales 1 MB apart."""
     torch = torch_cuda
@@ -738,7 +741,7 @@ def test_two_streams(q, torch_cuda):
                 o = [torch.empty(980, 2, 256, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
                 q.kv_cache_read_i8(*o, *dev[1:], slot)
                 q.kv_cache_write_i8(*c, *o, slot)
-                res.append((attn_run(q, torch, dev, lens, ctx, at), attn_run(q, torch, dev, lens, ctx, at, max_q=4096), o, c))
+                res.append((attn_run(q, torch, dev, lens, ctx, at), attn_run(q, torch, dev, lens, ctx, at, max_q=LARGE), o, c))
     torch.cuda.synchronize()
     for a, b, o, c in res:
         attn_check(torch, a, want, True)
