@@ -399,10 +399,10 @@ __global__ __launch_bounds__(512, 2) void attn_i8_tile_kernel(const AttnI8 a) {
   auto stage = [&](int it) __attribute__((always_inline)) {
     const int last = end - 1 - SK * it, slot = it & (kRing - 1);   // last: the last row that is there
     const uint32_t t = tid_here(), pr = t / CH, pc = t % CH, r = min(pr, (uint32_t)last), kc = 16 * (pc ^ (D == 256 ? pr & 15 : (pr >> 1) & 7)), vc = 16 * pc;
-    load_to_lds(kp + (int64_t)it * SK * a.k.ld, __umul24(r, kld) + kc, lds0 + slot * 8192 + 1024 * wave);
-    load_to_lds(vp + (int64_t)it * SK * a.v.ld, __umul24(r, vld) + vc, lds0 + kRaw + slot * 8192 + 1024 * wave);
+    load_to_lds<5>(kp + (int64_t)it * SK * a.k.ld, __umul24(r, kld) + kc, lds0 + slot * 8192 + 1024 * wave);
+    load_to_lds<5>(vp + (int64_t)it * SK * a.v.ld, __umul24(r, vld) + vc, lds0 + kRaw + slot * 8192 + 1024 * wave);
     if (scales)
-      load_word_to_lds(sp + it * SK * sld, 4 * __umul24(min(t % SK, (uint32_t)last), (uint32_t)sld), lds0 + kS + (it & (2 * kRing - 1)) * kScales + 256 * wave);
+      load_word_to_lds<5>(sp + it * SK * sld, 4 * __umul24(min(t % SK, (uint32_t)last), (uint32_t)sld), lds0 + kS + (it & (2 * kRing - 1)) * kScales + 256 * wave);
   };
   const int n = seq_tiles(end, SK);
 #pragma unroll

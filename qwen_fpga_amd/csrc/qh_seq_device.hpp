@@ -78,13 +78,19 @@ __device__ __forceinline__ __attribute__((address_space(3))) T* lds_at(uint32_t 
 // flight itself (s_waitcnt vmcnt before the barrier that hands a stage over): the compiler waits for every such load
 // before any transposing LDS read.  Nothing is returned to a register.  The compiler counts no wait states before an
 // asm statement: m0 needs one after it is set, and a scalar register that a vector instruction wrote (a spilled one, read
-// back from a vector register's lane) five before a load takes its address from it.
+// back from a vector register's lane) five before a load takes its address from it.  WAIT is 5 where a kernel spills such
+// a base; for all of them a test reads the compiled code.  (Five everywhere: packed attention 357 -> 364 us, the delta rule
+// 87 -> 91.)
+template <int WAIT = 1>
 __device__ __forceinline__ void load_to_lds(const char* base, uint32_t off, uint32_t to) {
-  asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"{m0}"(__builtin_amdgcn_readfirstlane(to)), "v"(off), "s"(base) : "memory");
+  asm volatile("s_nop %3\n\tglobal_load_lds_dwordx4 %1, %2" ::"{m0}"(__builtin_amdgcn_readfirstlane(to)), "v"(off), "s"(base), "n"(WAIT - 1)
+               : "memory");
 }
 // 4 bytes per lane from base + off to LDS at `to` + 4 lane.
+template <int WAIT = 1>
 __device__ __forceinline__ void load_word_to_lds(const float* base, uint32_t off, uint32_t to) {
-  asm volatile("s_nop 4\n\tglobal_load_lds_dword %1, %2" ::"{m0}"(__builtin_amdgcn_readfirstlane(to)), "v"(off), "s"(base) : "memory");
+  asm volatile("s_nop %3\n\tglobal_load_lds_dword %1, %2" ::"{m0}"(__builtin_amdgcn_readfirstlane(to)), "v"(off), "s"(base), "n"(WAIT - 1)
+               : "memory");
 }
 
 }  // namespace qh
