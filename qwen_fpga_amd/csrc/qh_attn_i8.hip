@@ -545,23 +545,41 @@ __global__ __launch_bounds__(512, 2) void attn_i8_tile_kernel(const AttnI8 a) {
     constexpr bool part = decltype(PART)::value;
     const int h = (uint32_t)(tid_here() & 63) / NR, kb = SK * it + 4 * h;
     float st[4 * NK];
-    each<NK>([&](auto I) {
-      each<4>([&](auto R) {
-        constexpr int i = I, r = R;
-        auto d = [&](int p) { return BF16 ? dg[p][i / 4][4 * (i % 4) + r] : dg[p][i % NM][r]; };
-        float x = (float)(d(0) * 256 + d(1));   // a whole number below 2^30
-        // (fp32: the row's unit first, a sum of three digits times a large scale could overflow)
-        if constexpr (!BF16) x = __builtin_fmaf(x, 256.0f * fac, (float)d(NP - 1) * fac);
-        st[4 * i + r] = x * lane_of_16<(4 * i + r) % 16>(ksc[(4 * i + r) / 16]);
-        if (part && kb + KS * i + r >= seen) st[4 * i + r] = kNegInf;
+    // bfloat16: the scores without the row's unit, which the exponent's multiplication brings; where a scale of K could take
+    // a whole number beyond a float's range, and in fp32 (a sum of three digits), the unit comes first
+    bool far = !BF16;
+    if constexpr (BF16) {
+      bool any = false;
+#pragma unroll
+      for (int q = 0; q < NSC; ++q) any |= !(fabsf(ksc[q]) < 0x1p96f);
+      far = __ballot(any) != 0;
+    }
+    const float after = far ? 1.0f : fac;
+    auto scores = [&](auto FAR) __attribute__((always_inline)) {
+      each<NK>([&](auto I) {
+        each<4>([&](auto R) {
+          constexpr int i = I, r = R;
+          auto d = [&](int p) { return BF16 ? dg[p][i / 4][4 * (i % 4) + r] : dg[p][i % NM][r]; };
+          float x = (float)(d(0) * 256 + d(1));   // a whole number below 2^30
+          if constexpr (!BF16)
+            x = __builtin_fmaf(x, 256.0f * fac, (float)d(NP - 1) * fac);
+          else if constexpr (decltype(FAR)::value)
+            x *= fac;
+          st[4 * i + r] = x * lane_of_16<(4 * i + r) % 16>(ksc[(4 * i + r) / 16]);
+          if (part && kb + KS * i + r >= seen) st[4 * i + r] = kNegInf;
+        });
       });
-    });
+    };
+    if (BF16 && far)
+      scores(std::true_type{});
+    else
+      scores(std::false_type{});
     float mt = st[0];
 #pragma unroll
     for (int r = 1; r < 4 * NK; ++r) mt = fmaxf(mt, st[r]);
     if constexpr (!BF16) mt = fmaxf(mt, xor_perm<16>(mt));
     mt = fmaxf(mt, xor_perm<32>(mt));
-    if constexpr (BF16) mt = mt == kNegInf ? kNegInf : mt * fac;   // (0 times it is not it)
+    if constexpr (BF16) mt = mt == kNegInf ? kNegInf : mt * after;   // (0 times it is not it)
     const bool up = mt > m + 8.0f;                       // (as in the form for few rows)
     if (__ballot(up) != 0) {
       const float mn = up ? mt : m, al = __builtin_amdgcn_exp2f(m - (mn == kNegInf ? 0.0f : mn));
@@ -578,7 +596,7 @@ __global__ __launch_bounds__(512, 2) void attn_i8_tile_kernel(const AttnI8 a) {
       each<4>([&](auto R) {
         constexpr int i = I, r = R;
         const bool hidden = part && kb + KS * i + r >= seen;
-        float p = __builtin_amdgcn_exp2f(BF16 ? __builtin_fmaf(st[4 * i + r], fac, -mu) : st[4 * i + r] - mu);
+        float p = __builtin_amdgcn_exp2f(BF16 ? __builtin_fmaf(st[4 * i + r], after, -mu) : st[4 * i + r] - mu);
         if (BF16 && hidden) p = 0.0f;   // (a unit of 0)
         ps += p;
         const float v = p * lane_of_16<(4 * i + r) % 16>(vsc[(4 * i + r) / 16]);

@@ -340,7 +340,6 @@ def attn_inputs(torch, seed, lens, ctx, h, kvh, d, bf16, gap=0, qscale=2.0):
     return (qq, *sides), at_k
 
 
-
 def attn_run(q, torch, dev, lens, ctx, at_k, scale=None, max_q=None, max_k=None, out=None):
     qq, kq = dev[:2]
     t, h, d = qq.shape
@@ -506,6 +505,25 @@ def test_attention_queries_of_any_size(q, torch_cuda, bf16, size):
     if size < 2.0 ** -125:     # the row's unit has steps of 2^-149: up to 2^-150 off, times sums of 256 codes of 128 and 30 (scales up to 1e30)
         tol = tol + 1e-6 * inp[4].abs().max().double() * 127
     attn_check(torch, attn_run(q, torch, dev, lens, ctx, at), (wo, tol), bf16)
+
+
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+@pytest.mark.parametrize("max_q", [1, LARGE])
+@pytest.mark.parametrize("d", [128, 256])
+def test_attention_keys_near_the_end_of_the_range(q, torch_cuda, bf16, max_q, d):
+    """Scales of K near 2^106: a sum of digits times codes (2^23 and more) times the scale is beyond a float, the score is not."""
+    torch = torch_cuda
+    lens, ctx = [70, 1], [150, 300]
+    inp, at = attn_inputs(torch, 16, lens, ctx, 2, 1, d, bf16)
+    inp = list(inp)
+    inp[0] = inp[0] * 2.0 ** -105
+    inp[2] = inp[2] * 2.0 ** 111
+    dev, want = both(torch, inp, at, lens, ctx, 1 / math.sqrt(d), bf16)
+    attn_check(torch, attn_run(q, torch, dev, lens, ctx, at, max_q=max_q), want, bf16)
+    inp[2][40:] = inp[2][40:] * 2.0 ** -111     # these scales among ordinary ones: stages with and without them
+    inp[0] = inp[0] * 2.0 ** 100
+    dev, want = both(torch, inp, at, lens, ctx, 1 / math.sqrt(d), bf16)
+    attn_check(torch, attn_run(q, torch, dev, lens, ctx, at, max_q=max_q), want, bf16)
 
 
 @pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
