@@ -296,13 +296,13 @@ int qh_attention_seq(void* out, int64_t ldo, int64_t hso, const void* q, int64_t
  * These three calls take no sequences: a token is a row of its operands. */
 #define QH_ROPE_MAX_TOKENS (1 << 23)
 
-/* Norms of queries and keys for each head, with the position rotation, in one pass: qh_rmsnorm of every head's row (y = x / sqrt(mean(x^2) + eps) *
- * (1 + w), w = q_norm or k_norm [head_dim] fp32, 16-byte aligned), then elements i and i + rope_dim / 2 of it
- * (i < rope_dim / 2) turned by pos[token] * theta^(-2 i / rope_dim); the others stay (qh_rope_cos_sin and qh_apply_rope are that for
- * rope_dim 64 and theta 1e7).  rope_dim: a multiple of 16, 0 .. head_dim.  pos [tokens] int32, any value.  The angles are formed
- * in 64 bits, where qh_rope_cos_sin rounds the position times the frequency to fp32 as the reference does: at
- * position p the two are up to p 2^-24 apart, in radians.  All arithmetic is fp32, an output is rounded once.  q_out (k_out) may be q (k) itself:
- * the same pointer and strides. */
+/* Norms of queries and keys for each head, with the position rotation, in one pass: qh_rmsnorm of every head's row
+ * (y = x / sqrt(mean(x^2) + eps) * (1 + w), w = q_norm or k_norm [head_dim] fp32, 16-byte aligned), then elements i and
+ * i + rope_dim / 2 of it (i < rope_dim / 2) turned by pos[token] * theta^(-2 i / rope_dim); the others stay
+ * (qh_rope_cos_sin and qh_apply_rope are that for rope_dim 64 and theta 1e7).  rope_dim: a multiple of 16, 0 .. head_dim.
+ * pos [tokens] int32, any value.  The angles are formed in 64 bits, where qh_rope_cos_sin rounds the position times the
+ * frequency to fp32 as the reference does: at position p the two are up to p 2^-24 apart, in radians.  All arithmetic is
+ * fp32, an output is rounded once.  q_out (k_out) may be q (k) itself: the same pointer and strides. */
 int qh_qk_norm_rope_seq(void* q_out, int64_t ldqo, int64_t hsqo, void* k_out, int64_t ldko, int64_t hsko, const void* q,
                         int64_t ldq, int64_t hsq, const void* k, int64_t ldk, int64_t hsk, int type, const float* q_norm,
                         const float* k_norm, const int32_t* pos, int tokens, int heads, int kv_heads, int head_dim, int rope_dim,
@@ -311,15 +311,15 @@ int qh_qk_norm_rope_seq(void* q_out, int64_t ldqo, int64_t hsqo, void* k_out, in
 /* Rows of the cache from new keys and values k, v [tokens][kv_heads][head_dim] of `type`: token t goes to row slot[t]
  * (int64, on the device).  scale = largest magnitude / 127 (1 for zeros), code = rint(x / scale): qh_quant_rows of each
  * head's row, bit for bit; one that is not finite gets scale NaN and codes 0 (and what attends to it is NaN).  A token
- * whose slot lies outside 0 .. rows - 1 is skipped (a batch's unused places: -1); rows that no token names are left as they were.
- * Two tokens may not name one row: it then holds a mixture of both.  tokens * kv_heads: up to 2^26. */
+ * whose slot lies outside 0 .. rows - 1 is skipped (a batch's unused places: -1); rows that no token names are left as
+ * they were.  Two tokens may not name one row: it then holds a mixture of both.  tokens * kv_heads: up to 2^26. */
 int qh_kv_cache_write_i8(int8_t* kq, int64_t ldkq, int64_t hskq, float* ks, int64_t ldks, int64_t hsks, int8_t* vq, int64_t ldvq,
                          int64_t hsvq, float* vs, int64_t ldvs, int64_t hsvs, const void* k, int64_t ldk, int64_t hsk, const void* v,
                          int64_t ldv, int64_t hsv, int type, const int64_t* slot, int64_t rows, int tokens, int kv_heads,
                          int head_dim, void* stream);
-/* The values that rows of the cache stand for: k, v [tokens][kv_heads][head_dim] of `type`, token t from row slot[t], code * scale in
- * fp32, rounded once more to bfloat16.  A token whose slot lies outside 0 .. rows - 1 is left as it was; a row may be
- * read many times. */
+/* The values that rows of the cache stand for: k, v [tokens][kv_heads][head_dim] of `type`, token t from row slot[t],
+ * code * scale in fp32, rounded once more to bfloat16.  A token whose slot lies outside 0 .. rows - 1 is left as it was; a
+ * row may be read many times. */
 int qh_kv_cache_read_i8(void* k, int64_t ldk, int64_t hsk, void* v, int64_t ldv, int64_t hsv, int type, const int8_t* kq,
                         int64_t ldkq, int64_t hskq, const float* ks, int64_t ldks, int64_t hsks, const int8_t* vq, int64_t ldvq,
                         int64_t hsvq, const float* vs, int64_t ldvs, int64_t hsvs, const int64_t* slot, int64_t rows, int tokens,
@@ -327,13 +327,15 @@ int qh_kv_cache_read_i8(void* k, int64_t ldk, int64_t hsk, void* v, int64_t ldv,
 
 #define QH_ATTN_I8_MAX_LD (1 << 24)
 
-/* qh_attention_seq over the cache, whose row strides (of codes and of scales) are below QH_ATTN_I8_MAX_LD: the same sequences, key ranges, rows without keys, limits and workspace rules; q and
- * out of `type`.  Codes and scales of keys that a row does not see have no influence on it; a row that sees a
- * scale of V that is not finite gives nothing finite, and NaN where that or one of K is NaN.  A query row takes part as whole numbers, its largest magnitude being 32639
- * (QH_BF16: an element is off by 2^-16 of the row's largest at most) or 8355704 (QH_F32: 2^-24), so that sums of products with
- * codes are exact; scores, the softmax and sums are fp32.  Probabilities times V's scales enter the product with the
- * codes exactly for QH_F32; for QH_BF16 in two bfloat16 parts in the form for few rows (off by 2^-16 of sum p |v| at
- * most) and rounded to bfloat16 once in the one for prompts (2^-8). */
+/* qh_attention_seq over the cache, whose row strides (of codes and of scales) are below QH_ATTN_I8_MAX_LD: the same
+ * sequences, key ranges, rows without keys, limits and workspace rules; q and out of `type`.  Codes and scales of keys that
+ * a row does not see have no influence on it; a row that sees a scale of V that is not finite gives nothing finite, and NaN
+ * where that or one of K is NaN.
+ * A query row takes part as whole numbers, its largest magnitude being 32639 (QH_BF16: an element is off by 2^-16 of the
+ * row's largest at most) or 8355704 (QH_F32: 2^-24), so that sums of products with codes are exact; scores, the softmax and
+ * sums are fp32 (256 times the sum of the values' magnitudes over the keys that a row sees has to be finite there).
+ * Probabilities times V's scales enter the product with the codes exactly for QH_F32; for QH_BF16 in two bfloat16 parts in
+ * the form for few rows (off by 2^-16 of sum p |v| at most) and rounded to bfloat16 once in the one for prompts (2^-8). */
 size_t qh_attention_seq_i8_workspace(int q_rows, int n_seq, int max_q, int max_k, int heads, int kv_heads, int head_dim,
                                      int type);
 int qh_attention_seq_i8(void* out, int64_t ldo, int64_t hso, const void* q, int64_t ldq, int64_t hsq, int type, const int8_t* kq,

@@ -74,7 +74,8 @@ __device__ __forceinline__ uint32_t larger_of(uint32_t top, const u32x4 (&q)[BF1
     for (int c = 0; c < 4; ++c) {
       if constexpr (BF16) {
         typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
-        top = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, top), __builtin_bit_cast(u16x2, q[i][c] & 0x7fff7fffu)));
+        const u16x2 two = __builtin_bit_cast(u16x2, q[i][c] & 0x7fff7fffu);
+        top = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, top), two));
       } else {
         top = max(top, q[i][c] & 0x7fffffffu);
       }
@@ -97,8 +98,8 @@ __device__ __forceinline__ uint32_t code_float(uint32_t x) {
   if constexpr (B == 3) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_3" : "=v"(f) : "v"(x));
   return f;
 }
-// Byte C of eight rows as bfloat16, rows 2 i and 2 i + 1 in dword i.  A code has eight bits, a bfloat16 as well: the upper half of
-// the float is all of it.
+// Byte C of eight rows as bfloat16, rows 2 i and 2 i + 1 in dword i.  A code has eight bits, a bfloat16 as well: the upper
+// half of the float is all of it.
 template <int C, typename V>
 __device__ __forceinline__ u32x4 widen(const V (&rows)[8]) {
   u32x4 t;
@@ -123,8 +124,15 @@ __device__ __forceinline__ void each(F&& f) {
 
 // Few query rows: a workgroup takes 16 rows (tokens x query heads of one kv head) and one chunk of the keys, its four
 // waves every fourth step of 32 keys.  S^T = K Q^T runs on the int8 MFMAs, a product for each digit of Q, so that K goes
-// from memory into them as it is; O^T = V^T P^T on the bfloat16 ones, P (times V's scales) cut into two bfloat16 parts, which leave
-// out 2^-16 of it at most (bfloat16), or three, which leave out nothing (fp32).  V's codes are widened in registers, 1.5 instructions an element.
+// from memory into them as it is; O^T = V^T P^T on the bfloat16 ones, P (times V's scales) cut into two bfloat16 parts,
+// which leave out 2^-16 of it at most (bfloat16), or three, which leave out nothing (fp32).  V's codes are widened in
+// registers, 1.5 instructions an element.
+// Bound by memory where there are keys for all CUs: one token behind 131070 keys, 8 / 2 heads of 256 (135 MB), 28.3 us, 4.8
+// TB/s (and 8 to join).  With fewer keys by what follows one after the other: one key 7 us, 128 more for each workgroup 1.7
+// us more; 16 tokens of 42000 keys together (43 MB) 16.5, 2.6 TB/s.  With many rows by the vector instructions that widen V,
+// which every 16 rows do again: 1500 tokens 43 us (fp32 51).  Three instructions a code instead of 1.5 and spilled
+// registers took twice as long; Q asked for before K, no loads behind the last step, chunks of a multiple of 128 keys and 384,
+// 768 or 1024 units instead of 512 made no difference or took longer.
 template <bool BF16, int D>
 __global__ __launch_bounds__(256, 2) void attn_i8_split_kernel(const AttnI8 a) {
   constexpr int NP = Row<BF16>::NP;       // digits of Q, parts of P
@@ -358,9 +366,15 @@ __global__ __launch_bounds__(256, 2) void attn_i8_split_kernel(const AttnI8 a) {
 // (16) rows a wave, with the products of the form for few rows.  Keys come 8 KB of codes at a time (a stage: 32 keys of 256
 // elements, 64 of 128) by global -> LDS loads, three stages ahead.  K's codes stay codes; V's are widened to bfloat16 once a
 // workgroup, one stage ahead, by the wave that loaded them.  16-byte chunk c of K's row r stands at chunk c ^ (r % 16) (128
-// elements: c ^ (r / 2 % 8)), so that 16 keys of one chunk lie in all banks, and chunk c of V's widened row r at c ^ (4 (r % 4) + 2 (r / 4 % 2)),
-// as the transposing reads take four keys of 32 elements or eight of 16.  P (times V's scales) is rounded to bfloat16 once for
-// bfloat16 (2^-8 of sum p |v|) and taken in three parts for fp32 (exact).
+// elements: c ^ (r / 2 % 8)), so that 16 keys of one chunk lie in all banks, and chunk c of V's widened row r at
+// c ^ (4 (r % 4) + 2 (r / 4 % 2)), as the transposing reads take four keys of 32 elements or eight of 16.  P (times V's scales)
+// is rounded to bfloat16 once for bfloat16 (2^-8 of sum p |v|: a second part would double the products with V) and taken in
+// three parts for fp32 (exact).
+// A stage takes 2.1 us (bfloat16, 256 elements): its products would take 0.85 at the pipe's peak and 1.9 at the rates that
+// large products of the two types reach here (2107 and 1205 T/s).  A product comes every 46 cycles of a wave's turn, not
+// 32, as each fragment is read from LDS by all eight waves, and the vector instructions of the SIMD's other wave take 5
+// to 7 cycles each beside them.  16345 packed tokens, 8 / 2 heads of 256: 437 us, 840 TFLOP/s (fp32 725 us).  Without turns,
+// the waves of a SIMD took 5 to 8% longer; with V widened in the probabilities' turn, or the loads sent for there, longer as well.
 template <bool BF16, int D>
 __global__ __launch_bounds__(512, 2) void attn_i8_tile_kernel(const AttnI8 a) {
   constexpr int E = BF16 ? 2 : 4, kTile = tile_rows(BF16), NR = kTile / 8, NP = Row<BF16>::NP;
@@ -387,8 +401,8 @@ __global__ __launch_bounds__(512, 2) void attn_i8_tile_kernel(const AttnI8 a) {
   const int end = min(sees(r0 + kTile - 1), piece);
   if (at.split > 0 && end <= 0) return;   // (a unit of no key that the tile sees)
 
-  // A thread's place in a stage is row tid / CH, chunk tid % CH.  (What follows from the thread's number alone is formed where it
-  // is used, by tid_here: held over the loop it would not fit the registers.)
+  // A thread's place in a stage is row tid / CH, chunk tid % CH.  (What follows from the thread's number alone is formed
+  // where it is used, by tid_here: held over the loop it would not fit the registers.)
   const char* kp = static_cast<const char*>(a.k.p) + (at.ks + k0) * a.k.ld + kvh * a.k.hs;
   const char* vp = static_cast<const char*>(a.v.p) + (at.ks + k0) * a.v.ld + kvh * a.v.hs;
   const uint32_t kld = (uint32_t)a.k.ld, vld = (uint32_t)a.v.ld;   // (below 2^24: the entry point's rule)
@@ -398,11 +412,13 @@ __global__ __launch_bounds__(512, 2) void attn_i8_tile_kernel(const AttnI8 a) {
   const int64_t sld = wave == 0 ? a.ldks : a.ldvs;
   auto stage = [&](int it) __attribute__((always_inline)) {
     const int last = end - 1 - SK * it, slot = it & (kRing - 1);   // last: the last row that is there
-    const uint32_t t = tid_here(), pr = t / CH, pc = t % CH, r = min(pr, (uint32_t)last), kc = 16 * (pc ^ (D == 256 ? pr & 15 : (pr >> 1) & 7)), vc = 16 * pc;
+    const uint32_t t = tid_here(), pr = t / CH, pc = t % CH, r = min(pr, (uint32_t)last);
+    const uint32_t kc = 16 * (pc ^ (D == 256 ? pr & 15 : (pr >> 1) & 7)), vc = 16 * pc;
     load_to_lds<5>(kp + (int64_t)it * SK * a.k.ld, __umul24(r, kld) + kc, lds0 + slot * 8192 + 1024 * wave);
     load_to_lds<5>(vp + (int64_t)it * SK * a.v.ld, __umul24(r, vld) + vc, lds0 + kRaw + slot * 8192 + 1024 * wave);
     if (scales)
-      load_word_to_lds<5>(sp + it * SK * sld, 4 * __umul24(min(t % SK, (uint32_t)last), (uint32_t)sld), lds0 + kS + (it & (2 * kRing - 1)) * kScales + 256 * wave);
+      load_word_to_lds<5>(sp + it * SK * sld, 4 * __umul24(min(t % SK, (uint32_t)last), (uint32_t)sld),
+                          lds0 + kS + (it & (2 * kRing - 1)) * kScales + 256 * wave);
   };
   const int n = seq_tiles(end, SK);
 #pragma unroll
@@ -458,8 +474,8 @@ __global__ __launch_bounds__(512, 2) void attn_i8_tile_kernel(const AttnI8 a) {
   // a lane holds four neighbours of its row from place(i) on, i below NQ
   auto place = [&](int i) { return BF16 ? 32 * (i >> 2) + 8 * (i & 3) + 4 * h : 16 * i + 4 * h; };
   constexpr int KS = 4 * LR;   // a lane's quad i of scores is of the keys KS i + 4 h ..
-  // A turn at the matrix pipe: O^T += V^T P^T of stage it - 1 (not in the FIRST turn), and S^T of stage it, digit by digit, if
-  // there is one (not in the LAST); between the products the thread's 16 codes of stage it of V are widened.  The
+  // A turn at the matrix pipe: O^T += V^T P^T of stage it - 1 (not in the FIRST turn), and S^T of stage it, digit by
+  // digit, if there is one (not in the LAST); between the products the thread's 16 codes of stage it of V are widened.  The
   // fragments of V and K come from LDS kAhead products before they are used: the order is the program's, which the
   // compiler left to itself does not keep (it waited for each fragment right after asking for it).
   constexpr int kAhead = 3, NV = NT * NK / 2, NKF = NF * NM;
@@ -468,7 +484,8 @@ __global__ __launch_bounds__(512, 2) void attn_i8_tile_kernel(const AttnI8 a) {
   auto matrix = [&](int it, auto FIRST, auto LAST) __attribute__((always_inline)) {
     constexpr bool first = decltype(FIRST)::value, last = decltype(LAST)::value;
     constexpr int i0 = first ? NV : 0, i1 = last ? NV : NV + NKF;
-    const uint32_t tid = tid_here(), ln = tid & 63, h = ln / NR, j = ln % NR, vx = (ln & 15) >> 2;   // vx: the key of four that this lane's transposing read brings
+    const uint32_t tid = tid_here(), ln = tid & 63, h = ln / NR, j = ln % NR;
+    const uint32_t vx = (ln & 15) >> 2;   // the key of four that this lane's transposing read brings
     const uint32_t kl = lds0 + (it & (kRing - 1)) * 8192 + j * D + 16 * (h ^ (D == 256 ? j & 15 : (j >> 1) & 7));
     const uint32_t vl = lds0 + kV + ((it - 1) & 1) * kWide + (4 * h + vx) * D * 2 +
                         ((BF16 ? 32 * ((ln >> 4) & 1) : 0) ^ (64 * vx + 32 * (h & 1))) + 16 * ((ln & 3) >> 1) + 8 * (ln & 1);
@@ -476,7 +493,8 @@ __global__ __launch_bounds__(512, 2) void attn_i8_tile_kernel(const AttnI8 a) {
     auto ask = [&](auto I, u32x4& to) __attribute__((always_inline)) {
       constexpr int i = I;
       if constexpr (i < NV) {
-        // tile t of the elements, keys 16 kk + 4 h .., + 8 of element 32 t + lane % 32 (fp32: 32 kk + 4 h .., + 16 of 16 t + lane % 16)
+        // tile t of the elements, keys 16 kk + 4 h .., + 8 of element 32 t + lane % 32 (fp32: 32 kk + 4 h .., + 16 of
+        // 16 t + lane % 16)
         constexpr int t = i / (NK / 2), kk = i % (NK / 2);
         const uint32_t p = (BF16 ? (vl ^ (64 * (t & 3))) + 256 * (t >> 2) : (vl ^ (32 * (t & 7))) + 256 * (t >> 3)) + 4 * KS * D * kk;
         union {
@@ -545,41 +563,36 @@ __global__ __launch_bounds__(512, 2) void attn_i8_tile_kernel(const AttnI8 a) {
     constexpr bool part = decltype(PART)::value;
     const int h = (uint32_t)(tid_here() & 63) / NR, kb = SK * it + 4 * h;
     float st[4 * NK];
-    // bfloat16: the scores without the row's unit, which the exponent's multiplication brings; where a scale of K could take
-    // a whole number beyond a float's range, and in fp32 (a sum of three digits), the unit comes first
-    bool far = !BF16;
+    // bfloat16: the scores without the row's unit, which the exponent's multiplication brings.  Where a scale of K could take
+    // a whole number beyond a float's range, 2^32 goes from the scales to the units; as a branch hardly any stage takes it.
+    float unit = fac;
     if constexpr (BF16) {
-      bool any = false;
+      bool far = false;
 #pragma unroll
-      for (int q = 0; q < NSC; ++q) any |= !(fabsf(ksc[q]) < 0x1p96f);
-      far = __ballot(any) != 0;
+      for (int q = 0; q < NSC; ++q) far |= !(fabsf(ksc[q]) < 0x1p96f);
+      if (__ballot(far) != 0) {
+        unit = fminf(fac * 0x1p32f, 0x1.fffffep127f);
+#pragma unroll
+        for (int q = 0; q < NSC; ++q) ksc[q] *= 0x1p-32f;
+      }
     }
-    const float after = far ? 1.0f : fac;
-    auto scores = [&](auto FAR) __attribute__((always_inline)) {
-      each<NK>([&](auto I) {
-        each<4>([&](auto R) {
-          constexpr int i = I, r = R;
-          auto d = [&](int p) { return BF16 ? dg[p][i / 4][4 * (i % 4) + r] : dg[p][i % NM][r]; };
-          float x = (float)(d(0) * 256 + d(1));   // a whole number below 2^30
-          if constexpr (!BF16)
-            x = __builtin_fmaf(x, 256.0f * fac, (float)d(NP - 1) * fac);
-          else if constexpr (decltype(FAR)::value)
-            x *= fac;
-          st[4 * i + r] = x * lane_of_16<(4 * i + r) % 16>(ksc[(4 * i + r) / 16]);
-          if (part && kb + KS * i + r >= seen) st[4 * i + r] = kNegInf;
-        });
+    each<NK>([&](auto I) {
+      each<4>([&](auto R) {
+        constexpr int i = I, r = R;
+        auto d = [&](int p) { return BF16 ? dg[p][i / 4][4 * (i % 4) + r] : dg[p][i % NM][r]; };
+        float x = (float)(d(0) * 256 + d(1));   // a whole number below 2^30
+        // (fp32: the row's unit first, a sum of three digits times a large scale could overflow)
+        if constexpr (!BF16) x = __builtin_fmaf(x, 256.0f * fac, (float)d(NP - 1) * fac);
+        st[4 * i + r] = x * lane_of_16<(4 * i + r) % 16>(ksc[(4 * i + r) / 16]);
+        if (part && kb + KS * i + r >= seen) st[4 * i + r] = kNegInf;
       });
-    };
-    if (BF16 && far)
-      scores(std::true_type{});
-    else
-      scores(std::false_type{});
+    });
     float mt = st[0];
 #pragma unroll
     for (int r = 1; r < 4 * NK; ++r) mt = fmaxf(mt, st[r]);
     if constexpr (!BF16) mt = fmaxf(mt, xor_perm<16>(mt));
     mt = fmaxf(mt, xor_perm<32>(mt));
-    if constexpr (BF16) mt = mt == kNegInf ? kNegInf : mt * after;   // (0 times it is not it)
+    if constexpr (BF16) mt = mt == kNegInf ? kNegInf : mt * unit;   // (0 times it is not it)
     const bool up = mt > m + 8.0f;                       // (as in the form for few rows)
     if (__ballot(up) != 0) {
       const float mn = up ? mt : m, al = __builtin_amdgcn_exp2f(m - (mn == kNegInf ? 0.0f : mn));
@@ -591,12 +604,18 @@ __global__ __launch_bounds__(512, 2) void attn_i8_tile_kernel(const AttnI8 a) {
         for (int r = 0; r < VW; ++r) acc[t][r] *= al;
     }
     const float mu = m == kNegInf ? 0.0f : m;
+    // (bfloat16: the exponent's product is not rounded, the maximum was: 2^-24 of a score of 2^31 would be too large a power)
+    if (BF16 && __ballot(fabsf(mu) >= 0x1p20f) != 0) {
+#pragma unroll
+      for (int i = 0; i < 4 * NK; ++i) st[i] *= unit;
+      unit = 1.0f;
+    }
     float ps = 0.0f;
     each<NK>([&](auto I) {
       each<4>([&](auto R) {
         constexpr int i = I, r = R;
         const bool hidden = part && kb + KS * i + r >= seen;
-        float p = __builtin_amdgcn_exp2f(BF16 ? __builtin_fmaf(st[4 * i + r], after, -mu) : st[4 * i + r] - mu);
+        float p = __builtin_amdgcn_exp2f(BF16 ? __builtin_fmaf(st[4 * i + r], unit, -mu) : st[4 * i + r] - mu);
         if (BF16 && hidden) p = 0.0f;   // (a unit of 0)
         ps += p;
         const float v = p * lane_of_16<(4 * i + r) % 16>(vsc[(4 * i + r) / 16]);
@@ -619,13 +638,13 @@ __global__ __launch_bounds__(512, 2) void attn_i8_tile_kernel(const AttnI8 a) {
     }
     __builtin_amdgcn_sched_barrier(0);
   };
-  // The two waves of a SIMD (w and w + 4) take turns at the matrix pipe: while the one forms stage it - 1's outputs and stage
-  // it's scores, the other turns its scores into probabilities, and a barrier ends each turn.  In turn t = 0, 1 .. the first four
-  // waves are at the matrix pipe when t is even, with it = t / 2, and at the probabilities of stage (t - 1) / 2 when t is odd; the
-  // last four are one turn behind.  In its turn at the matrix pipe a wave also widens its part of stage it (in turn 2 it or 2 it + 1;
-  // read from turn 2 it + 2 on; the place held stage it - 2, last read in turn 2 it - 1), sends for its part of stage it + 3
-  // (in the place of stage it - 1, whose K was last read in turn 2 it - 1; the scales, read until turn 2 it, have places of
-  // their own) and waits for its part of stage it + 1 (read from turn 2 it + 2 on).
+  // The two waves of a SIMD (w and w + 4) take turns at the matrix pipe: while the one forms stage it - 1's outputs and
+  // stage it's scores, the other turns its scores into probabilities, and a barrier ends each turn.  In turn t = 0, 1 .. the
+  // first four waves are at the matrix pipe when t is even, with it = t / 2, and at the probabilities of stage (t - 1) / 2
+  // when t is odd; the last four are one turn behind.  In its turn at the matrix pipe a wave also widens its part of stage it
+  // (in turn 2 it or 2 it + 1; read from turn 2 it + 2 on; the place held stage it - 2, last read in turn 2 it - 1), sends for
+  // its part of stage it + 3 (in the place of stage it - 1, whose K was last read in turn 2 it - 1; the scales, read until
+  // turn 2 it, have places of their own) and waits for its part of stage it + 1 (read from turn 2 it + 2 on).
   const int second = wave >> 2;
   if (n > 0) {
     landed(min(n - 1, 2));
@@ -633,7 +652,7 @@ __global__ __launch_bounds__(512, 2) void attn_i8_tile_kernel(const AttnI8 a) {
     if (second) barrier();
     const int full = max(min(sees(r0), end), 0) / SK;  // stages that every row sees whole
     auto turns = [&](int it, auto FIRST, auto PART) __attribute__((always_inline)) {
-      __builtin_amdgcn_s_setprio(2);   // (before the other wave's vector instructions: 2.79 -> 2.58 us a stage)
+      __builtin_amdgcn_s_setprio(2);   // (before the other wave's vector instructions: 8% of a stage)
       if (it + kRing - 1 < n) stage(it + kRing - 1);
       matrix(it, FIRST, std::false_type{});
       __builtin_amdgcn_s_setprio(0);

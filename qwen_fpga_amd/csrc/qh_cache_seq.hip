@@ -39,10 +39,11 @@ __device__ __forceinline__ void store8(char* p, const float (&x)[8]) {
 }
 
 // y = x / sqrt(mean(x^2) + eps) * (1 + w) of each head, then elements i and i + rot / 2 (i < rot / 2) turned by the
-// angle pos * theta^(-2 i / rot).  WPT waves take a token, D / 8 lanes a head's row; the first rows are on their way while a wave
-// forms the token's angles, counted in turns in 64 bits (a float holds an angle of 131071 to 2^-7), and a lane
-// reads the other element of a pair from the lane that holds it.  Bound by memory: 16345 tokens of 8 and 2 heads of 256 in
-// bfloat16 (168 MB) 38.7 us, 4.3 TB/s; with two rows of a wave on their way at once 39.9, with five (fewer waves) 45.
+// angle pos * theta^(-2 i / rot).  WPT waves take a token, D / 8 lanes a head's row; the first rows are on their way while
+// a wave forms the token's angles, counted in turns in 64 bits (a float holds an angle of 131071 to 2^-7), and a lane reads
+// the other element of a pair from the lane that holds it.  Bound by memory: 16345 tokens of 8 and 2 heads of 256 in bfloat16
+// (168 MB) 36.7 us, 4.6 TB/s; with two rows of a wave on their way at once 39.9, with five (fewer waves) 45; 1500 in fp32
+// (31 MB) 9.6 us; one token 3.3, a launch.
 template <bool BF16, int D, int WPT>
 __global__ __launch_bounds__(256) void norm_rope_kernel(const NormRope a) {
   constexpr int L = D / 8, E = BF16 ? 2 : 4, NG = 64 / L;   // rows of a wave at a time
@@ -134,7 +135,8 @@ struct RowsAt {
 };
 
 // The scale is the row's largest magnitude over 127 and a code rint(x / scale), half to even, as quant_rows has them, bit
-// for bit; a row that is not finite gets scale NaN and codes 0.
+// for bit; a row that is not finite gets scale NaN and codes 0.  Bound by memory: 16345 bfloat16 tokens of 2 heads of 256
+// (51 MB) 15.1 us, 3.4 TB/s; 35 tokens 3.1, a launch.
 template <bool BF16, int D, int R>
 __global__ __launch_bounds__(256) void cache_write_kernel(const CacheSeq a) {
   constexpr int L = D / 8, E = BF16 ? 2 : 4;
@@ -172,6 +174,8 @@ __global__ __launch_bounds__(256) void cache_write_kernel(const CacheSeq a) {
   }
 }
 
+// Code times scale in fp32, rounded once more to bfloat16.  Bound by memory: 60001 bfloat16 tokens of 2 heads of 256 (185
+// MB) 35.2 us, 5.2 TB/s; 641 fp32 ones 3.8, a launch.
 template <bool BF16, int D, int R>
 __global__ __launch_bounds__(256) void cache_read_kernel(const CacheSeq a) {
   constexpr int E = BF16 ? 2 : 4;
@@ -195,12 +199,13 @@ __global__ __launch_bounds__(256) void cache_read_kernel(const CacheSeq a) {
     float x[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = (float)(int8_t)(q[u][i >> 2] >> (8 * (i & 3))) * s[u];
-    store8<BF16>(const_cast<char*>(static_cast<const char*>(a.x[side])) + (at.tok * a.ld[side] + (r - side * a.heads) * a.hs[side] + 8 * at.c) * E, x);
+    char* to = const_cast<char*>(static_cast<const char*>(a.x[side]));
+    store8<BF16>(to + (at.tok * a.ld[side] + (r - side * a.heads) * a.hs[side] + 8 * at.c) * E, x);
   }
 }
 
-// One row at a time up to 16384 of them (2048 workgroups of heads of 256): 35 tokens of 2 heads written in 3.1 us and 4.0 four at a time, 641
-// read in 3.3 and 3.9; 16345 written in 16.6 and 15.2, 60001 read in 62 and 35.
+// One row at a time up to 16384 of them (2048 workgroups of heads of 256): 35 tokens of 2 heads written in 3.1 us and in
+// 4.0 four at a time, 641 read in 3.3 and 3.9; 16345 written in 16.6 and 15.2, 60001 read in 62 and 35.
 template <typename One, typename Four>
 hipError_t launch_rows(const CacheSeq& a, One one, Four four, hipStream_t s) {
   const bool few = 2ll * a.tokens * a.heads <= 16384;
@@ -224,9 +229,11 @@ hipError_t launch_norm_rope(const NormRope& a, hipStream_t s) {
       four<<<(unsigned)a.tokens, 256, 0, s>>>(a);
   };
   if (a.dim == 256)
-    a.bf16 ? go(norm_rope_kernel<true, 256, 1>, norm_rope_kernel<true, 256, 4>) : go(norm_rope_kernel<false, 256, 1>, norm_rope_kernel<false, 256, 4>);
+    a.bf16 ? go(norm_rope_kernel<true, 256, 1>, norm_rope_kernel<true, 256, 4>)
+           : go(norm_rope_kernel<false, 256, 1>, norm_rope_kernel<false, 256, 4>);
   else
-    a.bf16 ? go(norm_rope_kernel<true, 128, 1>, norm_rope_kernel<true, 128, 4>) : go(norm_rope_kernel<false, 128, 1>, norm_rope_kernel<false, 128, 4>);
+    a.bf16 ? go(norm_rope_kernel<true, 128, 1>, norm_rope_kernel<true, 128, 4>)
+           : go(norm_rope_kernel<false, 128, 1>, norm_rope_kernel<false, 128, 4>);
   return hipGetLastError();
 }
 

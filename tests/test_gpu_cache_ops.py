@@ -479,9 +479,10 @@ def test_attention_bounds_too_small_or_large(q, torch_cuda, monkeypatch, bf16):
 
 @pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
 def test_attention_large_scores(q, torch_cuda, bf16):
-    """Scores far apart (one key takes all), equal scores, a scale of 0 (the mean of the keys), a negative one."""
+    """Scores far apart (one key takes all), equal scores, a scale of 0 (the mean of the keys), a negative one, and
+    scores of 2^40 (whose rounding is more than a power of two holds)."""
     torch = torch_cuda
-    for scale in (4.0, 0.0, -0.3):
+    for scale in (4.0, 0.0, -0.3, 1e10):
         inp, at = attn_inputs(torch, 7, [20, 1], [30, 400], 2, 1, 128, bf16)
         dev, want = both(torch, inp, at, [20, 1], [30, 400], scale, bf16)
         attn_check(torch, attn_run(q, torch, dev, [20, 1], [30, 400], at, scale=scale), want, bf16)
