@@ -300,7 +300,7 @@ int qh_attention_seq(void* out, int64_t ldo, int64_t hso, const void* q, int64_t
  * (y = x / sqrt(mean(x^2) + eps) * (1 + w), w = q_norm or k_norm [head_dim] fp32, 16-byte aligned), then elements i and
  * i + rope_dim / 2 of it (i < rope_dim / 2) turned by pos[token] * theta^(-2 i / rope_dim); the others stay
  * (qh_rope_cos_sin and qh_apply_rope are that for rope_dim 64 and theta 1e7).  rope_dim: a multiple of 16, 0 .. head_dim.
- * pos [tokens] int32, any value.  The angles are formed in 64 bits, where qh_rope_cos_sin rounds the position times the
+ * theta: 1 or more.  pos [tokens] int32, any value.  The angles are formed in 64 bits, where qh_rope_cos_sin rounds the position times the
  * frequency to fp32 as the reference does: at position p the two are up to p 2^-24 apart, in radians.  All arithmetic is
  * fp32, an output is rounded once.  q_out (k_out) may be q (k) itself: the same pointer and strides. */
 int qh_qk_norm_rope_seq(void* q_out, int64_t ldqo, int64_t hsqo, void* k_out, int64_t ldko, int64_t hsko, const void* q,

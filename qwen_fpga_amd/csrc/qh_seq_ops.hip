@@ -201,7 +201,7 @@ int qh_qk_norm_rope_seq(void* q_out, int64_t ldqo, int64_t hsqo, void* k_out, in
                         const float* k_norm, const int32_t* pos, int tokens, int heads, int kv_heads, int head_dim, int rope_dim,
                         double theta, float eps, void* stream) {
   if (!type_ok(type) || tokens < 0 || heads <= 0 || kv_heads <= 0 || (head_dim != 128 && head_dim != 256) || rope_dim < 0 ||
-      rope_dim > head_dim || rope_dim % 16 != 0 || !std::isfinite(theta) || theta <= 0.0 || !std::isfinite(eps) || eps < 0.0f)
+      rope_dim > head_dim || rope_dim % 16 != 0 || !std::isfinite(theta) || theta < 1.0 || !std::isfinite(eps) || eps < 0.0f)
     return QH_EINVAL;
   if (tokens == 0) return QH_OK;
   if (tokens > QH_ROPE_MAX_TOKENS || (int64_t)tokens * ((int64_t)heads + kv_heads) > kMaxUnits) return QH_ERANGE;
@@ -260,8 +260,9 @@ int qh_kv_cache_read_i8(void* k, int64_t ldk, int64_t hsk, void* v, int64_t ldv,
 }
 
 size_t qh_attention_seq_i8_workspace(int q_rows, int n_seq, int max_q, int max_k, int heads, int kv_heads, int head_dim, int type) {
-  if (!type_ok(type) || q_rows <= 0 || n_seq <= 0 || n_seq > QH_ATTN_MAX_SEQ || max_q < 0 || max_k < 0 || max_k > kMaxKeys || heads <= 0 || kv_heads <= 0 ||
-      heads % kv_heads != 0 || (head_dim != 128 && head_dim != 256) || (int64_t)q_rows * heads > kMaxUnits)
+  if (!type_ok(type) || q_rows <= 0 || n_seq <= 0 || n_seq > QH_ATTN_MAX_SEQ || max_q < 0 || max_k < 0 || max_k > kMaxKeys ||
+      heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || (head_dim != 128 && head_dim != 256) ||
+      (int64_t)q_rows * heads > kMaxUnits)
     return 0;
   return attn_i8_form(q_rows, n_seq, max_q, max_k, heads, kv_heads, head_dim, type == QH_BF16).bytes;
 }

@@ -106,7 +106,7 @@ def changed(kw, at):
 
 @pytest.mark.parametrize("kw", [
     dict(type=2), dict(tokens=-1), dict(heads=0), dict(kv_heads=0), dict(d=64), dict(rope_dim=-16), dict(rope_dim=8), dict(rope_dim=144),
-    dict(theta=0.0), dict(theta=float("nan")), dict(theta=float("inf")), dict(eps=-1.0), dict(eps=float("nan")), dict(q_out=None),
+    dict(theta=0.0), dict(theta=0.999), dict(theta=float("nan")), dict(theta=float("inf")), dict(eps=-1.0), dict(eps=float("nan")), dict(q_out=None),
     dict(k_out=None), dict(q=None), dict(k=None), dict(q_norm=None), dict(k_norm=None), dict(pos=None), dict(ldqo=128), dict(ldqo=0),
     dict(hsqo=64), dict(ldko=64), dict(ldq=258), dict(hsk=128, ldk=-128), "q_out+4", "k+8", "q_norm+4", "k_norm+8", "q_out=k", "q_out=k_out",
     "k_out=q", "k_out=pos", "q_out=q_norm", "q+128", dict(ldq=128, hsq=384),

@@ -89,6 +89,12 @@ def test_norm_rope(q, torch_cuda, tokens, h, kvh, d, rot, bf16):
     q2, k2 = dev[0].transpose(0, 1).contiguous().transpose(0, 1), kk.cuda()
     q.qk_norm_rope_seq(q2, k2, q2, k2, *dev[2:], rot)
     assert torch.equal(q2, qo) and torch.equal(k2, ko)
+    # in place in the rows of one projection, queries and keys beside each other and beside others' columns
+    row = torch.full((tokens, (h + kvh) * d + 16), 7.0, dtype=dt, device="cuda")
+    q3, k3 = row[:, :h * d].view(tokens, h, d), row[:, h * d:(h + kvh) * d].view(tokens, kvh, d)
+    q3.copy_(qk[:, :, :d]), k3.copy_(kk)          # (dev[0] may have been q2)
+    q.qk_norm_rope_seq(q3, k3, q3, k3, *dev[2:], rot)
+    assert torch.equal(q3, qo) and torch.equal(k3, ko) and (row[:, (h + kvh) * d:] == 7).all()
 
 
 def test_norm_rope_is_the_one_token_ops(q, torch_cuda):
@@ -511,9 +517,10 @@ def test_attention_queries_of_any_size(q, torch_cuda, bf16, size):
 @pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
 @pytest.mark.parametrize("max_q", [1, LARGE])
 @pytest.mark.parametrize("d", [128, 256])
-def test_attention_keys_near_the_end_of_the_range(q, torch_cuda, bf16, max_q, d):
+def test_attention_keys_near_the_end_of_the_range(q, torch_cuda, monkeypatch, bf16, max_q, d):
     """Scales of K near 2^106: a sum of digits times codes (2^23 and more) times the scale is beyond a float, the score is not."""
     torch = torch_cuda
+    monkeypatch.setattr(sys.modules[__name__], "MAX_Q", max_q)      # (the bound of the form)
     lens, ctx = [70, 1], [150, 300]
     inp, at = attn_inputs(torch, 16, lens, ctx, 2, 1, d, bf16)
     inp = list(inp)
@@ -768,6 +775,41 @@ def test_two_streams(q, torch_cuda):
         assert torch.equal(a, res[0][0]) and torch.equal(b, res[0][1])
         assert torch.equal(o[0].cpu(), (inp[1].float() * inp[2][..., None]).bfloat16())
         assert torch.equal(c[0].cpu(), code_oracle(torch, o[0].cpu())[0])
+
+
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+@pytest.mark.parametrize("max_q", [4, LARGE])
+def test_attention_replayed(q, torch_cuda, monkeypatch, bf16, max_q):
+    """A call whose keys are split (a second kernel joins them), captured once and replayed with other lengths and ranges on the
+    device, eager work between: the eager call's bits each time, rows behind the last sequence as they were."""
+    torch = torch_cuda
+    monkeypatch.setattr(sys.modules[__name__], "MAX_Q", max_q)      # (the bound of the form)
+    h, kvh, d, rows, t, n, max_k = 4, 2, 128, 6000, 12, 4, 6000
+    inp, _ = attn_inputs(torch, 17, [t], [rows], h, kvh, d, bf16)
+    dev = [x.cuda() for x in inp]
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    cu, at, kl = i32([0] * (n + 1)), torch.zeros(n, dtype=torch.int64, device="cuda"), i32([0] * n)
+    out = torch.empty(t, h, d, dtype=dev[0].dtype, device="cuda")
+    nb = q.attention_seq_i8_workspace(t, n, max_q, max_k, h, kvh, d, q.BF16 if bf16 else q.F32)
+    assert nb > 0
+    ws = [torch.full((nb,), 0xFF, dtype=torch.uint8, device="cuda") for _ in range(2)]     # the graph's own, and one for eager calls
+    call = lambda w: q.attention_seq_i8(out, *dev, cu, at, kl, w, max_q, max_k)
+    call(ws[1])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(ws[0])
+    for lens, ctx, k0 in (([1, 1, 1, 1], [5000, 3, 600, 4000], [0, 17, 5400, 2000]), ([4, 0, 3, 1], [6000, 9, 2, 1], [0, 5, 5998, 3]),
+                          ([0, 0, 0, 2], [0, 0, 0, 3100], [0, 0, 0, 2900]), ([4, 4, 4, 0], [900, 800, 700, 0], [1, 2000, 5300, 0])):
+        cu.copy_(i32(starts(lens))), at.copy_(torch.tensor(k0)), kl.copy_(i32(ctx))
+        got = []
+        for run in (lambda: call(ws[1]), graph.replay, graph.replay):
+            out.fill_(7.0)
+            run()
+            torch.cuda.synchronize()
+            got.append(out.clone())
+        assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2]) and (got[0][sum(lens):] == 7).all()
+        want = attn_oracle(torch, inp[0][:sum(lens)], *inp[1:], lens, ctx, k0, 1 / math.sqrt(d), bf16)
+        attn_check(torch, got[0], want, bf16)
 
 
 @pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
