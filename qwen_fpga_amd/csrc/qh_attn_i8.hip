@@ -740,6 +740,7 @@ AttnForm attn_i8_form(int64_t q_rows, int n_seq, int max_q, int max_k, int heads
     }
     f.bytes = (size_t)f.limit * tile_part_floats(f.tile, dim) * sizeof(float);
   } else if (max_k > kMinChunk + few_whole((q_rows * G + 15) / 16 * kv_heads)) {
+    // (splitting may pay, with a second kernel: the workgroups, which know the lengths, decide)
     f.limit = 1;
     f.bytes = (size_t)(seq_tiles_max(q_rows * G, n_seq, 16) * kv_heads + kFill) * part_floats(dim) * sizeof(float);
   }
