@@ -81,8 +81,9 @@ __device__ __forceinline__ bool find_unit(const AttnSeq& a, int b, Unit& o) {
       o.nsplit = of(ns);
       o.chunk = chunk;
       const int in = b - base - (of(JOIN ? it : iu) - of(JOIN ? tiles : tiles * ns));
-      o.tile = JOIN ? in : in / o.nsplit;
-      o.split = JOIN ? 0 : in - o.tile * o.nsplit;
+      const int nth = JOIN ? in : in / o.nsplit;
+      o.tile = WHOLE && !JOIN ? of(tiles) - 1 - nth : nth;   // (the last tiles see the most keys: they start first)
+      o.split = JOIN ? 0 : in - nth * o.nsplit;
       o.first = first + of(iu) - of(tiles * ns) + o.tile * o.nsplit;
       return o.tile >= 0 && o.tile < of(tiles);   // (bounds that overlap can make more tiles than an int counts)
     }

@@ -130,9 +130,10 @@ __device__ __forceinline__ void each(F&& f) {
 // Bound by memory where there are keys for all CUs: one token behind 131070 keys, 8 / 2 heads of 256 (135 MB), 28.3 us, 4.8
 // TB/s (and 8 to join).  With fewer keys by what follows one after the other: one key 7 us, 128 more for each workgroup 1.7
 // us more; 16 tokens of 42000 keys together (43 MB) 16.5, 2.6 TB/s.  With many rows by the vector instructions that widen V,
-// which every 16 rows do again: 1500 tokens 43 us (fp32 51).  Three instructions a code instead of 1.5 and spilled
-// registers took twice as long; Q asked for before K, no loads behind the last step, chunks of a multiple of 128 keys and 384,
-// 768 or 1024 units instead of 512 made no difference or took longer.
+// which every 16 rows do again: 1500 tokens 39 us (fp32 42).  The tiles that see the most keys start first (2000 tokens in
+// fp32 68 -> 61 us).  Three instructions a code instead of 1.5 and spilled registers took twice as long; Q asked for before K,
+// no loads behind the last step, chunks of a multiple of 128 keys and 384, 768 or 1024 units instead of 512 made no difference
+// or took longer.
 template <bool BF16, int D>
 __global__ __launch_bounds__(256, 2) void attn_i8_split_kernel(const AttnI8 a) {
   constexpr int NP = Row<BF16>::NP;       // digits of Q, parts of P
@@ -351,7 +352,9 @@ __global__ __launch_bounds__(256, 2) void attn_i8_split_kernel(const AttnI8 a) {
         }
       }
   } else {
-    float* pp = a.part + (size_t)blockIdx.x * part_floats(D);   // (unit first + split, kv head)
+    const int64_t place = (int64_t)(at.first + at.split) * a.kv_heads + kvh;
+    if (at.first < 0 || place >= (int64_t)gridDim.x) return;   // (bounds that overlap can make more units than there is place for)
+    float* pp = a.part + place * part_floats(D);
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -725,10 +728,10 @@ AttnForm attn_i8_form(int64_t q_rows, int n_seq, int max_q, int max_k, int heads
   AttnForm f = {0, 0, 0};
   // Pairs of a query row and a key it sees, about (where there is one sequence, or several of equal length).  The form for
   // prompts takes a workgroup of 512 threads a CU and 2 us for every 32 keys however few rows there are, the one for few
-  // rows takes half as long again where there is work for all CUs.  few / prompts, bfloat16, 8 / 2 heads of 256: 1024
-  // tokens 24 / 47 us, 1500 41 / 50, 2000 59 / 59, 6000 382 / 210, 512 behind 1488 29 / 47, 512 behind 3488 75 / 54, 300
-  // behind 15700 160 / 79, 64 behind 31936 59 / 75; 8 / 8 heads of 128: 1500 27 / 39, 2000 40 / 46, 6000 261 / 148; fp32,
-  // 8 / 2 heads of 256: 1500 47 / 51, 2000 67 / 68, 6000 425 / 353, 512 behind 3488 78 / 56.
+  // rows half as long again where there is work for all CUs.  few / prompts, bfloat16, 8 / 2 heads of 256: 1024 tokens 22
+  // / 47 us, 1500 39 / 49, 2000 55 / 58, 3000 109 / 84, 6000 356 / 210, 512 behind 1488 29 / 47, 512 behind 3488 74 / 54, 300
+  // behind 15700 160 / 79, 64 behind 31936 57 / 75; 8 / 8 heads of 128: 1500 25 / 39, 2000 37 / 47, 3000 75 / 61; fp32, 8 / 2
+  // heads of 256: 1500 42 / 51, 2000 61 / 68, 6000 397 / 355, 512 behind 3488 78 / 56.
   const int64_t pairs = q_rows * heads * (std::max(max_k, max_q) - max_q / 2);
   if ((int64_t)max_q * G > 256 && pairs >= 15000000) {
     f.tile = tile_rows(bf16);

@@ -43,7 +43,7 @@ __device__ __forceinline__ void store8(char* p, const float (&x)[8]) {
 // a wave forms the token's angles, counted in turns in 64 bits (a float holds an angle of 131071 to 2^-7), and a lane reads
 // the other element of a pair from the lane that holds it.  Bound by memory: 16345 tokens of 8 and 2 heads of 256 in bfloat16
 // (168 MB) 36.7 us, 4.6 TB/s; with two rows of a wave on their way at once 39.9, with five (fewer waves) 45; 1500 in fp32
-// (31 MB) 9.6 us; one token 3.3, a launch.
+// (31 MB) 9.1 us; one token 3.3, a launch.
 template <bool BF16, int D, int WPT>
 __global__ __launch_bounds__(256) void norm_rope_kernel(const NormRope a) {
   constexpr int L = D / 8, E = BF16 ? 2 : 4, NG = 64 / L;   // rows of a wave at a time
@@ -221,9 +221,12 @@ hipError_t launch_rows(const CacheSeq& a, One one, Four four, hipStream_t s) {
 }  // namespace
 
 hipError_t launch_norm_rope(const NormRope& a, hipStream_t s) {
-  // Waves of a token: four up to 1024 tokens, which fill the chip's 1024 SIMDs once.
+  // Waves of a token: four where there are few tokens for the chip's 1024 SIMDs, and for many rows of fp32.  Four and one, 8
+  // and 2 heads of 256, bfloat16: 1100 tokens 5.9 and 7.6 us, 1500 7.2 and 8.2, 2000 8.9 and 8.7, 4000 12.8 and 11.4, 16000
+  // 45 and 36; fp32: 1100 8.0 and 9.0, 1500 9.1 and 9.6, 2000 10.8 and 10.4, 4000 20.0 and 20.2, 8000 34.8 and 39, 16000 63
+  // and 67.
   auto go = [&](auto one, auto four) {
-    if (a.tokens > 1024)
+    if (a.tokens > 1792 && (a.bf16 || a.tokens < 4096))
       one<<<(unsigned)((a.tokens + 3) / 4), 256, 0, s>>>(a);
     else
       four<<<(unsigned)a.tokens, 256, 0, s>>>(a);
