@@ -65,6 +65,7 @@ def rope_check(torch, got, want, bf16):
 ROPE = [  # tokens, heads, kv heads, dim, rotated
     (1, 8, 2, 256, 64), (1, 1, 1, 128, 128), (2, 3, 1, 256, 256), (5, 6, 2, 128, 32), (7, 16, 4, 128, 16), (33, 8, 2, 256, 0),
     (64, 32, 1, 256, 64), (65, 2, 2, 128, 64), (300, 8, 8, 128, 96), (1000, 8, 2, 256, 48), (3, 1, 40, 256, 240),
+    (1801, 3, 1, 128, 64), (2000, 5, 2, 256, 48), (4097, 2, 3, 128, 16), (4096, 1, 1, 256, 32),   # another number of waves a token
 ]
 
 
@@ -186,6 +187,7 @@ def cache_new(torch, rows, kvh, d, layout):
 CACHE = [  # tokens, rows, kv heads, dim
     (1, 1, 1, 128), (1, 40, 2, 256), (3, 9, 1, 256), (15, 16, 3, 128), (16, 33, 8, 128), (17, 1000, 2, 256), (129, 200, 5, 128),
     (700, 900, 2, 256), (5, 4000, 40, 256),
+    (3000, 3333, 3, 128), (1700, 2000, 5, 256), (8200, 9000, 1, 128),      # four rows of a token at a time
 ]
 
 
@@ -371,6 +373,10 @@ def both(torch, inp, at, lens, ctx, scale, bf16):
     return [x.cuda() for x in inp], attn_oracle(torch, *inp, lens, ctx, at, scale, bf16)
 
 
+def short(x):
+    return str(x)[:40]
+
+
 ATTN = [  # lens, keys, heads, kv heads, dim
     ([1], [1], 1, 1, 128), ([1], [1], 8, 2, 256), ([1, 1, 1], [7, 300, 1], 8, 2, 256), ([1, 1], [2500, 15], 4, 4, 128),
     ([1], [5000], 8, 2, 256), ([2, 3], [33, 64], 6, 2, 128), ([4], [1000], 16, 1, 128), ([1], [777], 32, 1, 256), ([1], [31], 2, 1, 128),
@@ -378,10 +384,11 @@ ATTN = [  # lens, keys, heads, kv heads, dim
     ([63, 0, 65], [63, 5, 70], 4, 2, 128), ([127, 1], [127, 129], 8, 2, 256), ([129], [400], 2, 1, 256), ([200, 90], [200, 90], 3, 3, 128),
     ([300], [300], 8, 2, 256), ([33], [2000], 2, 1, 128), ([260], [261], 1, 1, 256), ([520], [520], 4, 1, 128), ([5], [5], 3, 1, 256),
     ([200, 1], [1400, 900], 8, 2, 256), ([1] * 70, [1500 - 20 * i for i in range(70)], 4, 1, 128), ([100, 7], [3000, 100], 4, 2, 128),
+    ([1] * 135, [10 + i for i in range(134)] + [6000], 4, 2, 128), ([90, 600], [90, 5000], 2, 1, 128),
 ]
 
 
-@pytest.mark.parametrize("lens,ctx,h,kvh,d", ATTN, ids=str)
+@pytest.mark.parametrize("lens,ctx,h,kvh,d", ATTN, ids=short)
 @pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
 def test_attention(q, torch_cuda, lens, ctx, h, kvh, d, bf16):
     torch = torch_cuda
@@ -599,7 +606,7 @@ def prompts(monkeypatch):
 
 @pytest.mark.parametrize("lens,ctx,h,kvh,d", ATTN + [
     ([700], [3000], 8, 2, 256), ([130, 1], [4100, 2000], 2, 2, 128), ([40], [9000], 4, 4, 128), ([1023, 0, 513], [1023, 4, 800], 4, 1, 256),
-    ([257], [700], 12, 4, 256)], ids=str)
+    ([257], [700], 12, 4, 256)], ids=short)
 @pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
 def test_prompt_form(prompts, q, torch_cuda, lens, ctx, h, kvh, d, bf16):
     test_attention(q, torch_cuda, lens, ctx, h, kvh, d, bf16)
