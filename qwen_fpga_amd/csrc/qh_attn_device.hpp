@@ -33,8 +33,8 @@ constexpr int kFill = 512, kMinChunk = 128;
 // and 17 us, 1024 24 and 28, 512 behind 1488 29 and 32, 100 single tokens of 1500 keys each 44 and 52, one of 500 12
 // and 13; where it splits, 256 tokens behind 7744 95 and 62, 16 single tokens of 900 23 and 17.
 __host__ __device__ __forceinline__ int few_whole(int64_t tiles) { return 384 + (int)(tiles > 192 ? 1536 : 8 * tiles); }
-// Unit b of the split kernel, or (JOIN) the units of row tile b.  WHOLE: no tile is split where that
-// would save no more than joining costs (few_whole).
+// Unit b of the split kernel, or (JOIN) the units of row tile b.  WHOLE: no tile is split where that would save no more
+// than joining costs (few_whole), and a sequence's last tiles come first.
 template <bool JOIN, bool WHOLE = false>
 __device__ __forceinline__ bool find_unit(const AttnSeq& a, int b, Unit& o) {
   const int lane = threadIdx.x & 63, G = a.heads / a.kv_heads;
@@ -96,8 +96,8 @@ __device__ __forceinline__ bool find_unit(const AttnSeq& a, int b, Unit& o) {
 // Partials of a unit and kv head: 16 rows of D sums, their maxima, their sums of exponentials.
 constexpr size_t part_floats(int D) { return 16 * D + 32; }
 
-// Joins the splits of a tile's rows, every fourth row in a workgroup: sixteen waves take every sixteenth split, four
-// in flight, each with a running maximum of its own.
+// Joins the splits of a tile's rows, every gridDim.y-th row in a workgroup: sixteen waves take every sixteenth split,
+// four in flight, each with a running maximum of its own.
 template <bool BF16, int D, bool WHOLE = false>
 __global__ __launch_bounds__(1024) void attn_join_kernel(const AttnSeq a) {
   constexpr int W = D / 64, NW = 16, U = 4;   // elements of a lane; waves; splits in flight

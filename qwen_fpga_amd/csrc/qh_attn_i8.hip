@@ -352,7 +352,7 @@ __global__ __launch_bounds__(256, 2) void attn_i8_split_kernel(const AttnI8 a) {
         }
       }
   } else {
-    const int64_t place = (int64_t)(at.first + at.split) * a.kv_heads + kvh;
+    const int64_t place = ((int64_t)at.first + at.split) * a.kv_heads + kvh;
     if (at.first < 0 || place >= (int64_t)gridDim.x) return;   // (bounds that overlap can make more units than there is place for)
     float* pp = a.part + place * part_floats(D);
 #pragma unroll
