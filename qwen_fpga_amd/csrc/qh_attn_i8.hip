@@ -716,8 +716,11 @@ hipError_t launch(const AttnI8& a, hipStream_t s) {
   const unsigned tiles = (unsigned)(seq_tiles_max(rows, a.n_seq, 16) * a.kv_heads);
   attn_i8_split_kernel<BF16, D><<<a.limit > 0 ? tiles + kFill : tiles, 256, 0, s>>>(a);
   // rows of a tile side by side where there are few tiles (4 tokens behind 29996 keys: 16 workgroups 23 us, 4 36), few
-  // workgroups where there are many, most of which find nothing to join (16 x 128 behind 1872: 4 106 us, 1 97)
-  if (a.limit > 0) attn_join_kernel<BF16, D, true><<<dim3(tiles, tiles >= 256 ? 1 : tiles >= 64 ? 4 : 16), 1024, 0, s>>>(a);
+  // workgroups where there are many, most of which find nothing to join (16 x 128 behind 1872: 4 106 us, 1 97), and none for
+  // rows that max_q does not promise
+  const int64_t there = std::max<int64_t>((int64_t)a.max_q * (a.heads / a.kv_heads), 1);
+  const unsigned side = (unsigned)std::min<int64_t>(there, tiles >= 256 ? 1 : tiles >= 64 ? 4 : 16);
+  if (a.limit > 0) attn_join_kernel<BF16, D, true><<<dim3(tiles, side), 1024, 0, s>>>(a);
   return hipGetLastError();
 }
 

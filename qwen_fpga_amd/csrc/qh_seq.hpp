@@ -187,6 +187,7 @@ struct CacheSeq {
 struct AttnI8 : AttnSeq {
   const float *ks = nullptr, *vs = nullptr;   // scales, (r, h) at ks + r * ldks + h * hsks
   int64_t ldks = 0, hsks = 0, ldvs = 0, hsvs = 0;
+  int max_q = 0;                  // the caller's bound
 };
 
 hipError_t launch_attn_i8(const AttnI8& a, hipStream_t s);

@@ -309,6 +309,7 @@ int qh_attention_seq_i8(void* out, int64_t ldo, int64_t hso, const void* q, int6
   a.hsks = hsks;
   a.ldvs = ldvs;
   a.hsvs = hsvs;
+  a.max_q = max_q;
   a.cu_q = cu_q;
   a.k_start = k_start;
   a.k_len = k_len;
