@@ -607,11 +607,14 @@ __global__ __launch_bounds__(512, 2) void attn_i8_tile_kernel(const AttnI8 a) {
         for (int r = 0; r < VW; ++r) acc[t][r] *= al;
     }
     const float mu = m == kNegInf ? 0.0f : m;
-    // (bfloat16: the exponent's product is not rounded, the maximum was: 2^-24 of a score of 2^31 would be too large a power)
-    if (BF16 && __ballot(fabsf(mu) >= 0x1p20f) != 0) {
+    // (bfloat16: the exponent's product is not rounded, the maximum was: 2^-24 of a score of 2^31 would be too large a power.
+    // A row's own maximum decides: the other rows of the wave have no influence on it)
+    const bool large = fabsf(mu) >= 0x1p20f;
+    if (BF16 && __ballot(large) != 0) {
+      const float by = large ? unit : 1.0f;
 #pragma unroll
-      for (int i = 0; i < 4 * NK; ++i) st[i] *= unit;
-      unit = 1.0f;
+      for (int i = 0; i < 4 * NK; ++i) st[i] *= by;
+      unit = large ? 1.0f : unit;
     }
     float ps = 0.0f;
     each<NK>([&](auto I) {

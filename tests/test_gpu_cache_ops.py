@@ -902,3 +902,32 @@ def test_layer_over_the_cache(q, torch_cuda, bf16):
             assert all(same(torch, a, b) for a, b in zip(r, res[0]))
         assert (out1[len(live):] == 7).all()
         stage_check(row1, pos1.cpu(), out1, res[0][1], res[0][2], None, cu, held)
+
+
+# ------------------------------------------------------------------ rows of a wave are their own affair
+
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+@pytest.mark.parametrize("max_q", [1, LARGE])
+@pytest.mark.parametrize("d", [128, 256])
+def test_attention_large_scores_of_other_rows(q, torch_cuda, bf16, max_q, d):
+    """Scores of 2^18 to 2^20 whose keys differ by a few powers of two, where a product rounded before it is subtracted and one
+    that is not give different probabilities; a key behind a row takes the rows that see it past 2^20.  The rows that do not
+    keep their bits."""
+    torch = torch_cuda
+    g, n, h, kvh, hit, u = gen(torch, 22), 100, 4, 2, 67, 16
+    k0 = torch.randint(20, 128, (kvh, d), generator=g) * (1 - 2 * torch.randint(0, 2, (kvh, d), generator=g))
+    kq = k0.expand(n, kvh, d).clone()
+    kq[..., :u] = torch.randint(-127, 128, (n, kvh, u), generator=g)
+    qq = torch.sign(k0).float().repeat_interleave(h // kvh, 0) * (0.5 + 0.5 * torch.rand(n, h, d, generator=g))
+    qq[..., :u] = torch.randn(n, h, u, generator=g) * 2.0 ** -13 * d / 128
+    ks, vs = torch.full((n, kvh), 2.0 ** -7), torch.rand(n, kvh, generator=g) + 0.5
+    vq = torch.randint(-127, 128, (n, kvh, d), generator=g)
+    inp = [qq.to(torch.bfloat16 if bf16 else torch.float32), kq.to(torch.int8), ks, vq.to(torch.int8), vs]
+    dots = torch.einsum("thd,mhd->htm", inp[0].double(), kq.repeat_interleave(h // kvh, 1).double()) * 2.0 ** -7
+    scale = 0.95 * 2.0 ** 20 / math.log2(math.e) / dots.max().item()
+    p = torch.softmax((dots * scale)[:, hit - 3:hit, :hit - 3], -1).amax(-1)
+    assert dots.min() * scale * math.log2(math.e) > 2.0 ** 18 and p.median() < 0.7      # several keys have a part in a row
+    clean = attn_run(q, torch, [x.cuda() for x in inp], [n], [n], [0], scale=scale, max_q=max_q)
+    inp[2][hit] *= 16
+    got = attn_run(q, torch, [x.cuda() for x in inp], [n], [n], [0], scale=scale, max_q=max_q)
+    assert torch.equal(got[:hit], clean[:hit])
