@@ -574,7 +574,8 @@ __global__ __launch_bounds__(512, 2) void attn_i8_tile_kernel(const AttnI8 a) {
 #pragma unroll
       for (int q = 0; q < NSC; ++q) far |= !(fabsf(ksc[q]) < 0x1p96f);
       if (__ballot(far) != 0) {
-        unit = fminf(fac * 0x1p32f, 0x1.fffffep127f);
+        unit = fac * 0x1p32f;
+        if (unit > 0x1.fffffep127f) unit = 0x1.fffffep127f;   // (a row that is NaN stays it)
 #pragma unroll
         for (int q = 0; q < NSC; ++q) ksc[q] *= 0x1p-32f;
       }

@@ -931,3 +931,23 @@ def test_attention_large_scores_of_other_rows(q, torch_cuda, bf16, max_q, d):
     inp[2][hit] *= 16
     got = attn_run(q, torch, [x.cuda() for x in inp], [n], [n], [0], scale=scale, max_q=max_q)
     assert torch.equal(got[:hit], clean[:hit])
+
+
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+@pytest.mark.parametrize("max_q", [1, LARGE])
+@pytest.mark.parametrize("d", [128, 256])
+@pytest.mark.parametrize("bad_q", [math.nan, math.inf], ids=str)
+@pytest.mark.parametrize("bad_k", [math.nan, math.inf, 2.0 ** 97], ids=str)
+def test_attention_bad_queries_beside_bad_scales(q, torch_cuda, bf16, max_q, d, bad_q, bad_k):
+    """Query rows that are not finite, one before and one behind a key of the same 32 whose scale is large or not finite:
+    both are NaN, and the rows that do not see the key keep their bits."""
+    torch = torch_cuda
+    lens, ctx = [70, 1], [90, 300]
+    inp, at = attn_inputs(torch, 23, lens, ctx, 4, 2, d, bf16)
+    clean = attn_run(q, torch, [x.cuda() for x in inp], lens, ctx, at, max_q=max_q)
+    inp[2][at[0] + 28, 0] = bad_k                  # the tokens from 8 on see it
+    inp[0][3, 1, 5], inp[0][50, 0, d - 1] = bad_q, bad_q
+    got = attn_run(q, torch, [x.cuda() for x in inp], lens, ctx, at, max_q=max_q)
+    assert torch.isnan(got[3, 1]).all() and torch.isnan(got[50, 0]).all()
+    got[3, 1] = clean[3, 1]
+    assert torch.equal(got[:8], clean[:8]) and torch.equal(got[:, 2:], clean[:, 2:]) and torch.equal(got[70:], clean[70:])
