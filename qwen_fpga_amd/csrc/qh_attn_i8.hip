@@ -566,18 +566,17 @@ __global__ __launch_bounds__(512, 2) void attn_i8_tile_kernel(const AttnI8 a) {
     constexpr bool part = decltype(PART)::value;
     const int h = (uint32_t)(tid_here() & 63) / NR, kb = SK * it + 4 * h;
     float st[4 * NK];
-    // bfloat16: the scores without the row's unit, which the exponent's multiplication brings.  Where a scale of K could take
-    // a whole number beyond a float's range, 2^32 goes from the scales to the units; as a branch hardly any stage takes it.
+    // bfloat16: the scores without the row's unit, which the exponent's multiplication brings.  A scale of K that could take a
+    // whole number beyond a float's range is taken 2^32 smaller; the rows that see its key then put unit and 2^32 to their
+    // scores below.  A row's own keys decide, so that others have no influence; hardly any stage takes the branch.
     float unit = fac;
+    uint64_t far[NSC] = {}, any = 0;   // the lanes that hold such a scale
     if constexpr (BF16) {
-      bool far = false;
 #pragma unroll
-      for (int q = 0; q < NSC; ++q) far |= !(fabsf(ksc[q]) < 0x1p96f);
-      if (__ballot(far) != 0) {
-        unit = fac * 0x1p32f;
-        if (unit > 0x1.fffffep127f) unit = 0x1.fffffep127f;   // (a row that is NaN stays it)
-#pragma unroll
-        for (int q = 0; q < NSC; ++q) ksc[q] *= 0x1p-32f;
+      for (int q = 0; q < NSC; ++q) {
+        const bool large = !(fabsf(ksc[q]) < 0x1p96f);
+        any |= far[q] = __ballot(large);
+        ksc[q] = large ? ksc[q] * 0x1p-32f : ksc[q];
       }
     }
     each<NK>([&](auto I) {
@@ -591,6 +590,23 @@ __global__ __launch_bounds__(512, 2) void attn_i8_tile_kernel(const AttnI8 a) {
         if (part && kb + KS * i + r >= seen) st[4 * i + r] = kNegInf;
       });
     });
+    if (BF16 && any != 0) {
+      float by[NSC], most = 1.0f;
+#pragma unroll
+      for (int q = 0; q < NSC; ++q) by[q] = far[q] >> (tid_here() & 63) & 1 ? 0x1p32f : 1.0f;
+      auto of = [&](auto I) { return lane_of_16<I % 16>(by[I / 16]); };
+      int to = seen - kb;
+      asm volatile("" : "+v"(to));   // (masks kept from the loop above would not fit the scalar registers)
+      each<4 * NK>([&](auto I) { most = fmaxf(most, part && KS * (I / 4) + I % 4 >= to ? 1.0f : of(I)); });
+      most = fmaxf(most, xor_perm<32>(most));
+      const bool sees = most != 1.0f;
+      const float first = sees ? fac : 1.0f;
+      unit = sees ? 1.0f : fac;
+      each<4 * NK>([&](auto I) {   // (all lanes take part in reading another's)
+        const float f = of(I);
+        st[I] = st[I] * first * (sees ? f : 1.0f);
+      });
+    }
     float mt = st[0];
 #pragma unroll
     for (int r = 1; r < 4 * NK; ++r) mt = fmaxf(mt, st[r]);

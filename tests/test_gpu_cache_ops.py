@@ -951,3 +951,25 @@ def test_attention_bad_queries_beside_bad_scales(q, torch_cuda, bf16, max_q, d, 
     assert torch.isnan(got[3, 1]).all() and torch.isnan(got[50, 0]).all()
     got[3, 1] = clean[3, 1]
     assert torch.equal(got[:8], clean[:8]) and torch.equal(got[:, 2:], clean[:, 2:]) and torch.equal(got[70:], clean[70:])
+
+
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+@pytest.mark.parametrize("max_q", [1, LARGE])
+@pytest.mark.parametrize("d", [128, 256])
+@pytest.mark.parametrize("bad", [2.0 ** 97, 3e38, math.inf, math.nan], ids=str)
+def test_attention_small_scales_beside_hidden_large_ones(q, torch_cuda, bf16, max_q, d, bad):
+    """Queries near 2^100 and scales of K near 2^-104, where a scale moved down by 2^32 would lose bits: a large scale of a key
+    behind them has no influence; and queries near 2^115, whose unit times 2^32 is beyond a float."""
+    torch = torch_cuda
+    lens, ctx = [70, 1], [90, 300]
+    inp, at = attn_inputs(torch, 24, lens, ctx, 4, 2, d, bf16)
+    inp = list(inp)
+    for up in (100, 115):
+        now = list(inp)
+        now[0], now[2] = inp[0] * 2.0 ** up, inp[2] * 2.0 ** -(up + 4)
+        clean = attn_run(q, torch, [x.cuda() for x in now], lens, ctx, at, max_q=max_q)
+        attn_check(torch, clean, attn_oracle(torch, *now, lens, ctx, at, 1 / math.sqrt(d), bf16), bf16)
+        now[2] = now[2].clone()
+        now[2][at[0] + 28] = bad                        # the tokens from 8 on see it
+        got = attn_run(q, torch, [x.cuda() for x in now], lens, ctx, at, max_q=max_q)
+        assert torch.equal(got[:8], clean[:8]) and torch.equal(got[70:], clean[70:])
