@@ -749,14 +749,7 @@ hipError_t launch(const AttnI8& a, hipStream_t s) {
 AttnForm attn_i8_form(int64_t q_rows, int n_seq, int max_q, int max_k, int heads, int kv_heads, int dim, bool bf16) {
   const int G = heads / kv_heads;
   AttnForm f = {0, 0, 0};
-  // Pairs of a query row and a key it sees, about (where there is one sequence, or several of equal length).  The form for
-  // prompts takes a workgroup of 512 threads a CU and 2 us for every 32 keys however few rows there are, the one for few
-  // rows half as long again where there is work for all CUs.  few / prompts, bfloat16, 8 / 2 heads of 256: 1024 tokens 22
-  // / 47 us, 1500 39 / 49, 2000 55 / 58, 3000 109 / 84, 6000 356 / 210, 512 behind 1488 29 / 47, 512 behind 3488 74 / 54, 300
-  // behind 15700 160 / 79, 64 behind 31936 57 / 75; 8 / 8 heads of 128: 1500 25 / 39, 2000 37 / 47, 3000 75 / 61; fp32, 8 / 2
-  // heads of 256: 1500 42 / 51, 2000 61 / 68, 6000 397 / 355, 512 behind 3488 78 / 56.
-  const int64_t pairs = q_rows * heads * (std::max(max_k, max_q) - max_q / 2);
-  if ((int64_t)max_q * G > 256 && pairs >= 15000000) {
+  if (attn_i8_prompts(q_rows, n_seq, max_q, max_k, heads, kv_heads, dim, tile_rows(bf16), bf16)) {
     f.tile = tile_rows(bf16);
     const int64_t tiles = seq_tiles_max(q_rows * G, n_seq, f.tile) * kv_heads;
     // two workspace places a CU: the chunks are such that more are hardly ever taken

@@ -61,6 +61,28 @@ QH_SEQ_FN float code_scale(float top) {
   return !(top > 0.0f) ? 1.0f : s > 0.0f ? s : 0x1p-149f;
 }
 
+// Whether attention over an int8 cache takes the form for prompts (a workgroup for `tile` rows, 512 threads, about 2 us for
+// every 32 keys however few rows there are) and not the one for few rows (16 rows), by bounds that the host knows: it does
+// where a sequence has more than 256 rows a kv head, there is work for all CUs, and the tiles are full enough.
+// Work: pairs of a query row and a key that it sees, about.  few / prompts, bfloat16, 8 / 2 heads of 256: 1024 tokens 22 / 47 us,
+// 1500 39 / 49, 2000 55 / 58, 3000 109 / 84, 6000 356 / 210, 512 behind 1488 29 / 47, 512 behind 3488 74 / 54, 300
+// behind 15700 160 / 79, 64 behind 31936 57 / 75; 8 / 8 heads of 128: 1500 25 / 39, 2000 37 / 47, 3000 75 / 61; fp32, 8 / 2
+// heads of 256: 1500 42 / 51, 2000 61 / 68, 6000 397 / 355, 512 behind 3488 78 / 56.
+// Tiles: a sequence of max_q tokens, the others' of equal lengths, each with a tile that it does not fill.  A tile of the
+// form for prompts costs as much as 9 (heads of 128: 8; fp32, whose tiles have 128 rows: 6) of 16 rows.  Single tokens and one
+// prompt, whose tiles stand few / prompts as given, 8 / 2 heads of 256, bfloat16: 31 behind 30000 keys and 65 tokens 202 / 490 us
+// (1.7 times as many tiles), 255 behind 8000 and 128 tokens 387 / 1089 (1.3), 31 behind 4000 and 512 behind 3488 88 / 117 (4.2), 100
+// behind 4000 and 4000 tokens 244 / 372 (6.9), 31 behind 4000 and 2048 76 / 140 (8.7), 7 behind 4000 and 512 behind 3488 83 / 71
+// (9.1), 31 behind 4000 and 8000 634 / 480 (13); 16 x 80 behind 4000 132 / 117 (9.6); 8 / 8 heads of 128: 31 behind 4000 and 8000
+// 461 / 382 (8.5), 7 behind 4000 and 512 behind 3488 60 / 78 (4.4); fp32, 8 / 2 heads of 256: 64 x 300 216 / 170 (7.3), 7 behind 4000
+// and 512 behind 3488 85 / 72 (5.9), 31 behind 4000 and 2048 81 / 144 (5.7).
+inline bool attn_i8_prompts(int64_t q_rows, int n_seq, int max_q, int max_k, int heads, int kv_heads, int dim, int tile, bool bf16) {
+  const int64_t G = heads / kv_heads, longest = max_q * G, rest = q_rows > max_q ? (q_rows - max_q) * G : 0;
+  const int64_t pairs = q_rows * heads * ((max_k > max_q ? max_k : max_q) - max_q / 2);
+  auto tiles = [&](int rows) { return (longest + rest) / rows + n_seq - 1; };
+  return longest > 256 && pairs >= 15000000 && tiles(16) >= (!bf16 ? 6 : dim == 256 ? 9 : 8) * tiles(tile);
+}
+
 // A float as the sum of three bfloat16, eight bits of it each: the upper halves of p[0], p[1], p[2].
 struct Cut {
   uint32_t p[3];

@@ -225,3 +225,33 @@ def test_any_operator_may_be_the_first(call):
             f"try:\n    q.{call}\nexcept TypeError as e:\n    assert 'CUDA' in str(e), e\nelse:\n    raise SystemExit('taken')\n")
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=ROOT)
     assert r.returncode == 0, r.stderr
+
+
+def prompts(q, q_rows, n_seq, max_q, max_k, heads, kv_heads, dim, bf16):
+    """Whether a call takes the form for prompts, by its workspace: 512 places (or two tiles' and more) of `tile` rows; the one for
+    few rows asks for those of 16 rows, or for none."""
+    nb = q.attention_seq_i8_workspace(q_rows, n_seq, max_q, max_k, heads, kv_heads, dim, q.BF16 if bf16 else q.F32)
+    tile, rows = 256 if bf16 else 128, q_rows * (heads // kv_heads)
+    few = (min(rows // 16 + n_seq, rows) * kv_heads + 512) * (16 * dim + 32) * 4
+    assert max_k > 3000                                  # (fewer keys may need no workspace in either form)
+    if nb in (0, few):
+        return False
+    assert nb % (tile * (dim + 2) * 4) == 0 and 0 < nb // (tile * (dim + 2) * 4) <= 512
+    return True
+
+
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 256), (8, 8, 128)])
+def test_attention_form_of_mixed_calls(q, bf16, heads, kv_heads, dim):
+    """Single tokens beside a short part of a prompt take the form for few rows, whatever the pairs come to when all rows see the
+    longest keys; a long prompt beside a few of them takes the one for prompts, and so do equal sequences that fill tiles."""
+    f = lambda *a: prompts(q, *a, heads, kv_heads, dim, bf16)
+    for single, keys, part in ((31, 30000, 65), (31, 30000, 512), (255, 8000, 128), (31, 4000, 512), (100, 4000, 1000), (128, 4000, 300),
+                               (60000, 8000, 4096)):
+        assert not f(single + part, single + 1, part, keys)
+    assert f(7 + 8000, 8, 8000, 8000) and f(31 + 20000, 32, 20000, 20000)
+    assert f(1, 1, 1 << 26, 4000) and f(300, 150, 1 << 26, 4000)          # a bound of many rows asks for it
+    if heads > kv_heads:
+        assert f(64 * 400, 64, 400, 4000)
+    # as before for one sequence
+    assert f(4000, 1, 4000, 8000) and f(512, 1, 512, 8000) and not f(512, 1, 512, 3001) and not f(1, 1, 1, 131071)

@@ -973,3 +973,23 @@ def test_attention_small_scales_beside_hidden_large_ones(q, torch_cuda, bf16, ma
         now[2][at[0] + 28] = bad                        # the tokens from 8 on see it
         got = attn_run(q, torch, [x.cuda() for x in now], lens, ctx, at, max_q=max_q)
         assert torch.equal(got[:8], clean[:8]) and torch.equal(got[70:], clean[70:])
+
+
+@pytest.mark.parametrize("single,keys,part", [(31, 6000, 300), (60, 6000, 300), (8, 4000, 20)])
+@pytest.mark.parametrize("d", [128, 256])
+def test_attention_single_tokens_beside_a_part_of_a_prompt(q, torch_cuda, d, single, keys, part):
+    """bfloat16: single tokens keep the two parts of P (2^-16) beside a part of a prompt, as on their own.  Queries of 0 take the mean
+    of the values: three of four keys hold c x and the fourth -3 c x, so that what rounding leaves of c and of 3 c is all there is."""
+    torch = torch_cuda
+    lens, ctx, h, kvh = [1] * single + [part], [keys - 4 * i for i in range(single)] + [part], 8, 2
+    inp, at = attn_inputs(torch, 25, lens, ctx, h, kvh, d, True)
+    g = gen(torch, 26)
+    inp[0][:single] = 0.0
+    for i in range(single):
+        r = slice(at[i], at[i] + ctx[i])
+        x, c = inp[3][at[i]].clone(), torch.rand(kvh, generator=g) + 0.5
+        inp[3][r], inp[4][r] = x, c
+        inp[3][at[i] + 3:at[i] + ctx[i]:4], inp[4][at[i] + 3:at[i] + ctx[i]:4] = -x, 3 * c
+    got = attn_run(q, torch, [x.cuda() for x in inp], lens, ctx, at)
+    want = attn_oracle(torch, inp[0][:single], *inp[1:], lens[:single], ctx[:single], at[:single], 1 / math.sqrt(d), True)   # (its max_q is 1)
+    attn_check(torch, got[:single], want, True)
