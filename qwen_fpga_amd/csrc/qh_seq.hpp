@@ -64,10 +64,18 @@ QH_SEQ_FN float code_scale(float top) {
 // Whether attention over an int8 cache takes the form for prompts (a workgroup for `tile` rows, 512 threads, about 2 us for
 // every 32 keys however few rows there are) and not the one for few rows (16 rows), by bounds that the host knows: it does
 // where a sequence has more than 256 rows a kv head, there is work for all CUs, and the tiles are full enough.
-// Work: pairs of a query row and a key that it sees, about.  few / prompts, bfloat16, 8 / 2 heads of 256: 1024 tokens 22 / 47 us,
-// 1500 39 / 49, 2000 55 / 58, 3000 109 / 84, 6000 356 / 210, 512 behind 1488 29 / 47, 512 behind 3488 74 / 54, 300
-// behind 15700 160 / 79, 64 behind 31936 57 / 75; 8 / 8 heads of 128: 1500 25 / 39, 2000 37 / 47, 3000 75 / 61; fp32, 8 / 2
-// heads of 256: 1500 42 / 51, 2000 61 / 68, 6000 397 / 355, 512 behind 3488 78 / 56.
+// Work: pairs of a query row and a key that it sees, about.  A prompt behind a long prefix is split in either form; one that
+// begins its sequence costs the form for few rows no split, and fp32 hardly gains by the other: so 15 million pairs where there
+// are twice as many keys as new tokens, else 20 (fp32: 33).  few / prompts:
+//   8 / 2 heads of 256, bfloat16: 1500 tokens 40 / 52 us, 2000 (16 million) 57 / 61, 2300 (21) 75 / 66, 3000 109 / 88, 4000 174 / 126;
+//     512 behind 1488 31 / 48, behind 2500 (11) 45 / 52, behind 3488 (15) 76 / 57, 300 behind 15700 162 / 85
+//   fp32: 1500 tokens 43 / 53, 2000 62 / 70, 2300 82 / 84, 3000 (36) 119 / 120, 4000 192 / 197; 512 behind 3488 80 / 58
+//   8 / 8 heads of 128, bfloat16: 1500 26 / 39, 2000 38 / 49, 2300 55 / 52, 3000 76 / 64, 4000 118 / 89; 512 behind 2500 35 / 38, behind
+//     3488 54 / 43
+//   fp32: 2000 40 / 51, 3000 78 / 89, 4000 124 / 136; 512 behind 3488 56 / 44
+//   16 / 4 heads of 128, bfloat16: 1500 (18) 40 / 54, 2000 (32) 59 / 63, 2300 86 / 75; 256 behind 3840 (16) 54 / 43; fp32: 1500 42 / 60,
+//     2000 62 / 85, 2300 (42) 90 / 97, 2600 110 / 107; 256 behind 3840 57 / 45
+//   64 tokens behind 31936 keys (256 rows a kv head of 8 / 2) 60 / 78, 80 86 / 83
 // Tiles: a sequence of max_q tokens, the others' of equal lengths, each with a tile that it does not fill.  A tile of the
 // form for prompts costs as much as 9 (heads of 128: 8; fp32, whose tiles have 128 rows: 6) of 16 rows.  Single tokens and one
 // prompt, whose tiles stand few / prompts as given, 8 / 2 heads of 256, bfloat16: 31 behind 30000 keys and 65 tokens 202 / 490 us
@@ -80,7 +88,8 @@ inline bool attn_i8_prompts(int64_t q_rows, int n_seq, int max_q, int max_k, int
   const int64_t G = heads / kv_heads, longest = max_q * G, rest = q_rows > max_q ? (q_rows - max_q) * G : 0;
   const int64_t pairs = q_rows * heads * ((max_k > max_q ? max_k : max_q) - max_q / 2);
   auto tiles = [&](int rows) { return (longest + rest) / rows + n_seq - 1; };
-  return longest > 256 && pairs >= 15000000 && tiles(16) >= (!bf16 ? 6 : dim == 256 ? 9 : 8) * tiles(tile);
+  const int64_t from = max_k / 2 >= max_q ? 15000000 : bf16 ? 20000000 : 33000000;
+  return longest > 256 && pairs >= from && tiles(16) >= (!bf16 ? 6 : dim == 256 ? 9 : 8) * tiles(tile);
 }
 
 // A float as the sum of three bfloat16, eight bits of it each: the upper halves of p[0], p[1], p[2].

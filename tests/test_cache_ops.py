@@ -255,3 +255,40 @@ def test_attention_form_of_mixed_calls(q, bf16, heads, kv_heads, dim):
         assert f(64 * 400, 64, 400, 4000)
     # as before for one sequence
     assert f(4000, 1, 4000, 8000) and f(512, 1, 512, 8000) and not f(512, 1, 512, 3001) and not f(1, 1, 1, 131071)
+
+
+FORMS = r"""
+#include <cstdio>
+#include <initializer_list>
+#include "qh_seq.hpp"
+using namespace qh;
+#define REQUIRE(c) do { if (!(c)) { std::printf("line %d: %s\n", __LINE__, #c); return 1; } } while (0)
+int main() {
+  auto one = [](int n, int past, int heads, int kv, int dim, bool bf16) {
+    return attn_i8_prompts(n, 1, n, n + past, heads, kv, dim, bf16 ? 256 : 128, bf16);
+  };
+  for (bool bf16 : {false, true}) {
+    for (int n : {1, 64, 512, 1024, 1500, 2000}) REQUIRE(!one(n, 0, 8, 2, 256, bf16) && !one(n, 0, 8, 8, 128, bf16));
+    REQUIRE(!one(512, 1488, 8, 2, 256, bf16) && one(512, 3488, 8, 2, 256, bf16) && one(300, 15700, 8, 2, 256, bf16));
+    REQUIRE(!one(512, 1488, 8, 8, 128, bf16) && one(512, 3488, 8, 8, 128, bf16) && !one(64, 31936, 8, 2, 256, bf16));
+    REQUIRE(one(256, 3840, 16, 4, 128, bf16) && one(6000, 0, 8, 2, 256, bf16));
+    REQUIRE(one(1 << 26, 0, 1, 1, 128, bf16) && attn_i8_prompts(1, 1, 1 << 26, 1, 1, 1, 128, bf16 ? 256 : 128, bf16));
+  }
+  REQUIRE(one(2300, 0, 8, 2, 256, true) && one(3000, 0, 8, 8, 128, true) && one(2000, 0, 16, 4, 128, true));
+  REQUIRE(!one(2300, 0, 8, 2, 256, false) && !one(2000, 0, 16, 4, 128, false) && !one(1500, 0, 16, 4, 128, true));
+  // the most that a call can have stays within 64 bits
+  REQUIRE(attn_i8_prompts(0x7fffffff, 1, 0x7fffffff, 1 << 30, 1, 1, 128, 256, true));
+  REQUIRE(!attn_i8_prompts(0x7fffffff / 64, 65536, 1, 1 << 30, 64, 1, 128, 256, true));
+  return 0;
+}
+"""
+
+
+def test_attention_form(tmp_path):
+    """What was the faster form on the card, by the rule itself (which the few keys that need no workspace do not show)."""
+    src, exe = tmp_path / "t.cpp", tmp_path / "t"
+    src.write_text(FORMS)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Wextra", "-Werror", "-ftrapv", "-I",
+                    os.path.join(ROOT, "qwen_fpga_amd", "csrc"), "-o", str(exe), str(src)], check=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert r.returncode == 0, r.stdout + r.stderr
