@@ -274,7 +274,7 @@ int main() {
     REQUIRE(one(256, 3840, 16, 4, 128, bf16) && one(6000, 0, 8, 2, 256, bf16));
     REQUIRE(one(1 << 26, 0, 1, 1, 128, bf16) && attn_i8_prompts(1, 1, 1 << 26, 1, 1, 1, 128, bf16 ? 256 : 128, bf16));
   }
-  REQUIRE(one(2300, 0, 8, 2, 256, true) && one(3000, 0, 8, 8, 128, true) && one(2000, 0, 16, 4, 128, true));
+  REQUIRE(one(2300, 0, 8, 2, 256, true) && one(3000, 0, 8, 8, 128, true) && one(2300, 0, 16, 4, 128, true));
   REQUIRE(!one(2300, 0, 8, 2, 256, false) && !one(2000, 0, 16, 4, 128, false) && !one(1500, 0, 16, 4, 128, true));
   // the most that a call can have stays within 64 bits
   REQUIRE(attn_i8_prompts(0x7fffffff, 1, 0x7fffffff, 1 << 30, 1, 1, 128, 256, true));

@@ -993,3 +993,34 @@ def test_attention_single_tokens_beside_a_part_of_a_prompt(q, torch_cuda, d, sin
     got = attn_run(q, torch, [x.cuda() for x in inp], lens, ctx, at)
     want = attn_oracle(torch, inp[0][:single], *inp[1:], lens[:single], ctx[:single], at[:single], 1 / math.sqrt(d), True)   # (its max_q is 1)
     attn_check(torch, got[:single], want, True)
+
+
+@pytest.fixture
+def two_parts(monkeypatch):
+    """The bound of the form for few rows: P in two parts whatever the number of rows."""
+    monkeypatch.setattr(sys.modules[__name__], "p_rounding", lambda lens, G, bf16: 2.0 ** -16 if bf16 else 0.0)
+
+
+@pytest.mark.parametrize("lens,ctx,h,kvh,d", ATTN, ids=short)
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+def test_few_rows_keep_two_parts(two_parts, q, torch_cuda, lens, ctx, h, kvh, d, bf16):
+    """All of these take the form for few rows by their own lengths.  Queries are small, so that their own rounding does not hide P's."""
+    torch = torch_cuda
+    inp, at = attn_inputs(torch, sum(lens) + sum(ctx) + h, lens, ctx, h, kvh, d, bf16, gap=3, qscale=0.02)
+    dev, want = both(torch, inp, at, lens, ctx, 1 / math.sqrt(d), bf16)
+    attn_check(torch, attn_run(q, torch, dev, lens, ctx, at), want, bf16)
+
+
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+@pytest.mark.parametrize("n,past,h,kvh,d", [
+    (2200, 0, 8, 8, 128), (500, 1490, 8, 2, 256),                                 # few rows, the last before the form changes
+    (2300, 0, 8, 2, 256), (512, 3500, 8, 2, 256), (2900, 0, 8, 8, 128),           # prompts in bfloat16 (and in fp32 behind a prefix)
+])
+def test_attention_on_both_sides_of_the_form(q, torch_cuda, monkeypatch, n, past, h, kvh, d, bf16):
+    """The form that a call takes by its own sizes, at the bound of that form."""
+    torch = torch_cuda
+    if n <= 500 or n == 2200:
+        monkeypatch.setattr(sys.modules[__name__], "p_rounding", lambda lens, G, bf16: 2.0 ** -16 if bf16 else 0.0)
+    inp, at = attn_inputs(torch, n, [n], [n + past], h, kvh, d, bf16, gap=5, qscale=0.02)
+    dev, want = both(torch, inp, at, [n], [n + past], 1 / math.sqrt(d), bf16)
+    attn_check(torch, attn_run(q, torch, dev, [n], [n + past], at), want, bf16)
