@@ -310,7 +310,8 @@ int qh_qk_norm_rope_seq(void* q_out, int64_t ldqo, int64_t hsqo, void* k_out, in
 
 /* Rows of the cache from new keys and values k, v [tokens][kv_heads][head_dim] of `type`: token t goes to row slot[t]
  * (int64, on the device).  scale = largest magnitude / 127 (1 for zeros), code = rint(x / scale): qh_quant_rows of each
- * head's row, bit for bit; one that is not finite gets scale NaN and codes 0 (and what attends to it is NaN).  A token
+ * head's row, bit for bit (but a scale that is 0 in fp32 there is the smallest number, 2^-149, here); one that is not
+ * finite gets scale NaN and codes 0 (and what attends to it is NaN).  A token
  * whose slot lies outside 0 .. rows - 1 is skipped (a batch's unused places: -1); rows that no token names are left as
  * they were.  Two tokens may not name one row: it then holds a mixture of both.  tokens * kv_heads: up to 2^26. */
 int qh_kv_cache_write_i8(int8_t* kq, int64_t ldkq, int64_t hskq, float* ks, int64_t ldks, int64_t hsks, int8_t* vq, int64_t ldvq,

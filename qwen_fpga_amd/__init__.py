@@ -781,7 +781,8 @@ def _cache_operands(name: str, kq, ks, vq, vs, k, v, slot):
 def kv_cache_write_i8(kq, ks, vq, vs, k, v, slot, stream=None):
     """Keys and values quantised into rows of the cache: token t of k, v [tokens, kv_heads, dim] (float32 or bfloat16,
     any row and head strides) goes to row slot[t] (int64 on the device; one outside the cache, such as -1, is skipped).
-    quant_rows of each head's row, bit for bit: scale = largest magnitude / 127, and NaN where the row is not finite.
+    quant_rows of each head's row, bit for bit: scale = largest magnitude / 127 (2^-149 at least; 1 for zeros), and NaN
+    where the row is not finite.
     Two tokens may not name the same row."""
     fn = _op("qh_kv_cache_write_i8")
     ty, cache, new, where = _cache_operands("qh_kv_cache_write_i8", kq, ks, vq, vs, k, v, slot)

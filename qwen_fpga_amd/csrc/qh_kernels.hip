@@ -420,8 +420,9 @@ hipError_t launch_quant(int8_t* q, float* sx, const float* x, int n, hipStream_t
 // 16-bit shift), its amax taken with the xor tree (max is exact in any order),
 // and written as one dword of four int8 per lane and chunk; other rows take
 // two passes over memory.  s = amax/127 (1 if amax == 0) and the quotient
-// RN(w/s) is Markstein's correction from rs = RN(1/s), exact on |w| <= amax.
-// A row holding a NaN or an infinity gets scale NaN and q = 0.
+// RN(w/s) is Markstein's correction from rs = RN(1/s), exact on |w| <= amax where
+// the remainder is no subnormal number; below 2^-100 (1/s may be infinite) the division
+// itself.  A row holding a NaN or an infinity gets scale NaN and q = 0.
 constexpr int kQRowRegs = 16;
 __device__ __forceinline__ float qr_widen(float v) { return v; }
 __device__ __forceinline__ float qr_widen(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
@@ -468,13 +469,19 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(int8_t* q, float* scale
     bad = !wave_all(!bad);
     const float s = bad ? __builtin_nanf("") : quant_scale(am);
     const float rs = 1.0f / s;
+    const bool small = s < 0x1p-100f;
 #pragma unroll
     for (int c = 0; c < REGS; ++c) {
       const int i = 4 * (lane + 64 * c);
       if (i < cols) {
         int t[4];
+        if (small) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) t[k] = bad ? 0 : quant_one_r(v[c][k], s, rs);
+          for (int k = 0; k < 4; ++k) t[k] = quant_one(v[c][k], s);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) t[k] = bad ? 0 : quant_one_r(v[c][k], s, rs);
+        }
         *as_global_w(reinterpret_cast<uint32_t*>(qr + i)) = pack4(t[0], t[1], t[2], t[3]);
       }
     }
@@ -490,7 +497,11 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(int8_t* q, float* scale
   bad = !wave_all(!bad);
   const float s = bad ? __builtin_nanf("") : quant_scale(am);
   const float rs = 1.0f / s;
-  for (int i = lane; i < cols; i += 64) qr[i] = bad ? (int8_t)0 : (int8_t)quant_one_r(qr_widen(wr[i]), s, rs);
+  if (s < 0x1p-100f) {
+    for (int i = lane; i < cols; i += 64) qr[i] = (int8_t)quant_one(qr_widen(wr[i]), s);
+  } else {
+    for (int i = lane; i < cols; i += 64) qr[i] = bad ? (int8_t)0 : (int8_t)quant_one_r(qr_widen(wr[i]), s, rs);
+  }
   if (lane == 0) scale[row] = s;
 }
 template <typename T>

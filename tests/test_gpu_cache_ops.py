@@ -1024,3 +1024,19 @@ def test_attention_on_both_sides_of_the_form(q, torch_cuda, monkeypatch, n, past
     inp, at = attn_inputs(torch, n, [n], [n + past], h, kvh, d, bf16, gap=5, qscale=0.02)
     dev, want = both(torch, inp, at, [n], [n + past], 1 / math.sqrt(d), bf16)
     attn_check(torch, attn_run(q, torch, dev, [n], [n + past], at), want, bf16)
+
+
+@pytest.mark.parametrize("d", [128, 256])
+def test_cache_rows_are_quant_rows_at_any_size(q, torch_cuda, d):
+    """The packer's operator and the cache's agree bit for bit from the smallest rows whose scale is not 0 in fp32 on."""
+    torch = torch_cuda
+    g, n = gen(torch, d + 1), 260
+    x = torch.randn(n, 1, d, generator=g) * (2.0 ** (torch.arange(n).double() - 142)).float()[:, None, None]
+    x = torch.where(torch.isfinite(x), x, 1.0)
+    assert (x.abs().amax(-1) / 127 > 0).all()
+    c = cache_new(torch, n, 1, d, "rows")
+    q.kv_cache_write_i8(*c, x.cuda(), x.cuda(), torch.arange(n, device="cuda"))
+    pq, ps = torch.empty(n, d, dtype=torch.int8, device="cuda"), torch.empty(n, device="cuda")
+    q.quant_rows(pq, ps, x.reshape(n, d).cuda(), n, d)
+    for codes, sc in ((c[0], c[1]), (c[2], c[3])):
+        assert torch.equal(codes[:, 0], pq) and torch.equal(sc[:, 0], ps)

@@ -74,6 +74,29 @@ def test_quant_rows_matches_oracle(q, orc, torch_cuda, rows, cols, off):
     assert np.isnan(s_o[3]) and np.isnan(s_o[4]) and s_o[1] == 1.0 and s_o[2] == 1.0
 
 
+@pytest.mark.parametrize("cols,off", [(1024, 0), (256, 0), (128, 0), (1000, 1), (5000, 0)])
+def test_quant_rows_of_very_small_numbers(q, orc, torch_cuda, cols, off):
+    """Rows down to the smallest number, whose 1 / scale is infinite or whose scale is 0 in fp32, as the definition has them."""
+    torch = torch_cuda
+    rng = np.random.default_rng(cols)
+    rows = 60
+    w = (rng.standard_normal((rows, cols)) * 2.0 ** (-148.0 + np.arange(rows))[:, None]).astype(np.float32)
+    w[0] = np.sign(w[0]) * 2.0 ** -149
+    w[1, 1:] = 0.0
+    w[1, 0] = 2.0 ** -149
+    bits = (w.view(np.uint32) >> 16).astype(np.uint16)
+    for x, src in ((w, torch.from_numpy(w)), ((bits.astype(np.uint32) << 16).view(np.float32), torch.from_numpy(bits.view(np.int16)))):
+        q_o, s_o = orc.quant_rows(x)
+        buf = torch.zeros(rows * cols + 16, dtype=src.dtype, device="cuda")
+        wd = buf[off:off + rows * cols].view(rows, cols)
+        wd.copy_(src)
+        qd = torch.empty(rows * cols + 16, dtype=torch.int8, device="cuda")[off:off + rows * cols].view(rows, cols)
+        sd = torch.empty(rows, device="cuda")
+        q.quant_rows(qd, sd, wd, rows, cols)
+        np.testing.assert_array_equal(sd.cpu().numpy(), s_o)
+        np.testing.assert_array_equal(qd.cpu().numpy(), q_o)
+
+
 def test_quant_rows_rejects_bad_arguments(q, torch_cuda):
     torch = torch_cuda
     w = torch.zeros((4, 8), device="cuda")
