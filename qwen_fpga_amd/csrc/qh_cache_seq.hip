@@ -221,12 +221,9 @@ hipError_t launch_rows(const CacheSeq& a, One one, Four four, hipStream_t s) {
 }  // namespace
 
 hipError_t launch_norm_rope(const NormRope& a, hipStream_t s) {
-  // Waves of a token: four where there are few tokens for the chip's 1024 SIMDs, and for many rows of fp32.  Four and one, 8
-  // and 2 heads of 256, bfloat16: 1100 tokens 5.9 and 7.6 us, 1500 7.2 and 8.2, 2000 8.9 and 8.7, 4000 12.8 and 11.4, 16000
-  // 45 and 36; fp32: 1100 8.0 and 9.0, 1500 9.1 and 9.6, 2000 10.8 and 10.4, 4000 20.0 and 20.2, 8000 34.8 and 39, 16000 63
-  // and 67.
+  const bool single = norm_rope_waves(a.tokens, (int64_t)a.heads + a.kv_heads, a.dim, a.bf16) == 1;
   auto go = [&](auto one, auto four) {
-    if (a.tokens > 1792 && (a.bf16 || a.tokens < 4096))
+    if (single)
       one<<<(unsigned)((a.tokens + 3) / 4), 256, 0, s>>>(a);
     else
       four<<<(unsigned)a.tokens, 256, 0, s>>>(a);

@@ -61,6 +61,23 @@ QH_SEQ_FN float code_scale(float top) {
   return !(top > 0.0f) ? 1.0f : s > 0.0f ? s : 0x1p-149f;
 }
 
+// Waves that take a token of `rows` heads (queries' and keys') in the norms with the rotation, one or four; a wave takes 512 / dim
+// rows at a time, `groups` times in all.  One / four, us:
+//   one group (1 / 1 heads of 256 or fewer): three of four would form angles for nothing; bfloat16 100 tokens 3.7 / 3.5, 1000 3.7
+//     / 3.8, 4000 4.7 / 6.7, 16000 11.4 / 17.9; fp32 4000 6.4 / 7.7, 16000 14.9 / 19.0
+//   3 to 5 (4 / 1 and 8 / 2 of 256, 8 / 8 and 16 / 4 of 128): four where there are few tokens for the chip's 1024 SIMDs; 8 / 2 bfloat16
+//     1000 7.5 / 5.9, 1500 8.5 / 7.3, 2000 8.9 / 9.1, 4000 11.5 / 12.8, 16000 37 / 43; fp32 1500 9.9 / 9.4, 2000 10.9 / 11.3, 4000 16.0
+//     / 16.8, 6000 28.8 / 27.6, 8000 39.7 / 35.7, 16000 63.9 / 63.2; 4 / 1 fp32 8000 16.5 / 17.1; 8 / 8 bfloat16 2000 7.4 / 7.3, 4000
+//     9.9 / 11.4, fp32 2000 9.4 / 10.3, 8000 30.2 / 29.6
+//   10 and more (32 / 8): 32 / 8 of 128 bfloat16 2000 13.3 / 12.0, 4000 17.7 / 17.6, 6000 26.7 / 28.6, 8000 40.6 / 36.6, 16000 62 / 68;
+//     of 256 2000 22.1 / 17.7, 8000 74 / 57; fp32 of 128 2000 18.3 / 15.7, 8000 74 / 62
+inline int norm_rope_waves(int tokens, int64_t rows, int dim, bool bf16) {
+  const int64_t groups = (rows * dim + 511) / 512;
+  if (groups == 1) return 1;
+  if (groups >= 10 || tokens <= 1792) return 4;
+  return !bf16 && groups >= 5 && tokens >= 4096 ? 4 : 1;
+}
+
 // Whether attention over an int8 cache takes the form for prompts (a workgroup for `tile` rows, 512 threads, about 2 us for
 // every 32 keys however few rows there are) and not the one for few rows (16 rows), by bounds that the host knows: it does
 // where a sequence has more than 256 rows a kv head, there is work for all CUs, and the tiles are full enough.

@@ -292,3 +292,35 @@ def test_attention_form(tmp_path):
                     os.path.join(ROOT, "qwen_fpga_amd", "csrc"), "-o", str(exe), str(src)], check=True)
     r = subprocess.run([str(exe)], capture_output=True, text=True)
     assert r.returncode == 0, r.stdout + r.stderr
+
+
+WAVES = r"""
+#include <cstdio>
+#include <initializer_list>
+#include "qh_seq.hpp"
+using namespace qh;
+#define REQUIRE(c) do { if (!(c)) { std::printf("line %d: %s\n", __LINE__, #c); return 1; } } while (0)
+int main() {
+  for (bool bf16 : {false, true}) {
+    // never a wave without rows
+    for (int tokens : {1, 100, 1792, 1793, 4096, 16000, 1 << 23})
+      for (int dim : {128, 256})
+        for (int rows = 2; rows <= 512 / dim; ++rows) REQUIRE(norm_rope_waves(tokens, rows, dim, bf16) == 1);
+    // rows of the call, not its tokens alone
+    for (int tokens : {1, 1000, 2000, 3000, 8000}) REQUIRE(norm_rope_waves(tokens, 40, 256, bf16) == 4);
+    REQUIRE(norm_rope_waves(1500, 10, 256, bf16) == 4 && norm_rope_waves(2000, 10, 256, bf16) == 1 && norm_rope_waves(2000, 20, 128, bf16) == 1);
+    REQUIRE(norm_rope_waves(8000, 5, 256, bf16) == 1 && norm_rope_waves(1 << 23, 0x1fffffffell, 256, bf16) == 4);
+  }
+  REQUIRE(norm_rope_waves(8000, 10, 256, true) == 1 && norm_rope_waves(8000, 10, 256, false) == 4 && norm_rope_waves(4000, 10, 256, false) == 1);
+  return 0;
+}
+"""
+
+
+def test_norm_rope_waves(tmp_path):
+    src, exe = tmp_path / "t.cpp", tmp_path / "t"
+    src.write_text(WAVES)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Wextra", "-Werror", "-ftrapv", "-I", os.path.join(ROOT, "qwen_fpga_amd", "csrc"),
+                    "-o", str(exe), str(src)], check=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert r.returncode == 0, r.stdout + r.stderr

@@ -1040,3 +1040,11 @@ def test_cache_rows_are_quant_rows_at_any_size(q, torch_cuda, d):
     q.quant_rows(pq, ps, x.reshape(n, d).cuda(), n, d)
     for codes, sc in ((c[0], c[1]), (c[2], c[3])):
         assert torch.equal(codes[:, 0], pq) and torch.equal(sc[:, 0], ps)
+
+
+@pytest.mark.parametrize("tokens,h,kvh,d,rot", [
+    (1, 1, 1, 256, 64), (513, 2, 2, 128, 32), (2, 3, 1, 128, 128), (5000, 1, 1, 256, 64),       # a wave whose rows it takes at once
+    (1900, 32, 8, 128, 64), (1800, 20, 1, 256, 96), (4100, 8, 2, 256, 64), (4097, 4, 1, 256, 16)], ids=str)
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+def test_norm_rope_numbers_of_waves(q, torch_cuda, tokens, h, kvh, d, rot, bf16):
+    test_norm_rope(q, torch_cuda, tokens, h, kvh, d, rot, bf16)
