@@ -332,11 +332,16 @@ int qh_kv_cache_read_i8(void* k, int64_t ldk, int64_t hsk, void* v, int64_t ldv,
  * sequences, key ranges, rows without keys, limits and workspace rules; q and out of `type`.  Codes and scales of keys that
  * a row does not see have no influence on it; a row that sees a scale of V that is not finite gives nothing finite, and NaN
  * where that or one of K is NaN.
+ * A sequence's keys are one range of rows: rows that were written into slots anywhere can be read back (above), not
+ * attended to.
  * A query row takes part as whole numbers, its largest magnitude being 32639 (QH_BF16: an element is off by 2^-16 of the
  * row's largest at most) or 8355704 (QH_F32: 2^-24), so that sums of products with codes are exact; scores, the softmax and
- * sums are fp32 (256 times the sum of the values' magnitudes over the keys that a row sees has to be finite there).
+ * sums are fp32 (256 times the sum of the values' magnitudes over the keys that a row sees has to be finite there, and so
+ * has scale times a row's product with the codes of a key, before K's scale).
  * Probabilities times V's scales enter the product with the codes exactly for QH_F32; for QH_BF16 in two bfloat16 parts in
- * the form for few rows (off by 2^-16 of sum p |v| at most) and rounded to bfloat16 once in the one for prompts (2^-8). */
+ * the form for few rows (off by 2^-16 of sum p |v| at most) and rounded to bfloat16 once in the one for prompts (2^-8).
+ * bfloat16 prompts of 3000 tokens and more: qh_kv_cache_read_i8 and qh_attention_seq are 5 to 14% faster (8000 tokens, 8 / 2 heads
+ * of 256 322 us for 372), for scratch of the values' size and code times scale rounded to bfloat16. */
 size_t qh_attention_seq_i8_workspace(int q_rows, int n_seq, int max_q, int max_k, int heads, int kv_heads, int head_dim,
                                      int type);
 int qh_attention_seq_i8(void* out, int64_t ldo, int64_t hso, const void* q, int64_t ldq, int64_t hsq, int type, const int8_t* kq,
