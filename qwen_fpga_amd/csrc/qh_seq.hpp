@@ -102,9 +102,10 @@ inline int norm_rope_waves(int tokens, int64_t rows, int dim, bool bf16) {
 // 461 / 382 (8.5), 7 behind 4000 and 512 behind 3488 60 / 78 (4.4); fp32, 8 / 2 heads of 256: 64 x 300 216 / 170 (7.3), 7 behind 4000
 // and 512 behind 3488 85 / 72 (5.9), 31 behind 4000 and 2048 81 / 144 (5.7).
 inline bool attn_i8_prompts(int64_t q_rows, int n_seq, int max_q, int max_k, int heads, int kv_heads, int dim, int tile, bool bf16) {
-  const int64_t G = heads / kv_heads, longest = max_q * G, rest = q_rows > max_q ? (q_rows - max_q) * G : 0;
+  const int64_t G = heads / kv_heads, longest = max_q * G, rest = q_rows > max_q ? q_rows - max_q : 0;
+  const int64_t others = n_seq - 1 < rest ? n_seq - 1 : rest;   // (the places of a batch that no token is left for are empty)
   const int64_t pairs = q_rows * heads * ((max_k > max_q ? max_k : max_q) - max_q / 2);
-  auto tiles = [&](int rows) { return (longest + rest) / rows + n_seq - 1; };
+  auto tiles = [&](int rows) { return (longest + rest * G) / rows + others; };
   const int64_t from = max_k / 2 >= max_q ? 15000000 : bf16 ? 20000000 : 33000000;
   return longest > 256 && pairs >= from && tiles(16) >= (!bf16 ? 6 : dim == 256 ? 9 : 8) * tiles(tile);
 }

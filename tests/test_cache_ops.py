@@ -249,6 +249,7 @@ def test_attention_form_of_mixed_calls(q, bf16, heads, kv_heads, dim):
     for single, keys, part in ((31, 30000, 65), (31, 30000, 512), (255, 8000, 128), (31, 4000, 512), (100, 4000, 1000), (128, 4000, 300),
                                (60000, 8000, 4096)):
         assert not f(single + part, single + 1, part, keys)
+    assert f(4096, 64, 4096, 8192) and f(4100, 256, 4096, 8192)           # places that are empty, as the rows tell, count for nothing
     assert f(7 + 8000, 8, 8000, 8000) and f(31 + 20000, 32, 20000, 20000)
     assert f(1, 1, 1 << 26, 4000) and f(300, 150, 1 << 26, 4000)          # a bound of many rows asks for it
     if heads > kv_heads:
