@@ -1048,3 +1048,57 @@ def test_cache_rows_are_quant_rows_at_any_size(q, torch_cuda, d):
 @pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
 def test_norm_rope_numbers_of_waves(q, torch_cuda, tokens, h, kvh, d, rot, bf16):
     test_norm_rope(q, torch_cuda, tokens, h, kvh, d, rot, bf16)
+
+
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+@pytest.mark.parametrize("max_q", [1, LARGE])
+@pytest.mark.parametrize("d", [128, 256])
+def test_attention_inputs_that_repeat(q, torch_cuda, bf16, max_q, d):
+    """Strides of 0: one scale for all rows or for all heads, one row of codes for all, one head of keys for two; the first
+    sequence behind rows of none; sequences whose keys are the same rows."""
+    torch = torch_cuda
+    lens, ctx, h, kvh, rows = [40, 1, 70], [150, 400, 290], 4, 2, 420
+    at = [20, 20, 100]
+    inp, _ = attn_inputs(torch, 31, lens, [rows], h, kvh, d, bf16)
+    qq, kq, ks, vq, vs = inp
+    for host in ((kq, ks[:1].expand(rows, kvh), vq, vs[:, :1].expand(rows, kvh)), (kq[:, :1].expand(rows, kvh, d), ks, vq[5:6].expand(rows, kvh, d), vs),
+                 (kq[7:8].expand(rows, kvh, d), ks[3:4, :1].expand(rows, kvh), vq, vs)):
+        dev = [qq.cuda()]
+        for x in host:      # the same strides on the device
+            base = x[tuple(slice(0, 1) if s == 0 else slice(None) for s in x.stride())].contiguous().cuda()
+            dev.append(base.expand(x.shape))
+            assert 0 in dev[-1].stride() or 0 not in x.stride()
+        want = attn_oracle(torch, qq, *host, lens, ctx, at, 1 / math.sqrt(d), bf16)
+        pre = 3
+        out = torch.full((pre + sum(lens), h, d), 7.0, dtype=qq.dtype, device="cuda")
+        dev[0] = torch.cat([dev[0][:pre], dev[0]])
+        i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+        ws = torch.empty(q.attention_seq_i8_workspace(out.shape[0], 3, max_q, rows, h, kvh, d), dtype=torch.uint8, device="cuda")
+        q.attention_seq_i8(out, *dev, i32([pre + x for x in starts(lens)]), torch.tensor(at, dtype=torch.int64, device="cuda"), i32(ctx), ws, max_q, rows)
+        assert (out[:pre] == 7).all()
+        attn_check(torch, out[pre:], want, bf16)
+
+
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+def test_norms_and_cache_inputs_that_repeat(q, torch_cuda, bf16):
+    """Strides of 0 in what is read: one row of queries for all tokens, one head of keys for all, one row of new values for all tokens,
+    one scale for the cache's rows."""
+    torch = torch_cuda
+    g, dt = gen(torch, 32), torch.bfloat16 if bf16 else torch.float32
+    x, y = torch.randn(1, 4, 128, generator=g).to(dt), torch.randn(30, 1, 128, generator=g).to(dt)
+    w, pos = torch.randn(128, generator=g), torch.arange(30, dtype=torch.int32)
+    qo, ko = torch.empty(30, 4, 128, dtype=dt, device="cuda"), torch.empty(30, 2, 128, dtype=dt, device="cuda")
+    q.qk_norm_rope_seq(qo, ko, x.cuda().expand(30, 4, 128), y.cuda().expand(30, 2, 128), w.cuda(), w.cuda(), pos.cuda())
+    rope_check(torch, qo, rope_oracle(torch, x.expand(30, 4, 128), w, pos, 64), bf16)
+    rope_check(torch, ko, rope_oracle(torch, y.expand(30, 2, 128), w, pos, 64), bf16)
+    c = cache_new(torch, 40, 2, 128, "rows")
+    slot = torch.randperm(40, generator=g)[:30]
+    q.kv_cache_write_i8(*c, y.cuda().expand(30, 2, 128), x[:, :2].cuda().expand(30, 2, 128), slot.cuda())
+    for src, cq, cs in ((y.expand(30, 2, 128), c[0], c[1]), (x[:, :2].expand(30, 2, 128), c[2], c[3])):
+        codes, sc = code_oracle(torch, src)
+        assert torch.equal(cq[slot.cuda()].cpu(), codes) and torch.equal(cs[slot.cuda()].cpu(), sc)
+    one = torch.rand(1, 2, generator=g)
+    o = [torch.empty(30, 2, 128, dtype=dt, device="cuda") for _ in range(2)]
+    q.kv_cache_read_i8(*o, c[0][:1].expand(40, 2, 128), one.cuda().expand(40, 2), c[2], one.cuda().expand(40, 2), slot.cuda())
+    assert torch.equal(o[0].cpu(), (c[0][:1].cpu().float() * one[..., None]).expand(30, 2, 128).to(dt))
+    assert torch.equal(o[1].cpu(), (c[2].cpu()[slot].float() * one[..., None]).to(dt))
