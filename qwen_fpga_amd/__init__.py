@@ -815,11 +815,12 @@ def attention_seq_i8(out, q, kq, ks, vq, vs, cu_q, k_start, k_len, workspace, ma
                      scale: Optional[float] = None, stream=None):
     """attention_seq over an int8 cache (kv_cache_write_i8's): q, out [q_rows, heads, dim] (float32 or bfloat16, any row
     and head strides), kq, vq int8 [k_rows, kv_heads, dim], ks, vs float32 [k_rows, kv_heads]; sequences, key ranges,
-    bounds and workspace (attention_seq_i8_workspace(...) bytes) as there: a sequence's keys are one range of rows of the cache, not
-    slots anywhere.  A row that sees a scale that is NaN gives NaN.  A query row takes part as whole numbers, off by 2^-16 of its largest element at most (bfloat16) or 2^-24
-    (float32); bfloat16: the form for prompts rounds the probabilities to bfloat16 for their product with the codes (2^-8 of
-    sum p |v|), the one for few rows takes them in two parts (2^-16).  bfloat16 prompts of 3000 tokens and more: kv_cache_read_i8 and
-    attention_seq are 5 to 14% faster, for scratch of the values' size and another rounding."""
+    bounds and workspace (attention_seq_i8_workspace(...) bytes) as there: a sequence's keys are one range of rows of the
+    cache, not slots anywhere.  A row that sees a scale that is NaN gives NaN.  A query row takes part as whole numbers, off
+    by 2^-16 of its largest element at most (bfloat16) or 2^-24 (float32); bfloat16: the form for prompts rounds the
+    probabilities to bfloat16 for their product with the codes (2^-8 of sum p |v|), the one for few rows takes them in two
+    parts (2^-16).  bfloat16 prompts of 3000 tokens and more: kv_cache_read_i8 and attention_seq are 5 to 14% faster, for
+    scratch of the values' size and another rounding."""
     fn = _op("qh_attention_seq_i8")
     nq, nk, n = _dims(q, 3, "q"), _dims(kq, 3, "kq"), _dims(k_len, 1, "k_len")[0]
     (rows, heads, d), (krows, kvh, _) = nq, nk
